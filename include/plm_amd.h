@@ -469,6 +469,89 @@ int plm_voronoi_assign(int32_t dtype, const void* logits, int64_t ld_logits, con
                        void* stream);
 size_t plm_voronoi_assign_workspace_bytes(int64_t n_problems, int64_t n_targets, int64_t k, int64_t n_items);
 
+/*
+ * Attention over a paged cache of keys and values: the step between the QKV linear and attn-out.
+ *
+ * A cache holds `pages` pages of `page` tokens (16, 32, 64 or 128) for kv_heads heads of head_dim
+ * dimensions (a multiple of 8, at most 256; padded with zeros to chunks of 64), keys and values apart,
+ * as bf16 / fp16 or as e4m3 codes times one power of two per (page, head). Page (id, head) is
+ * page / 16 x ceil(head_dim / 64) units of 16 tokens x 64 dimensions in the order the matrix
+ * instructions read; with n = token % 16 and e = dimension % 64 a unit holds
+ *   e4m3 keys     [4, 16, 16]      at [e / 16, n, e % 16]
+ *   e4m3 values   [4, 16, 4, 4]    at [n / 4, e / 4, e % 4, n % 4]
+ *   16-bit keys   [2, 4, 16, 8]    at [e / 8 % 2, e / 16, n, e % 8]
+ *   16-bit values [2, 4, 16, 2, 4] at [e / 2 % 2, n / 4, e / 4, e % 2, n % 4]
+ * k, v: [pages, kv_heads, page / 16, chunks, unit]; k_scale, v_scale: float [pages, kv_heads] (NULL for
+ * 16-bit caches), powers of two in [2^-64, 2^127].
+ *
+ * Rows of a call: `total` rows of `seqs` sequences, one after the other; sequence b's are
+ * [row_starts[b], row_starts[b + 1]) (row_starts NULL: max_rows each, total = seqs * max_rows), at most
+ * max_rows of them, and follow a context of lengths[b] tokens: row i is token lengths[b] + i. Token t
+ * of sequence b is in page table[b, t / page] (int32, row stride table_stride, table_width entries).
+ * lengths, row_starts and positions are int64, all on the device. An entry outside [0, pages) is a page
+ * that is not there: rows for it are not stored, its tokens are not seen, they read as zeros. Row
+ * tensors have their dimensions contiguous; q_row, q_head, ... are strides in elements, multiples of 8;
+ * bases are 16-byte aligned.
+ */
+enum plm_cache_type { PLM_CACHE_BF16 = 0, PLM_CACHE_F16 = 1, PLM_CACHE_E4M3 = 2 };
+
+typedef struct plm_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages;
+  int32_t kv_heads, page, head_dim, type;
+} plm_kv_cache;
+
+/*
+ * Turns the rows' queries and keys by their positions and stores keys and values in the cache.
+ * rope: float [rope_rows, rotary], a position's rotary / 2 cosines, then its sines (NULL: no rotation);
+ * dimensions past `rotary` stay. A pair is (i, i + rotary / 2), or with side_by_side (2 i, 2 i + 1):
+ * (a, b) becomes (a cos - b sin, b cos + a sin). Row r's position is positions[r], or its token number
+ * where positions is NULL; a position that the table does not hold turns into NaN.
+ * q_out: contiguous [total, heads, head_dim] (q NULL: no queries). It must not overlap q.
+ * 8-bit pages: a page's scale is the least power of two that its rows need (largest magnitude <= 448
+ * scale); it grows with them, the rows that stay are then rounded again, and starts anew with the
+ * page's first row. What is not finite becomes NaN and has no part in the scale.
+ * No two sequences may append to the same page in one call.
+ */
+int plm_kv_append(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int32_t heads,
+                  void* q_out, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                  int64_t v_head, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table,
+                  int64_t table_stride, int64_t table_width, const int64_t* lengths, const int64_t* row_starts,
+                  const float* rope, int64_t rope_rows, int32_t rotary, int32_t side_by_side,
+                  const int64_t* positions, void* stream);
+
+/* Tokens [first[b], min(first[b] + most, ends[b])) of every sequence as values of `dtype`: k, v
+ * contiguous [seqs, most, kv_heads, head_dim], zeros past ends[b]. */
+int plm_kv_read(int32_t dtype, const plm_kv_cache* cache, const int32_t* table, int64_t table_stride,
+                int64_t table_width, const int64_t* first, const int64_t* ends, int64_t seqs, int64_t most, void* k,
+                void* v, void* stream);
+
+/*
+ * out[row, head] = softmax over the tokens that the row sees of (scale * q . key), times the values;
+ * head h reads key head h / (heads / kv_heads). The rows' own keys and values are in the cache already.
+ * Row i of sequence b sees
+ *   mask NULL: tokens t <= lengths[b] + i;
+ *   mask (uint32 [mask_rows, mask_words]): the context, and own row j where bit j % 32 of
+ *     mask[i, j / 32] is set;
+ * and with window > 0 of these only t > position - window or t < sinks, the position being positions[r]
+ * (positions NULL: lengths[b] + i); under a mask the window holds for the context alone. A row that sees
+ * nothing is zero. out: contiguous [total, heads, head_dim].
+ * Workspace: plm_attend_workspace_bytes (0: none needed), 16-byte aligned, its counters (the first
+ * PLM_ATTEND_COUNTER_BYTES) zero before the first call; each call leaves them zero. Calls that may run at
+ * the same time need workspaces of their own.
+ */
+#define PLM_ATTEND_COUNTER_BYTES 16384
+int plm_attend(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int32_t heads,
+               void* out, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table, int64_t table_stride,
+               int64_t table_width, const int64_t* lengths, const int64_t* row_starts, int64_t window, int64_t sinks,
+               const uint32_t* mask, int64_t mask_rows, int64_t mask_words, const int64_t* positions, float scale,
+               void* workspace, size_t workspace_bytes, void* stream);
+size_t plm_attend_workspace_bytes(int32_t kv_heads, int32_t page, int32_t head_dim, int32_t heads, int64_t total,
+                                  int64_t seqs, int64_t max_rows, int64_t table_width);
+
 /* Human-readable name of a status code. */
 const char* plm_status_string(int32_t status);
 

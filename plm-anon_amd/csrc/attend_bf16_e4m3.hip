@@ -1,0 +1,11 @@
+// Attention over e4m3 pages, bf16 rows: the kernels of attend.h, a translation unit of its own so that
+// the build compiles them in parallel.
+#include "attend.h"
+
+namespace plm {
+
+hipError_t attend_bf16_e4m3(const AttendArgs& a, int tiles, unsigned grid, hipStream_t s) {
+  return attend_pick<DT_BF16, true>(a, tiles, grid, s);
+}
+
+}  // namespace plm

@@ -1,0 +1,510 @@
+// The paged cache's append (with the position rotation of keys and queries) and its read, declared in
+// include/plm_amd.h.
+//
+// Rotation: dimensions (a, b) of a pair become (a cos - b sin, b cos + a sin) in fp32; a pair is (i,
+// i + rotary / 2), or (2 i, 2 i + 1) side by side. A query is rounded once to the model's type, a key
+// once to what the cache holds.
+//
+// 8-bit pages: codes times one power of two per (page, head). Appending rows needs their largest
+// magnitude first: a workgroup owns one (page, head) of the keys or of the values, keeps its new rows
+// in registers while it finds it, and rounds the rows that stay again only where the scale grows.
+#include <hip/hip_runtime.h>
+
+#include "kv_cache.h"
+#include "plm_amd.h"
+
+namespace plm {
+
+struct AppendArgs {
+  KvCache cache;
+  KvRows rows;
+  const uint16_t* q;
+  const uint16_t* new_k;
+  const uint16_t* new_v;
+  uint16_t* q_out;  // contiguous [total, heads, dim]
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int64_t* positions;
+  const float* rope;  // [rope_rows, rotary]: cosines, then sines
+  int64_t rope_rows;
+  int heads, rotary, side_by_side, page_slots, kv_blocks, q_blocks;
+};
+
+// Dimensions [e0, e0 + 8) of a row, as fp32, turned. `turn` is the position's row of the rotation table,
+// null where the table does not hold the position: what it would have turned is NaN.
+template <int DT>
+__device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float* turn, int rotary, bool side_by_side,
+                                         float (&out)[8]) {
+  const u32x4 own = *reinterpret_cast<const u32x4*>(x + e0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[i] = from_bits16<DT>(static_cast<uint16_t>(own[i / 2] >> (16 * (i & 1))));
+  if (e0 >= rotary) return;
+  const int half = rotary >> 1;
+  if (turn == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e0 + i < rotary) out[i] = __builtin_nanf("");
+  } else if (side_by_side) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      if (e0 + i < rotary) {
+        const float c = turn[(e0 + i) >> 1], s = turn[half + ((e0 + i) >> 1)];
+        const float a = out[i], b = out[i + 1];
+        out[i] = fmaf(a, c, -(b * s));
+        out[i + 1] = fmaf(b, c, a * s);
+      }
+    }
+  } else if ((half & 7) == 0) {
+    // The partners are eight consecutive dimensions too.
+    const bool low = e0 < half;
+    const u32x4 other = *reinterpret_cast<const u32x4*>(x + (low ? e0 + half : e0 - half));
+    const float* at = turn + (low ? e0 : e0 - half);
+    float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      *reinterpret_cast<f32x4*>(c + i) = *reinterpret_cast<const f32x4*>(at + i);
+      *reinterpret_cast<f32x4*>(s + i) = *reinterpret_cast<const f32x4*>(at + half + i);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float o = from_bits16<DT>(static_cast<uint16_t>(other[i / 2] >> (16 * (i & 1))));
+      out[i] = fmaf(out[i], c[i], low ? -(o * s[i]) : o * s[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = e0 + i;
+      if (e < rotary) {
+        const bool low = e < half;
+        const float o = from_bits16<DT>(x[low ? e + half : e - half]);
+        const int at = low ? e : e - half;
+        out[i] = fmaf(out[i], turn[at], low ? -(o * turn[half + at]) : o * turn[half + at]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ const float* turn_of(const AppendArgs& a, int row, int slot, bool& none) {
+  none = a.rope == nullptr;
+  if (none) return nullptr;
+  const int64_t at = a.positions != nullptr ? a.positions[row] : slot;
+  return at >= 0 && at < a.rope_rows ? a.rope + at * a.rotary : nullptr;
+}
+
+template <int DT>
+__device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    o[i] = to_bits16<DT>(x[2 * i]) | (static_cast<uint32_t>(to_bits16<DT>(x[2 * i + 1])) << 16);
+  return o;
+}
+
+template <int DT>
+__device__ __forceinline__ void append_queries(const AppendArgs& a, int block) {
+  const int b = block / a.q_blocks;
+  const KvSeq seq = kv_seq(a.rows, b, a.cache.page_shift);
+  const int per_head = a.cache.dim >> 3, per_row = per_head * a.heads;
+  const int64_t at = static_cast<int64_t>(block - b * a.q_blocks) * blockDim.x + threadIdx.x;
+  const int i = static_cast<int>(at / per_row);
+  if (i >= seq.rows) return;
+  const int rest = static_cast<int>(at - static_cast<int64_t>(i) * per_row);
+  const int head = rest / per_head, e0 = (rest - head * per_head) << 3;
+  const int64_t row = seq.start + i;
+  bool none;
+  const float* turn = turn_of(a, static_cast<int>(row), seq.context + i, none);
+  float x[8];
+  rotated8<DT>(a.q + row * a.q_row + head * a.q_head, e0, turn, none ? 0 : a.rotary, a.side_by_side != 0, x);
+  *reinterpret_cast<u32x4*>(a.q_out + (row * a.heads + head) * a.cache.dim + e0) = pack8<DT>(x);
+}
+
+// 16 fp32 values of unit x of the workgroup's page: for keys 16 dimensions of one token, for values 4
+// dimensions (i / 4) of 4 tokens (i % 4); zero where a token is not new.
+struct PageUnit {
+  int token, e;    // first token in the page, first dimension
+  int64_t offset;  // bytes from the (page, head)'s start to its 16 (e4m3) or first 16 (16-bit) bytes
+};
+
+template <bool VALUES, bool E8>
+__device__ __forceinline__ PageUnit page_unit(const KvCache& c, int x) {
+  PageUnit p;
+  constexpr int bytes = E8 ? 1024 : 2048;  // of a unit of 16 tokens x 64 dimensions
+  if constexpr (VALUES) {
+    const int per = c.dim >> 2;
+    p.token = (x / per) << 2;
+    p.e = (x % per) << 2;
+    p.offset = (static_cast<int64_t>(p.token >> 4) * c.chunks + (p.e >> 6)) * bytes +
+               ((p.token & 15) >> 2) * 256 + ((p.e & 63) >> 2) * 16;
+  } else {
+    const int groups = (c.dim + 15) >> 4;
+    const int y = x >> 4;
+    p.token = (x & 15) + ((y / groups) << 4);
+    p.e = (y % groups) << 4;
+    p.offset = (static_cast<int64_t>(p.token >> 4) * c.chunks + (p.e >> 6)) * bytes + ((p.e & 63) >> 4) * 256 +
+               (p.token & 15) * 16;
+  }
+  return p;
+}
+
+template <int DT, bool VALUES>
+__device__ __forceinline__ void new_values(const AppendArgs& a, const KvSeq& seq, const PageUnit& p, int base, int head,
+                                           float (&x)[16]) {
+  const int end = seq.context + seq.rows;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+  if constexpr (VALUES) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int slot = base + p.token + n;
+      if (slot >= seq.context && slot < end) {
+        const int64_t row = seq.start + (slot - seq.context);
+        const u32x2 w = *reinterpret_cast<const u32x2*>(a.new_v + row * a.v_row + head * a.v_head + p.e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * j + n] = from_bits16<DT>(static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1))));
+      }
+    }
+  } else {
+    const int slot = base + p.token;
+    if (slot >= seq.context && slot < end) {
+      const int row = seq.start + (slot - seq.context);
+      bool none;
+      const float* turn = turn_of(a, row, slot, none);
+      const uint16_t* from = a.new_k + static_cast<int64_t>(row) * a.k_row + head * a.k_head;
+      float half[8];
+      rotated8<DT>(from, p.e, turn, none ? 0 : a.rotary, a.side_by_side != 0, half);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = half[i];
+      if (p.e + 8 < a.cache.dim) {
+        rotated8<DT>(from, p.e + 8, turn, none ? 0 : a.rotary, a.side_by_side != 0, half);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[8 + i] = half[i];
+      }
+    }
+  }
+}
+
+// Rows of one page of one head into an 8-bit cache. UPT units of 16 values per thread.
+template <int DT, bool VALUES, int UPT>
+__device__ __forceinline__ void append_page_fp8(const AppendArgs& a, const KvSeq& seq, int64_t id, int base, int head,
+                                                float* red) {
+  const KvCache& c = a.cache;
+  const int count = VALUES ? (c.page >> 2) * (c.dim >> 2) : c.page * ((c.dim + 15) >> 4);
+  const int end = seq.context + seq.rows;
+  float x[UPT][16];
+  PageUnit p[UPT];
+  float amax = 0.0f;
+#pragma unroll
+  for (int u = 0; u < UPT; ++u) {
+    const int at = threadIdx.x + u * 256;
+    p[u] = page_unit<VALUES, true>(c, min(at, count - 1));
+    new_values<DT, VALUES>(a, seq, p[u], base, head, x[u]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float m = fabsf(x[u][i]);
+      amax = m < __builtin_inff() ? fmaxf(amax, m) : amax;  // what is not finite has no part in the scale
+    }
+  }
+  float* held = (VALUES ? c.v_scale : c.k_scale) + id * c.heads + head;
+  const bool stays = base < seq.context;  // the page holds rows from before
+  const float before = stays ? *held : 0.0f;
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
+  __syncthreads();
+  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float wanted = fp8_scale_of(amax);
+  const float scale = stays ? fmaxf(before, wanted) : wanted;
+  const float inverse = 1.0f / scale;
+  const bool again = stays && scale > before;
+  const float ratio = before * inverse;  // a power of two, at most 1
+  char* page = (VALUES ? c.v : c.k) + (id * c.heads + head) * (static_cast<int64_t>(c.page) * c.chunks * 64);
+#pragma unroll
+  for (int u = 0; u < UPT; ++u) {
+    const int at = threadIdx.x + u * 256;
+    if (at >= count) continue;
+    const int first = base + p[u].token, last = first + (VALUES ? 4 : 1);  // slots [first, last)
+    const bool any_new = last > seq.context && first < end, any_old = first < seq.context;
+    if (!any_new && !(again && any_old)) continue;
+    u32x4* to = reinterpret_cast<u32x4*>(page + p[u].offset);
+    const u32x4 old = any_old ? *to : u32x4{0u, 0u, 0u, 0u};
+    u32x4 word;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float y[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float rounded = fp8_value(old[j], n) * ratio;
+        y[n] = (VALUES ? first + n : first) < seq.context ? rounded : x[u][4 * j + n] * inverse;
+      }
+      word[j] = fp8_word(y[0], y[1], y[2], y[3]);
+    }
+    *to = word;
+  }
+  if (threadIdx.x == 0) *held = scale;
+}
+
+template <int DT, bool VALUES>
+__device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq& seq, int64_t id, int base, int head) {
+  const KvCache& c = a.cache;
+  const int count = VALUES ? (c.page >> 2) * (c.dim >> 2) : c.page * ((c.dim + 15) >> 4);
+  const int end = seq.context + seq.rows;
+  char* page = (VALUES ? c.v : c.k) + (id * c.heads + head) * (static_cast<int64_t>(c.page) * c.chunks * 128);
+  for (int at = threadIdx.x; at < count; at += 256) {
+    const PageUnit p = page_unit<VALUES, false>(c, at);
+    const int first = base + p.token, last = first + (VALUES ? 4 : 1);
+    if (last <= seq.context || first >= end) continue;
+    float x[16];
+    new_values<DT, VALUES>(a, seq, p, base, head, x);
+    u32x4* to = reinterpret_cast<u32x4*>(page + p.offset);  // the second 16 bytes lie 1 KiB on
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[8 * h + i];
+      u32x4 word = pack8<DT>(y);
+      if constexpr (VALUES) {
+        if (first < seq.context) {  // tokens from before share the word: lanes n of both dimensions
+          const u32x4 old = to[64 * h];
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            if (first + n < seq.context) {
+              const uint32_t keep = 0xffffu << (16 * (n & 1));
+              word[n / 2] = (word[n / 2] & ~keep) | (old[n / 2] & keep);
+              word[2 + n / 2] = (word[2 + n / 2] & ~keep) | (old[2 + n / 2] & keep);
+            }
+        }
+      } else if (p.e + 8 * h >= c.dim) {
+        continue;
+      }
+      to[64 * h] = word;
+    }
+  }
+}
+
+template <int DT, bool E8, int UPT>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+  __shared__ float red[4];
+  int block = blockIdx.x;
+  if (block >= a.kv_blocks) {
+    append_queries<DT>(a, block - a.kv_blocks);
+    return;
+  }
+  const bool values = block & 1;
+  block >>= 1;
+  const int head = block % a.cache.heads;
+  block /= a.cache.heads;
+  const int b = block / a.page_slots;
+  const KvSeq seq = kv_seq(a.rows, b, a.cache.page_shift);
+  const int number = (seq.context >> a.cache.page_shift) + block % a.page_slots;
+  const int base = number << a.cache.page_shift;
+  if (seq.rows == 0 || number >= a.rows.width || base >= seq.context + seq.rows) return;
+  const int64_t id = a.rows.table[b * a.rows.table_stride + number];
+  if (id < 0 || id >= a.cache.pages) return;
+  if constexpr (E8) {
+    if (values) append_page_fp8<DT, true, UPT>(a, seq, id, base, head, red);
+    else append_page_fp8<DT, false, UPT>(a, seq, id, base, head, red);
+  } else {
+    if (values) append_page_16<DT, true>(a, seq, id, base, head);
+    else append_page_16<DT, false>(a, seq, id, base, head);
+  }
+}
+
+struct ReadArgs {
+  KvCache cache;
+  const int32_t* table;
+  const int64_t* first;
+  const int64_t* ends;
+  uint16_t* k;  // [seqs, most, heads, dim]
+  uint16_t* v;
+  int64_t table_stride;
+  int width, seqs, most, blocks;  // blocks per (sequence, keys or values)
+};
+
+// Thread: keys, 8 dimensions of one token; values, 4 dimensions of the 4 tokens that share their words.
+template <int DT, bool E8>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+  const KvCache& c = a.cache;
+  int block = blockIdx.x;
+  const int within = block % a.blocks;
+  block /= a.blocks;
+  const bool values = block & 1;
+  const int b = block >> 1;
+  const int64_t most_tokens = static_cast<int64_t>(a.width) << c.page_shift;
+  const int64_t first = a.first[b], end = min(a.ends[b], most_tokens);
+  const int64_t x = static_cast<int64_t>(within) * 256 + threadIdx.x;
+  constexpr int bytes = E8 ? 1024 : 2048;
+  const int64_t head_bytes = static_cast<int64_t>(c.page >> 4) * c.chunks * bytes;
+  if (!values) {
+    const int per_head = c.dim >> 3, per = per_head * c.heads;
+    const int64_t i = x / per;
+    if (i >= a.most) return;
+    const int rest = static_cast<int>(x - i * per);
+    const int head = rest / per_head, e = (rest - head * per_head) << 3;
+    const int64_t t = first + i;
+    u32x4 out = u32x4{0u, 0u, 0u, 0u};
+    if (t >= 0 && t < end) {
+      const int64_t id = a.table[b * a.table_stride + (t >> c.page_shift)];
+      if (id >= 0 && id < c.pages) {
+        const int n = static_cast<int>(t & (c.page - 1));
+        const char* from = c.k + (id * c.heads + head) * head_bytes +
+                           (static_cast<int64_t>(n >> 4) * c.chunks + (e >> 6)) * bytes + ((e & 63) >> 4) * 256 +
+                           (n & 15) * 16;
+        if constexpr (E8) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(from + (e & 8));
+          const float scale = c.k_scale[id * c.heads + head];
+          float y[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = fp8_value(w[j / 4], j & 3) * scale;
+          out = pack8<DT>(y);
+        } else {
+          out = *reinterpret_cast<const u32x4*>(from + (e & 8) * 128);
+        }
+      }
+    }
+    *reinterpret_cast<u32x4*>(a.k + ((static_cast<int64_t>(b) * a.most + i) * c.heads + head) * c.dim + e) = out;
+    return;
+  }
+  const int per_head = c.dim >> 2, per = per_head * c.heads;
+  const int64_t quad = x / per;  // the quad of tokens, from the one that holds `first`
+  const int rest = static_cast<int>(x - quad * per);
+  const int head = rest / per_head, e = (rest - head * per_head) << 2;
+  const int64_t t0 = ((first >> 2) + quad) << 2;
+  if (t0 - first >= a.most) return;
+  u32x4 w[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+  float scale = 1.0f;
+  if (t0 >= 0 && t0 < end) {
+    const int64_t id = a.table[b * a.table_stride + (t0 >> c.page_shift)];
+    if (id >= 0 && id < c.pages) {
+      const int n = static_cast<int>(t0 & (c.page - 1));
+      const char* from = c.v + (id * c.heads + head) * head_bytes +
+                         (static_cast<int64_t>(n >> 4) * c.chunks + (e >> 6)) * bytes + ((n & 15) >> 2) * 256 +
+                         ((e & 63) >> 2) * 16;
+      w[0] = *reinterpret_cast<const u32x4*>(from);
+      if constexpr (E8) scale = c.v_scale[id * c.heads + head];
+      else w[1] = *reinterpret_cast<const u32x4*>(from + 1024);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int64_t i = t0 + n - first;
+    if (i < 0 || i >= a.most) continue;
+    u32x2 out = u32x2{0u, 0u};
+    if (t0 + n < end) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t half;
+        if constexpr (E8) half = to_bits16<DT>(fp8_value(w[0][j], n) * scale);
+        else half = (w[j / 2][2 * (j & 1) + n / 2] >> (16 * (n & 1))) & 0xffffu;
+        out[j / 2] |= half << (16 * (j & 1));
+      }
+    }
+    *reinterpret_cast<u32x2*>(a.v + ((static_cast<int64_t>(b) * a.most + i) * c.heads + head) * c.dim + e) = out;
+  }
+}
+
+namespace {
+
+template <int DT, bool E8>
+void append_go(const AppendArgs& a, unsigned grid, hipStream_t s) {
+  const int units = a.cache.page * ((a.cache.dim + 15) / 16);
+  if constexpr (!E8) {
+    append_kernel<DT, false, 1><<<grid, 256, 0, s>>>(a);
+  } else {
+    if (units <= 256) append_kernel<DT, true, 1><<<grid, 256, 0, s>>>(a);
+    else if (units <= 512) append_kernel<DT, true, 2><<<grid, 256, 0, s>>>(a);
+    else if (units <= 1024) append_kernel<DT, true, 4><<<grid, 256, 0, s>>>(a);
+    else append_kernel<DT, true, 8><<<grid, 256, 0, s>>>(a);
+  }
+}
+
+}  // namespace
+}  // namespace plm
+
+extern "C" {
+
+int plm_kv_append(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int32_t heads,
+                  void* q_out, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                  int64_t v_head, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table,
+                  int64_t table_stride, int64_t table_width, const int64_t* lengths, const int64_t* row_starts,
+                  const float* rope, int64_t rope_rows, int32_t rotary, int32_t side_by_side,
+                  const int64_t* positions, void* stream) {
+  plm::AppendArgs a{};
+  if (!plm::kv_cache_of(cache, a.cache) || !plm::kv_type_fits(cache, dtype)) return PLM_ERR_ARGUMENT;
+  if (!plm::kv_rows_of(a.cache, total, seqs, max_rows, table, table_stride, table_width, lengths, row_starts, a.rows))
+    return PLM_ERR_ARGUMENT;
+  if (k == nullptr || v == nullptr) return PLM_ERR_ARGUMENT;
+  if (q != nullptr && (heads < 1 || heads > 4096 || q_out == nullptr)) return PLM_ERR_ARGUMENT;
+  if (rope != nullptr && (rotary < 2 || rotary > cache->head_dim || rotary % 2 != 0 || rope_rows < 1))
+    return PLM_ERR_ARGUMENT;
+  if ((q_row | q_head | k_row | k_head | v_row | v_head) % 8 != 0) return PLM_ERR_ALIGNMENT;
+  for (const void* p : {q, static_cast<const void*>(q_out), k, v, static_cast<const void*>(cache->k),
+                        static_cast<const void*>(cache->v), static_cast<const void*>(rope)})
+    if (!plm::aligned16_ptr(p)) return PLM_ERR_ALIGNMENT;
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_out = static_cast<uint16_t*>(q_out);
+  a.new_k = static_cast<const uint16_t*>(k);
+  a.new_v = static_cast<const uint16_t*>(v);
+  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  a.positions = positions;
+  a.rope = rope;
+  a.rope_rows = rope_rows;
+  a.heads = heads;
+  a.rotary = rotary;
+  a.side_by_side = side_by_side;
+  const int64_t page = cache->page;
+  a.page_slots = static_cast<int>((page - 1 + max_rows + page - 1) / page);
+  const int64_t kv_blocks = seqs * a.page_slots * cache->kv_heads * 2;
+  const int64_t q_blocks = q == nullptr ? 0 : (max_rows * heads * (cache->head_dim / 8) + 255) / 256;
+  if (kv_blocks + q_blocks * seqs >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
+  a.kv_blocks = static_cast<int>(kv_blocks);
+  a.q_blocks = static_cast<int>(q_blocks);
+  const unsigned grid = static_cast<unsigned>(kv_blocks + q_blocks * seqs);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool e8 = cache->type == PLM_CACHE_E4M3;
+  if (dtype == PLM_BF16) e8 ? plm::append_go<plm::DT_BF16, true>(a, grid, s) : plm::append_go<plm::DT_BF16, false>(a, grid, s);
+  else e8 ? plm::append_go<plm::DT_F16, true>(a, grid, s) : plm::append_go<plm::DT_F16, false>(a, grid, s);
+  return hipGetLastError() == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
+}
+
+int plm_kv_read(int32_t dtype, const plm_kv_cache* cache, const int32_t* table, int64_t table_stride,
+                int64_t table_width, const int64_t* first, const int64_t* ends, int64_t seqs, int64_t most, void* k,
+                void* v, void* stream) {
+  plm::ReadArgs a{};
+  if (!plm::kv_cache_of(cache, a.cache) || !plm::kv_type_fits(cache, dtype)) return PLM_ERR_ARGUMENT;
+  if (seqs < 1 || seqs > (1 << 20) || most < 1 || most >= (1 << 30) || table == nullptr || first == nullptr ||
+      ends == nullptr || k == nullptr || v == nullptr)
+    return PLM_ERR_ARGUMENT;
+  if (table_width < 1 || table_width > ((int64_t{1} << 29) >> a.cache.page_shift) || table_stride < table_width)
+    return PLM_ERR_ARGUMENT;
+  for (const void* p : {static_cast<const void*>(k), static_cast<const void*>(v), static_cast<const void*>(cache->k),
+                        static_cast<const void*>(cache->v)})
+    if (!plm::aligned16_ptr(p)) return PLM_ERR_ALIGNMENT;
+  a.table = table;
+  a.first = first;
+  a.ends = ends;
+  a.k = static_cast<uint16_t*>(k);
+  a.v = static_cast<uint16_t*>(v);
+  a.table_stride = table_stride;
+  a.width = static_cast<int>(table_width);
+  a.seqs = static_cast<int>(seqs);
+  a.most = static_cast<int>(most);
+  // Keys: an item per token and 8 dimensions; values: per quad of tokens (one more where `first` is
+  // inside a quad) and 4 dimensions, never more items than keys have but for that quad.
+  const int64_t key_items = most * cache->kv_heads * (cache->head_dim / 8);
+  const int64_t value_items = ((most + 3) / 4 + 1) * cache->kv_heads * (cache->head_dim / 4);
+  const int64_t blocks = ((key_items > value_items ? key_items : value_items) + 255) / 256;
+  if (blocks * seqs * 2 >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
+  a.blocks = static_cast<int>(blocks);
+  const unsigned grid = static_cast<unsigned>(blocks * seqs * 2);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool e8 = cache->type == PLM_CACHE_E4M3;
+  if (dtype == PLM_BF16) {
+    if (e8) plm::read_kernel<plm::DT_BF16, true><<<grid, 256, 0, s>>>(a);
+    else plm::read_kernel<plm::DT_BF16, false><<<grid, 256, 0, s>>>(a);
+  } else {
+    if (e8) plm::read_kernel<plm::DT_F16, true><<<grid, 256, 0, s>>>(a);
+    else plm::read_kernel<plm::DT_F16, false><<<grid, 256, 0, s>>>(a);
+  }
+  return hipGetLastError() == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -18,6 +18,9 @@ PLM_BF16, PLM_F16 = 0, 1
 PLM_ROUND_F32, PLM_ROUND_BF16, PLM_ROUND_F16 = 0, 1, 2
 PLM_RULE_NUCLEUS, PLM_RULE_FLOOR = 0, 1
 PLM_OUT_MODEL, PLM_OUT_F32, PLM_OUT_SILU_MUL = 0, 1, 2   # plm_chain_gemm.out_f32
+PLM_CACHE_BF16, PLM_CACHE_F16, PLM_CACHE_E4M3 = 0, 1, 2   # plm_kv_cache.type
+# PLM_ATTEND_COUNTER_BYTES: the zero-between-calls start of an attention workspace.
+ATTEND_COUNTER_BYTES = 16384
 DTYPE_CODES = {torch.bfloat16: PLM_BF16, torch.float16: PLM_F16}
 # PLM_WORKSPACE_COUNTER_BYTES: the zero-between-calls counter area at the start of every workspace.
 COUNTER_BYTES = 1 << 18
@@ -66,6 +69,10 @@ EXPORTS = (
     "plm_voronoi_argmin",
     "plm_voronoi_assign",
     "plm_voronoi_assign_workspace_bytes",
+    "plm_kv_append",
+    "plm_kv_read",
+    "plm_attend",
+    "plm_attend_workspace_bytes",
     "plm_status_string",
 )
 
@@ -89,6 +96,14 @@ class ChainGemm(ctypes.Structure):
                 ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("split_k", ctypes.c_int32), ("dep", ctypes.c_int32),
                 ("out_f32", ctypes.c_int32), ("consumed", ctypes.c_int32), ("arrive_base", ctypes.c_int32),
                 ("done_base", ctypes.c_int32), ("partial_offset", ctypes.c_int64)]
+
+
+class KvCache(ctypes.Structure):
+    """``struct plm_kv_cache``: a paged cache's tensors and sizes."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("page", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("type", ctypes.c_int32)]
 
 
 _lib: ctypes.CDLL | None = None
@@ -182,6 +197,18 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.plm_voronoi_assign.restype = ctypes.c_int
     lib.plm_voronoi_assign_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_i64]
     lib.plm_voronoi_assign_workspace_bytes.restype = c_sz
+    cache_p = ctypes.POINTER(KvCache)
+    rows = [c_i64, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_p]
+    lib.plm_kv_append.argtypes = [c_i32, cache_p, c_p, c_i64, c_i64, c_i32, c_p, c_p, c_i64, c_i64, c_p, c_i64, c_i64, *rows,
+                                  c_p, c_i64, c_i32, c_i32, c_p, c_p]
+    lib.plm_kv_append.restype = ctypes.c_int
+    lib.plm_kv_read.argtypes = [c_i32, cache_p, c_p, c_i64, c_i64, c_p, c_p, c_i64, c_i64, c_p, c_p, c_p]
+    lib.plm_kv_read.restype = ctypes.c_int
+    lib.plm_attend.argtypes = [c_i32, cache_p, c_p, c_i64, c_i64, c_i32, c_p, *rows, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_f,
+                               c_p, c_sz, c_p]
+    lib.plm_attend.restype = ctypes.c_int
+    lib.plm_attend_workspace_bytes.argtypes = [c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_i64, c_i64]
+    lib.plm_attend_workspace_bytes.restype = c_sz
     lib.plm_status_string.argtypes = [c_i32]
     lib.plm_status_string.restype = ctypes.c_char_p
 
