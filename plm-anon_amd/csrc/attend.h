@@ -117,33 +117,29 @@ __device__ __forceinline__ AttendItem attend_item(const AttendArgs& a, int index
     const uint64_t past = __ballot(items + to > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      const int first = items + __shfl(to - mine, at);
+      auto of = [&](int v) { return __builtin_amdgcn_readfirstlane(__shfl(v, at)); };
       it.b = base + at;
-      it.ranges = __shfl(ranges, at);
-      const int tiles = __shfl(s.tiles, at);
-      const int rest = index - first;
+      it.ranges = of(ranges);
+      const int tiles = of(s.tiles), rest = index - (items + of(to - mine));
       if (rest < 0 || tiles < 1) return AttendItem{};
       it.head = rest % heads;
       const int x = rest / heads;
       it.range = x % it.ranges;
       it.tile = tiles - 1 - x / it.ranges;  // a causal tile's work grows with its number: the longest first
-      it.group = groups + __shfl(group_to, at) - tiles * heads + it.tile * heads + it.head;
-      it.slot = slots + __shfl(slot_to, at) - tiles * it.ranges * heads + it.tile * it.ranges * heads + it.head;
-      it.b = __builtin_amdgcn_readfirstlane(it.b);
-      it.ranges = __builtin_amdgcn_readfirstlane(it.ranges);
-      it.head = __builtin_amdgcn_readfirstlane(it.head);
-      it.range = __builtin_amdgcn_readfirstlane(it.range);
-      it.tile = __builtin_amdgcn_readfirstlane(it.tile);
-      it.group = __builtin_amdgcn_readfirstlane(it.group);
-      it.slot = __builtin_amdgcn_readfirstlane(it.slot);
+      it.group = groups + of(group_to) - tiles * heads + it.tile * heads + it.head;
+      it.slot = slots + of(slot_to) - tiles * it.ranges * heads + it.tile * it.ranges * heads + it.head;
       return it;
     }
-    items += __shfl(to, 63);
-    groups += __shfl(group_to, 63);
-    slots += __shfl(slot_to, 63);
+    items += __builtin_amdgcn_readlane(to, 63);
+    groups += __builtin_amdgcn_readlane(group_to, 63);
+    slots += __builtin_amdgcn_readlane(slot_to, 63);
   }
   return it;
 }
+
+// The larger of two, NaN if either is: unlike fmaxf it needs no quieting of its operands, and three values are one
+// instruction. A score that is NaN makes its row NaN, whatever the maximum.
+__device__ __forceinline__ float larger_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // The lane's value and its partner's, 32 (WIDE) or 16 lanes away, in either order.
 template <bool WIDE>
@@ -165,8 +161,8 @@ __device__ __forceinline__ void lane_pair(float v, float& a, float& b) {
 __device__ __forceinline__ float column_max(float v) {
   float a, b;
   lane_pair<true>(v, a, b);
-  lane_pair<false>(fmaxf(a, b), a, b);
-  return fmaxf(a, b);
+  lane_pair<false>(larger_of(a, b), a, b);
+  return larger_of(a, b);
 }
 
 __device__ __forceinline__ float column_sum(float v) {
@@ -176,9 +172,12 @@ __device__ __forceinline__ float column_sum(float v) {
   return a + b;
 }
 
+// Two values in the model's type, rounded to nearest even, as one word.
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return to_bits16<DT>(a) | (static_cast<uint32_t>(to_bits16<DT>(b)) << 16);
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == DT_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
 }
 
 // Whether a 16-bit pair holds an infinity or a NaN.
@@ -188,6 +187,11 @@ __device__ __forceinline__ bool pair_not_finite(uint32_t w) {
   return (w & e) == e || ((w >> 16) & e) == e;
 }
 
+// Whether any of four e4m3 codes is NaN (all seven bits below the sign).
+__device__ __forceinline__ bool fp8_not_finite(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+
+// Scales are at least this (a masked score times a scale of zero would be NaN).
+constexpr float kLeastScale = 1.0f / 18446744073709551616.0f;
 constexpr float kMinusInf = -__builtin_inff();
 // The running maximum follows a larger one only where that is more than this (base 2) above it, so most
 // steps leave the accumulators alone; exponentials then reach 2^kSlack, exact in fp32 sums. fp16
@@ -197,18 +201,279 @@ constexpr float kSlack = 6.0f;
 template <int DT>
 constexpr float kShift = DT == DT_F16 ? 8.0f : 0.0f;
 
+// Token x of a step's 32: its place among the eight of the lanes that hold it.
+struct TokenOf {
+  int slot, holder;
+  u32x4 only;  // masks that leave this token alone
+  __device__ __forceinline__ TokenOf(int x, int g) {
+    slot = ((x >> 4) << 2) | (x & 3);
+    holder = (x & 15) >> 2;
+    const uint32_t half = holder == g ? 0xffffu << (16 * (slot & 1)) : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) only[i] = (slot >> 1) == i ? half : 0u;
+  }
+  // Whether the lane's column sees it, from the bits of the lanes that hold it.
+  __device__ __forceinline__ bool seen(uint32_t bits, int step, int col) const {
+    return ((__shfl(static_cast<int>(bits), holder * 16 + col) >> (8 * step + slot)) & 1) != 0;
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ void take_token(u32x4 v, u32x4 p, bool sees, f32x4& o) {
+  const f32x4 sum = mfma_16x16x32<DT>(v, p, o);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = sees ? sum[r] : o[r];
+}
+
+// The queries of a wavefront's NC x 16 columns: lane l has column l % 16 of each sixteen.
+template <int NC>
+struct AttendColumns {
+  int row[NC], head[NC], window_lo[NC];
+  bool real[NC];  // others repeat the sequence's last column and are not stored
+
+  __device__ __forceinline__ void set(const AttendArgs& a, const KvSeq& seq, const AttendItem& it, int first, int columns,
+                                      int col) {
+    constexpr int far = 1 << 30;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int x = first + 16 * n + col, y = min(x, columns - 1);
+      real[n] = x < columns;
+      row[n] = y / a.group;
+      head[n] = it.head * a.group + y - row[n] * a.group;
+      const int64_t p = a.positions != nullptr ? a.positions[seq.start + row[n]] : seq.context + row[n];
+      window_lo[n] = a.window > 0 ? max(static_cast<int>(min(max(p, static_cast<int64_t>(-far)), static_cast<int64_t>(far))) - a.window + 1, 0) : 0;
+    }
+  }
+
+  // Whether column n sees token t of a page that is there.
+  __device__ __forceinline__ bool sees(const AttendArgs& a, const KvSeq& seq, int n, int t) const {
+    if (t >= seq.context + seq.rows) return false;
+    const bool near = t >= window_lo[n] || t < a.sinks;
+    if (a.mask == nullptr) return near && t <= seq.context + row[n];
+    if (t < seq.context) return near;
+    const int i = t - seq.context;
+    return (i >> 5) < a.mask_words && row[n] < a.mask_rows &&
+           ((a.mask[static_cast<int64_t>(row[n]) * a.mask_words + (i >> 5)] >> (i & 31)) & 1u) != 0;
+  }
+
+  // Bit 4 u + r: column n sees token t0 + 16 u + 4 g + r; units without a page (`held`) are not seen. A loop, since
+  // only tiles at an edge come here: unrolled, its loads of mask words would take the registers of all others.
+  template <int UNITS>
+  __device__ __forceinline__ uint32_t seen_bits(const AttendArgs& a, const KvSeq& seq, int n, int t0, int g,
+                                                uint32_t held) const {
+    uint32_t bits = 0;
+#pragma unroll 1
+    for (int u = 0; u < UNITS; ++u) {
+      uint32_t four = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) four |= static_cast<uint32_t>(sees(a, seq, n, t0 + 16 * u + 4 * g + r)) << r;
+      if ((held >> u) & 1u) bits |= four << (4 * u);
+    }
+    return bits;
+  }
+
+  template <int DT, int C>
+  __device__ __forceinline__ void queries(const AttendArgs& a, const KvSeq& seq, int g, u32x4 (&q)[NC][C][2]) const {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const uint16_t* from = a.q + (seq.start + row[n]) * a.q_row + head[n] * a.q_head;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int e = 64 * c + 16 * g + 8 * h;
+          q[n][c][h] = real[n] && e < a.cache.dim ? *reinterpret_cast<const u32x4*>(from + e) : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+  }
+
+  // The finished sums over l, in the model's type.
+  template <int DT, int C>
+  __device__ __forceinline__ void store(const AttendArgs& a, const KvSeq& seq, int g, const f32x4 (&o)[NC][C][4],
+                                        const float (&l)[NC]) const {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      if (!real[n]) continue;
+      const float inverse = l[n] == 0.0f ? 0.0f : 1.0f / l[n];  // a row that sees nothing is zero
+      uint16_t* at = a.out + (static_cast<int64_t>(seq.start + row[n]) * a.heads + head[n]) * a.cache.dim;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int e = 64 * c + 16 * g;
+        u32x4 word[2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // dimensions e + 2 i, e + 2 i + 1
+          const int r = i / 2, j = 2 * (i & 1);
+          word[i / 4][i % 4] = pack2<DT>(o[n][c][j][r] * inverse, o[n][c][j + 1][r] * inverse);
+        }
+        if (e < a.cache.dim) *reinterpret_cast<u32x4*>(at + e) = word[0];
+        if (e + 8 < a.cache.dim) *reinterpret_cast<u32x4*>(at + e + 8) = word[1];
+      }
+    }
+  }
+};
+
+// The tokens that a tile of columns looks at: steps of `STEP` tokens, the sinks' first, then from the window's
+// (or the sequence's) first on. Step s begins at token_of(s).
+template <int STEP>
+struct AttendWalk {
+  int whole;            // tokens before this are seen by every column, the window apart
+  int lo_most, sinks;   // tokens from lo_most on, and before `sinks`, are inside every column's window
+  int sink_steps, first, steps;
+  int from, to;         // the range's steps
+
+  template <int NC>
+  __device__ __forceinline__ void set(const AttendArgs& a, const KvSeq& seq, const AttendItem& it, int cols, int columns,
+                                      const AttendColumns<NC>& c, int lo_least) {
+    const int row_lo = it.tile * cols / a.group, row_hi = (min((it.tile + 1) * cols, columns) - 1) / a.group;
+    const int end = a.mask != nullptr ? seq.context + seq.rows : seq.context + row_hi + 1;
+    whole = a.mask != nullptr ? seq.context : seq.context + row_lo + 1;
+    sinks = a.sinks;
+    // Under a mask the window holds for the context alone: the rows' own tokens are always walked.
+    if (a.mask != nullptr) lo_least = min(lo_least, seq.context);
+    const int last = (end + STEP - 1) / STEP;
+    first = min(lo_least / STEP, last);
+    sink_steps = min((min(a.sinks, 1 << 29) + STEP - 1) / STEP, first);
+    steps = sink_steps + last - first;
+    from = static_cast<int>(static_cast<int64_t>(steps) * it.range / it.ranges);
+    to = static_cast<int>(static_cast<int64_t>(steps) * (it.range + 1) / it.ranges);
+  }
+  __device__ __forceinline__ int token_of(int s) const { return STEP * (s < sink_steps ? s : first + s - sink_steps); }
+  __device__ __forceinline__ bool edge(int t0) const { return t0 + STEP > whole || (t0 < lo_most && t0 + STEP > sinks); }
+};
+
+// Least and largest first token of the columns' windows over the sixteen lanes of a group (0 without a window).
+template <int NC>
+__device__ __forceinline__ void window_bounds(const AttendArgs& a, const AttendColumns<NC>& c, int& least, int& most) {
+  least = most = 0;
+  if (a.window <= 0) return;
+  least = 1 << 30;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    least = min(least, c.window_lo[n]);
+    most = max(most, c.window_lo[n]);
+  }
+#pragma unroll
+  for (int x = 8; x > 0; x >>= 1) {
+    least = min(least, __shfl_xor(least, x));
+    most = max(most, __shfl_xor(most, x));
+  }
+  least = __builtin_amdgcn_readfirstlane(least);
+  most = __builtin_amdgcn_readfirstlane(most);
+}
+
+// A partial result's slot: [cols][pad] sums, then [cols] maxima and [cols] sums of exponentials. Written and read
+// past the XCD's own L2 (tile.h).
+template <int NC, int C>
+__device__ __forceinline__ void attend_publish(const AttendArgs& a, const AttendItem& it, int cols, int first, int g, int col,
+                                               const AttendColumns<NC>& c, const f32x4 (&o)[NC][C][4], const float (&m)[NC],
+                                               const float (&l)[NC]) {
+  constexpr int PAD = 64 * C;
+  const uint32_t bytes = static_cast<uint32_t>(attend_slot_floats(cols, PAD) * 4);
+  char* mine = reinterpret_cast<char*>(a.partials) + static_cast<int64_t>(it.slot + it.range * a.cache.heads) * bytes;
+  const __amdgpu_buffer_rsrc_t rs = make_rsrc(mine, bytes);
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    if (!c.real[n]) continue;
+    const int at = first + 16 * n + col;
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 x = {o[n][k][0][r], o[n][k][1][r], o[n][k][2][r], o[n][k][3][r]};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rs, (at * PAD + 64 * k + 16 * g + 4 * r) * 4, 0,
+                                               kCoherent);
+      }
+    if (g == 0) {
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m[n]), rs, (cols * PAD + at) * 4, 0, kCoherent);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, l[n]), rs, (cols * PAD + cols + at) * 4, 0, kCoherent);
+    }
+  }
+}
+
+// Joins a group's ranges, by every thread of the workgroup that arrived last. `shared`: (kAttendMost + 1) * cols floats.
+template <int DT, int C>
+__device__ __forceinline__ void attend_join(const AttendArgs& a, const KvSeq& seq, const AttendItem& it, int cols, int columns,
+                                            float* shared) {
+  constexpr int PAD = 64 * C;
+  const uint32_t bytes = static_cast<uint32_t>(attend_slot_floats(cols, PAD) * 4);
+  const int live = min(cols, columns - it.tile * cols), threads = blockDim.x, dim = a.cache.dim;
+  float* weight = shared;               // [ranges][cols]
+  float* total = weight + it.ranges * cols;
+  auto slot_of = [&](int range) {
+    return reinterpret_cast<const char*>(a.partials) + static_cast<int64_t>(it.slot + range * a.cache.heads) * bytes;
+  };
+  for (int i = threadIdx.x; i < it.ranges * cols; i += threads) {
+    const int range = i / cols, c = i - range * cols;
+    weight[i] = c < live ? collect(reinterpret_cast<const float*>(slot_of(range)) + cols * PAD + c) : kMinusInf;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < live; c += threads) {
+    float top = kMinusInf, sum = 0.0f;
+    for (int range = 0; range < it.ranges; ++range) top = fmaxf(top, weight[range * cols + c]);
+    for (int range = 0; range < it.ranges; ++range) {
+      const float m = weight[range * cols + c];
+      const float x = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+      weight[range * cols + c] = x;
+      sum += x * collect(reinterpret_cast<const float*>(slot_of(range)) + cols * PAD + cols + c);
+    }
+    total[c] = sum == 0.0f ? 0.0f : 1.0f / sum;
+  }
+  __syncthreads();
+  const int quads = dim >> 2;
+  for (int i = threadIdx.x; i < live * quads; i += threads) {
+    const int c = i / quads, e = (i - c * quads) << 2;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int range = 0; range < it.ranges; ++range) {
+      const __amdgpu_buffer_rsrc_t rs = make_rsrc(slot_of(range), bytes);
+      const f32x4 x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (c * PAD + e) * 4, 0, kCoherent));
+      sum += x * weight[range * cols + c];
+    }
+    sum *= total[c];
+    const int x = it.tile * cols + c, row = x / a.group;
+    uint16_t* at = a.out + (static_cast<int64_t>(seq.start + row) * a.heads + it.head * a.group + x - row * a.group) * dim;
+    *reinterpret_cast<u32x2*>(at + e) = u32x2{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
+  }
+}
+
+// Chunk c of the unit at byte `at` (the same in every lane). Dimensions past the head's, in the last chunk, are not
+// read: a lane whose are (`inside` false) gets zeros.
+template <bool E8, int C>
+__device__ __forceinline__ void load_chunk_of(__amdgpu_buffer_rsrc_t rs, int c, int lane, bool inside, u32x4 (&x)[E8 ? 1 : 2]) {
+#pragma unroll
+  for (int h = 0; h < (E8 ? 1 : 2); ++h) {
+    const uint32_t off = static_cast<uint32_t>((c * (E8 ? 1 : 2) + h) * 1024 + lane * 16);
+    x[h] = buffer_load16(rs, c == C - 1 && !inside ? kOutOfRange : off);
+  }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t unit_rsrc(const char* base, int64_t at, uint32_t bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base) + static_cast<uint64_t>(at);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(p));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(p >> 32));
+  return make_rsrc(reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo), bytes);
+}
+
+template <bool E8, int C>
+__device__ __forceinline__ void load_unit(const char* base, int64_t at, int lane, bool inside, u32x4 (&x)[C][E8 ? 1 : 2]) {
+  const __amdgpu_buffer_rsrc_t rs = unit_rsrc(base, at, C * (E8 ? 1024 : 2048));
+#pragma unroll
+  for (int c = 0; c < C; ++c) load_chunk_of<E8, C>(rs, c, lane, inside, x[c]);
+}
+
 // A wavefront's state and its walk over tokens.
 template <int DT, bool E8, int C, int NC>
 struct AttendWave {
   static constexpr int kLoads = E8 ? 1 : 2;  // of 16 bytes per lane, unit and chunk
   static constexpr int kUnitBytes = 1024 * kLoads;
 
-  struct Step {
-    u32x4 k[2][C][kLoads], v[2][C][kLoads];
+  // Where a step's two units are.
+  struct Place {
+    int64_t at[2];
     float ks[2], vs[2];
     bool held[2];  // the unit's page is a page of the cache
   };
 
+  u32x4 k[2][C][kLoads], v[2][C][kLoads];
   f32x4 o[NC][C][4];
   u32x4 q[NC][C][2];
   float m[NC], l[NC];
@@ -224,7 +489,7 @@ struct AttendWave {
     const bool good = id >= 0 && id < a.cache.pages;
     page_id = good ? id : -1;
     if constexpr (E8) {
-      page_ks = good ? a.cache.k_scale[static_cast<int64_t>(id) * a.cache.heads + head] : 0.0f;
+      page_ks = good ? fmaxf(a.cache.k_scale[static_cast<int64_t>(id) * a.cache.heads + head], kLeastScale) : kLeastScale;
       page_vs = good ? a.cache.v_scale[static_cast<int64_t>(id) * a.cache.heads + head] : 0.0f;
       float most = page_vs;
 #pragma unroll
@@ -243,7 +508,8 @@ struct AttendWave {
     }
   }
 
-  __device__ __forceinline__ void fetch(const AttendArgs& a, int b, int head, int t0, int last_page, int lane, Step& s) {
+  __device__ __forceinline__ Place place(const AttendArgs& a, int b, int head, int t0, int last_page, int lane) {
+    Place s;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int t = t0 + 16 * u;
@@ -256,27 +522,29 @@ struct AttendWave {
         s.vs[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, page_vs), number - page_first));
       }
       const int unit = (t & (a.cache.page - 1)) >> 4;
-      const int64_t at = ((static_cast<int64_t>(max(id, 0)) * a.cache.heads + head) * (a.cache.page >> 4) + unit) *
-                         (a.cache.chunks * kUnitBytes);
-      const char* k = a.cache.k + at;
-      const char* v = a.cache.v + at;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int h = 0; h < kLoads; ++h) {
-          const uint32_t off = c * kUnitBytes + h * 1024 + lane * 16;
-          // Dimensions past the head's are not read: 16 (keys) or 4 (values) of them per lane.
-          s.k[u][c][h] = 64 * c + 16 * (lane >> 4) < a.cache.dim ? *reinterpret_cast<const u32x4*>(k + off) : u32x4{0u, 0u, 0u, 0u};
-          s.v[u][c][h] = 64 * c + 4 * (lane & 15) < a.cache.dim ? *reinterpret_cast<const u32x4*>(v + off) : u32x4{0u, 0u, 0u, 0u};
-        }
+      s.at[u] = ((static_cast<int64_t>(max(id, 0)) * a.cache.heads + head) * (a.cache.page >> 4) + unit) *
+                (a.cache.chunks * kUnitBytes);
     }
+    return s;
+  }
+
+  __device__ __forceinline__ void keys(const AttendArgs& a, const Place& s, int lane) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_unit<E8, C>(a.cache.k, s.at[u], lane, 16 * (lane >> 4) < a.cache.dim - 64 * (C - 1), k[u]);
+  }
+  __device__ __forceinline__ void values(const AttendArgs& a, const Place& s, int lane) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_unit<E8, C>(a.cache.v, s.at[u], lane, 4 * (lane & 15) < a.cache.dim - 64 * (C - 1), v[u]);
   }
 };
 
+// Wavefronts per SIMD to leave registers for.
+constexpr int attend_waves(int chunks, int nc) { return chunks * nc == 1 ? 4 : chunks * nc == 2 ? 3 : chunks * nc <= 4 ? 2 : 1; }
+
 template <int DT, bool E8, int C, int NC, int W>
-__global__ __launch_bounds__(64 * W) void attend_kernel(AttendArgs a) {
-  constexpr int COLS = 16 * NC, PAD = 64 * C;
-  extern __shared__ char lds[];
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_waves(C, NC)))) void attend_kernel(AttendArgs a) {
+  constexpr int COLS = 16 * NC;
+  extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
@@ -287,73 +555,37 @@ __global__ __launch_bounds__(64 * W) void attend_kernel(AttendArgs a) {
   seq.rows = __builtin_amdgcn_readfirstlane(seq.rows);
   seq.context = __builtin_amdgcn_readfirstlane(seq.context);
   const int columns = seq.rows * a.group;
-  const int dim = a.cache.dim;
 
   using Wave = AttendWave<DT, E8, C, NC>;
   Wave w;
   w.ref = 0.0f;
   w.page_first = -64;
-  int row[NC], place[NC], window_lo[NC], head_of[NC];
-  bool real[NC];
-  constexpr int kFar = 1 << 30;
+  AttendColumns<NC> cols;
+  cols.set(a, seq, it, it.tile * COLS, columns, col);
+  cols.template queries<DT, C>(a, seq, g, w.q);
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
-    const int x = it.tile * COLS + 16 * n + col;
-    real[n] = x < columns;
-    row[n] = min(x, columns - 1) / a.group;
-    head_of[n] = it.head * a.group + min(x, columns - 1) % a.group;
-    const int64_t at = seq.start + row[n];
-    const int64_t p = a.positions != nullptr ? a.positions[at] : seq.context + row[n];
-    place[n] = static_cast<int>(min(max(p, static_cast<int64_t>(-kFar)), static_cast<int64_t>(kFar)));
-    window_lo[n] = a.window > 0 ? max(place[n] - a.window + 1, 0) : 0;
-    const uint16_t* from = a.q + at * a.q_row + head_of[n] * a.q_head;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int e = 64 * c + 16 * g + 8 * h;
-        w.q[n][c][h] = real[n] && e < dim ? *reinterpret_cast<const u32x4*>(from + e) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) w.o[n][c][2 * h + j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      }
+      for (int j = 0; j < 4; ++j) w.o[n][c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     w.m[n] = kMinusInf;
     w.l[n] = 0.0f;
   }
-
-  // The tile's tokens: [0, 32 sink_steps) and [32 first, end).
+  AttendWalk<kStep> walk;
+  int lo_least;
+  window_bounds(a, cols, lo_least, walk.lo_most);
+  walk.set(a, seq, it, COLS, columns, cols, lo_least);
   const int end = seq.context + seq.rows;
-  const int row_lo = it.tile * COLS / a.group, row_hi = min((it.tile + 1) * COLS, columns) - 1;
-  const int tile_end = a.mask != nullptr ? end : seq.context + row_hi / a.group + 1;
-  const int whole = a.mask != nullptr ? seq.context : seq.context + row_lo + 1;  // seen by every column, window apart
-  int lo_least = 0, lo_most = 0;
-  if (a.window > 0) {
-    lo_least = kFar;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      lo_least = min(lo_least, window_lo[n]);
-      lo_most = max(lo_most, window_lo[n]);
-    }
-#pragma unroll
-    for (int x = 8; x > 0; x >>= 1) {
-      lo_least = min(lo_least, __shfl_xor(lo_least, x));
-      lo_most = max(lo_most, __shfl_xor(lo_most, x));
-    }
-    // Under a mask the window holds for the context alone: the rows' own tokens are always walked.
-    if (a.mask != nullptr) lo_least = min(lo_least, seq.context);
-    lo_least = __builtin_amdgcn_readfirstlane(lo_least);
-    lo_most = __builtin_amdgcn_readfirstlane(lo_most);
-  }
-  const int last_step = (tile_end + kStep - 1) / kStep;
-  const int first = min(lo_least / kStep, last_step);
-  const int sink_steps = min((a.sinks + kStep - 1) / kStep, first);
-  const int steps = sink_steps + last_step - first;
-  const int from = static_cast<int>(static_cast<int64_t>(steps) * it.range / it.ranges);
-  const int to = static_cast<int>(static_cast<int64_t>(steps) * (it.range + 1) / it.ranges);
   const int last_page = (end + a.cache.page - 1) >> a.cache.page_shift;
-  auto token_of = [&](int s) { return kStep * (s < sink_steps ? s : first + s - sink_steps); };
 
-  auto compute = [&](const typename Wave::Step& s, int t0) {
-    const bool edge = t0 + kStep > whole || (a.window > 0 && t0 < lo_most && t0 + kStep > a.sinks) || !s.held[0] || !s.held[1];
+  // One step. Keys and values have one set of registers each, refilled for the wavefront's next step as soon as the
+  // product that reads them is issued, so about a step's bytes are in flight throughout.
+  typename Wave::Place s;
+  auto step = [&](int number) {
+    const int t0 = walk.token_of(number);
+    const bool more = number + W < walk.to;
+    const bool edge = walk.edge(t0) || !s.held[0] || !s.held[1];
     // S^T of both units, all columns.
     f32x4 score[NC][2];
 #pragma unroll
@@ -364,12 +596,12 @@ __global__ __launch_bounds__(64 * W) void attend_kernel(AttendArgs a) {
       for (int c = 0; c < C; ++c) {
         u32x4 k0, k1;
         if constexpr (E8) {
-          const u32x4 x = s.k[u][c][0];
+          const u32x4 x = w.k[u][c][0];
           k0 = fp8_eight<DT>(x[0], x[1], 1.0f);
           k1 = fp8_eight<DT>(x[2], x[3], 1.0f);
         } else {
-          k0 = s.k[u][c][0];
-          k1 = s.k[u][c][1];
+          k0 = w.k[u][c][0];
+          k1 = w.k[u][c][1];
         }
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
@@ -378,43 +610,57 @@ __global__ __launch_bounds__(64 * W) void attend_kernel(AttendArgs a) {
         }
       }
     }
+    typename Wave::Place next = s;
+    if (more) {
+      next = w.place(a, it.b, it.head, walk.token_of(number + W), last_page, lane);
+      w.keys(a, next, lane);
+    }
+    uint32_t seen[NC];
+    bool odd = false;  // a value that is not finite, where some columns may not look: 0 * it would reach them
+    if (edge) {
+      const uint32_t held = static_cast<uint32_t>(s.held[0]) | static_cast<uint32_t>(s.held[1]) << 1;
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        seen[n] = cols.template seen_bits<2>(a, seq, n, t0, g, held);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) score[n][u][r] = (seen[n] >> (4 * u + r)) & 1u ? score[n][u][r] : kMinusInf;
+      }
+      // Tokens that are no one's, past the end or of a page that is not there, have values of zero.
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int live = s.held[u] ? min(max(end - (t0 + 16 * u + 4 * g), 0), 4) : 0;  // of the lane's four tokens
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int h = 0; h < Wave::kLoads; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (E8) {
+                w.v[u][c][h][i] &= live == 4 ? ~0u : (1u << (8 * live)) - 1u;
+                odd = odd || fp8_not_finite(w.v[u][c][h][i]);
+              } else {
+                const int two = min(max(live - 2 * (i & 1), 0), 2);
+                w.v[u][c][h][i] &= two == 2 ? ~0u : (1u << (16 * two)) - 1u;
+                odd = odd || pair_not_finite<DT>(w.v[u][c][h][i]);
+              }
+            }
+      }
+    }
     u32x4 p[NC];
-    uint32_t seen_bits[NC];  // bit 4 u + r: token t0 + 16 u + 4 g + r is seen by the lane's column
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) score[n][u] *= E8 ? a.scale * s.ks[u] : a.scale;
-      if (edge) {
-        seen_bits[n] = 0;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int t = t0 + 16 * u + 4 * g + r;
-            const bool near = t >= window_lo[n] || t < a.sinks;
-            bool seen;
-            if (a.mask == nullptr) {
-              seen = near && t <= seq.context + row[n];
-            } else if (t < seq.context) {
-              seen = near;
-            } else {
-              const int i = t - seq.context;
-              seen = i < seq.rows && (i >> 5) < a.mask_words && row[n] < a.mask_rows &&
-                     ((a.mask[static_cast<int64_t>(row[n]) * a.mask_words + (i >> 5)] >> (i & 31)) & 1u) != 0;
-            }
-            seen = seen && t < end && s.held[u];
-            seen_bits[n] |= static_cast<uint32_t>(seen) << (4 * u + r);
-            score[n][u][r] = seen ? score[n][u][r] : kMinusInf;
-          }
-      }
       float top = kMinusInf;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) top = fmaxf(top, score[n][u][r]);
+        for (int r = 0; r < 4; ++r) top = larger_of(top, score[n][u][r]);
       top = column_max(top);
       if (__any(top > w.m[n] + kSlack)) {
-        const float next = fmaxf(w.m[n], top);
+        const float next = larger_of(w.m[n], top);
         const float less = w.m[n] == next ? 1.0f : __builtin_amdgcn_exp2f(w.m[n] - next);
         w.m[n] = next;
         w.l[n] *= less;
@@ -437,35 +683,25 @@ __global__ __launch_bounds__(64 * W) void attend_kernel(AttendArgs a) {
     // O^T += V^T P^T: operand j of a chunk has dimensions 4 (l % 16) + j as rows.
     const float less = w.ref > 0.0f ? 1.0f / w.ref : 0.0f;
     float ratio[2] = {1.0f, 1.0f};
-    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};  // per pair of tokens: 16-bit masks of those that any column may see
     if constexpr (E8) {
       ratio[0] = s.vs[0] * less;
       ratio[1] = s.vs[1] * less;
-    }
-    if (edge) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int t = t0 + 16 * u + 4 * g + 2 * r;
-          keep[2 * u + r] = (s.held[u] && t < end ? 0xffffu : 0u) | (s.held[u] && t + 1 < end ? 0xffff0000u : 0u);
-        }
     }
     auto values_of = [&](int c, int j) {
       u32x4 v;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if constexpr (E8) {
-          v[2 * u] = fp8_pair<DT>(s.v[u][c][0][j], ratio[u], false);
-          v[2 * u + 1] = fp8_pair<DT>(s.v[u][c][0][j], ratio[u], true);
+          v[2 * u] = fp8_pair<DT>(w.v[u][c][0][j], ratio[u], false);
+          v[2 * u + 1] = fp8_pair<DT>(w.v[u][c][0][j], ratio[u], true);
         } else {
-          v[2 * u] = s.v[u][c][j / 2][2 * (j & 1)];
-          v[2 * u + 1] = s.v[u][c][j / 2][2 * (j & 1) + 1];
+          v[2 * u] = w.v[u][c][j / 2][2 * (j & 1)];
+          v[2 * u + 1] = w.v[u][c][j / 2][2 * (j & 1) + 1];
         }
       }
       return v;
     };
-    if (!edge) {
+    if (!__any(odd)) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -474,56 +710,32 @@ __global__ __launch_bounds__(64 * W) void attend_kernel(AttendArgs a) {
 #pragma unroll
           for (int n = 0; n < NC; ++n) w.o[n][c][j] = mfma_16x16x32<DT>(v, p[n], w.o[n][c][j]);
         }
-      return;
-    }
-    // A value that is not finite where some columns do not look: 0 * it would reach them. Where an
-    // operand has one, its tokens go one at a time, and only the columns that see a token take its result.
+    } else {
+      // One token at a time, and only the columns that see it take the result.
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u32x4 v = values_of(c, j);
-        bool odd = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] &= keep[i];
-          odd = odd || pair_not_finite<DT>(v[i]);
-        }
-        if (!__any(odd)) {
-#pragma unroll
-          for (int n = 0; n < NC; ++n) w.o[n][c][j] = mfma_16x16x32<DT>(v, p[n], w.o[n][c][j]);
-          continue;
-        }
+        for (int j = 0; j < 4; ++j) {
+          // Opaque to the compiler, which would otherwise form the operands of both branches ahead of them, all at once.
+          asm volatile("" : "+v"(w.v[0][c][E8 ? 0 : j / 2]), "+v"(w.v[1][c][E8 ? 0 : j / 2]));
+          const u32x4 v = values_of(c, j);
 #pragma unroll 1
-        for (int x = 0; x < kStep; ++x) {
-          const int slot = ((x >> 4) << 2) | (x & 3);  // the token's place among a lane's eight
-          const int holder = (x & 15) >> 2;            // the lanes that hold it
-          const uint32_t half = holder == g ? 0xffffu << (16 * (slot & 1)) : 0u;
-          u32x4 only;
+          for (int x = 0; x < kStep; ++x) {
+            const TokenOf t(x, g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) only[i] = (slot >> 1) == i ? half : 0u;
-#pragma unroll
-          for (int n = 0; n < NC; ++n) {
-            const bool sees = ((__shfl(static_cast<int>(seen_bits[n]), holder * 16 + col) >> slot) & 1) != 0;
-            const f32x4 sum = mfma_16x16x32<DT>(v & only, p[n] & only, w.o[n][c][j]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) w.o[n][c][j][r] = sees ? sum[r] : w.o[n][c][j][r];
+            for (int n = 0; n < NC; ++n) take_token<DT>(v & t.only, p[n] & t.only, t.seen(seen[n], 0, col), w.o[n][c][j]);
           }
         }
-      }
+    }
+    s = next;
+    if (more) w.values(a, s, lane);
   };
 
-  {
-    typename Wave::Step next;
-    int s = from + wave;
-    if (s < to) w.fetch(a, it.b, it.head, token_of(s), last_page, lane, next);
-    while (s < to) {
-      const typename Wave::Step now = next;
-      const int t0 = token_of(s);
-      s += W;
-      if (s < to) w.fetch(a, it.b, it.head, token_of(s), last_page, lane, next);
-      compute(now, t0);
-    }
+  if (walk.from + wave < walk.to) {
+    s = w.place(a, it.b, it.head, walk.token_of(walk.from + wave), last_page, lane);
+    w.keys(a, s, lane);
+    w.values(a, s, lane);
+    for (int number = walk.from + wave; number < walk.to; number += W) step(number);
   }
 
   // Every wavefront's result in plain units, then joined by halves through LDS.
@@ -578,141 +790,19 @@ __global__ __launch_bounds__(64 * W) void attend_kernel(AttendArgs a) {
   }
 
   if (it.ranges == 1) {
-    if (wave != 0) return;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      if (!real[n]) continue;
-      const float inverse = w.l[n] == 0.0f ? 0.0f : 1.0f / w.l[n];  // a row that sees nothing is zero
-      uint16_t* at = a.out + (static_cast<int64_t>(seq.start + row[n]) * a.heads + head_of[n]) * dim;
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int e = 64 * c + 16 * g;
-        u32x4 word[2];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // dimensions e + 2 i, e + 2 i + 1
-          const int r = i / 2, j = 2 * (i & 1);
-          word[i / 4][i % 4] = pack2<DT>(w.o[n][c][j][r] * inverse, w.o[n][c][j + 1][r] * inverse);
-        }
-        if (e < dim) *reinterpret_cast<u32x4*>(at + e) = word[0];
-        if (e + 8 < dim) *reinterpret_cast<u32x4*>(at + e + 8) = word[1];
-      }
-    }
+    if (wave == 0) cols.template store<DT, C>(a, seq, g, w.o, w.l);
     return;
   }
-
-  // A range of several: the partial result goes to the group's slot `range`; the group's last workgroup
-  // joins them. Slot: [COLS][PAD] sums, then [COLS] maxima and [COLS] sums of exponentials.
-  constexpr uint32_t kSlotBytes = static_cast<uint32_t>(attend_slot_floats(COLS, PAD) * 4);
-  const int heads = a.cache.heads;
-  if (wave == 0) {
-    char* mine = reinterpret_cast<char*>(a.partials) + static_cast<int64_t>(it.slot + it.range * heads) * kSlotBytes;
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(mine, kSlotBytes);
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      if (!real[n]) continue;
-      const int at = 16 * n + col;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const f32x4 x = {w.o[n][c][0][r], w.o[n][c][1][r], w.o[n][c][2][r], w.o[n][c][3][r]};
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rs,
-                                                 (at * PAD + 64 * c + 16 * g + 4 * r) * 4, 0, kCoherent);
-        }
-      if (g == 0) {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, w.m[n]), rs, (COLS * PAD + at) * 4, 0, kCoherent);
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, w.l[n]), rs, (COLS * PAD + COLS + at) * 4, 0, kCoherent);
-      }
-    }
-  }
-  if (!arrive_last(a.counters + it.group, it.ranges)) return;
-  // Weights of the ranges per column in LDS, then every thread joins four dimensions of a column.
-  const int live = min(COLS, columns - it.tile * COLS);
-  float* weight = shared;                     // [ranges][COLS]
-  float* total = weight + a.most * COLS;      // [COLS]
-  auto slot_of = [&](int range) {
-    return reinterpret_cast<const char*>(a.partials) + static_cast<int64_t>(it.slot + range * heads) * kSlotBytes;
-  };
-  for (int i = threadIdx.x; i < it.ranges * COLS; i += 64 * W) {
-    const int range = i / COLS, c = i % COLS;
-    weight[i] = c < live ? collect(reinterpret_cast<const float*>(slot_of(range)) + COLS * PAD + c) : kMinusInf;
-  }
-  __syncthreads();
-  if (static_cast<int>(threadIdx.x) < live) {
-    float top = kMinusInf, sum = 0.0f;
-    for (int range = 0; range < it.ranges; ++range) top = fmaxf(top, weight[range * COLS + threadIdx.x]);
-    for (int range = 0; range < it.ranges; ++range) {
-      const float m = weight[range * COLS + threadIdx.x];
-      const float x = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-      weight[range * COLS + threadIdx.x] = x;
-      sum += x * collect(reinterpret_cast<const float*>(slot_of(range)) + COLS * PAD + COLS + threadIdx.x);
-    }
-    total[threadIdx.x] = sum == 0.0f ? 0.0f : 1.0f / sum;
-  }
-  __syncthreads();
-  const int quads = dim >> 2;
-  for (int i = threadIdx.x; i < live * quads; i += 64 * W) {
-    const int c = i / quads, e = (i - c * quads) << 2;
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int range = 0; range < it.ranges; ++range) {
-      const __amdgpu_buffer_rsrc_t rs = make_rsrc(slot_of(range), kSlotBytes);
-      const f32x4 x = __builtin_bit_cast(
-          f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (c * PAD + e) * 4, 0, kCoherent));
-      sum += x * weight[range * COLS + c];
-    }
-    sum *= total[c];
-    const int x = it.tile * COLS + c;
-    uint16_t* at = a.out + (static_cast<int64_t>(seq.start + x / a.group) * a.heads + it.head * a.group + x % a.group) * dim;
-    *reinterpret_cast<u32x2*>(at + e) = u32x2{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
-  }
+  // One range of several: the partial result goes to the group's slot; the group's last workgroup joins them.
+  if (wave == 0) attend_publish<NC, C>(a, it, COLS, 0, g, col, cols, w.o, w.m, w.l);
+  if (arrive_last(a.counters + it.group, it.ranges)) attend_join<DT, C>(a, seq, it, COLS, columns, shared);
 }
 
-// Columns of a tile and wavefronts of a workgroup for heads of C chunks, by the columns that the longest
-// sequence may have per key head.
-inline int attend_column_tiles(int chunks, int64_t columns) {
-  if (columns <= 16) return 1;
-  if (columns <= 32 || chunks > 2) return 2;
-  return 4;
-}
-
-hipError_t attend_bf16_e4m3(const AttendArgs& a, int tiles, unsigned grid, hipStream_t s);
-hipError_t attend_bf16_model(const AttendArgs& a, int tiles, unsigned grid, hipStream_t s);
-hipError_t attend_f16_e4m3(const AttendArgs& a, int tiles, unsigned grid, hipStream_t s);
-hipError_t attend_f16_model(const AttendArgs& a, int tiles, unsigned grid, hipStream_t s);
+hipError_t attend_bf16_e4m3(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);
+hipError_t attend_bf16_model(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);
+hipError_t attend_f16_e4m3(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);
+hipError_t attend_f16_model(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);
 
 constexpr int kAttendMost = 64;  // ranges per group, at most
-
-template <int DT, bool E8, int C, int NC>
-hipError_t attend_launch(const AttendArgs& a, unsigned grid, hipStream_t s) {
-  constexpr int W = NC == 1 ? 8 : 4;
-  constexpr size_t join = static_cast<size_t>(W / 2) * NC * (C * 16 + 2) * 64 * 4;
-  constexpr size_t weights = static_cast<size_t>(kAttendMost + 1) * 16 * NC * 4;
-  constexpr size_t bytes = join > weights ? join : weights;
-  auto* kern = &attend_kernel<DT, E8, C, NC, W>;
-  if (bytes > 64 * 1024) {
-    static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                                         hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-    if (raised != hipSuccess) return raised;
-  }
-  kern<<<grid, 64 * W, bytes, s>>>(a);
-  return hipGetLastError();
-}
-
-template <int DT, bool E8>
-hipError_t attend_pick(const AttendArgs& a, int tiles, unsigned grid, hipStream_t s) {
-  switch (a.cache.chunks * 8 + tiles) {
-    case 8 + 1: return attend_launch<DT, E8, 1, 1>(a, grid, s);
-    case 8 + 2: return attend_launch<DT, E8, 1, 2>(a, grid, s);
-    case 8 + 4: return attend_launch<DT, E8, 1, 4>(a, grid, s);
-    case 16 + 1: return attend_launch<DT, E8, 2, 1>(a, grid, s);
-    case 16 + 2: return attend_launch<DT, E8, 2, 2>(a, grid, s);
-    case 16 + 4: return attend_launch<DT, E8, 2, 4>(a, grid, s);
-    case 24 + 1: return attend_launch<DT, E8, 3, 1>(a, grid, s);
-    case 24 + 2: return attend_launch<DT, E8, 3, 2>(a, grid, s);
-    case 32 + 1: return attend_launch<DT, E8, 4, 1>(a, grid, s);
-    case 32 + 2: return attend_launch<DT, E8, 4, 2>(a, grid, s);
-  }
-  return hipErrorInvalidValue;
-}
 
 }  // namespace plm

@@ -10,8 +10,8 @@ namespace plm {
 namespace {
 
 struct AttendPlan {
-  int tiles;         // column tiles of 16 per workgroup
-  int target, least; // AttendArgs
+  int columns;        // of a workgroup's tile
+  int target, least;  // AttendArgs
   int64_t grid, bytes;
 };
 
@@ -22,9 +22,9 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
                        int64_t max_rows, int64_t table_width) {
   AttendPlan p{};
   const int64_t group = heads / kv_heads, chunks = (head_dim + 63) / 64;
-  p.tiles = attend_column_tiles(static_cast<int>(chunks), max_rows * group);
-  const int64_t columns = 16 * p.tiles;
-  const int64_t groups = kv_heads * (seqs + total * group / columns);
+  const int64_t most = max_rows * group;
+  p.columns = most <= 16 ? 16 : most <= 32 ? 32 : most <= 256 ? 64 : 128;
+  const int64_t groups = kv_heads * (seqs + total * group / p.columns);
   const int64_t capacity = (table_width * page + kStep - 1) / kStep;
   p.least = 8;
   p.target = capacity > p.least ? 512 : 0;
@@ -33,7 +33,7 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   // a cut sequence has less than twice load / chunk of them, and a chunk is load / target at least.
   if (p.target > 0)
     p.bytes = PLM_ATTEND_COUNTER_BYTES +
-              2 * p.target * attend_slot_floats(static_cast<int>(columns), static_cast<int>(64 * chunks)) * 4;
+              2 * p.target * attend_slot_floats(p.columns, static_cast<int>(64 * chunks)) * 4;
   return p;
 }
 
@@ -103,8 +103,8 @@ int plm_attend(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t 
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool e8 = cache->type == PLM_CACHE_E4M3;
   hipError_t err;
-  if (dtype == PLM_BF16) err = e8 ? plm::attend_bf16_e4m3(a, p.tiles, grid, s) : plm::attend_bf16_model(a, p.tiles, grid, s);
-  else err = e8 ? plm::attend_f16_e4m3(a, p.tiles, grid, s) : plm::attend_f16_model(a, p.tiles, grid, s);
+  if (dtype == PLM_BF16) err = e8 ? plm::attend_bf16_e4m3(a, p.columns, grid, s) : plm::attend_bf16_model(a, p.columns, grid, s);
+  else err = e8 ? plm::attend_f16_e4m3(a, p.columns, grid, s) : plm::attend_f16_model(a, p.columns, grid, s);
   return err == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 

@@ -1,11 +1,11 @@
 // Attention over e4m3 pages, bf16 rows: the kernels of attend.h, a translation unit of its own so that
 // the build compiles them in parallel.
-#include "attend.h"
+#include "attend_pick.h"
 
 namespace plm {
 
-hipError_t attend_bf16_e4m3(const AttendArgs& a, int tiles, unsigned grid, hipStream_t s) {
-  return attend_pick<DT_BF16, true>(a, tiles, grid, s);
+hipError_t attend_bf16_e4m3(const AttendArgs& a, int columns, unsigned grid, hipStream_t s) {
+  return attend_pick<DT_BF16, true>(a, columns, grid, s);
 }
 
 }  // namespace plm

@@ -1,0 +1,58 @@
+// Which kernel a launch of plm_attend takes (a translation unit per type of rows and cache includes it).
+#pragma once
+
+#include "attend.h"
+#include "attend_tile.h"
+
+namespace plm {
+
+template <typename Kernel>
+hipError_t attend_go(Kernel kern, const AttendArgs& a, unsigned grid, unsigned threads, size_t bytes, hipStream_t s) {
+  if (bytes > 64 * 1024) {
+    const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                                  hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (raised != hipSuccess) return raised;
+  }
+  kern<<<grid, threads, bytes, s>>>(a);
+  return hipGetLastError();
+}
+
+constexpr size_t attend_join_bytes(int columns) { return static_cast<size_t>(kAttendMost + 1) * columns * 4; }
+constexpr size_t larger(size_t a, size_t b) { return a > b ? a : b; }
+
+template <int DT, bool E8, int C, int NC>
+hipError_t attend_stream(const AttendArgs& a, unsigned grid, hipStream_t s) {
+  constexpr int W = 4;
+  constexpr size_t waves = static_cast<size_t>(W / 2) * NC * (C * 16 + 2) * 64 * 4;
+  return attend_go(&attend_kernel<DT, E8, C, NC, W>, a, grid, 64 * W, larger(waves, attend_join_bytes(16 * NC)), s);
+}
+
+template <int DT, bool E8, int C, int NC>
+hipError_t attend_tiled(const AttendArgs& a, unsigned grid, hipStream_t s) {
+  constexpr size_t sets = static_cast<size_t>(2) * attend_set_bytes(C);
+  return attend_go(&attend_tile_kernel<DT, E8, C, NC>, a, grid, 256, larger(sets, attend_join_bytes(64 * NC)), s);
+}
+
+template <int DT, bool E8, int C>
+hipError_t attend_columns(const AttendArgs& a, int columns, unsigned grid, hipStream_t s) {
+  switch (columns) {
+    case 16: return attend_stream<DT, E8, C, 1>(a, grid, s);
+    case 32: return attend_stream<DT, E8, C, 2>(a, grid, s);
+    case 64: return attend_tiled<DT, E8, C, 1>(a, grid, s);
+    case 128: return attend_tiled<DT, E8, C, 2>(a, grid, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+template <int DT, bool E8>
+hipError_t attend_pick(const AttendArgs& a, int columns, unsigned grid, hipStream_t s) {
+  switch (a.cache.chunks) {
+    case 1: return attend_columns<DT, E8, 1>(a, columns, grid, s);
+    case 2: return attend_columns<DT, E8, 2>(a, columns, grid, s);
+    case 3: return attend_columns<DT, E8, 3>(a, columns, grid, s);
+    case 4: return attend_columns<DT, E8, 4>(a, columns, grid, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace plm
