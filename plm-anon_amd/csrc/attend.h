@@ -15,6 +15,8 @@
 // are joined by the last of their workgroups to finish, through partial results in device memory.
 #pragma once
 
+#include <type_traits>
+
 #include "kv_cache.h"
 
 namespace plm {
@@ -481,6 +483,20 @@ struct AttendWave {
   int page_id, page_first;  // lane i: page number page_first + i of the sequence
   float page_ks, page_vs;
 
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      m[n] = kMinusInf;
+      l[n] = 0.0f;
+    }
+    ref = 0.0f;
+    page_first = -64;
+  }
+
   __device__ __forceinline__ void pages(const AttendArgs& a, int b, int head, int number, int last, int lane) {
     page_first = number;
     const int at = number + lane;
@@ -538,11 +554,16 @@ struct AttendWave {
   }
 };
 
-// Wavefronts per SIMD to leave registers for.
-constexpr int attend_waves(int chunks, int nc) { return chunks * nc == 1 ? 4 : chunks * nc == 2 ? 3 : chunks * nc <= 4 ? 2 : 1; }
+// Wavefronts per SIMD to leave registers for: as many as hold the accumulators, the queries and a step's keys and
+// values without spilling (512 registers over them).
+constexpr int attend_waves(bool e8, int chunks, int nc) {
+  if (chunks == 1) return nc == 1 ? 4 : 3;
+  if (chunks == 2) return e8 && nc == 1 ? 3 : 2;
+  return e8 || chunks == 3 ? 2 : 1;
+}
 
 template <int DT, bool E8, int C, int NC, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_waves(C, NC)))) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_waves(E8, C, NC)))) void attend_kernel(AttendArgs a) {
   constexpr int COLS = 16 * NC;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63;
@@ -558,20 +579,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
 
   using Wave = AttendWave<DT, E8, C, NC>;
   Wave w;
-  w.ref = 0.0f;
-  w.page_first = -64;
   AttendColumns<NC> cols;
   cols.set(a, seq, it, it.tile * COLS, columns, col);
   cols.template queries<DT, C>(a, seq, g, w.q);
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w.o[n][c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    w.m[n] = kMinusInf;
-    w.l[n] = 0.0f;
-  }
   AttendWalk<kStep> walk;
   int lo_least;
   window_bounds(a, cols, lo_least, walk.lo_most);
@@ -581,10 +591,15 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
 
   // One step. Keys and values have one set of registers each, refilled for the wavefront's next step as soon as the
   // product that reads them is issued, so about a step's bytes are in flight throughout.
+  // CAREFUL: a value that is not finite was met in a step that some columns do not see whole, where 0 * it would reach
+  // them. The walk is then done again with one token at a time in such steps: apart from the usual one, whose registers
+  // it would take.
   typename Wave::Place s;
-  auto step = [&](int number) {
+  bool odd = false;
+  auto step = [&](auto careful, int number) {
+    constexpr bool CAREFUL = decltype(careful)::value;
     const int t0 = walk.token_of(number);
-    const bool more = number + W < walk.to;
+    const bool more = !CAREFUL && number + W < walk.to;
     const bool edge = walk.edge(t0) || !s.held[0] || !s.held[1];
     // S^T of both units, all columns.
     f32x4 score[NC][2];
@@ -616,7 +631,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
       w.keys(a, next, lane);
     }
     uint32_t seen[NC];
-    bool odd = false;  // a value that is not finite, where some columns may not look: 0 * it would reach them
     if (edge) {
       const uint32_t held = static_cast<uint32_t>(s.held[0]) | static_cast<uint32_t>(s.held[1]) << 1;
 #pragma unroll
@@ -701,7 +715,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
       }
       return v;
     };
-    if (!__any(odd)) {
+    if (!CAREFUL || !edge) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -711,13 +725,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
           for (int n = 0; n < NC; ++n) w.o[n][c][j] = mfma_16x16x32<DT>(v, p[n], w.o[n][c][j]);
         }
     } else {
-      // One token at a time, and only the columns that see it take the result.
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          // Opaque to the compiler, which would otherwise form the operands of both branches ahead of them, all at once.
-          asm volatile("" : "+v"(w.v[0][c][E8 ? 0 : j / 2]), "+v"(w.v[1][c][E8 ? 0 : j / 2]));
           const u32x4 v = values_of(c, j);
 #pragma unroll 1
           for (int x = 0; x < kStep; ++x) {
@@ -731,11 +742,22 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
     if (more) w.values(a, s, lane);
   };
 
+  w.begin();
   if (walk.from + wave < walk.to) {
     s = w.place(a, it.b, it.head, walk.token_of(walk.from + wave), last_page, lane);
     w.keys(a, s, lane);
     w.values(a, s, lane);
-    for (int number = walk.from + wave; number < walk.to; number += W) step(number);
+    for (int number = walk.from + wave; number < walk.to; number += W) step(std::false_type{}, number);
+    if (__any(odd)) {
+      w.begin();
+#pragma unroll 1
+      for (int number = walk.from + wave; number < walk.to; number += W) {
+        s = w.place(a, it.b, it.head, walk.token_of(number), last_page, lane);
+        w.keys(a, s, lane);
+        w.values(a, s, lane);
+        step(std::true_type{}, number);
+      }
+    }
   }
 
   // Every wavefront's result in plain units, then joined by halves through LDS.

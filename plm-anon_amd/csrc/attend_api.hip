@@ -23,7 +23,7 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   AttendPlan p{};
   const int64_t group = heads / kv_heads, chunks = (head_dim + 63) / 64;
   const int64_t most = max_rows * group;
-  p.columns = most <= 16 ? 16 : most <= 32 ? 32 : most <= 256 ? 64 : 128;
+  p.columns = most <= 16 ? 16 : chunks > 2 ? 64 : most <= 32 ? 32 : most <= 256 ? 64 : 128;
   const int64_t groups = kv_heads * (seqs + total * group / p.columns);
   const int64_t capacity = (table_width * page + kStep - 1) / kStep;
   p.least = 8;

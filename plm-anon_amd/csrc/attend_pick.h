@@ -35,11 +35,11 @@ hipError_t attend_tiled(const AttendArgs& a, unsigned grid, hipStream_t s) {
 
 template <int DT, bool E8, int C>
 hipError_t attend_columns(const AttendArgs& a, int columns, unsigned grid, hipStream_t s) {
-  switch (columns) {
-    case 16: return attend_stream<DT, E8, C, 1>(a, grid, s);
-    case 32: return attend_stream<DT, E8, C, 2>(a, grid, s);
-    case 64: return attend_tiled<DT, E8, C, 1>(a, grid, s);
-    case 128: return attend_tiled<DT, E8, C, 2>(a, grid, s);
+  if (columns == 16) return attend_stream<DT, E8, C, 1>(a, grid, s);
+  if (columns == 64) return attend_tiled<DT, E8, C, 1>(a, grid, s);
+  if constexpr (C <= 2) {  // of longer heads so many columns' sums do not fit the registers
+    if (columns == 32) return attend_stream<DT, E8, C, 2>(a, grid, s);
+    if (columns == 128) return attend_tiled<DT, E8, C, 2>(a, grid, s);
   }
   return hipErrorInvalidValue;
 }

@@ -14,17 +14,13 @@
 namespace plm {
 
 constexpr int kTile = 64;  // tokens staged at once
-constexpr int attend_set_bytes(int chunks) { return 16 * chunks * 1024 + 16; }
-
-// Wavefronts per SIMD to leave registers for.
-constexpr int attend_tile_waves(int chunks, int nc) { return chunks * nc <= 4 ? 2 : 1; }
+constexpr int attend_set_bytes(int chunks) { return 16 * chunks * 1024; }
 
 template <int DT, bool E8, int C, int NC>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attend_tile_waves(C, NC)))) void attend_tile_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attend_tile_kernel(AttendArgs a) {
   constexpr int COLS = 64 * NC;
   constexpr int kUnitBytes = E8 ? 1024 : 2048, kLoads = E8 ? 1 : 2;
-  // Bytes of a set: keys, values, and a flag per wavefront: it staged a value that is not finite.
-  constexpr int kKeys = 8 * C * 1024, kSet = attend_set_bytes(C);
+  constexpr int kKeys = 8 * C * 1024, kSet = attend_set_bytes(C);  // bytes of a set: keys, then values
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -46,15 +42,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attend_tile
   cols.template queries<DT, C>(a, seq, g, q);
   f32x4 o[NC][C][4];
   float m[NC], l[NC];
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[n][c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    m[n] = kMinusInf;
-    l[n] = 0.0f;
-  }
   // The walk is the workgroup's: bounds over all four wavefronts' windows.
   AttendWalk<kTile> walk;
   int lo_least, lo_most;
@@ -135,11 +122,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attend_tile
       }
     }
   };
+  bool odd = false;  // staged a value that is not finite for columns that may not all look (see attend_kernel)
   auto store = [&](int t0, char* set) {
     const bool edge = walk.edge(t0) || unit_held != 15u;
     const bool cut = t0 + kTile > end || unit_held != 15u;  // tokens that are no one's: values there are zero
     const float less = DT == DT_F16 ? (ref > 0.0f ? 1.0f / ref : 0.0f) : 1.0f;
-    bool odd = false;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const int job = wave + 4 * i;
@@ -188,16 +175,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attend_tile
         }
       }
     }
-    if (edge) {
-      odd = __any(odd);
-      if (lane == 0) reinterpret_cast<int*>(set + kSet - 16)[wave] = odd;
-    }
   };
 
-  auto compute = [&](const char* set, int t0, const float (&ks)[4], uint32_t held) {
+  auto compute = [&](auto careful, const char* set, int t0, const float (&ks)[4], uint32_t held) {
+    constexpr bool CAREFUL = decltype(careful)::value;
     const bool edge = walk.edge(t0) || held != 15u;
-    const int* flags = reinterpret_cast<const int*>(set + kSet - 16);
-    const bool odd = edge && (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
     const char* keys = set + lane * 16;
     const char* values = keys + kKeys;
     f32x4 s[NC][4];
@@ -262,7 +244,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attend_tile
       }
       l[n] += sum;
     }
-    if (!odd) {
+    if (!CAREFUL || !edge) {
 #pragma unroll
       for (int pair = 0; pair < 2; ++pair)
 #pragma unroll
@@ -275,7 +257,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attend_tile
           }
       return;
     }
-    // Values that are not finite, where some columns may not look: as in attend_kernel, a token at a time.
+    // One token at a time, as in attend_kernel.
 #pragma unroll
     for (int pair = 0; pair < 2; ++pair)
 #pragma unroll
@@ -293,10 +275,40 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attend_tile
         }
   };
 
+  // The accumulators follow `ref` when the set that was staged with the new one is up.
+  auto follow = [&]() {
+    if constexpr (E8 && DT == DT_F16) {
+      if (next_ref > ref) {
+        const float less = ref / next_ref;
+        ref = next_ref;
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][c][j] *= less;
+      }
+    }
+  };
+  auto begin = [&]() {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      m[n] = kMinusInf;
+      l[n] = 0.0f;
+    }
+    page_first = -64;
+    ref = next_ref = DT == DT_F16 ? 0.0f : 1.0f;
+  };
+
+  begin();
   if (walk.from < walk.to) {
     int t0 = walk.token_of(walk.from);
     fetch(t0);
-    ref = next_ref;
+    follow();
     store(t0, lds);
     __syncthreads();
     int set = 0;
@@ -309,24 +321,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attend_tile
         t0 = walk.token_of(s + 1);
         fetch(t0);
       }
-      compute(lds + set * kSet, now, ks, held);
+      compute(std::false_type{}, lds + set * kSet, now, ks, held);
       set ^= 1;
       if (more) {
-        if constexpr (E8 && DT == DT_F16) {
-          if (next_ref > ref) {
-            const float less = ref / next_ref;
-            ref = next_ref;
-#pragma unroll
-            for (int n = 0; n < NC; ++n)
-#pragma unroll
-              for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[n][c][j] *= less;
-          }
-        }
+        follow();
         store(t0, lds + set * kSet);
       }
       __syncthreads();
+    }
+    if (__syncthreads_or(odd)) {
+      begin();
+#pragma unroll 1
+      for (int s = walk.from; s < walk.to; ++s) {
+        t0 = walk.token_of(s);
+        fetch(t0);
+        follow();
+        store(t0, lds);
+        __syncthreads();
+        compute(std::true_type{}, lds, t0, unit_ks, unit_held);
+        __syncthreads();
+      }
     }
   }
 
