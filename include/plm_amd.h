@@ -539,11 +539,9 @@ int plm_kv_read(int32_t dtype, const plm_kv_cache* cache, const int32_t* table, 
  * and with window > 0 of these only t > position - window or t < sinks, the position being positions[r]
  * (positions NULL: lengths[b] + i); under a mask the window holds for the context alone. A row that sees
  * nothing is zero. out: contiguous [total, heads, head_dim].
- * Workspace: plm_attend_workspace_bytes (0: none needed), 16-byte aligned, its counters (the first
- * PLM_ATTEND_COUNTER_BYTES) zero before the first call; each call leaves them zero. Calls that may run at
- * the same time need workspaces of their own.
+ * Workspace: plm_attend_workspace_bytes (0: none needed), 16-byte aligned, of any content; calls that may
+ * run at the same time need workspaces of their own.
  */
-#define PLM_ATTEND_COUNTER_BYTES 16384
 int plm_attend(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int32_t heads,
                void* out, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table, int64_t table_stride,
                int64_t table_width, const int64_t* lengths, const int64_t* row_starts, int64_t window, int64_t sinks,

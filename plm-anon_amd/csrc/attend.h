@@ -12,7 +12,7 @@
 //
 // A workgroup's W wavefronts take every W-th step of 32 tokens of one range of one (sequence, tile of
 // columns, key head), and are joined through LDS at the end. Ranges of the same (sequence, tile, head)
-// are joined by the last of their workgroups to finish, through partial results in device memory.
+// leave partial results in device memory, which a second launch joins (attend_join.hip).
 #pragma once
 
 #include <type_traits>
@@ -29,16 +29,17 @@ struct AttendArgs {
   int64_t q_row, q_head;
   const int64_t* positions;  // [total]; null: context + row
   const uint32_t* mask;      // [mask_rows, mask_words]; null: causal
-  int* counters;             // one per (sequence, tile, head) of several ranges, zero between calls
   float* partials;           // slots of attend_slot_floats(columns, padded dim)
   float scale;               // times log2 e
   int heads, group, window, sinks, mask_rows, mask_words;
   int target;   // workgroups that the work is split over, at most; 0: never split
+  float per_target;  // a little more than 1 / target
   int least;    // steps of a range, at least
-  int most;     // ranges per group, at most
 };
 
-constexpr int kStep = 32;  // tokens of a step
+constexpr int kStep = 32;        // tokens of a step
+constexpr int kAttendMost = 64;  // ranges per group, at most
+constexpr int kJoinColumns = 8;  // columns of a workgroup of the joining launch
 
 __host__ __device__ constexpr int64_t attend_slot_floats(int columns, int padded) {
   return static_cast<int64_t>(columns) * (padded + 2);
@@ -66,74 +67,88 @@ __device__ __forceinline__ AttendShare attend_share(const AttendArgs& a, int b) 
   return s;
 }
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
-  return v;
+// Inclusive sums over the wavefront's lanes, by DPP: shifts inside rows of 16, then the rows' last lanes handed on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
 }
-
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int below = __shfl_up(v, d);
-    if (lane >= d) v += below;
-  }
-  return v;
+__device__ __forceinline__ int wave_scan(int v) {
+  v = scan_step<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = scan_step<0x112, 0xf>(v);
+  v = scan_step<0x114, 0xf>(v);
+  v = scan_step<0x118, 0xf>(v);
+  v = scan_step<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
+  return scan_step<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float scan_step(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float wave_total(float v) {
+  v = scan_step<0x111, 0xf>(v);
+  v = scan_step<0x112, 0xf>(v);
+  v = scan_step<0x114, 0xf>(v);
+  v = scan_step<0x118, 0xf>(v);
+  v = scan_step<0x142, 0xa>(v);
+  v = scan_step<0x143, 0xc>(v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 struct AttendItem {
   int b, tile, head, range, ranges;  // ranges == 0: nothing to do
-  int group;                         // number of the (sequence, tile, head) among those of several ranges
-  int slot;                          // first of the group's partial slots, in steps of `heads`
+  int slot;                          // the group's first partial slot; its ranges' are `heads` slots apart
 };
 
-// Which range of which group workgroup `index` takes. The work of the whole call (steps x tiles x heads,
-// from the lengths on the device) is cut so that about `target` workgroups share it evenly, whatever the
-// sequences' lengths and the table's width: a launch sized on the host alone would have to cut the widest
-// sequence the table could hold. Every wavefront scans the sequences by itself, 64 at a time.
-template <int COLS>
+// Which range of which group (sequence, tile, key head) workgroup `index` takes; with JOIN, which group of several
+// ranges is number `index`. The work of the whole call (steps x tiles x heads, from the lengths on the device) is cut
+// so that about `target` workgroups share it evenly, whatever the sequences' lengths and the table's width: a launch
+// cut on the host alone would have to go by the longest sequence that the table could hold. Every wavefront scans the
+// sequences by itself, 64 at a time.
+template <int COLS, bool JOIN>
 __device__ __forceinline__ AttendItem attend_item(const AttendArgs& a, int index, int lane) {
   const int heads = a.cache.heads;
   AttendItem it{};
   int chunk = 1 << 30;
-  AttendShare own = attend_share<COLS>(a, lane);
+  const AttendShare own = attend_share<COLS>(a, lane);
   if (a.target > 0) {
-    int64_t load = 0;
+    // In fp32, rounded up by more than its sums can be off: a chunk is never less than load / target.
+    float load = 0.0f;
     for (int base = 0; base < a.rows.seqs; base += 64) {
       const AttendShare s = base == 0 ? own : attend_share<COLS>(a, base + lane);
-      load += static_cast<int64_t>(s.tiles) * s.steps;
+      load += static_cast<float>(s.tiles) * static_cast<float>(s.steps);
     }
-    load = wave_sum64(load) * heads;
-    chunk = static_cast<int>(min(max((load + a.target - 1) / a.target, static_cast<int64_t>(a.least)), int64_t{1} << 30));
+    const float cut = ceilf(wave_total(load) * static_cast<float>(heads) * a.per_target);
+    chunk = max(static_cast<int>(fminf(cut, static_cast<float>(1 << 30))), a.least);
   }
-  int items = 0, groups = 0, slots = 0;
+  int items = 0, slots = 0;
   for (int base = 0; base < a.rows.seqs; base += 64) {
     const AttendShare s = base == 0 ? own : attend_share<COLS>(a, base + lane);
-    const int ranges = min(max((s.steps + chunk - 1) / chunk, 1), a.most);
-    const int mine = s.tiles * ranges * heads;
-    const int to = wave_scan(mine, lane);
-    // Only groups of several ranges have a counter and slots.
-    const int split = ranges > 1 ? s.tiles * heads : 0;
-    const int group_to = a.target > 0 ? wave_scan(split, lane) : 0;
-    const int slot_to = a.target > 0 ? wave_scan(split * ranges, lane) : 0;
+    const int ranges = min(max((s.steps + chunk - 1) / chunk, 1), kAttendMost);
+    const int split = ranges > 1 ? s.tiles * heads : 0;  // groups of several ranges: they alone have slots
+    const int mine = JOIN ? split : s.tiles * heads * ranges;
+    const int to = wave_scan(mine);
+    const int slot_to = a.target > 0 ? wave_scan(split * ranges) : 0;
     const uint64_t past = __ballot(items + to > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      auto of = [&](int v) { return __builtin_amdgcn_readfirstlane(__shfl(v, at)); };
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
       it.b = base + at;
       it.ranges = of(ranges);
       const int tiles = of(s.tiles), rest = index - (items + of(to - mine));
       if (rest < 0 || tiles < 1) return AttendItem{};
-      it.head = rest % heads;
       const int x = rest / heads;
-      it.range = x % it.ranges;
-      it.tile = tiles - 1 - x / it.ranges;  // a causal tile's work grows with its number: the longest first
-      it.group = groups + of(group_to) - tiles * heads + it.tile * heads + it.head;
-      it.slot = slots + of(slot_to) - tiles * it.ranges * heads + it.tile * it.ranges * heads + it.head;
+      it.head = rest - x * heads;
+      if constexpr (JOIN) {
+        it.tile = x;
+      } else {
+        const int y = x / it.ranges;
+        it.range = x - y * it.ranges;
+        it.tile = tiles - 1 - y;  // a causal tile's work grows with its number: the longest first
+      }
+      it.slot = slots + of(slot_to) + (it.tile - tiles) * it.ranges * heads + it.head;
       return it;
     }
     items += __builtin_amdgcn_readlane(to, 63);
-    groups += __builtin_amdgcn_readlane(group_to, 63);
     slots += __builtin_amdgcn_readlane(slot_to, 63);
   }
   return it;
@@ -247,29 +262,44 @@ struct AttendColumns {
     }
   }
 
-  // Whether column n sees token t of a page that is there.
-  __device__ __forceinline__ bool sees(const AttendArgs& a, const KvSeq& seq, int n, int t) const {
-    if (t >= seq.context + seq.rows) return false;
-    const bool near = t >= window_lo[n] || t < a.sinks;
-    if (a.mask == nullptr) return near && t <= seq.context + row[n];
-    if (t < seq.context) return near;
-    const int i = t - seq.context;
-    return (i >> 5) < a.mask_words && row[n] < a.mask_rows &&
-           ((a.mask[static_cast<int64_t>(row[n]) * a.mask_words + (i >> 5)] >> (i & 31)) & 1u) != 0;
-  }
-
-  // Bit 4 u + r: column n sees token t0 + 16 u + 4 g + r; units without a page (`held`) are not seen. A loop, since
-  // only tiles at an edge come here: unrolled, its loads of mask words would take the registers of all others.
+  // Bit 4 u + r: column n sees token t0 + 16 u + 4 g + r; units without a page (`held`) are not seen. Called where a
+  // step is at an edge of what its columns see.
   template <int UNITS>
   __device__ __forceinline__ uint32_t seen_bits(const AttendArgs& a, const KvSeq& seq, int n, int t0, int g,
                                                 uint32_t held) const {
-    uint32_t bits = 0;
-#pragma unroll 1
-    for (int u = 0; u < UNITS; ++u) {
-      uint32_t four = 0;
+    const int first = t0 + 4 * g, end = a.mask != nullptr ? seq.context + seq.rows : seq.context + row[n] + 1;
+    uint64_t own = ~uint64_t{0};  // bit i: token t0 + i by the mask
+    if (a.mask != nullptr && t0 + 16 * UNITS > seq.context) {
+      // The 16 UNITS bits from own row t0 - context on: three words of the row cover them.
+      const int i0 = max(t0 - seq.context, 0);
+      const uint32_t* from = a.mask + static_cast<int64_t>(row[n]) * a.mask_words;
+      uint32_t word[3];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) four |= static_cast<uint32_t>(sees(a, seq, n, t0 + 16 * u + 4 * g + r)) << r;
-      if ((held >> u) & 1u) bits |= four << (4 * u);
+      for (int i = 0; i < 3; ++i) {
+        const int at = (i0 >> 5) + i;
+        word[i] = at < a.mask_words && row[n] < a.mask_rows ? from[at] : 0u;
+      }
+      const uint64_t low = word[0] | static_cast<uint64_t>(word[1]) << 32, high = word[1] | static_cast<uint64_t>(word[2]) << 32;
+      own = (low >> (i0 & 31) & 0xffffffffu) | (high >> (i0 & 31)) << 32;
+      const int before = seq.context - t0;  // tokens of the context come first
+      if (before > 0) own = own << before | ((uint64_t{1} << before) - 1);
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      if (((held >> u) & 1u) == 0) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = first + 16 * u + r;
+        const bool near = t >= window_lo[n] || t < a.sinks || (a.mask != nullptr && t >= seq.context);
+        bits |= static_cast<uint32_t>(near && t < end) << (4 * u + r);
+      }
+    }
+    if (a.mask != nullptr) {
+      uint32_t by_mask = 0;
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) by_mask |= (static_cast<uint32_t>(own >> (16 * u + 4 * g)) & 15u) << (4 * u);
+      bits &= by_mask;
     }
     return bits;
   }
@@ -336,8 +366,10 @@ struct AttendWalk {
     first = min(lo_least / STEP, last);
     sink_steps = min((min(a.sinks, 1 << 29) + STEP - 1) / STEP, first);
     steps = sink_steps + last - first;
-    from = static_cast<int>(static_cast<int64_t>(steps) * it.range / it.ranges);
-    to = static_cast<int>(static_cast<int64_t>(steps) * (it.range + 1) / it.ranges);
+    // At most 2^24 steps (a table holds 2^29 tokens) and kAttendMost ranges: inside 32 bits.
+    const uint32_t n = static_cast<uint32_t>(steps), r = static_cast<uint32_t>(it.range), all = static_cast<uint32_t>(it.ranges);
+    from = all == 1 ? 0 : static_cast<int>(n * r / all);
+    to = all == 1 ? steps : static_cast<int>(n * (r + 1) / all);
   }
   __device__ __forceinline__ int token_of(int s) const { return STEP * (s < sink_steps ? s : first + s - sink_steps); }
   __device__ __forceinline__ bool edge(int t0) const { return t0 + STEP > whole || (t0 < lo_most && t0 + STEP > sinks); }
@@ -363,16 +395,13 @@ __device__ __forceinline__ void window_bounds(const AttendArgs& a, const AttendC
   most = __builtin_amdgcn_readfirstlane(most);
 }
 
-// A partial result's slot: [cols][pad] sums, then [cols] maxima and [cols] sums of exponentials. Written and read
-// past the XCD's own L2 (tile.h).
+// A partial result's slot: [cols][pad] sums, then [cols] maxima and [cols] sums of exponentials.
 template <int NC, int C>
 __device__ __forceinline__ void attend_publish(const AttendArgs& a, const AttendItem& it, int cols, int first, int g, int col,
                                                const AttendColumns<NC>& c, const f32x4 (&o)[NC][C][4], const float (&m)[NC],
                                                const float (&l)[NC]) {
   constexpr int PAD = 64 * C;
-  const uint32_t bytes = static_cast<uint32_t>(attend_slot_floats(cols, PAD) * 4);
-  char* mine = reinterpret_cast<char*>(a.partials) + static_cast<int64_t>(it.slot + it.range * a.cache.heads) * bytes;
-  const __amdgpu_buffer_rsrc_t rs = make_rsrc(mine, bytes);
+  float* mine = a.partials + static_cast<int64_t>(it.slot + it.range * a.cache.heads) * attend_slot_floats(cols, PAD);
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     if (!c.real[n]) continue;
@@ -380,60 +409,13 @@ __device__ __forceinline__ void attend_publish(const AttendArgs& a, const Attend
 #pragma unroll
     for (int k = 0; k < C; ++k)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const f32x4 x = {o[n][k][0][r], o[n][k][1][r], o[n][k][2][r], o[n][k][3][r]};
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rs, (at * PAD + 64 * k + 16 * g + 4 * r) * 4, 0,
-                                               kCoherent);
-      }
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(mine + at * PAD + 64 * k + 16 * g + 4 * r) =
+            f32x4{o[n][k][0][r], o[n][k][1][r], o[n][k][2][r], o[n][k][3][r]};
     if (g == 0) {
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m[n]), rs, (cols * PAD + at) * 4, 0, kCoherent);
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, l[n]), rs, (cols * PAD + cols + at) * 4, 0, kCoherent);
+      mine[cols * PAD + at] = m[n];
+      mine[cols * PAD + cols + at] = l[n];
     }
-  }
-}
-
-// Joins a group's ranges, by every thread of the workgroup that arrived last. `shared`: (kAttendMost + 1) * cols floats.
-template <int DT, int C>
-__device__ __forceinline__ void attend_join(const AttendArgs& a, const KvSeq& seq, const AttendItem& it, int cols, int columns,
-                                            float* shared) {
-  constexpr int PAD = 64 * C;
-  const uint32_t bytes = static_cast<uint32_t>(attend_slot_floats(cols, PAD) * 4);
-  const int live = min(cols, columns - it.tile * cols), threads = blockDim.x, dim = a.cache.dim;
-  float* weight = shared;               // [ranges][cols]
-  float* total = weight + it.ranges * cols;
-  auto slot_of = [&](int range) {
-    return reinterpret_cast<const char*>(a.partials) + static_cast<int64_t>(it.slot + range * a.cache.heads) * bytes;
-  };
-  for (int i = threadIdx.x; i < it.ranges * cols; i += threads) {
-    const int range = i / cols, c = i - range * cols;
-    weight[i] = c < live ? collect(reinterpret_cast<const float*>(slot_of(range)) + cols * PAD + c) : kMinusInf;
-  }
-  __syncthreads();
-  for (int c = threadIdx.x; c < live; c += threads) {
-    float top = kMinusInf, sum = 0.0f;
-    for (int range = 0; range < it.ranges; ++range) top = fmaxf(top, weight[range * cols + c]);
-    for (int range = 0; range < it.ranges; ++range) {
-      const float m = weight[range * cols + c];
-      const float x = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-      weight[range * cols + c] = x;
-      sum += x * collect(reinterpret_cast<const float*>(slot_of(range)) + cols * PAD + cols + c);
-    }
-    total[c] = sum == 0.0f ? 0.0f : 1.0f / sum;
-  }
-  __syncthreads();
-  const int quads = dim >> 2;
-  for (int i = threadIdx.x; i < live * quads; i += threads) {
-    const int c = i / quads, e = (i - c * quads) << 2;
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int range = 0; range < it.ranges; ++range) {
-      const __amdgpu_buffer_rsrc_t rs = make_rsrc(slot_of(range), bytes);
-      const f32x4 x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (c * PAD + e) * 4, 0, kCoherent));
-      sum += x * weight[range * cols + c];
-    }
-    sum *= total[c];
-    const int x = it.tile * cols + c, row = x / a.group;
-    uint16_t* at = a.out + (static_cast<int64_t>(seq.start + row) * a.heads + it.head * a.group + x - row * a.group) * dim;
-    *reinterpret_cast<u32x2*>(at + e) = u32x2{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
   }
 }
 
@@ -538,8 +520,10 @@ struct AttendWave {
         s.vs[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, page_vs), number - page_first));
       }
       const int unit = (t & (a.cache.page - 1)) >> 4;
-      s.at[u] = ((static_cast<int64_t>(max(id, 0)) * a.cache.heads + head) * (a.cache.page >> 4) + unit) *
-                (a.cache.chunks * kUnitBytes);
+      // A page of one head is at most 128 KiB, a page of all heads 128 MiB.
+      const uint32_t page_bytes = static_cast<uint32_t>(a.cache.page >> 4) * (C * kUnitBytes);
+      s.at[u] = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(max(id, 0))) * (page_bytes * a.cache.heads) +
+                                     page_bytes * static_cast<uint32_t>(head) + static_cast<uint32_t>(unit) * (C * kUnitBytes));
     }
     return s;
   }
@@ -569,7 +553,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const AttendItem it = attend_item<COLS>(a, blockIdx.x, lane);
+  const AttendItem it = attend_item<COLS, false>(a, blockIdx.x, lane);
   if (it.ranges == 0) return;
   KvSeq seq = kv_seq(a.rows, it.b, a.cache.page_shift);
   seq.start = __builtin_amdgcn_readfirstlane(seq.start);
@@ -815,9 +799,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
     if (wave == 0) cols.template store<DT, C>(a, seq, g, w.o, w.l);
     return;
   }
-  // One range of several: the partial result goes to the group's slot; the group's last workgroup joins them.
   if (wave == 0) attend_publish<NC, C>(a, it, COLS, 0, g, col, cols, w.o, w.m, w.l);
-  if (arrive_last(a.counters + it.group, it.ranges)) attend_join<DT, C>(a, seq, it, COLS, columns, shared);
 }
 
 hipError_t attend_bf16_e4m3(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);
@@ -825,6 +807,7 @@ hipError_t attend_bf16_model(const AttendArgs& a, int columns, unsigned grid, hi
 hipError_t attend_f16_e4m3(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);
 hipError_t attend_f16_model(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);
 
-constexpr int kAttendMost = 64;  // ranges per group, at most
+// Joins the groups of several ranges, `groups` at most.
+hipError_t attend_join(int32_t dtype, const AttendArgs& a, int columns, unsigned groups, hipStream_t s);
 
 }  // namespace plm

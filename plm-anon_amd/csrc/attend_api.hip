@@ -12,7 +12,7 @@ namespace {
 struct AttendPlan {
   int columns;        // of a workgroup's tile
   int target, least;  // AttendArgs
-  int64_t grid, bytes;
+  int64_t grid, groups, bytes;
 };
 
 // The launch of a call, from what the host knows: sizes, never the lengths. The work is cut on the device
@@ -24,16 +24,17 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   const int64_t group = heads / kv_heads, chunks = (head_dim + 63) / 64;
   const int64_t most = max_rows * group;
   p.columns = most <= 16 ? 16 : chunks > 2 ? 64 : most <= 32 ? 32 : most <= 256 ? 64 : 128;
-  const int64_t groups = kv_heads * (seqs + total * group / p.columns);
+  p.groups = kv_heads * (seqs + total * group / p.columns);
   const int64_t capacity = (table_width * page + kStep - 1) / kStep;
   p.least = 8;
   p.target = capacity > p.least ? 512 : 0;
-  p.grid = groups + p.target;
-  // A group of several ranges has two at least, and there are 2 * target ranges of such groups at most:
-  // a cut sequence has less than twice load / chunk of them, and a chunk is load / target at least.
-  if (p.target > 0)
-    p.bytes = PLM_ATTEND_COUNTER_BYTES +
-              2 * p.target * attend_slot_floats(p.columns, static_cast<int>(64 * chunks)) * 4;
+  p.grid = p.groups + p.target;
+  // There are 2 * target ranges of groups of several at most: a cut sequence has less than twice load / chunk of
+  // them, and a chunk is load / target at least. Such a group has two at least.
+  if (p.target > 0) {
+    p.groups = std::min<int64_t>(p.groups, p.target);
+    p.bytes = 2 * p.target * attend_slot_floats(p.columns, static_cast<int>(64 * chunks)) * 4;
+  }
   return p;
 }
 
@@ -44,8 +45,6 @@ bool attend_sizes(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t head
          seqs >= 1 && seqs <= (1 << 20) && max_rows >= 1 && max_rows <= total && total < (1 << 28) &&
          total * (heads / kv_heads) < (int64_t{1} << 30) && table_width >= 1 && table_width * page <= (int64_t{1} << 29);
 }
-
-static_assert(512 * sizeof(int) <= PLM_ATTEND_COUNTER_BYTES, "a counter per group of several ranges");
 
 }  // namespace
 }  // namespace plm
@@ -87,8 +86,7 @@ int plm_attend(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t 
   a.q_head = q_head;
   a.positions = positions;
   a.mask = mask;
-  a.counters = static_cast<int*>(workspace);
-  a.partials = p.bytes > 0 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + PLM_ATTEND_COUNTER_BYTES) : nullptr;
+  a.partials = static_cast<float*>(workspace);
   a.scale = scale * 1.44269504088896340736f;
   a.heads = heads;
   a.group = heads / cache->kv_heads;
@@ -97,14 +95,16 @@ int plm_attend(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t 
   a.mask_rows = static_cast<int>(mask_rows);
   a.mask_words = static_cast<int>(mask_words);
   a.target = p.target;
+  a.per_target = p.target > 0 ? 1.001f / static_cast<float>(p.target) : 0.0f;
   a.least = p.least;
-  a.most = plm::kAttendMost;
   const unsigned grid = static_cast<unsigned>(p.grid);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool e8 = cache->type == PLM_CACHE_E4M3;
   hipError_t err;
   if (dtype == PLM_BF16) err = e8 ? plm::attend_bf16_e4m3(a, p.columns, grid, s) : plm::attend_bf16_model(a, p.columns, grid, s);
   else err = e8 ? plm::attend_f16_e4m3(a, p.columns, grid, s) : plm::attend_f16_model(a, p.columns, grid, s);
+  if (err == hipSuccess && p.target > 0)
+    err = plm::attend_join(dtype, a, p.columns, static_cast<unsigned>(p.groups), s);
   return err == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 

@@ -17,20 +17,17 @@ hipError_t attend_go(Kernel kern, const AttendArgs& a, unsigned grid, unsigned t
   return hipGetLastError();
 }
 
-constexpr size_t attend_join_bytes(int columns) { return static_cast<size_t>(kAttendMost + 1) * columns * 4; }
-constexpr size_t larger(size_t a, size_t b) { return a > b ? a : b; }
-
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_stream(const AttendArgs& a, unsigned grid, hipStream_t s) {
   constexpr int W = 4;
   constexpr size_t waves = static_cast<size_t>(W / 2) * NC * (C * 16 + 2) * 64 * 4;
-  return attend_go(&attend_kernel<DT, E8, C, NC, W>, a, grid, 64 * W, larger(waves, attend_join_bytes(16 * NC)), s);
+  return attend_go(&attend_kernel<DT, E8, C, NC, W>, a, grid, 64 * W, waves, s);
 }
 
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_tiled(const AttendArgs& a, unsigned grid, hipStream_t s) {
   constexpr size_t sets = static_cast<size_t>(2) * attend_set_bytes(C);
-  return attend_go(&attend_tile_kernel<DT, E8, C, NC>, a, grid, 256, larger(sets, attend_join_bytes(64 * NC)), s);
+  return attend_go(&attend_tile_kernel<DT, E8, C, NC>, a, grid, 256, sets, s);
 }
 
 template <int DT, bool E8, int C>

@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const AttendItem it = attend_item<COLS>(a, blockIdx.x, lane);
+  const AttendItem it = attend_item<COLS, false>(a, blockIdx.x, lane);
   if (it.ranges == 0) return;
   KvSeq seq = kv_seq(a.rows, it.b, a.cache.page_shift);
   seq.start = __builtin_amdgcn_readfirstlane(seq.start);
@@ -91,6 +91,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   uint32_t unit_held = 0;  // bit u: unit u's page is there
   auto fetch = [&](int t0) {
     int64_t base[4];
+    // A page of one head is at most 128 KiB, a page of all heads 128 MiB.
+    const uint32_t page_bytes = static_cast<uint32_t>(a.cache.page >> 4) * (C * kUnitBytes);
     unit_held = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -103,8 +105,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
         unit_ks[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, page_ks), number - page_first));
         unit_vs[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, page_vs), number - page_first));
       }
-      base[u] = ((static_cast<int64_t>(max(id, 0)) * a.cache.heads + it.head) * (a.cache.page >> 4) +
-                 ((t & (a.cache.page - 1)) >> 4)) * (a.cache.chunks * kUnitBytes);
+      base[u] = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(max(id, 0))) * (page_bytes * a.cache.heads) +
+                                     page_bytes * static_cast<uint32_t>(it.head) +
+                                     static_cast<uint32_t>((t & (a.cache.page - 1)) >> 4) * (C * kUnitBytes));
     }
 #pragma unroll
     for (int i = 0; i < C; ++i) {
@@ -359,8 +362,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     return;
   }
   attend_publish<NC, C>(a, it, COLS, first_col, g, col, cols, o, m, l);
-  if (arrive_last(a.counters + it.group, it.ranges))
-    attend_join<DT, C>(a, seq, it, COLS, columns, reinterpret_cast<float*>(lds));
 }
 
 }  // namespace plm

@@ -222,27 +222,6 @@ def read_kv(cache: PagedCache, table: torch.Tensor, first: torch.Tensor, ends: t
     return k, v
 
 
-# The attention's workspaces: counters that every call leaves zero, then partial results. One per device and
-# stream, since calls on two streams may run at the same time.
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
-
-
-def _workspace(dev: torch.device, stream: int, sizes: tuple) -> tuple[int, int]:
-    need = int(_lib.lib().plm_attend_workspace_bytes(*sizes))
-    if need == 0:
-        return 0, 0
-    if torch.cuda.is_current_stream_capturing():
-        # The graph's own memory, its counters cleared in every replay: replays may run beside eager calls.
-        buf = torch.empty(need, dtype=torch.uint8, device=dev)
-        buf[: _lib.ATTEND_COUNTER_BYTES].zero_()
-        return buf.data_ptr(), need
-    key = (torch.cuda.current_device() if dev.index is None else dev.index, stream)
-    buf = _workspaces.get(key)
-    if buf is None or buf.numel() < need:
-        buf = _workspaces[key] = torch.zeros(max(need, 2 * buf.numel() if buf is not None else 0), dtype=torch.uint8, device=dev)
-    return buf.data_ptr(), need
-
-
 def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
            row_starts: torch.Tensor | None = None, max_rows: int | None = None, window: int | None = None, sinks: int = 0,
            mask: torch.Tensor | None = None, positions: torch.Tensor | None = None,
@@ -277,10 +256,12 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: tor
     at = None if positions is None else _index(positions, "positions", (total,), dev)
     out = torch.empty((total, heads, dim), dtype=dtype, device=dev)
     stream = _lib.stream_handle(dev)
-    space, size = _workspace(dev, stream, (cache.kv_heads, cache.page, dim, heads, total, rows[1], most, rows[5]))
+    size = _lib.lib().plm_attend_workspace_bytes(cache.kv_heads, cache.page, dim, heads, total, rows[1], most, rows[5])
+    space = torch.empty(size, dtype=torch.uint8, device=dev) if size else None   # partial results: this call's alone
     status = _lib.lib().plm_attend(code, cache._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, out.data_ptr(), *rows,
                                    0 if window is None else window, sinks, *mask_args, at,
-                                   1 / math.sqrt(dim) if scale is None else scale, space, size, stream)
+                                   1 / math.sqrt(dim) if scale is None else scale,
+                                   None if space is None else space.data_ptr(), size, stream)
     if status:
         _lib.check(status, f"plm_attend({total} rows, {rows[1]} sequences, heads {heads}/{cache.kv_heads} of {dim})")
     return out
