@@ -39,7 +39,7 @@ struct AttendArgs {
 
 constexpr int kStep = 32;        // tokens of a step
 constexpr int kAttendMost = 64;  // ranges per group, at most
-constexpr int kJoinColumns = 8;  // columns of a workgroup of the joining launch
+constexpr int kJoinColumns = 8;  // columns that a workgroup of the joining launch takes at a time, at most
 
 __host__ __device__ constexpr int64_t attend_slot_floats(int columns, int padded) {
   return static_cast<int64_t>(columns) * (padded + 2);
@@ -267,7 +267,7 @@ struct AttendColumns {
   template <int UNITS>
   __device__ __forceinline__ uint32_t seen_bits(const AttendArgs& a, const KvSeq& seq, int n, int t0, int g,
                                                 uint32_t held) const {
-    const int first = t0 + 4 * g, end = a.mask != nullptr ? seq.context + seq.rows : seq.context + row[n] + 1;
+    const int end = a.mask != nullptr ? seq.context + seq.rows : seq.context + row[n] + 1;
     uint64_t own = ~uint64_t{0};  // bit i: token t0 + i by the mask
     if (a.mask != nullptr && t0 + 16 * UNITS > seq.context) {
       // The 16 UNITS bits from own row t0 - context on: three words of the row cover them.
@@ -284,23 +284,15 @@ struct AttendColumns {
       const int before = seq.context - t0;  // tokens of the context come first
       if (before > 0) own = own << before | ((uint64_t{1} << before) - 1);
     }
+    // What is left of the step's tokens by the row's end and the window, as bits like `own`.
+    const auto below = [](int n) { return n <= 0 ? uint64_t{0} : n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1; };
+    uint64_t near = ~below(window_lo[n] - t0) | below(a.sinks - t0);
+    if (a.mask != nullptr) near |= ~below(seq.context - t0);
+    own &= near & below(end - t0);
+    const uint64_t mine = own >> (4 * g);
     uint32_t bits = 0;
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      if (((held >> u) & 1u) == 0) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = first + 16 * u + r;
-        const bool near = t >= window_lo[n] || t < a.sinks || (a.mask != nullptr && t >= seq.context);
-        bits |= static_cast<uint32_t>(near && t < end) << (4 * u + r);
-      }
-    }
-    if (a.mask != nullptr) {
-      uint32_t by_mask = 0;
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) by_mask |= (static_cast<uint32_t>(own >> (16 * u + 4 * g)) & 15u) << (4 * u);
-      bits &= by_mask;
-    }
+    for (int u = 0; u < UNITS; ++u) bits |= ((held >> u) & 1u ? static_cast<uint32_t>(mine >> (16 * u)) & 15u : 0u) << (4 * u);
     return bits;
   }
 
@@ -808,6 +800,6 @@ hipError_t attend_f16_e4m3(const AttendArgs& a, int columns, unsigned grid, hipS
 hipError_t attend_f16_model(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);
 
 // Joins the groups of several ranges, `groups` at most.
-hipError_t attend_join(int32_t dtype, const AttendArgs& a, int columns, unsigned groups, hipStream_t s);
+hipError_t attend_join(int32_t dtype, const AttendArgs& a, int columns, int64_t groups, hipStream_t s);
 
 }  // namespace plm

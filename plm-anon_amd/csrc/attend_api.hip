@@ -26,8 +26,9 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   p.columns = most <= 16 ? 16 : chunks > 2 ? 64 : most <= 32 ? 32 : most <= 256 ? 64 : 128;
   p.groups = kv_heads * (seqs + total * group / p.columns);
   const int64_t capacity = (table_width * page + kStep - 1) / kStep;
-  p.least = 8;
-  p.target = capacity > p.least ? 512 : 0;
+  p.least = p.columns <= 32 ? 16 : 8;
+  // A single sequence's groups are alike: where they fill the device there is nothing to even out.
+  p.target = capacity > p.least && !(seqs == 1 && p.groups >= 256) ? 512 : 0;
   p.grid = p.groups + p.target;
   // There are 2 * target ranges of groups of several at most: a cut sequence has less than twice load / chunk of
   // them, and a chunk is load / target at least. Such a group has two at least.
@@ -104,7 +105,7 @@ int plm_attend(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t 
   if (dtype == PLM_BF16) err = e8 ? plm::attend_bf16_e4m3(a, p.columns, grid, s) : plm::attend_bf16_model(a, p.columns, grid, s);
   else err = e8 ? plm::attend_f16_e4m3(a, p.columns, grid, s) : plm::attend_f16_model(a, p.columns, grid, s);
   if (err == hipSuccess && p.target > 0)
-    err = plm::attend_join(dtype, a, p.columns, static_cast<unsigned>(p.groups), s);
+    err = plm::attend_join(dtype, a, p.columns, p.groups, s);
   return err == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 

@@ -2,83 +2,107 @@
 //   out = sum_j 2^(m_j - m) o_j / sum_j 2^(m_j - m) l_j, m the largest m_j.
 // A launch of its own: joined by the last workgroup of each group to finish, a group's partial results came through one
 // CU, past its caches, at about 50 GB/s (a round's 56 rows over 4007 tokens: 16 groups of 16 ranges, 11 us of 25).
-// Here a workgroup takes eight columns of a group, thread by thread four dimensions of one.
+// Here a workgroup takes `take` columns of a group at a time, thread by thread four dimensions of one.
 #include "attend.h"
 
 namespace plm {
 
 template <int DT, int COLS>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
-  constexpr int kSlices = COLS / kJoinColumns;
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int take, int slices) {
   __shared__ float weight[kAttendMost][kJoinColumns], sums[kAttendMost][kJoinColumns], total[kJoinColumns];
-  const int slice = blockIdx.x % kSlices;
-  const AttendItem it = attend_item<COLS, true>(a, blockIdx.x / kSlices, threadIdx.x & 63);
-  if (it.ranges < 2) return;
-  const KvSeq seq = kv_seq(a.rows, it.b, a.cache.page_shift);
-  const int first = it.tile * COLS + slice * kJoinColumns;  // column of the sequence
-  const int live = min(kJoinColumns, seq.rows * a.group - first);
-  if (live <= 0) return;
-  const int pad = 64 * a.cache.chunks, dim = a.cache.dim;
+  __shared__ f32x4 parts[256];
+  const int pad = 64 * a.cache.chunks, dim = a.cache.dim, quads = dim >> 2;
   const int64_t apart = attend_slot_floats(COLS, pad) * a.cache.heads;  // from a range to the next
-  const float* slot = a.partials + it.slot * attend_slot_floats(COLS, pad);
-  for (int i = threadIdx.x; i < it.ranges * kJoinColumns; i += 256) {
-    const int range = i / kJoinColumns, c = i % kJoinColumns;
-    const float* from = slot + range * apart + COLS * pad + slice * kJoinColumns + c;
-    weight[range][c] = c < live ? from[0] : 0.0f;
-    sums[range][c] = c < live ? from[COLS] : 0.0f;
-  }
-  __syncthreads();
-  if (threadIdx.x < kJoinColumns) {
-    const int c = threadIdx.x;
-    constexpr float none = -__builtin_inff();
-    float top = none, sum = 0.0f;
-    for (int range = 0; range < it.ranges; ++range) top = fmaxf(top, weight[range][c]);
-    for (int range = 0; range < it.ranges; ++range) {
-      const float m = weight[range][c], x = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-      weight[range][c] = x;
-      sum += x * sums[range][c];
+  // A thread's share: every `lanes`-th range of four dimensions of a column.
+  const int work = take * quads, lanes = 256 / work, share = threadIdx.x / work;
+  const int c = (threadIdx.x - share * work) / quads, e = (threadIdx.x - share * work - c * quads) << 2;
+  for (int index = blockIdx.x;; index += gridDim.x) {
+    const AttendItem it = attend_item<COLS, true>(a, index / slices, threadIdx.x & 63);
+    if (it.ranges < 2) return;
+    const int slice = index % slices;
+    const KvSeq seq = kv_seq(a.rows, it.b, a.cache.page_shift);
+    const int first = it.tile * COLS + slice * take;  // column of the sequence
+    const int live = min(take, seq.rows * a.group - first);
+    if (live <= 0) continue;
+    const float* slot = a.partials + it.slot * attend_slot_floats(COLS, pad);
+    // The first eight of the thread's loads go with the maxima's and sums'.
+    const bool mine = share < lanes && c < live;
+    const float* from = slot + (slice * take + c) * pad + e;
+    f32x4 part[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (mine) part[k] = *reinterpret_cast<const f32x4*>(from + min(share + k * lanes, it.ranges - 1) * apart);
+    for (int i = threadIdx.x; i < it.ranges * take; i += 256) {
+      const int range = i / take, x = i - range * take;
+      const float* at = slot + range * apart + COLS * pad + slice * take + x;
+      weight[range][x] = x < live ? at[0] : 0.0f;
+      sums[range][x] = x < live ? at[COLS] : 0.0f;
     }
-    total[c] = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing is zero
-  }
-  __syncthreads();
-  const int quads = dim >> 2;
-  for (int i = threadIdx.x; i < live * quads; i += 256) {
-    const int c = i / quads, e = (i - c * quads) << 2;
-    const float* from = slot + (slice * kJoinColumns + c) * pad + e;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < take) {
+      const int x = threadIdx.x;
+      float top = -__builtin_inff(), sum = 0.0f;
+      for (int range = 0; range < it.ranges; ++range) top = fmaxf(top, weight[range][x]);
+      for (int range = 0; range < it.ranges; ++range) {
+        const float m = weight[range][x], y = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        weight[range][x] = y;
+        sum += y * sums[range][x];
+      }
+      total[x] = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing is zero
+    }
+    __syncthreads();
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int base = 0; base < it.ranges; base += 8) {
-      f32x4 part[8];
+    if (mine) {
+      for (int base = share; base < it.ranges; base += 8 * lanes) {
+        if (base != share) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) part[k] = *reinterpret_cast<const f32x4*>(from + min(base + k, it.ranges - 1) * apart);
+          for (int k = 0; k < 8; ++k)
+            part[k] = *reinterpret_cast<const f32x4*>(from + min(base + k * lanes, it.ranges - 1) * apart);
+        }
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (base + k < it.ranges) sum += part[k] * weight[base + k][c];
+        for (int k = 0; k < 8; ++k)
+          if (base + k * lanes < it.ranges) sum += part[k] * weight[base + k * lanes][c];
+      }
     }
-    sum *= total[c];
-    const int column = first + c, row = column / a.group;
-    uint16_t* at = a.out + (static_cast<int64_t>(seq.start + row) * a.heads + it.head * a.group + column - row * a.group) * dim;
-    *reinterpret_cast<u32x2*>(at + e) = u32x2{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
+    parts[threadIdx.x] = sum;
+    __syncthreads();
+    if (share == 0 && c < live) {
+      for (int k = 1; k < lanes; ++k) sum += parts[threadIdx.x + k * work];
+      sum *= total[c];
+      const int column = first + c, row = column / a.group;
+      uint16_t* at = a.out + (static_cast<int64_t>(seq.start + row) * a.heads + it.head * a.group + column - row * a.group) * dim;
+      *reinterpret_cast<u32x2*>(at + e) = u32x2{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
+    }
+    __syncthreads();
   }
 }
 
 namespace {
 
 template <int COLS>
-hipError_t join_go(int32_t dtype, const AttendArgs& a, unsigned groups, hipStream_t s) {
-  const unsigned grid = groups * (COLS / kJoinColumns);
-  if (dtype == PLM_BF16) attend_join_kernel<DT_BF16, COLS><<<grid, 256, 0, s>>>(a);
-  else attend_join_kernel<DT_F16, COLS><<<grid, 256, 0, s>>>(a);
+hipError_t join_go(int32_t dtype, const AttendArgs& a, int64_t groups, int columns, hipStream_t s) {
+  // Few columns per workgroup while the device has room for more of them, each of which costs a look at the lengths:
+  // cut decodes one at a time. What the grid does not cover is taken in turns.
+  const int quads = a.cache.dim / 4;
+  int take = 1;
+  while (take < kJoinColumns && 2 * take * quads <= 256 && groups * ((columns + take - 1) / take) > 512) take *= 2;
+  const int slices = (columns + take - 1) / take;
+  const unsigned grid = static_cast<unsigned>(groups * slices < 2048 ? groups * slices : 2048);
+  if (dtype == PLM_BF16) attend_join_kernel<DT_BF16, COLS><<<grid, 256, 0, s>>>(a, take, slices);
+  else attend_join_kernel<DT_F16, COLS><<<grid, 256, 0, s>>>(a, take, slices);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t attend_join(int32_t dtype, const AttendArgs& a, int columns, unsigned groups, hipStream_t s) {
+hipError_t attend_join(int32_t dtype, const AttendArgs& a, int columns, int64_t groups, hipStream_t s) {
+  const int64_t most = static_cast<int64_t>(a.rows.max_rows) * a.group;
+  const int live = static_cast<int>(most < columns ? most : columns);
   switch (columns) {
-    case 16: return join_go<16>(dtype, a, groups, s);
-    case 32: return join_go<32>(dtype, a, groups, s);
-    case 64: return join_go<64>(dtype, a, groups, s);
-    case 128: return join_go<128>(dtype, a, groups, s);
+    case 16: return join_go<16>(dtype, a, groups, live, s);
+    case 32: return join_go<32>(dtype, a, groups, live, s);
+    case 64: return join_go<64>(dtype, a, groups, live, s);
+    case 128: return join_go<128>(dtype, a, groups, live, s);
   }
   return hipErrorInvalidValue;
 }

@@ -14,6 +14,7 @@
 namespace plm {
 
 constexpr int kTile = 64;  // tokens staged at once
+constexpr int kNoLds = 0x1e;  // __builtin_amdgcn_sched_barrier: all but LDS accesses may move across
 constexpr int attend_set_bytes(int chunks) { return 16 * chunks * 1024; }
 
 template <int DT, bool E8, int C, int NC>
@@ -62,20 +63,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   walk.set(a, seq, it, COLS, columns, cols, lo_least);
   __syncthreads();
 
-  // Pages: lane i has number page_first + i of the sequence. fp16 values are staged in units of the largest scale
-  // of their pages so far (`ref`), which keeps codes times scale inside fp16; bf16 takes any scale.
-  int page_id = -1, page_first = -64;
-  float page_ks = 0.0f, page_vs = 0.0f, ref = DT == DT_F16 ? 0.0f : 1.0f, next_ref = ref;
+  // Pages: lane i has number page_first + i of the sequence: the byte where its head begins (bit 0: it is not there,
+  // and page 0 is read) and its scales. fp16 values are staged in units of the largest scale of their pages so far
+  // (`ref`), which keeps codes times scale inside fp16; bf16 takes any scale.
+  const uint32_t page_bytes = static_cast<uint32_t>(a.cache.page >> 4) * (C * kUnitBytes);  // of a head, 128 KiB at most
+  uint32_t page_lo = 1, page_hi = 0;
+  int page_first = -64;
+  float page_ks = kLeastScale, page_vs = 0.0f, ref = 1.0f, next_ref = 1.0f;
   auto pages = [&](int number) {
     page_first = number;
     const int at = number + lane;
-    int id = -1;
+    int64_t id = -1;
     if (at < last_page && at < a.rows.width) id = a.rows.table[it.b * a.rows.table_stride + at];
     const bool good = id >= 0 && id < a.cache.pages;
-    page_id = good ? id : -1;
+    const uint64_t byte = good ? static_cast<uint64_t>(id) * (page_bytes * static_cast<uint64_t>(a.cache.heads)) + page_bytes * static_cast<uint32_t>(it.head) : 1;
+    page_lo = static_cast<uint32_t>(byte);
+    page_hi = static_cast<uint32_t>(byte >> 32);
     if constexpr (E8) {
-      page_ks = good ? fmaxf(a.cache.k_scale[static_cast<int64_t>(id) * a.cache.heads + it.head], kLeastScale) : kLeastScale;
-      page_vs = good ? a.cache.v_scale[static_cast<int64_t>(id) * a.cache.heads + it.head] : 0.0f;
+      const int64_t of = good ? id * a.cache.heads + it.head : 0;
+      page_ks = good ? fmaxf(a.cache.k_scale[of], kLeastScale) : kLeastScale;
+      page_vs = good ? a.cache.v_scale[of] : 0.0f;
       if constexpr (DT == DT_F16) {
         float most = page_vs;
 #pragma unroll
@@ -84,100 +91,95 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       }
     }
   };
+  auto lane_float = [](float v, int at) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), at));
+  };
 
-  // A wavefront stages C jobs of 4 C: keys or values of a pair of units of one chunk.
-  u32x4 stage[C][2][kLoads];
-  float unit_ks[4], unit_vs[4];
-  uint32_t unit_held = 0;  // bit u: unit u's page is there
+  // A wavefront stages keys (wavefronts 0 and 1) or values (2 and 3) of one pair of the four units.
+  const int pair = wave & 1;
+  const bool values_role = wave >= 2;
+  const bool inside = (values_role ? 4 * col : 16 * g) < a.cache.dim - 64 * (C - 1);  // of the last chunk
+  const char* const role_base = values_role ? a.cache.v : a.cache.k;
+  struct Stage {
+    u32x4 x[2][C][kLoads];
+    float ks[4], vs[2];
+    uint32_t held;  // bit u: unit u's page is there
+    int t0;
+  };
+  Stage st;
   auto fetch = [&](int t0) {
-    int64_t base[4];
-    // A page of one head is at most 128 KiB, a page of all heads 128 MiB.
-    const uint32_t page_bytes = static_cast<uint32_t>(a.cache.page >> 4) * (C * kUnitBytes);
-    unit_held = 0;
+    const int shift = a.cache.page_shift, number = t0 >> shift;
+    if (number < page_first || ((t0 + 48) >> shift) >= page_first + 64) pages(number);
+    st.t0 = t0;
+    st.held = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int t = t0 + 16 * u;
-      const int number = t >> a.cache.page_shift;
-      if (number < page_first || number >= page_first + 64) pages(number);
-      const int id = __builtin_amdgcn_readlane(page_id, number - page_first);
-      unit_held |= static_cast<uint32_t>(id >= 0) << u;
-      if constexpr (E8) {
-        unit_ks[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, page_ks), number - page_first));
-        unit_vs[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, page_vs), number - page_first));
-      }
-      base[u] = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(max(id, 0))) * (page_bytes * a.cache.heads) +
-                                     page_bytes * static_cast<uint32_t>(it.head) +
-                                     static_cast<uint32_t>((t & (a.cache.page - 1)) >> 4) * (C * kUnitBytes));
+      const int at = ((t0 + 16 * u) >> shift) - page_first;
+      st.held |= (~static_cast<uint32_t>(__builtin_amdgcn_readlane(page_lo, at)) & 1u) << u;
+      if constexpr (E8) st.ks[u] = lane_float(page_ks, at);
     }
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int job = wave + 4 * i;
-      const bool values = job >= 2 * C;
-      const int x = values ? job - 2 * C : job, pair = x / C, c = x - pair * C;
-      const bool inside = (values ? 4 * col : 16 * g) < a.cache.dim - 64 * c;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const __amdgpu_buffer_rsrc_t rs =
-            unit_rsrc(values ? a.cache.v : a.cache.k, pair ? base[2 + u] : base[u], C * kUnitBytes);
-#pragma unroll
-        for (int h = 0; h < kLoads; ++h)
-          stage[i][u][h] = buffer_load16(rs, inside ? static_cast<uint32_t>(c * kUnitBytes + h * 1024 + lane * 16) : kOutOfRange);
-      }
+    for (int u = 0; u < 2; ++u) {
+      const int t = t0 + 32 * pair + 16 * u, at = (t >> shift) - page_first;
+      if constexpr (E8) st.vs[u] = lane_float(page_vs, at);
+      const uint64_t byte = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(page_hi, at))) << 32 |
+                            (static_cast<uint32_t>(__builtin_amdgcn_readlane(page_lo, at)) & ~1u);
+      load_unit<E8, C>(role_base, static_cast<int64_t>(byte + static_cast<uint32_t>((t & (a.cache.page - 1)) >> 4) * (C * kUnitBytes)),
+                       lane, inside, st.x[u]);
     }
   };
   bool odd = false;  // staged a value that is not finite for columns that may not all look (see attend_kernel)
-  auto store = [&](int t0, char* set) {
-    const bool edge = walk.edge(t0) || unit_held != 15u;
-    const bool cut = t0 + kTile > end || unit_held != 15u;  // tokens that are no one's: values there are zero
-    const float less = DT == DT_F16 ? (ref > 0.0f ? 1.0f / ref : 0.0f) : 1.0f;
+  auto store = [&](char* set) {
+    if (!values_role) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int job = wave + 4 * i;
-      const bool values = job >= 2 * C;
-      const int x = values ? job - 2 * C : job, pair = x / C, c = x - pair * C;
-      if (!values) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int c = 0; c < C; ++c) {
           char* to = set + ((2 * pair + u) * C + c) * 2048 + lane * 16;
           if constexpr (E8) {
-            *reinterpret_cast<u32x4*>(to) = fp8_eight<DT>(stage[i][u][0][0], stage[i][u][0][1], 1.0f);
-            *reinterpret_cast<u32x4*>(to + 1024) = fp8_eight<DT>(stage[i][u][0][2], stage[i][u][0][3], 1.0f);
+            const u32x4 x = st.x[u][c][0];
+            *reinterpret_cast<u32x4*>(to) = fp8_eight<DT>(x[0], x[1], 1.0f);
+            *reinterpret_cast<u32x4*>(to + 1024) = fp8_eight<DT>(x[2], x[3], 1.0f);
           } else {
-            *reinterpret_cast<u32x4*>(to) = stage[i][u][0];
-            *reinterpret_cast<u32x4*>(to + 1024) = stage[i][u][1];
+            *reinterpret_cast<u32x4*>(to) = st.x[u][c][0];
+            *reinterpret_cast<u32x4*>(to + 1024) = st.x[u][c][1];
           }
         }
-      } else {
-        char* to = set + kKeys + (pair * C + c) * 4096 + lane * 16;
-        const float r0 = (pair ? unit_vs[2] : unit_vs[0]) * less, r1 = (pair ? unit_vs[3] : unit_vs[1]) * less;
-        u32x4 keep = {~0u, ~0u, ~0u, ~0u};
-        if (cut) {
+      return;
+    }
+    const float less = DT == DT_F16 ? (ref > 0.0f ? 1.0f / ref : 0.0f) : 1.0f;
+    const float r0 = st.vs[0] * less, r1 = st.vs[1] * less;
+    const bool edge = walk.edge(st.t0) || st.held != 15u;
+    // Tokens that are no one's, past the end or of a page that is not there, have values of zero.
+    u32x4 keep = {~0u, ~0u, ~0u, ~0u};
+    if (st.t0 + kTile > end || st.held != 15u) {
 #pragma unroll
-          for (int i2 = 0; i2 < 4; ++i2) {
-            const int u = 2 * pair + i2 / 2, t = t0 + 16 * u + 4 * g + 2 * (i2 & 1);
-            const bool held = ((unit_held >> u) & 1u) != 0;
-            keep[i2] = (held && t < end ? 0xffffu : 0u) | (held && t + 1 < end ? 0xffff0000u : 0u);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          u32x4 v;
-          if constexpr (E8) {
-            v = u32x4{fp8_pair<DT>(stage[i][0][0][j], r0, false), fp8_pair<DT>(stage[i][0][0][j], r0, true),
-                      fp8_pair<DT>(stage[i][1][0][j], r1, false), fp8_pair<DT>(stage[i][1][0][j], r1, true)};
-          } else {
-            v = u32x4{stage[i][0][j / 2][2 * (j & 1)], stage[i][0][j / 2][2 * (j & 1) + 1], stage[i][1][j / 2][2 * (j & 1)],
-                      stage[i][1][j / 2][2 * (j & 1) + 1]};
-          }
-          v &= keep;
-          *reinterpret_cast<u32x4*>(to + j * 1024) = v;
-          if (edge) {
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) odd = odd || pair_not_finite<DT>(v[i2]);
-          }
-        }
+      for (int u = 0; u < 2; ++u) {
+        const bool held = ((st.held >> (2 * pair + u)) & 1u) != 0;
+        const int live = held ? end - (st.t0 + 32 * pair + 16 * u + 4 * g) : 0;  // of the lane's four tokens
+        keep[2 * u] = live >= 2 ? ~0u : live == 1 ? 0xffffu : 0u;
+        keep[2 * u + 1] = live >= 4 ? ~0u : live == 3 ? 0xffffu : 0u;
       }
     }
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x4 v;
+        if constexpr (E8) {
+          v = u32x4{fp8_pair<DT>(st.x[0][c][0][j], r0, false), fp8_pair<DT>(st.x[0][c][0][j], r0, true),
+                    fp8_pair<DT>(st.x[1][c][0][j], r1, false), fp8_pair<DT>(st.x[1][c][0][j], r1, true)};
+        } else {
+          v = u32x4{st.x[0][c][j / 2][2 * (j & 1)], st.x[0][c][j / 2][2 * (j & 1) + 1], st.x[1][c][j / 2][2 * (j & 1)],
+                    st.x[1][c][j / 2][2 * (j & 1) + 1]};
+        }
+        v &= keep;
+        *reinterpret_cast<u32x4*>(set + kKeys + ((pair * C + c) * 4 + j) * 1024 + lane * 16) = v;
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) odd = odd || pair_not_finite<DT>(v[i]);
+        }
+      }
   };
 
   auto compute = [&](auto careful, const char* set, int t0, const float (&ks)[4], uint32_t held) {
@@ -185,19 +187,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     const bool edge = walk.edge(t0) || held != 15u;
     const char* keys = set + lane * 16;
     const char* values = keys + kKeys;
+    // Operands come from LDS four at a time, the next four ahead of the products with the current: the products of
+    // one (chunk, half) with all four units are independent of each other and take longer than a read.
+    u32x4 x[2][4];
+    auto read_keys = [&](int ch, u32x4 (&to)[4]) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) to[u] = *reinterpret_cast<const u32x4*>(keys + (u * 2 * C + ch) * 1024);
+    };
+    auto read_values = [&](int pc, u32x4 (&to)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[j] = *reinterpret_cast<const u32x4*>(values + (pc * 4 + j) * 1024);
+    };
     f32x4 s[NC][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int n = 0; n < NC; ++n)
 #pragma unroll
-      for (int n = 0; n < NC; ++n) s[n][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int u = 0; u < 4; ++u) s[n][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    read_keys(0, x[0]);
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+    for (int ch = 0; ch < 2 * C; ++ch) {
+      if (ch + 1 < 2 * C) read_keys(ch + 1, x[(ch + 1) & 1]);
+      else read_values(0, x[(ch + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(kNoLds);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const u32x4 k = *reinterpret_cast<const u32x4*>(keys + ((u * C + c) * 2 + h) * 1024);
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int n = 0; n < NC; ++n) s[n][u] = mfma_16x16x32<DT>(k, q[n][c][h], s[n][u]);
-        }
+        for (int n = 0; n < NC; ++n) s[n][u] = mfma_16x16x32<DT>(x[ch & 1][u], q[n][ch / 2][ch & 1], s[n][u]);
     }
     uint32_t seen[NC];
     if (edge) {
@@ -249,15 +264,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     }
     if (!CAREFUL || !edge) {
 #pragma unroll
-      for (int pair = 0; pair < 2; ++pair)
+      for (int pc = 0; pc < 2 * C; ++pc) {
+        if (pc + 1 < 2 * C) read_values(pc + 1, x[(pc + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(kNoLds);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(values + ((pair * C + c) * 4 + j) * 1024);
-#pragma unroll
-            for (int n = 0; n < NC; ++n) o[n][c][j] = mfma_16x16x32<DT>(v, p[n][pair], o[n][c][j]);
-          }
+          for (int n = 0; n < NC; ++n) o[n][pc % C][j] = mfma_16x16x32<DT>(x[pc & 1][j], p[n][pc / C], o[n][pc % C][j]);
+      }
       return;
     }
     // One token at a time, as in attend_kernel.
@@ -304,31 +318,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       l[n] = 0.0f;
     }
     page_first = -64;
-    ref = next_ref = DT == DT_F16 ? 0.0f : 1.0f;
+    ref = next_ref = E8 && DT == DT_F16 ? 0.0f : 1.0f;
   };
 
   begin();
   if (walk.from < walk.to) {
-    int t0 = walk.token_of(walk.from);
-    fetch(t0);
-    follow();
-    store(t0, lds);
-    __syncthreads();
-    int set = 0;
-    for (int s = walk.from; s < walk.to; ++s) {
-      const float ks[4] = {unit_ks[0], unit_ks[1], unit_ks[2], unit_ks[3]};
-      const uint32_t held = unit_held;
-      const int now = t0;
-      const bool more = s + 1 < walk.to;
-      if (more) {
-        t0 = walk.token_of(s + 1);
-        fetch(t0);
-      }
-      compute(std::false_type{}, lds + set * kSet, now, ks, held);
-      set ^= 1;
-      if (more) {
+    // The first turn only fetches: one copy of the code, which short walks wait for too.
+#pragma unroll 1
+    for (int s = walk.from - 1; s < walk.to; ++s) {
+      const int t0 = st.t0, set = (s - walk.from) & 1;
+      const float ks[4] = {st.ks[0], st.ks[1], st.ks[2], st.ks[3]};
+      const uint32_t held = st.held;
+      if (s + 1 < walk.to) fetch(walk.token_of(s + 1));
+      if (s >= walk.from) compute(std::false_type{}, lds + set * kSet, t0, ks, held);
+      if (s + 1 < walk.to) {
         follow();
-        store(t0, lds + set * kSet);
+        store(lds + (set ^ 1) * kSet);
       }
       __syncthreads();
     }
@@ -336,12 +341,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       begin();
 #pragma unroll 1
       for (int s = walk.from; s < walk.to; ++s) {
-        t0 = walk.token_of(s);
-        fetch(t0);
+        fetch(walk.token_of(s));
         follow();
-        store(t0, lds);
+        store(lds);
         __syncthreads();
-        compute(std::true_type{}, lds, t0, unit_ks, unit_held);
+        compute(std::true_type{}, lds, st.t0, st.ks, st.held);
         __syncthreads();
       }
     }
