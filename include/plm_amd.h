@@ -504,30 +504,59 @@ typedef struct plm_kv_cache {
   int32_t kv_heads, page, head_dim, type;
 } plm_kv_cache;
 
+/* The rows of a call, as above; every field of a call's structs is 8 bytes. */
+typedef struct plm_kv_rows {
+  int64_t total, seqs, max_rows;
+  const int32_t* table;
+  int64_t table_stride, table_width;
+  const int64_t* lengths;
+  const int64_t* row_starts;
+} plm_kv_rows;
+
 /*
  * Turns the rows' queries and keys by their positions and stores keys and values in the cache.
- * rope: float [rope_rows, rotary], a position's rotary / 2 cosines, then its sines (NULL: no rotation);
- * dimensions past `rotary` stay. A pair is (i, i + rotary / 2), or with side_by_side (2 i, 2 i + 1):
- * (a, b) becomes (a cos - b sin, b cos + a sin). Row r's position is positions[r], or its token number
- * where positions is NULL; a position that the table does not hold turns into NaN.
+ * dtype: plm_dtype of the rows (of a 16-bit cache its own type). rope: float [rope_rows, rotary], a position's
+ * rotary / 2 cosines, then its sines (NULL: no rotation); dimensions past `rotary` stay. A pair is
+ * (i, i + rotary / 2), or with side_by_side (2 i, 2 i + 1): (a, b) becomes (a cos - b sin, b cos + a sin).
+ * Row r's position is positions[r], or its token number where positions is NULL; a position that the table
+ * does not hold turns into NaN.
  * q_out: contiguous [total, heads, head_dim] (q NULL: no queries). It must not overlap q.
  * 8-bit pages: a page's scale is the least power of two that its rows need (largest magnitude <= 448
  * scale); it grows with them, the rows that stay are then rounded again, and starts anew with the
  * page's first row. What is not finite becomes NaN and has no part in the scale.
  * No two sequences may append to the same page in one call.
  */
-int plm_kv_append(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int32_t heads,
-                  void* q_out, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
-                  int64_t v_head, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table,
-                  int64_t table_stride, int64_t table_width, const int64_t* lengths, const int64_t* row_starts,
-                  const float* rope, int64_t rope_rows, int32_t rotary, int32_t side_by_side,
-                  const int64_t* positions, void* stream);
+typedef struct plm_append_call {
+  int64_t dtype;
+  const plm_kv_cache* cache;
+  plm_kv_rows rows;
+  const void* q;
+  int64_t q_row, q_head, heads;
+  void* q_out;
+  const void* k;
+  int64_t k_row, k_head;
+  const void* v;
+  int64_t v_row, v_head;
+  const float* rope;
+  int64_t rope_rows, rotary, side_by_side;
+  const int64_t* positions;
+} plm_append_call;
+int plm_kv_append(const plm_append_call* call, void* stream);
 
 /* Tokens [first[b], min(first[b] + most, ends[b])) of every sequence as values of `dtype`: k, v
  * contiguous [seqs, most, kv_heads, head_dim], zeros past ends[b]. */
-int plm_kv_read(int32_t dtype, const plm_kv_cache* cache, const int32_t* table, int64_t table_stride,
-                int64_t table_width, const int64_t* first, const int64_t* ends, int64_t seqs, int64_t most, void* k,
-                void* v, void* stream);
+typedef struct plm_read_call {
+  int64_t dtype;
+  const plm_kv_cache* cache;
+  const int32_t* table;
+  int64_t table_stride, table_width;
+  const int64_t* first;
+  const int64_t* ends;
+  int64_t seqs, most;
+  void* k;
+  void* v;
+} plm_read_call;
+int plm_kv_read(const plm_read_call* call, void* stream);
 
 /*
  * out[row, head] = softmax over the tokens that the row sees of (scale * q . key), times the values;
@@ -538,17 +567,25 @@ int plm_kv_read(int32_t dtype, const plm_kv_cache* cache, const int32_t* table, 
  *     mask[i, j / 32] is set;
  * and with window > 0 of these only t > position - window or t < sinks, the position being positions[r]
  * (positions NULL: lengths[b] + i); under a mask the window holds for the context alone. A row that sees
- * nothing is zero. out: contiguous [total, heads, head_dim].
+ * nothing is zero. out: contiguous [total, heads, head_dim]. scale is positive.
  * Workspace: plm_attend_workspace_bytes (0: none needed), 16-byte aligned, of any content; calls that may
  * run at the same time need workspaces of their own.
  */
-int plm_attend(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int32_t heads,
-               void* out, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table, int64_t table_stride,
-               int64_t table_width, const int64_t* lengths, const int64_t* row_starts, int64_t window, int64_t sinks,
-               const uint32_t* mask, int64_t mask_rows, int64_t mask_words, const int64_t* positions, float scale,
-               void* workspace, size_t workspace_bytes, void* stream);
-size_t plm_attend_workspace_bytes(int32_t kv_heads, int32_t page, int32_t head_dim, int32_t heads, int64_t total,
-                                  int64_t seqs, int64_t max_rows, int64_t table_width);
+typedef struct plm_attend_call {
+  int64_t dtype;
+  const plm_kv_cache* cache;
+  plm_kv_rows rows;
+  const void* q;
+  int64_t q_row, q_head, heads;
+  void* out;
+  int64_t window, sinks;
+  const uint32_t* mask;
+  int64_t mask_rows, mask_words;
+  const int64_t* positions;
+  double scale;
+} plm_attend_call;
+int plm_attend(const plm_attend_call* call, void* workspace, size_t workspace_bytes, void* stream);
+size_t plm_attend_workspace_bytes(const plm_attend_call* call);
 
 /* Human-readable name of a status code. */
 const char* plm_status_string(int32_t status);

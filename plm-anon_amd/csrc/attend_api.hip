@@ -39,12 +39,19 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   return p;
 }
 
-bool attend_sizes(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t heads, int64_t total, int64_t seqs,
-                  int64_t max_rows, int64_t table_width) {
-  return kv_heads >= 1 && kv_heads <= 1024 && heads >= kv_heads && heads <= 4096 && heads % kv_heads == 0 &&
-         (page == 16 || page == 32 || page == 64 || page == 128) && head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0 &&
-         seqs >= 1 && seqs <= (1 << 20) && max_rows >= 1 && max_rows <= total && total < (1 << 28) &&
-         total * (heads / kv_heads) < (int64_t{1} << 30) && table_width >= 1 && table_width * page <= (int64_t{1} << 29);
+// The plan of a call whose numbers go together; false where they do not.
+bool attend_of(const plm_attend_call* call, AttendArgs& a, AttendPlan& p) {
+  if (call == nullptr) return false;
+  const plm_attend_call& h = *call;
+  if (!kv_cache_of(h.cache, a.cache) || !kv_type_fits(h.cache, h.dtype) || !kv_rows_of(a.cache, h.rows, a.rows)) return false;
+  const int64_t heads = a.cache.heads;
+  if (h.heads < heads || h.heads > 4096 || h.heads % heads != 0 || h.rows.total * (h.heads / heads) >= (int64_t{1} << 30))
+    return false;
+  if (h.window < 0 || h.sinks < 0 || !(h.scale > 0.0) || !(h.scale < 3.0e38)) return false;
+  if (h.mask != nullptr && (h.mask_rows < 1 || h.mask_words < 1 || h.mask_rows >= (1 << 28) || h.mask_words >= (1 << 24)))
+    return false;
+  p = attend_plan(heads, a.cache.page, a.cache.dim, h.heads, h.rows.total, h.rows.seqs, h.rows.max_rows, h.rows.table_width);
+  return p.grid < (int64_t{1} << 31);
 }
 
 }  // namespace
@@ -52,60 +59,49 @@ bool attend_sizes(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t head
 
 extern "C" {
 
-size_t plm_attend_workspace_bytes(int32_t kv_heads, int32_t page, int32_t head_dim, int32_t heads, int64_t total,
-                                  int64_t seqs, int64_t max_rows, int64_t table_width) {
-  if (!plm::attend_sizes(kv_heads, page, head_dim, heads, total, seqs, max_rows, table_width)) return 0;
-  return static_cast<size_t>(plm::attend_plan(kv_heads, page, head_dim, heads, total, seqs, max_rows, table_width).bytes);
+size_t plm_attend_workspace_bytes(const plm_attend_call* call) {
+  plm::AttendArgs a{};
+  plm::AttendPlan p{};
+  return plm::attend_of(call, a, p) ? static_cast<size_t>(p.bytes) : 0;
 }
 
-int plm_attend(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int32_t heads,
-               void* out, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table, int64_t table_stride,
-               int64_t table_width, const int64_t* lengths, const int64_t* row_starts, int64_t window, int64_t sinks,
-               const uint32_t* mask, int64_t mask_rows, int64_t mask_words, const int64_t* positions, float scale,
-               void* workspace, size_t workspace_bytes, void* stream) {
+int plm_attend(const plm_attend_call* call, void* workspace, size_t workspace_bytes, void* stream) {
   plm::AttendArgs a{};
-  if (!plm::kv_cache_of(cache, a.cache) || !plm::kv_type_fits(cache, dtype)) return PLM_ERR_ARGUMENT;
-  if (!plm::attend_sizes(cache->kv_heads, cache->page, cache->head_dim, heads, total, seqs, max_rows, table_width))
-    return PLM_ERR_ARGUMENT;
-  if (!plm::kv_rows_of(a.cache, total, seqs, max_rows, table, table_stride, table_width, lengths, row_starts, a.rows))
-    return PLM_ERR_ARGUMENT;
-  if (q == nullptr || out == nullptr || window < 0 || sinks < 0) return PLM_ERR_ARGUMENT;
-  if (mask != nullptr && (mask_rows < 1 || mask_words < 1 || mask_rows >= (1 << 28) || mask_words >= (1 << 24)))
-    return PLM_ERR_ARGUMENT;
-  if (q_row % 8 != 0 || q_head % 8 != 0) return PLM_ERR_ALIGNMENT;
-  for (const void* p : {q, static_cast<const void*>(out), static_cast<const void*>(cache->k),
-                        static_cast<const void*>(cache->v), static_cast<const void*>(workspace)})
-    if (!plm::aligned16_ptr(p)) return PLM_ERR_ALIGNMENT;
-  const plm::AttendPlan p =
-      plm::attend_plan(cache->kv_heads, cache->page, cache->head_dim, heads, total, seqs, max_rows, table_width);
+  plm::AttendPlan p{};
+  if (!plm::attend_of(call, a, p)) return PLM_ERR_ARGUMENT;
+  const plm_attend_call& h = *call;
+  if (h.q == nullptr || h.out == nullptr) return PLM_ERR_ARGUMENT;
+  if (h.q_row % 8 != 0 || h.q_head % 8 != 0) return PLM_ERR_ALIGNMENT;
+  for (const void* x : {h.q, static_cast<const void*>(h.out), static_cast<const void*>(a.cache.k),
+                        static_cast<const void*>(a.cache.v), static_cast<const void*>(workspace)})
+    if (!plm::aligned16_ptr(x)) return PLM_ERR_ALIGNMENT;
   if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(p.bytes))) return PLM_ERR_WORKSPACE;
-  if (p.grid >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   constexpr int64_t far = int64_t{1} << 30;
-  a.q = static_cast<const uint16_t*>(q);
-  a.out = static_cast<uint16_t*>(out);
-  a.q_row = q_row;
-  a.q_head = q_head;
-  a.positions = positions;
-  a.mask = mask;
+  a.q = static_cast<const uint16_t*>(h.q);
+  a.out = static_cast<uint16_t*>(h.out);
+  a.q_row = h.q_row;
+  a.q_head = h.q_head;
+  a.positions = h.positions;
+  a.mask = h.mask;
   a.partials = static_cast<float*>(workspace);
-  a.scale = scale * 1.44269504088896340736f;
-  a.heads = heads;
-  a.group = heads / cache->kv_heads;
-  a.window = static_cast<int>(window < far ? window : 0);  // longer than any cache: no window
-  a.sinks = static_cast<int>(std::min(sinks, far));
-  a.mask_rows = static_cast<int>(mask_rows);
-  a.mask_words = static_cast<int>(mask_words);
+  a.scale = static_cast<float>(h.scale * 1.44269504088896340736);
+  a.heads = static_cast<int>(h.heads);
+  a.group = a.heads / a.cache.heads;
+  a.window = static_cast<int>(h.window < far ? h.window : 0);  // longer than any cache: no window
+  a.sinks = static_cast<int>(std::min(h.sinks, far));
+  a.mask_rows = static_cast<int>(h.mask_rows);
+  a.mask_words = static_cast<int>(h.mask_words);
   a.target = p.target;
   a.per_target = p.target > 0 ? 1.001f / static_cast<float>(p.target) : 0.0f;
   a.least = p.least;
   const unsigned grid = static_cast<unsigned>(p.grid);
+  const int32_t dtype = static_cast<int32_t>(h.dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool e8 = cache->type == PLM_CACHE_E4M3;
+  const bool e8 = h.cache->type == PLM_CACHE_E4M3;
   hipError_t err;
   if (dtype == PLM_BF16) err = e8 ? plm::attend_bf16_e4m3(a, p.columns, grid, s) : plm::attend_bf16_model(a, p.columns, grid, s);
   else err = e8 ? plm::attend_f16_e4m3(a, p.columns, grid, s) : plm::attend_f16_model(a, p.columns, grid, s);
-  if (err == hipSuccess && p.target > 0)
-    err = plm::attend_join(dtype, a, p.columns, p.groups, s);
+  if (err == hipSuccess && p.target > 0) err = plm::attend_join(dtype, a, p.columns, p.groups, s);
   return err == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 

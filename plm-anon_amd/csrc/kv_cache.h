@@ -129,21 +129,20 @@ inline bool kv_cache_of(const plm_kv_cache* h, KvCache& c) {
   return true;
 }
 
-inline bool kv_type_fits(const plm_kv_cache* h, int32_t dtype) {
+inline bool kv_type_fits(const plm_kv_cache* h, int64_t dtype) {
   if (dtype != PLM_BF16 && dtype != PLM_F16) return false;
   return h->type == PLM_CACHE_E4M3 || h->type == (dtype == PLM_BF16 ? PLM_CACHE_BF16 : PLM_CACHE_F16);
 }
 
 // A call's rows; false where its numbers do not go together.
-inline bool kv_rows_of(const KvCache& c, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table,
-                       int64_t table_stride, int64_t table_width, const int64_t* lengths, const int64_t* row_starts,
-                       KvRows& r) {
-  if (total < 1 || total >= (1 << 28) || seqs < 1 || seqs > (1 << 20) || max_rows < 1 || max_rows > total) return false;
-  if (row_starts == nullptr && seqs * max_rows != total) return false;
-  if (table == nullptr || lengths == nullptr) return false;
-  if (table_width < 1 || table_width > ((int64_t{1} << 29) >> c.page_shift) || table_stride < table_width) return false;
-  r = {table, lengths, row_starts, table_stride, static_cast<int>(total), static_cast<int>(seqs),
-       static_cast<int>(max_rows), static_cast<int>(table_width)};
+inline bool kv_rows_of(const KvCache& c, const plm_kv_rows& h, KvRows& r) {
+  if (h.total < 1 || h.total >= (1 << 28) || h.seqs < 1 || h.seqs > (1 << 20) || h.max_rows < 1 || h.max_rows > h.total)
+    return false;
+  if (h.row_starts == nullptr && h.seqs * h.max_rows != h.total) return false;
+  if (h.table == nullptr || h.lengths == nullptr) return false;
+  if (h.table_width < 1 || h.table_width > ((int64_t{1} << 29) >> c.page_shift) || h.table_stride < h.table_width) return false;
+  r = {h.table, h.lengths, h.row_starts, h.table_stride, static_cast<int>(h.total), static_cast<int>(h.seqs),
+       static_cast<int>(h.max_rows), static_cast<int>(h.table_width)};
   return true;
 }
 

@@ -421,83 +421,79 @@ void append_go(const AppendArgs& a, unsigned grid, hipStream_t s) {
 
 extern "C" {
 
-int plm_kv_append(int32_t dtype, const plm_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int32_t heads,
-                  void* q_out, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
-                  int64_t v_head, int64_t total, int64_t seqs, int64_t max_rows, const int32_t* table,
-                  int64_t table_stride, int64_t table_width, const int64_t* lengths, const int64_t* row_starts,
-                  const float* rope, int64_t rope_rows, int32_t rotary, int32_t side_by_side,
-                  const int64_t* positions, void* stream) {
+int plm_kv_append(const plm_append_call* call, void* stream) {
+  if (call == nullptr) return PLM_ERR_ARGUMENT;
+  const plm_append_call& h = *call;
   plm::AppendArgs a{};
-  if (!plm::kv_cache_of(cache, a.cache) || !plm::kv_type_fits(cache, dtype)) return PLM_ERR_ARGUMENT;
-  if (!plm::kv_rows_of(a.cache, total, seqs, max_rows, table, table_stride, table_width, lengths, row_starts, a.rows))
+  if (!plm::kv_cache_of(h.cache, a.cache) || !plm::kv_type_fits(h.cache, h.dtype)) return PLM_ERR_ARGUMENT;
+  if (!plm::kv_rows_of(a.cache, h.rows, a.rows)) return PLM_ERR_ARGUMENT;
+  if (h.k == nullptr || h.v == nullptr) return PLM_ERR_ARGUMENT;
+  if (h.q != nullptr && (h.heads < 1 || h.heads > 4096 || h.q_out == nullptr)) return PLM_ERR_ARGUMENT;
+  if (h.rope != nullptr && (h.rotary < 2 || h.rotary > a.cache.dim || h.rotary % 2 != 0 || h.rope_rows < 1))
     return PLM_ERR_ARGUMENT;
-  if (k == nullptr || v == nullptr) return PLM_ERR_ARGUMENT;
-  if (q != nullptr && (heads < 1 || heads > 4096 || q_out == nullptr)) return PLM_ERR_ARGUMENT;
-  if (rope != nullptr && (rotary < 2 || rotary > cache->head_dim || rotary % 2 != 0 || rope_rows < 1))
-    return PLM_ERR_ARGUMENT;
-  if ((q_row | q_head | k_row | k_head | v_row | v_head) % 8 != 0) return PLM_ERR_ALIGNMENT;
-  for (const void* p : {q, static_cast<const void*>(q_out), k, v, static_cast<const void*>(cache->k),
-                        static_cast<const void*>(cache->v), static_cast<const void*>(rope)})
+  if ((h.q_row | h.q_head | h.k_row | h.k_head | h.v_row | h.v_head) % 8 != 0) return PLM_ERR_ALIGNMENT;
+  for (const void* p : {h.q, static_cast<const void*>(h.q_out), h.k, h.v, static_cast<const void*>(a.cache.k),
+                        static_cast<const void*>(a.cache.v), static_cast<const void*>(h.rope)})
     if (!plm::aligned16_ptr(p)) return PLM_ERR_ALIGNMENT;
-  a.q = static_cast<const uint16_t*>(q);
-  a.q_out = static_cast<uint16_t*>(q_out);
-  a.new_k = static_cast<const uint16_t*>(k);
-  a.new_v = static_cast<const uint16_t*>(v);
-  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  a.positions = positions;
-  a.rope = rope;
-  a.rope_rows = rope_rows;
-  a.heads = heads;
-  a.rotary = rotary;
-  a.side_by_side = side_by_side;
-  const int64_t page = cache->page;
+  a.q = static_cast<const uint16_t*>(h.q);
+  a.q_out = static_cast<uint16_t*>(h.q_out);
+  a.new_k = static_cast<const uint16_t*>(h.k);
+  a.new_v = static_cast<const uint16_t*>(h.v);
+  a.q_row = h.q_row, a.q_head = h.q_head, a.k_row = h.k_row, a.k_head = h.k_head, a.v_row = h.v_row, a.v_head = h.v_head;
+  a.positions = h.positions;
+  a.rope = h.rope;
+  a.rope_rows = h.rope_rows;
+  a.heads = static_cast<int>(h.heads);
+  a.rotary = static_cast<int>(h.rotary);
+  a.side_by_side = h.side_by_side != 0;
+  const int64_t page = a.cache.page, seqs = h.rows.seqs, max_rows = h.rows.max_rows;
   a.page_slots = static_cast<int>((page - 1 + max_rows + page - 1) / page);
-  const int64_t kv_blocks = seqs * a.page_slots * cache->kv_heads * 2;
-  const int64_t q_blocks = q == nullptr ? 0 : (max_rows * heads * (cache->head_dim / 8) + 255) / 256;
+  const int64_t kv_blocks = seqs * a.page_slots * a.cache.heads * 2;
+  const int64_t q_blocks = h.q == nullptr ? 0 : (max_rows * h.heads * (a.cache.dim / 8) + 255) / 256;
   if (kv_blocks + q_blocks * seqs >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   a.kv_blocks = static_cast<int>(kv_blocks);
   a.q_blocks = static_cast<int>(q_blocks);
   const unsigned grid = static_cast<unsigned>(kv_blocks + q_blocks * seqs);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool e8 = cache->type == PLM_CACHE_E4M3;
-  if (dtype == PLM_BF16) e8 ? plm::append_go<plm::DT_BF16, true>(a, grid, s) : plm::append_go<plm::DT_BF16, false>(a, grid, s);
+  const bool e8 = h.cache->type == PLM_CACHE_E4M3;
+  if (h.dtype == PLM_BF16) e8 ? plm::append_go<plm::DT_BF16, true>(a, grid, s) : plm::append_go<plm::DT_BF16, false>(a, grid, s);
   else e8 ? plm::append_go<plm::DT_F16, true>(a, grid, s) : plm::append_go<plm::DT_F16, false>(a, grid, s);
   return hipGetLastError() == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 
-int plm_kv_read(int32_t dtype, const plm_kv_cache* cache, const int32_t* table, int64_t table_stride,
-                int64_t table_width, const int64_t* first, const int64_t* ends, int64_t seqs, int64_t most, void* k,
-                void* v, void* stream) {
+int plm_kv_read(const plm_read_call* call, void* stream) {
+  if (call == nullptr) return PLM_ERR_ARGUMENT;
+  const plm_read_call& h = *call;
   plm::ReadArgs a{};
-  if (!plm::kv_cache_of(cache, a.cache) || !plm::kv_type_fits(cache, dtype)) return PLM_ERR_ARGUMENT;
-  if (seqs < 1 || seqs > (1 << 20) || most < 1 || most >= (1 << 30) || table == nullptr || first == nullptr ||
-      ends == nullptr || k == nullptr || v == nullptr)
+  if (!plm::kv_cache_of(h.cache, a.cache) || !plm::kv_type_fits(h.cache, h.dtype)) return PLM_ERR_ARGUMENT;
+  if (h.seqs < 1 || h.seqs > (1 << 20) || h.most < 1 || h.most >= (1 << 30) || h.table == nullptr || h.first == nullptr ||
+      h.ends == nullptr || h.k == nullptr || h.v == nullptr)
     return PLM_ERR_ARGUMENT;
-  if (table_width < 1 || table_width > ((int64_t{1} << 29) >> a.cache.page_shift) || table_stride < table_width)
+  if (h.table_width < 1 || h.table_width > ((int64_t{1} << 29) >> a.cache.page_shift) || h.table_stride < h.table_width)
     return PLM_ERR_ARGUMENT;
-  for (const void* p : {static_cast<const void*>(k), static_cast<const void*>(v), static_cast<const void*>(cache->k),
-                        static_cast<const void*>(cache->v)})
+  for (const void* p : {static_cast<const void*>(h.k), static_cast<const void*>(h.v), static_cast<const void*>(a.cache.k),
+                        static_cast<const void*>(a.cache.v)})
     if (!plm::aligned16_ptr(p)) return PLM_ERR_ALIGNMENT;
-  a.table = table;
-  a.first = first;
-  a.ends = ends;
-  a.k = static_cast<uint16_t*>(k);
-  a.v = static_cast<uint16_t*>(v);
-  a.table_stride = table_stride;
-  a.width = static_cast<int>(table_width);
-  a.seqs = static_cast<int>(seqs);
-  a.most = static_cast<int>(most);
+  a.table = h.table;
+  a.first = h.first;
+  a.ends = h.ends;
+  a.k = static_cast<uint16_t*>(h.k);
+  a.v = static_cast<uint16_t*>(h.v);
+  a.table_stride = h.table_stride;
+  a.width = static_cast<int>(h.table_width);
+  a.seqs = static_cast<int>(h.seqs);
+  a.most = static_cast<int>(h.most);
   // Keys: an item per token and 8 dimensions; values: per quad of tokens (one more where `first` is
   // inside a quad) and 4 dimensions, never more items than keys have but for that quad.
-  const int64_t key_items = most * cache->kv_heads * (cache->head_dim / 8);
-  const int64_t value_items = ((most + 3) / 4 + 1) * cache->kv_heads * (cache->head_dim / 4);
+  const int64_t key_items = h.most * a.cache.heads * (a.cache.dim / 8);
+  const int64_t value_items = ((h.most + 3) / 4 + 1) * a.cache.heads * (a.cache.dim / 4);
   const int64_t blocks = ((key_items > value_items ? key_items : value_items) + 255) / 256;
-  if (blocks * seqs * 2 >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
+  if (blocks * h.seqs * 2 >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   a.blocks = static_cast<int>(blocks);
-  const unsigned grid = static_cast<unsigned>(blocks * seqs * 2);
+  const unsigned grid = static_cast<unsigned>(blocks * h.seqs * 2);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool e8 = cache->type == PLM_CACHE_E4M3;
-  if (dtype == PLM_BF16) {
+  const bool e8 = h.cache->type == PLM_CACHE_E4M3;
+  if (h.dtype == PLM_BF16) {
     if (e8) plm::read_kernel<plm::DT_BF16, true><<<grid, 256, 0, s>>>(a);
     else plm::read_kernel<plm::DT_BF16, false><<<grid, 256, 0, s>>>(a);
   } else {

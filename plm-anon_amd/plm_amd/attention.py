@@ -28,7 +28,6 @@ from . import _lib
 
 PAGES = (16, 32, 64, 128)
 MAX_HEAD_DIM = 256
-MAX_ROPE_ROWS = 1 << 30
 _TYPES = {torch.bfloat16: _lib.PLM_CACHE_BF16, torch.float16: _lib.PLM_CACHE_F16, torch.float8_e4m3fn: _lib.PLM_CACHE_E4M3}
 LEAST_SCALE = 2.0 ** -64   # of an 8-bit page that holds nothing but zeros
 
@@ -73,10 +72,11 @@ class PagedCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.page, self.head_dim, self.dtype = pages, heads, page, head_dim, k.dtype
         self.device = k.device
+        self._index = k.get_device()
         self._handle = _lib.KvCache(k.data_ptr(), v.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
                                     0 if v_scale is None else v_scale.data_ptr(), pages, heads, page, head_dim,
                                     _TYPES[k.dtype])
-        self._ref = ctypes.byref(self._handle)
+        self._ref = ctypes.addressof(self._handle)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, *, page: int = 64,
@@ -98,52 +98,69 @@ class PagedCache:
         return cls(k, v, *scales, head_dim=head_dim)
 
 
-def _index(t: torch.Tensor, name: str, shape: tuple, dev: torch.device) -> int:
-    if t.dtype != torch.int64 or t.shape != shape or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int64 {list(shape)} tensor on {dev}, got {t.dtype} "
+# The checks below are on every call's path, where the host's time counts: one look at each property, strides only of
+# tensors that are not contiguous, messages formed for refusals alone.
+
+
+def _numbers(t: torch.Tensor, name: str, n: int, cache: PagedCache) -> int:
+    """Device pointer of ``n`` int64 numbers."""
+    if t.dtype is not torch.int64 or t.shape != (n,) or t.get_device() != cache._index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int64 [{n}] tensor on {cache.device}, got {t.dtype} "
                          f"{list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, total: int, heads: int | None, dim: int,
-          dev: torch.device) -> torch.Tensor:
-    """``t`` as [rows, heads, dim] rows that a kernel can read: dimensions contiguous, rows and heads on 16 bytes."""
-    if t.dim() != 3 or t.shape[0] != total or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [{total}, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
-    if t.dtype != dtype:
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, cache: PagedCache) -> tuple[torch.Tensor, int, int, int]:
+    """``t`` [rows, heads, dim] as a kernel can read it (dimensions contiguous, rows and heads on 16 bytes), its pointer
+    and the strides of its rows and heads."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != dev:
-        raise RuntimeError(f"{name} must be on the cache's GPU {dev}, got {t.device}")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    if t.get_device() != cache._index:
+        raise RuntimeError(f"{name} must be on the cache's GPU {cache.device}, got {t.device}")
+    at = t.data_ptr()
+    if at % 16 == 0:
+        if t.is_contiguous():
+            return t, at, shape[1] * shape[2], shape[2]
+        row, head, one = t.stride()
+        if one == 1 and row % 8 == 0 and head % 8 == 0:
+            return t, at, row, head
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), shape[1] * shape[2], shape[2]
+
+
+def _table(t: torch.Tensor, cache: PagedCache) -> tuple[int, int, int, int]:
+    """Sequences, pointer, row stride and width of a page table."""
+    if t.dim() == 2 and t.dtype is torch.int32 and t.get_device() == cache._index:
+        seqs, width = t.shape
+        if seqs and width:
+            if t.is_contiguous():
+                return seqs, t.data_ptr(), width, width
+            row, one = t.stride()
+            if (one == 1 or width == 1) and (row >= width or seqs == 1):
+                return seqs, t.data_ptr(), max(row, width), width
+    raise ValueError(f"table must be an int32 [seqs, pages] tensor with contiguous rows on {cache.device}, got {t.dtype} "
+                     f"{list(t.shape)} on {t.device}")
 
 
 def _call(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, row_starts: torch.Tensor | None,
-          max_rows: int | None) -> tuple[int, tuple]:
-    """``(max_rows, arguments)`` of a call's rows, from ``total`` to ``row_starts`` of the C entries."""
-    dev = cache.device
-    if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or table.shape[1] < 1 or table.stride(1) != 1:
-        raise ValueError(f"table must be an int32 [seqs, pages] tensor with contiguous rows on {dev}, got {table.dtype} "
-                         f"{tuple(table.shape)} on {table.device}")
-    seqs, width = table.shape
+          max_rows: int | None) -> tuple:
+    """plm_kv_rows of a call."""
+    seqs, at, stride, width = _table(table, cache)
     if row_starts is None:
-        if seqs < 1 or total % seqs:
+        if total % seqs:
             raise ValueError(f"{total} rows are no whole number for each of {seqs} sequences: row_starts is needed")
         each = total // seqs
         if max_rows is not None and max_rows != each:
             raise ValueError(f"max_rows must be {each} for {total} rows of {seqs} sequences, got {max_rows}")
-        max_rows, starts = each, None
-    else:
-        starts = _index(row_starts, "row_starts", (seqs + 1,), dev)
-        if max_rows is None:
-            max_rows = total
-        elif not 1 <= max_rows <= total:
-            raise ValueError(f"max_rows must be in [1, {total}], got {max_rows}")
-    stride = table.stride(0) if seqs > 1 else width
-    if stride < width:
-        raise ValueError("the table's rows must not overlap")
-    return max_rows, (total, seqs, max_rows, table.data_ptr(), stride, width, _index(lengths, "lengths", (seqs,), dev), starts)
+        return total, seqs, each, at, stride, width, _numbers(lengths, "lengths", seqs, cache), 0
+    starts = _numbers(row_starts, "row_starts", seqs + 1, cache)
+    if max_rows is None:
+        max_rows = total
+    elif not 1 <= max_rows <= total:
+        raise ValueError(f"max_rows must be in [1, {total}], got {max_rows}")
+    return total, seqs, max_rows, at, stride, width, _numbers(lengths, "lengths", seqs, cache), starts
 
 
 def _model_dtype(cache: PagedCache, dtype: torch.dtype) -> int:
@@ -168,33 +185,38 @@ def append_kv(cache: PagedCache, q: torch.Tensor | None, k: torch.Tensor, v: tor
     ``rope`` does not hold gives NaN. In an 8-bit cache a page's scale is the least power of two that its rows
     need: it grows with them (rows that stay are rounded again) and starts anew with the page's first row.
     ``lengths`` stays as it is. Two sequences may share pages, but not the ones this call appends to."""
-    total = k.shape[0] if k.dim() == 3 else 0
-    if total < 1:
-        raise ValueError(f"k must be [rows, {cache.kv_heads}, {cache.head_dim}] with at least one row, got {tuple(k.shape)}")
-    dev, dim, dtype = cache.device, cache.head_dim, k.dtype
+    if k.dim() != 3 or k.shape[0] < 1:
+        raise ValueError(f"k must be [rows, {cache.kv_heads}, {cache.head_dim}] with at least one row, got {list(k.shape)}")
+    dim, dtype, total = cache.head_dim, k.dtype, k.shape[0]
     code = _model_dtype(cache, dtype)
-    k = _rows(k, "k", dtype, total, cache.kv_heads, dim, dev)
-    v = _rows(v, "v", dtype, total, cache.kv_heads, dim, dev)
-    out, heads, q_args = None, 0, (0, 0, 0, 0, 0)
+    shape = (total, cache.kv_heads, dim)
+    k, k_at, k_row, k_head = _rows(k, "k", dtype, shape, cache)
+    v, v_at, v_row, v_head = _rows(v, "v", dtype, shape, cache)
+    out, q_at, q_row, q_head, heads, out_at = None, 0, 0, 0, 0, 0
     if q is not None:
-        q = _rows(q, "q", dtype, total, None, dim, dev)
-        heads = q.shape[1]
-        out = torch.empty((total, heads, dim), dtype=dtype, device=dev)
-        q_args = (q.data_ptr(), q.stride(0), q.stride(1), heads, out.data_ptr())
-    _, rows = _call(cache, total, table, lengths, row_starts, max_rows)
-    rope_args = (0, 0, 0)
+        heads = q.shape[1] if q.dim() == 3 else 0
+        q, q_at, q_row, q_head = _rows(q, "q", dtype, (total, heads, dim), cache)
+        if heads < 1:
+            raise ValueError("q must have at least one head")
+        out = q.new_empty((total, heads, dim))
+        out_at = out.data_ptr()
+    rows = _call(cache, total, table, lengths, row_starts, max_rows)
+    rope_at, rope_rows, rotary = 0, 0, 0
     if rope is not None:
-        if rope.dim() != 2 or rope.dtype != torch.float32 or rope.device != dev or not rope.is_contiguous():
-            raise ValueError(f"rope must be a contiguous float32 [positions, rotary] tensor on {dev}")
-        if rope.shape[0] < 1 or rope.shape[1] < 2 or rope.shape[1] % 2 or rope.shape[1] > dim:
-            raise ValueError(f"rope must hold an even number of entries up to {dim} per position, got {tuple(rope.shape)}")
-        if rope.data_ptr() % 16:
+        if rope.dim() != 2 or rope.dtype is not torch.float32 or rope.get_device() != cache._index or not rope.is_contiguous():
+            raise ValueError(f"rope must be a contiguous float32 [positions, rotary] tensor on {cache.device}")
+        rope_rows, rotary = rope.shape
+        if rope_rows < 1 or rotary < 2 or rotary % 2 or rotary > dim:
+            raise ValueError(f"rope must hold an even number of entries up to {dim} per position, got {list(rope.shape)}")
+        rope_at = rope.data_ptr()
+        if rope_at % 16:
             rope = rope.clone()
-        rope_args = (rope.data_ptr(), rope.shape[0], rope.shape[1])
-    at = None if positions is None else _index(positions, "positions", (total,), dev)
-    status = _lib.lib().plm_kv_append(code, cache._ref, *q_args, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                      v.stride(0), v.stride(1), *rows, *rope_args, bool(interleaved), at,
-                                      _lib.stream_handle(dev))
+            rope_at = rope.data_ptr()
+    at = 0 if positions is None else _numbers(positions, "positions", total, cache)
+    status = _lib.lib().plm_kv_append(
+        _lib.pack_append(code, cache._ref, *rows, q_at, q_row, q_head, heads, out_at, k_at, k_row, k_head, v_at, v_row, v_head,
+                         rope_at, rope_rows, rotary, bool(interleaved), at),
+        _lib.stream_handle(cache.device))
     if status:
         _lib.check(status, f"plm_kv_append({total} rows, {rows[1]} sequences, heads {heads}/{cache.kv_heads} of {dim})")
     return out
@@ -205,18 +227,14 @@ def read_kv(cache: PagedCache, table: torch.Tensor, first: torch.Tensor, ends: t
     """Keys and values of tokens ``[first[b], min(first[b] + most, ends[b]))`` as ``dtype``
     ``[seqs, most, kv_heads, head_dim]``, zeros after them."""
     code = _model_dtype(cache, dtype)
-    dev = cache.device
-    if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or table.shape[0] < 1 or table.shape[1] < 1 \
-            or table.stride(1) != 1:
-        raise ValueError(f"table must be an int32 [seqs, pages] tensor with contiguous rows on {dev}, got {table.dtype} "
-                         f"{tuple(table.shape)} on {table.device}")
     if most < 1:
         raise ValueError(f"most must be at least 1, got {most}")
-    seqs, width = table.shape
-    k, v = (torch.empty((seqs, most, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev) for _ in range(2))
-    status = _lib.lib().plm_kv_read(code, cache._ref, table.data_ptr(), table.stride(0) if seqs > 1 else width, width,
-                                    _index(first, "first", (seqs,), dev), _index(ends, "ends", (seqs,), dev), seqs, most,
-                                    k.data_ptr(), v.data_ptr(), _lib.stream_handle(dev))
+    seqs, table_at, stride, width = _table(table, cache)
+    first_at, ends_at = _numbers(first, "first", seqs, cache), _numbers(ends, "ends", seqs, cache)
+    k, v = torch.empty((2, seqs, most, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device).unbind(0)
+    status = _lib.lib().plm_kv_read(
+        _lib.pack_read(code, cache._ref, table_at, stride, width, first_at, ends_at, seqs, most, k.data_ptr(), v.data_ptr()),
+        _lib.stream_handle(cache.device))
     if status:
         _lib.check(status, f"plm_kv_read({seqs} sequences, most {most})")
     return k, v
@@ -235,33 +253,38 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: tor
     position being ``positions[row]`` or the row's token number; under a mask the window holds for the context
     alone. A row that sees nothing is zero. ``scale`` is 1 / sqrt(head_dim) unless given."""
     if q.dim() != 3 or q.shape[0] < 1:
-        raise ValueError(f"q must be [rows, heads, {cache.head_dim}] with at least one row, got {tuple(q.shape)}")
-    dev, dim, dtype, total, heads = cache.device, cache.head_dim, q.dtype, q.shape[0], q.shape[1]
+        raise ValueError(f"q must be [rows, heads, {cache.head_dim}] with at least one row, got {list(q.shape)}")
+    dim, dtype = cache.head_dim, q.dtype
+    total, heads, _ = shape = q.shape
     code = _model_dtype(cache, dtype)
-    q = _rows(q, "q", dtype, total, None, dim, dev)
+    q, q_at, q_row, q_head = _rows(q, "q", dtype, (total, heads, dim), cache)
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"the query heads must be a multiple of the cache's {cache.kv_heads}, got {heads}")
-    most, rows = _call(cache, total, table, lengths, row_starts, max_rows)
+    rows = _call(cache, total, table, lengths, row_starts, max_rows)
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1 token, got {window}")
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
-    mask_args = (None, 0, 0)
+    if scale is not None and not 0 < scale < math.inf:
+        raise ValueError(f"scale must be positive, got {scale}")
+    mask_at, mask_rows, mask_words = 0, 0, 0
     if mask is not None:
-        if mask.dim() != 2 or mask.dtype != torch.int32 or mask.device != dev or not mask.is_contiguous() \
+        most = rows[2]
+        if mask.dim() != 2 or mask.dtype is not torch.int32 or mask.get_device() != cache._index or not mask.is_contiguous() \
                 or mask.shape[0] < most or mask.shape[1] * 32 < most:
-            raise ValueError(f"mask must be a contiguous int32 [rows, words] tensor on {dev} with a bit for each of {most} "
-                             f"rows, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
-        mask_args = (mask.data_ptr(), mask.shape[0], mask.shape[1])
-    at = None if positions is None else _index(positions, "positions", (total,), dev)
-    out = torch.empty((total, heads, dim), dtype=dtype, device=dev)
-    stream = _lib.stream_handle(dev)
-    size = _lib.lib().plm_attend_workspace_bytes(cache.kv_heads, cache.page, dim, heads, total, rows[1], most, rows[5])
-    space = torch.empty(size, dtype=torch.uint8, device=dev) if size else None   # partial results: this call's alone
-    status = _lib.lib().plm_attend(code, cache._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, out.data_ptr(), *rows,
-                                   0 if window is None else window, sinks, *mask_args, at,
-                                   1 / math.sqrt(dim) if scale is None else scale,
-                                   None if space is None else space.data_ptr(), size, stream)
+            raise ValueError(f"mask must be a contiguous int32 [rows, words] tensor on {cache.device} with a bit for each of "
+                             f"{most} rows, got {mask.dtype} {list(mask.shape)} on {mask.device}")
+        mask_at, (mask_rows, mask_words) = mask.data_ptr(), mask.shape
+    at = 0 if positions is None else _numbers(positions, "positions", total, cache)
+    out = q.new_empty(shape)
+    call = _lib.pack_attend(code, cache._ref, *rows, q_at, q_row, q_head, heads, out.data_ptr(), window or 0, sinks, mask_at,
+                            mask_rows, mask_words, at, 1 / math.sqrt(dim) if scale is None else scale)
+    lib = _lib.lib()
+    space, size = 0, lib.plm_attend_workspace_bytes(call)
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=cache.device)   # partial results: this call's alone
+        space = work.data_ptr()
+    status = lib.plm_attend(call, space, size, _lib.stream_handle(cache.device))
     if status:
         _lib.check(status, f"plm_attend({total} rows, {rows[1]} sequences, heads {heads}/{cache.kv_heads} of {dim})")
     return out

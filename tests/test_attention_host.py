@@ -5,6 +5,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -21,7 +23,7 @@ def _stub(pages=4, heads=2, dim=64, page=32, dtype=E4M3):
     c.pages, c.kv_heads, c.page, c.head_dim, c.dtype, c.device = pages, heads, page, dim, dtype, torch.device("cpu")
     kind = {BF16: 0, FP16: 1, E4M3: 2}[dtype]
     c._handle = _lib.KvCache(1 << 20, 1 << 20, 1 << 20, 1 << 20, pages, heads, page, dim, kind)
-    c._ref = ctypes.byref(c._handle)
+    c._ref, c._index = ctypes.addressof(c._handle), -1
     return c
 
 
@@ -84,6 +86,8 @@ def test_cache_refuses():
     (dict(mask=torch.zeros(3, 1, dtype=torch.int64)), ValueError),
     (dict(mask=torch.zeros(3, 0, dtype=torch.int32)), ValueError),
     (dict(positions=torch.zeros(5, dtype=torch.int64)), ValueError),
+    (dict(scale=0.0), ValueError),
+    (dict(scale=math.nan), ValueError),
 ])
 def test_attend_refuses(change, error):
     c = _call()
@@ -124,53 +128,88 @@ def test_types_of_rows_and_cache_go_together():
         attention.read_kv(_stub(), c["table"].long(), c["lengths"], c["lengths"], 4, BF16)
 
 
+def test_structs_are_the_headers():
+    """The packed structs have the header's fields, in its order."""
+    text = (Path(__file__).resolve().parents[1] / "include" / "plm_amd.h").read_text()
+
+    def fields(name):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
+        found = []
+        for line in body.strip().split(";"):
+            words = line.replace("*", " ").replace(",", " ").split()
+            words = [w for w in words if w not in ("const", "void", "int64_t", "int32_t", "uint32_t", "float", "double")]
+            if words[:1] == ["plm_kv_rows"]:
+                words = list(fields("plm_kv_rows"))
+            elif words[:1] == ["plm_kv_cache"]:
+                words = words[1:]
+            found += words
+        return tuple(found)
+
+    assert fields("plm_kv_rows") == _lib.KV_ROWS
+    assert fields("plm_append_call") == _lib.APPEND_FIELDS
+    assert fields("plm_read_call") == _lib.READ_FIELDS
+    assert fields("plm_attend_call") == _lib.ATTEND_FIELDS
+    assert fields("plm_kv_cache") == tuple(name for name, _ in _lib.KvCache._fields_)
+
+
 def test_c_entries_refuse_before_a_launch():
     lib, f = _lib.lib(), 1 << 20   # never dereferenced
+    kept = []
 
     def cache(**more):
         fields = dict(k=f, v=f, k_scale=f, v_scale=f, pages=4, kv_heads=2, page=32, head_dim=64, type=2)
-        return ctypes.byref(_lib.KvCache(**{**fields, **more}))
+        kept.append(_lib.KvCache(**{**fields, **more}))
+        return ctypes.addressof(kept[-1])
 
-    def attend(c, dtype=0, q=f, q_row=256, q_head=64, heads=4, out=f, total=6, seqs=2, most=3, table=f, stride=3, width=3,
-               lengths=f, starts=None, window=0, sinks=0, mask=None, rows=0, words=0, space=f, size=1 << 30):
-        return lib.plm_attend(dtype, c, q, q_row, q_head, heads, out, total, seqs, most, table, stride, width, lengths, starts,
-                              window, sinks, mask, rows, words, None, 0.125, space, size, None)
+    rows = dict(total=6, seqs=2, max_rows=3, table=f, table_stride=3, table_width=3, lengths=f, row_starts=0)
 
+    def attend(space=f, size=1 << 30, **more):
+        call = dict(dtype=0, cache=cache(), **rows, q=f, q_row=256, q_head=64, heads=4, out=f, window=0, sinks=0, mask=0,
+                    mask_rows=0, mask_words=0, positions=0, scale=0.125)
+        assert set(more) <= set(call)
+        packed = _lib.pack_attend(*{**call, **more}.values())
+        return lib.plm_attend(packed, space, size, None), lib.plm_attend_workspace_bytes(packed)
+
+    assert lib.plm_attend(None, f, 1 << 30, None) == -1 and lib.plm_attend_workspace_bytes(None) == 0
     for bad in (dict(k=None), dict(pages=0), dict(kv_heads=0), dict(page=48), dict(head_dim=60), dict(head_dim=264),
                 dict(type=3), dict(k_scale=None), dict(type=1)):
-        assert attend(cache(**bad)) == -1, bad
-    assert attend(None) == -1
-    for bad in (dict(dtype=2), dict(heads=3), dict(heads=0), dict(total=0), dict(total=5), dict(seqs=0), dict(most=0),
-                dict(most=7, starts=f), dict(table=None), dict(lengths=None), dict(width=0), dict(stride=2), dict(q=None),
-                dict(out=None), dict(window=-1), dict(sinks=-1), dict(mask=f), dict(mask=f, rows=3)):
-        assert attend(cache(), **bad) == -1, bad
+        assert attend(cache=cache(**bad)) == (-1, 0), bad
+    for bad in (dict(cache=0), dict(dtype=2), dict(heads=3), dict(heads=0), dict(total=0), dict(total=5), dict(seqs=0),
+                dict(max_rows=0), dict(max_rows=7, row_starts=f), dict(table=0), dict(lengths=0), dict(table_width=0),
+                dict(table_stride=2), dict(window=-1), dict(sinks=-1), dict(mask=f), dict(mask=f, mask_rows=3), dict(scale=0.0),
+                dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf)):
+        assert attend(**bad) == (-1, 0), bad
+    for bad in (dict(q=0), dict(out=0)):
+        assert attend(**bad)[0] == -1, bad
     for bad in (dict(q=f + 2), dict(out=f + 8), dict(q_row=100), dict(q_head=4)):
-        assert attend(cache(), **bad) == -2, bad
-    sizes = (2, 32, 64, 4, 6, 2, 3, 64)
-    need = lib.plm_attend_workspace_bytes(*sizes)
-    assert need > 0
-    assert attend(cache(), stride=64, width=64, size=need - 1) == -4
-    assert attend(cache(), stride=64, width=64, space=None) == -4
-    assert lib.plm_attend_workspace_bytes(2, 32, 64, 4, 6, 2, 3, 1) == 0   # short tables are never cut
-    assert lib.plm_attend_workspace_bytes(2, 32, 64, 3, 6, 2, 3, 64) == 0
+        assert attend(**bad)[0] == -2, bad
+    wide = dict(table_stride=64, table_width=64)
+    need = attend(space=None, **wide)[1]
+    assert need > 0 and attend(size=need - 1, **wide) == (-4, need) and attend(space=None, **wide) == (-4, need)
+    assert attend(q=0)[1] == 0   # short tables are never cut
 
-    def append(c, dtype=0, q=f, heads=4, q_out=f, k=f, k_row=128, total=6, rope=f, rope_rows=9, rotary=64):
-        return lib.plm_kv_append(dtype, c, q, 256, 64, heads, q_out, k, k_row, 64, f, 128, 64, total, 2, 3, f, 3, 3, f, None,
-                                 rope, rope_rows, rotary, 0, None, None)
+    def append(**more):
+        call = dict(dtype=0, cache=cache(), **rows, q=f, q_row=256, q_head=64, heads=4, q_out=f, k=f, k_row=128, k_head=64, v=f,
+                    v_row=128, v_head=64, rope=f, rope_rows=9, rotary=64, side_by_side=0, positions=0)
+        assert set(more) <= set(call)
+        return lib.plm_kv_append(_lib.pack_append(*{**call, **more}.values()), None)
 
-    for bad in (dict(dtype=5), dict(heads=0), dict(q_out=None), dict(k=None), dict(total=7), dict(rotary=66), dict(rotary=3),
-                dict(rope_rows=0)):
-        assert append(cache(), **bad) == -1, bad
+    assert lib.plm_kv_append(None, None) == -1
+    for bad in (dict(dtype=5), dict(heads=0), dict(q_out=0), dict(k=0), dict(v=0), dict(total=7), dict(rotary=66), dict(rotary=3),
+                dict(rope_rows=0), dict(cache=cache(head_dim=0))):
+        assert append(**bad) == -1, bad
     for bad in (dict(k=f + 4), dict(rope=f + 4), dict(k_row=132), dict(q_out=f + 2)):
-        assert append(cache(), **bad) == -2, bad
-    assert append(cache(head_dim=0)) == -1
+        assert append(**bad) == -2, bad
 
-    def read(c, first=f, most=4, k=f, width=3):
-        return lib.plm_kv_read(0, c, f, 3, width, first, f, 2, most, k, f, None)
+    def read(**more):
+        call = dict(dtype=0, cache=cache(), table=f, table_stride=3, table_width=3, first=f, ends=f, seqs=2, most=4, k=f, v=f)
+        assert set(more) <= set(call)
+        return lib.plm_kv_read(_lib.pack_read(*{**call, **more}.values()), None)
 
-    for bad in (dict(first=None), dict(most=0), dict(width=0), dict(width=4), dict(k=None)):
-        assert read(cache(), **bad) == -1, bad
-    assert read(cache(), k=f + 2) == -2
+    assert lib.plm_kv_read(None, None) == -1
+    for bad in (dict(first=0), dict(ends=0), dict(most=0), dict(seqs=0), dict(table_width=0), dict(table_width=4), dict(k=0)):
+        assert read(**bad) == -1, bad
+    assert read(k=f + 2) == -2
 
 
 @pytest.mark.parametrize("k", [1, 2, 6, 7, 10])
