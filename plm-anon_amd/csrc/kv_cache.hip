@@ -26,7 +26,7 @@ struct AppendArgs {
   const int64_t* positions;
   const float* rope;  // [rope_rows, rotary]: cosines, then sines
   int64_t rope_rows;
-  int heads, rotary, side_by_side, page_slots, kv_blocks, q_blocks;
+  int heads, rotary, side_by_side, page_slots, parts, kv_blocks, q_blocks;
 };
 
 // Dimensions [e0, e0 + 8) of a row, as fp32, turned. `turn` is the position's row of the rotation table,
@@ -99,52 +99,117 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
   return o;
 }
 
+// Eight pairs, partners in `lo` and `hi`, turned.
 template <int DT>
+__device__ __forceinline__ void turned8(u32x4 lo, u32x4 hi, const float (&c)[8], const float (&s)[8], float* x, float* y) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float p = from_bits16<DT>(static_cast<uint16_t>(lo[k / 2] >> (16 * (k & 1))));
+    const float q = from_bits16<DT>(static_cast<uint16_t>(hi[k / 2] >> (16 * (k & 1))));
+    x[k] = fmaf(p, c[k], -(q * s[k]));
+    y[k] = fmaf(q, c[k], p * s[k]);
+  }
+}
+
+// Queries: a thread has one place of a row, and `take` heads of it: the cosines and sines, four times a query's bytes,
+// are then read once for all of them. Where a half is whole groups of 8, a place is both partners' groups.
+template <int DT, int TAKE>
 __device__ __forceinline__ void append_queries(const AppendArgs& a, int block) {
   const int b = block / a.q_blocks;
   const KvSeq seq = kv_seq(a.rows, b, a.cache.page_shift);
-  const int per_head = a.cache.dim >> 3, per_row = per_head * a.heads;
-  const int64_t at = static_cast<int64_t>(block - b * a.q_blocks) * blockDim.x + threadIdx.x;
-  const int i = static_cast<int>(at / per_row);
+  const int dim = a.cache.dim, rotary = a.rope != nullptr ? a.rotary : 0, half = rotary >> 1;
+  const bool paired = rotary > 0 && !a.side_by_side && (half & 7) == 0;
+  const int places = paired ? (dim - half) >> 3 : dim >> 3, per_row = places * ((a.heads + TAKE - 1) / TAKE);
+  const int at = (block - b * a.q_blocks) * 256 + static_cast<int>(threadIdx.x), i = at / per_row;
   if (i >= seq.rows) return;
-  const int rest = static_cast<int>(at - static_cast<int64_t>(i) * per_row);
-  const int head = rest / per_head, e0 = (rest - head * per_head) << 3;
+  const int rest = at - i * per_row, part = rest / places, place = rest - part * places;
   const int64_t row = seq.start + i;
   bool none;
   const float* turn = turn_of(a, static_cast<int>(row), seq.context + i, none);
-  float x[8];
-  rotated8<DT>(a.q + row * a.q_row + head * a.q_head, e0, turn, none ? 0 : a.rotary, a.side_by_side != 0, x);
-  *reinterpret_cast<u32x4*>(a.q_out + (row * a.heads + head) * a.cache.dim + e0) = pack8<DT>(x);
+  const uint16_t* from = a.q + row * a.q_row;
+  uint16_t* to = a.q_out + row * a.heads * dim;
+  const int head0 = part * TAKE;
+  if (paired && place < (half >> 3) && turn != nullptr) {
+    const int e = place << 3;
+    u32x4 lo[TAKE], hi[TAKE];
+#pragma unroll
+    for (int h = 0; h < TAKE; ++h) {
+      const uint16_t* x = from + min(head0 + h, a.heads - 1) * a.q_head + e;
+      lo[h] = *reinterpret_cast<const u32x4*>(x);
+      hi[h] = *reinterpret_cast<const u32x4*>(x + half);
+    }
+    float c[8], s[8];
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      *reinterpret_cast<f32x4*>(c + k) = *reinterpret_cast<const f32x4*>(turn + e + k);
+      *reinterpret_cast<f32x4*>(s + k) = *reinterpret_cast<const f32x4*>(turn + half + e + k);
+    }
+#pragma unroll
+    for (int h = 0; h < TAKE; ++h) {
+      if (head0 + h >= a.heads) continue;
+      float x[8], y[8];
+      turned8<DT>(lo[h], hi[h], c, s, x, y);
+      uint16_t* out = to + (head0 + h) * dim + e;
+      *reinterpret_cast<u32x4*>(out) = pack8<DT>(x);
+      *reinterpret_cast<u32x4*>(out + half) = pack8<DT>(y);
+    }
+    return;
+  }
+  // Everything else eight dimensions at a time: pairs side by side, halves of other sizes, what is not turned.
+  const bool both = paired && place < (half >> 3);  // a position that the table does not hold
+#pragma unroll 1
+  for (int h = head0; h < min(head0 + TAKE, a.heads); ++h)
+#pragma unroll 1
+    for (int k = 0; k < (both ? 2 : 1); ++k) {
+      const int e = paired && !both ? (place << 3) + half : (place << 3) + k * half;
+      float x[8];
+      rotated8<DT>(from + h * a.q_head, e, turn, rotary, a.side_by_side != 0, x);
+      *reinterpret_cast<u32x4*>(to + h * dim + e) = pack8<DT>(x);
+    }
 }
 
-// 16 fp32 values of unit x of the workgroup's page: for keys 16 dimensions of one token, for values 4
-// dimensions (i / 4) of 4 tokens (i % 4); zero where a token is not new.
+// A thread's 16 values of the workgroup's page. Values: 4 dimensions (i / 4, from e[0]) of 4 tokens (i % 4), one 16-byte
+// word in 8 bits and two, 1 KiB apart, in 16. Keys: dimensions [e[0], e[0] + 8) and [e[1], e[1] + 8) of one token, the
+// second maybe past the head's end; where halves are whole groups of 8 the two are partners, so that each is read once
+// and the cosines and sines serve both.
 struct PageUnit {
-  int token, e;    // first token in the page, first dimension
-  int64_t offset;  // bytes from the (page, head)'s start to its 16 (e4m3) or first 16 (16-bit) bytes
+  int token;     // the first token, in the page
+  int e[2];
+  int64_t at[2]; // bytes from the (page, head)'s start
 };
 
+__device__ __forceinline__ bool paired_halves(const AppendArgs& a) {
+  return a.rope != nullptr && !a.side_by_side && (a.rotary & 15) == 0;
+}
+
 template <bool VALUES, bool E8>
-__device__ __forceinline__ PageUnit page_unit(const KvCache& c, int x) {
+__device__ __forceinline__ PageUnit page_unit(const AppendArgs& a, int x) {
+  const KvCache& c = a.cache;
   PageUnit p;
   constexpr int bytes = E8 ? 1024 : 2048;  // of a unit of 16 tokens x 64 dimensions
   if constexpr (VALUES) {
     const int per = c.dim >> 2;
-    p.token = (x / per) << 2;
-    p.e = (x % per) << 2;
-    p.offset = (static_cast<int64_t>(p.token >> 4) * c.chunks + (p.e >> 6)) * bytes +
-               ((p.token & 15) >> 2) * 256 + ((p.e & 63) >> 2) * 16;
+    p.token = x / per;
+    p.e[0] = p.e[1] = (x - p.token * per) << 2;
+    p.token <<= 2;
+    p.at[0] = p.at[1] = ((p.token >> 4) * c.chunks + (p.e[0] >> 6)) * bytes + ((p.token & 15) >> 2) * 256 + ((p.e[0] & 63) >> 2) * 16;
   } else {
-    const int groups = (c.dim + 15) >> 4;
-    const int y = x >> 4;
-    p.token = (x & 15) + ((y / groups) << 4);
-    p.e = (y % groups) << 4;
-    p.offset = (static_cast<int64_t>(p.token >> 4) * c.chunks + (p.e >> 6)) * bytes + ((p.e & 63) >> 4) * 256 +
-               (p.token & 15) * 16;
+    const int per = (c.dim + 15) >> 4;
+    p.token = x / per;
+    const int place = x - p.token * per, pairs = paired_halves(a) ? a.rotary >> 4 : 0;
+    p.e[0] = place < pairs ? place << 3 : place << 4;
+    p.e[1] = place < pairs ? p.e[0] + (a.rotary >> 1) : p.e[0] + 8;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = p.e[k];
+      p.at[k] = ((p.token >> 4) * c.chunks + (e >> 6)) * bytes + ((e & 63) >> 4) * 256 + (p.token & 15) * 16 +
+                (E8 ? e & 8 : (e & 8) * 128);
+    }
   }
   return p;
 }
 
+// The unit's new values in fp32, zero where a token is not new.
 template <int DT, bool VALUES>
 __device__ __forceinline__ void new_values(const AppendArgs& a, const KvSeq& seq, const PageUnit& p, int base, int head,
                                            float (&x)[16]) {
@@ -157,28 +222,38 @@ __device__ __forceinline__ void new_values(const AppendArgs& a, const KvSeq& seq
       const int slot = base + p.token + n;
       if (slot >= seq.context && slot < end) {
         const int64_t row = seq.start + (slot - seq.context);
-        const u32x2 w = *reinterpret_cast<const u32x2*>(a.new_v + row * a.v_row + head * a.v_head + p.e);
+        const u32x2 w = *reinterpret_cast<const u32x2*>(a.new_v + row * a.v_row + head * a.v_head + p.e[0]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[4 * j + n] = from_bits16<DT>(static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1))));
       }
     }
   } else {
     const int slot = base + p.token;
-    if (slot >= seq.context && slot < end) {
-      const int row = seq.start + (slot - seq.context);
-      bool none;
-      const float* turn = turn_of(a, row, slot, none);
-      const uint16_t* from = a.new_k + static_cast<int64_t>(row) * a.k_row + head * a.k_head;
-      float half[8];
-      rotated8<DT>(from, p.e, turn, none ? 0 : a.rotary, a.side_by_side != 0, half);
+    if (slot < seq.context || slot >= end) return;
+    const int row = seq.start + (slot - seq.context);
+    bool none;
+    const float* turn = turn_of(a, row, slot, none);
+    const uint16_t* from = a.new_k + static_cast<int64_t>(row) * a.k_row + head * a.k_head;
+    const int rotary = none ? 0 : a.rotary;
+    if (turn != nullptr && paired_halves(a) && p.e[0] < (rotary >> 1)) {
+      const u32x4 lo = *reinterpret_cast<const u32x4*>(from + p.e[0]), hi = *reinterpret_cast<const u32x4*>(from + p.e[1]);
+      float c[8], s[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = half[i];
-      if (p.e + 8 < a.cache.dim) {
-        rotated8<DT>(from, p.e + 8, turn, none ? 0 : a.rotary, a.side_by_side != 0, half);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[8 + i] = half[i];
+      for (int k = 0; k < 8; k += 4) {
+        *reinterpret_cast<f32x4*>(c + k) = *reinterpret_cast<const f32x4*>(turn + p.e[0] + k);
+        *reinterpret_cast<f32x4*>(s + k) = *reinterpret_cast<const f32x4*>(turn + p.e[1] + k);
       }
+      turned8<DT>(lo, hi, c, s, x, x + 8);
+      return;
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (p.e[k] < a.cache.dim) {
+        float half[8];
+        rotated8<DT>(from, p.e[k], turn, rotary, a.side_by_side != 0, half);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[8 * k + i] = half[i];
+      }
   }
 }
 
@@ -189,13 +264,15 @@ __device__ __forceinline__ void append_page_fp8(const AppendArgs& a, const KvSeq
   const KvCache& c = a.cache;
   const int count = VALUES ? (c.page >> 2) * (c.dim >> 2) : c.page * ((c.dim + 15) >> 4);
   const int end = seq.context + seq.rows;
+  float* held = (VALUES ? c.v_scale : c.k_scale) + id * c.heads + head;
+  const bool stays = base < seq.context;  // the page holds rows from before
+  const float before = stays ? *held : 0.0f;
   float x[UPT][16];
   PageUnit p[UPT];
   float amax = 0.0f;
 #pragma unroll
   for (int u = 0; u < UPT; ++u) {
-    const int at = threadIdx.x + u * 256;
-    p[u] = page_unit<VALUES, true>(c, min(at, count - 1));
+    p[u] = page_unit<VALUES, true>(a, min(static_cast<int>(threadIdx.x) + u * 256, count - 1));
     new_values<DT, VALUES>(a, seq, p[u], base, head, x[u]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -203,9 +280,6 @@ __device__ __forceinline__ void append_page_fp8(const AppendArgs& a, const KvSeq
       amax = m < __builtin_inff() ? fmaxf(amax, m) : amax;  // what is not finite has no part in the scale
     }
   }
-  float* held = (VALUES ? c.v_scale : c.k_scale) + id * c.heads + head;
-  const bool stays = base < seq.context;  // the page holds rows from before
-  const float before = stays ? *held : 0.0f;
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
@@ -219,82 +293,104 @@ __device__ __forceinline__ void append_page_fp8(const AppendArgs& a, const KvSeq
   char* page = (VALUES ? c.v : c.k) + (id * c.heads + head) * (static_cast<int64_t>(c.page) * c.chunks * 64);
 #pragma unroll
   for (int u = 0; u < UPT; ++u) {
-    const int at = threadIdx.x + u * 256;
-    if (at >= count) continue;
+    if (static_cast<int>(threadIdx.x) + u * 256 >= count) continue;
     const int first = base + p[u].token, last = first + (VALUES ? 4 : 1);  // slots [first, last)
     const bool any_new = last > seq.context && first < end, any_old = first < seq.context;
     if (!any_new && !(again && any_old)) continue;
-    u32x4* to = reinterpret_cast<u32x4*>(page + p[u].offset);
-    const u32x4 old = any_old ? *to : u32x4{0u, 0u, 0u, 0u};
-    u32x4 word;
+    if constexpr (VALUES) {
+      u32x4* to = reinterpret_cast<u32x4*>(page + p[u].at[0]);
+      const u32x4 old = any_old ? *to : u32x4{0u, 0u, 0u, 0u};
+      u32x4 word;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float y[4];
+      for (int j = 0; j < 4; ++j) {
+        float y[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float rounded = fp8_value(old[j], n) * ratio;
-        y[n] = (VALUES ? first + n : first) < seq.context ? rounded : x[u][4 * j + n] * inverse;
+        for (int n = 0; n < 4; ++n)
+          y[n] = first + n < seq.context ? fp8_value(old[j], n) * ratio : x[u][4 * j + n] * inverse;
+        word[j] = fp8_word(y[0], y[1], y[2], y[3]);
       }
-      word[j] = fp8_word(y[0], y[1], y[2], y[3]);
+      *to = word;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        // The last 16 dimensions' second 8 may be padding: written, as zeros.
+        u32x2* to = reinterpret_cast<u32x2*>(page + p[u].at[k]);
+        const u32x2 old = any_old ? *to : u32x2{0u, 0u};
+        u32x2 word;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float y[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) y[n] = any_old ? fp8_value(old[j], n) * ratio : x[u][8 * k + 4 * j + n] * inverse;
+          word[j] = fp8_word(y[0], y[1], y[2], y[3]);
+        }
+        *to = word;
+      }
     }
-    *to = word;
   }
   if (threadIdx.x == 0) *held = scale;
 }
 
 template <int DT, bool VALUES>
-__device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq& seq, int64_t id, int base, int head) {
+__device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq& seq, int64_t id, int base, int head,
+                                               int part) {
   const KvCache& c = a.cache;
   const int count = VALUES ? (c.page >> 2) * (c.dim >> 2) : c.page * ((c.dim + 15) >> 4);
   const int end = seq.context + seq.rows;
   char* page = (VALUES ? c.v : c.k) + (id * c.heads + head) * (static_cast<int64_t>(c.page) * c.chunks * 128);
-  for (int at = threadIdx.x; at < count; at += 256) {
-    const PageUnit p = page_unit<VALUES, false>(c, at);
-    const int first = base + p.token, last = first + (VALUES ? 4 : 1);
-    if (last <= seq.context || first >= end) continue;
-    float x[16];
-    new_values<DT, VALUES>(a, seq, p, base, head, x);
-    u32x4* to = reinterpret_cast<u32x4*>(page + p.offset);  // the second 16 bytes lie 1 KiB on
+  const int at = part * 256 + static_cast<int>(threadIdx.x);
+  if (at >= count) return;
+  const PageUnit p = page_unit<VALUES, false>(a, at);
+  const int first = base + p.token, last = first + (VALUES ? 4 : 1);
+  if (last <= seq.context || first >= end) return;
+  float x[16];
+  new_values<DT, VALUES>(a, seq, p, base, head, x);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float y[8];
+  for (int h = 0; h < 2; ++h) {
+    u32x4* to = reinterpret_cast<u32x4*>(page + p.at[h] + (VALUES ? h * 1024 : 0));
+    float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[8 * h + i];
-      u32x4 word = pack8<DT>(y);
-      if constexpr (VALUES) {
-        if (first < seq.context) {  // tokens from before share the word: lanes n of both dimensions
-          const u32x4 old = to[64 * h];
+    for (int i = 0; i < 8; ++i) y[i] = x[8 * h + i];
+    u32x4 word = pack8<DT>(y);
+    if constexpr (VALUES) {
+      if (first < seq.context) {  // tokens from before share the word: lanes n of both dimensions
+        const u32x4 old = *to;
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-            if (first + n < seq.context) {
-              const uint32_t keep = 0xffffu << (16 * (n & 1));
-              word[n / 2] = (word[n / 2] & ~keep) | (old[n / 2] & keep);
-              word[2 + n / 2] = (word[2 + n / 2] & ~keep) | (old[2 + n / 2] & keep);
-            }
-        }
-      } else if (p.e + 8 * h >= c.dim) {
-        continue;
+        for (int n = 0; n < 4; ++n)
+          if (first + n < seq.context) {
+            const uint32_t keep = 0xffffu << (16 * (n & 1));
+            word[n / 2] = (word[n / 2] & ~keep) | (old[n / 2] & keep);
+            word[2 + n / 2] = (word[2 + n / 2] & ~keep) | (old[2 + n / 2] & keep);
+          }
       }
-      to[64 * h] = word;
+    } else if (p.e[h] >= c.dim) {
+      continue;
     }
+    *to = word;
   }
 }
 
-template <int DT, bool E8, int UPT>
+// A workgroup has a page of one head's keys or values (8 bits), 256 units of it (16 bits), or 256 places of queries.
+template <int DT, bool E8, int UPT, int TAKE>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ float red[4];
   int block = blockIdx.x;
   if (block >= a.kv_blocks) {
-    append_queries<DT>(a, block - a.kv_blocks);
+    append_queries<DT, TAKE>(a, block - a.kv_blocks);
     return;
   }
   const bool values = block & 1;
   block >>= 1;
+  int part = 0;
+  if constexpr (!E8) {
+    part = block % a.parts;
+    block /= a.parts;
+  }
   const int head = block % a.cache.heads;
   block /= a.cache.heads;
   const int b = block / a.page_slots;
   const KvSeq seq = kv_seq(a.rows, b, a.cache.page_shift);
-  const int number = (seq.context >> a.cache.page_shift) + block % a.page_slots;
+  const int number = (seq.context >> a.cache.page_shift) + block - b * a.page_slots;
   const int base = number << a.cache.page_shift;
   if (seq.rows == 0 || number >= a.rows.width || base >= seq.context + seq.rows) return;
   const int64_t id = a.rows.table[b * a.rows.table_stride + number];
@@ -303,8 +399,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     if (values) append_page_fp8<DT, true, UPT>(a, seq, id, base, head, red);
     else append_page_fp8<DT, false, UPT>(a, seq, id, base, head, red);
   } else {
-    if (values) append_page_16<DT, true>(a, seq, id, base, head);
-    else append_page_16<DT, false>(a, seq, id, base, head);
+    if (values) append_page_16<DT, true>(a, seq, id, base, head, part);
+    else append_page_16<DT, false>(a, seq, id, base, head, part);
   }
 }
 
@@ -316,38 +412,47 @@ struct ReadArgs {
   uint16_t* k;  // [seqs, most, heads, dim]
   uint16_t* v;
   int64_t table_stride;
-  int width, seqs, most, blocks;  // blocks per (sequence, keys or values)
+  int width, seqs, most, key_blocks, value_blocks;
 };
 
-// Thread: keys, 8 dimensions of one token; values, 4 dimensions of the 4 tokens that share their words.
+// Thread: keys, 8 dimensions of one token; values, 8 dimensions of the 4 tokens that share their words.
 template <int DT, bool E8>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const KvCache& c = a.cache;
-  int block = blockIdx.x;
-  const int within = block % a.blocks;
-  block /= a.blocks;
-  const bool values = block & 1;
-  const int b = block >> 1;
+  const bool values = static_cast<int>(blockIdx.x) >= a.key_blocks;
+  const int blocks = values ? a.value_blocks : a.key_blocks, block = static_cast<int>(blockIdx.x) - (values ? a.key_blocks : 0);
+  const int each = blocks / a.seqs, b = block / each;
   const int64_t most_tokens = static_cast<int64_t>(a.width) << c.page_shift;
   const int64_t first = a.first[b], end = min(a.ends[b], most_tokens);
-  const int64_t x = static_cast<int64_t>(within) * 256 + threadIdx.x;
+  const int x = (block - b * each) * 256 + static_cast<int>(threadIdx.x);
   constexpr int bytes = E8 ? 1024 : 2048;
   const int64_t head_bytes = static_cast<int64_t>(c.page >> 4) * c.chunks * bytes;
+  const int per_head = c.dim >> 3, per = per_head * c.heads;
+  // Item: a token (keys) or the quad of tokens from the one that holds `first` (values). Keys go by blocks of 8 tokens x 8
+  // places, whose 16-byte pieces lie side by side both in the cache (over tokens) and in the result (over places).
+  int item, rest;
+  if (values) {
+    item = x / per;
+    rest = x - item * per;
+  } else {
+    const int wide = (per + 7) >> 3, block8 = x >> 6, tokens8 = block8 / wide;
+    item = (tokens8 << 3) + ((x >> 3) & 7);
+    rest = ((block8 - tokens8 * wide) << 3) + (x & 7);
+    if (rest >= per) return;
+  }
+  const int head = rest / per_head, e = (rest - head * per_head) << 3;
+  const int64_t row = static_cast<int64_t>(c.heads) * c.dim;  // elements from a token to the next
+  const int64_t out0 = static_cast<int64_t>(b) * a.most * row + head * c.dim + e;
   if (!values) {
-    const int per_head = c.dim >> 3, per = per_head * c.heads;
-    const int64_t i = x / per;
-    if (i >= a.most) return;
-    const int rest = static_cast<int>(x - i * per);
-    const int head = rest / per_head, e = (rest - head * per_head) << 3;
-    const int64_t t = first + i;
+    if (item >= a.most) return;
+    const int64_t t = first + item;
     u32x4 out = u32x4{0u, 0u, 0u, 0u};
     if (t >= 0 && t < end) {
       const int64_t id = a.table[b * a.table_stride + (t >> c.page_shift)];
       if (id >= 0 && id < c.pages) {
         const int n = static_cast<int>(t & (c.page - 1));
-        const char* from = c.k + (id * c.heads + head) * head_bytes +
-                           (static_cast<int64_t>(n >> 4) * c.chunks + (e >> 6)) * bytes + ((e & 63) >> 4) * 256 +
-                           (n & 15) * 16;
+        const char* from = c.k + (id * c.heads + head) * head_bytes + ((n >> 4) * c.chunks + (e >> 6)) * bytes +
+                           ((e & 63) >> 4) * 256 + (n & 15) * 16;
         if constexpr (E8) {
           const u32x2 w = *reinterpret_cast<const u32x2*>(from + (e & 8));
           const float scale = c.k_scale[id * c.heads + head];
@@ -360,59 +465,67 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
         }
       }
     }
-    *reinterpret_cast<u32x4*>(a.k + ((static_cast<int64_t>(b) * a.most + i) * c.heads + head) * c.dim + e) = out;
+    *reinterpret_cast<u32x4*>(a.k + out0 + item * row) = out;
     return;
   }
-  const int per_head = c.dim >> 2, per = per_head * c.heads;
-  const int64_t quad = x / per;  // the quad of tokens, from the one that holds `first`
-  const int rest = static_cast<int>(x - quad * per);
-  const int head = rest / per_head, e = (rest - head * per_head) << 2;
-  const int64_t t0 = ((first >> 2) + quad) << 2;
+  const int64_t t0 = ((first >> 2) + item) << 2;
   if (t0 - first >= a.most) return;
-  u32x4 w[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+  u32x4 w[2][E8 ? 1 : 2];  // of dimensions e .. e + 3 and e + 4 .. e + 7
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int h = 0; h < (E8 ? 1 : 2); ++h) w[q][h] = u32x4{0u, 0u, 0u, 0u};
   float scale = 1.0f;
   if (t0 >= 0 && t0 < end) {
     const int64_t id = a.table[b * a.table_stride + (t0 >> c.page_shift)];
     if (id >= 0 && id < c.pages) {
       const int n = static_cast<int>(t0 & (c.page - 1));
-      const char* from = c.v + (id * c.heads + head) * head_bytes +
-                         (static_cast<int64_t>(n >> 4) * c.chunks + (e >> 6)) * bytes + ((n & 15) >> 2) * 256 +
-                         ((e & 63) >> 2) * 16;
-      w[0] = *reinterpret_cast<const u32x4*>(from);
+      const char* from = c.v + (id * c.heads + head) * head_bytes + ((n >> 4) * c.chunks + (e >> 6)) * bytes +
+                         ((n & 15) >> 2) * 256 + ((e & 63) >> 2) * 16;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int h = 0; h < (E8 ? 1 : 2); ++h) w[q][h] = *reinterpret_cast<const u32x4*>(from + q * 16 + h * 1024);
       if constexpr (E8) scale = c.v_scale[id * c.heads + head];
-      else w[1] = *reinterpret_cast<const u32x4*>(from + 1024);
     }
   }
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
     const int64_t i = t0 + n - first;
     if (i < 0 || i >= a.most) continue;
-    u32x2 out = u32x2{0u, 0u};
+    u32x4 out = u32x4{0u, 0u, 0u, 0u};
     if (t0 + n < end) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
+        const int k = j & 3;
         uint32_t half;
-        if constexpr (E8) half = to_bits16<DT>(fp8_value(w[0][j], n) * scale);
-        else half = (w[j / 2][2 * (j & 1) + n / 2] >> (16 * (n & 1))) & 0xffffu;
+        if constexpr (E8) half = to_bits16<DT>(fp8_value(w[j / 4][0][k], n) * scale);
+        else half = (w[j / 4][k / 2][2 * (k & 1) + n / 2] >> (16 * (n & 1))) & 0xffffu;
         out[j / 2] |= half << (16 * (j & 1));
       }
     }
-    *reinterpret_cast<u32x2*>(a.v + ((static_cast<int64_t>(b) * a.most + i) * c.heads + head) * c.dim + e) = out;
+    *reinterpret_cast<u32x4*>(a.v + out0 + i * row) = out;
   }
 }
 
 namespace {
 
+template <int DT, bool E8, int UPT>
+void append_take(const AppendArgs& a, int take, unsigned grid, hipStream_t s) {
+  if (take == 4) append_kernel<DT, E8, UPT, 4><<<grid, 256, 0, s>>>(a);
+  else append_kernel<DT, E8, UPT, 1><<<grid, 256, 0, s>>>(a);
+}
+
 template <int DT, bool E8>
-void append_go(const AppendArgs& a, unsigned grid, hipStream_t s) {
+void append_go(const AppendArgs& a, int take, unsigned grid, hipStream_t s) {
   const int units = a.cache.page * ((a.cache.dim + 15) / 16);
   if constexpr (!E8) {
-    append_kernel<DT, false, 1><<<grid, 256, 0, s>>>(a);
+    append_take<DT, false, 1>(a, take, grid, s);
   } else {
-    if (units <= 256) append_kernel<DT, true, 1><<<grid, 256, 0, s>>>(a);
-    else if (units <= 512) append_kernel<DT, true, 2><<<grid, 256, 0, s>>>(a);
-    else if (units <= 1024) append_kernel<DT, true, 4><<<grid, 256, 0, s>>>(a);
-    else append_kernel<DT, true, 8><<<grid, 256, 0, s>>>(a);
+    if (units <= 256) append_take<DT, true, 1>(a, take, grid, s);
+    else if (units <= 512) append_take<DT, true, 2>(a, take, grid, s);
+    else if (units <= 1024) append_take<DT, true, 4>(a, take, grid, s);
+    else append_take<DT, true, 8>(a, take, grid, s);
   }
 }
 
@@ -448,16 +561,22 @@ int plm_kv_append(const plm_append_call* call, void* stream) {
   a.side_by_side = h.side_by_side != 0;
   const int64_t page = a.cache.page, seqs = h.rows.seqs, max_rows = h.rows.max_rows;
   a.page_slots = static_cast<int>((page - 1 + max_rows + page - 1) / page);
-  const int64_t kv_blocks = seqs * a.page_slots * a.cache.heads * 2;
-  const int64_t q_blocks = h.q == nullptr ? 0 : (max_rows * h.heads * (a.cache.dim / 8) + 255) / 256;
-  if (kv_blocks + q_blocks * seqs >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
+  const bool e8 = h.cache->type == PLM_CACHE_E4M3;
+  a.parts = e8 ? 1 : (a.cache.page * ((a.cache.dim + 15) / 16) + 255) / 256;
+  const int64_t kv_blocks = seqs * a.page_slots * a.cache.heads * a.parts * 2;
+  // Four heads per thread once that leaves a few wavefronts for every SIMD; below, latency is all there is.
+  const int take = h.heads >= 4 && h.rows.total * h.heads * (a.cache.dim / 8) >= (1 << 19) ? 4 : 1;
+  const int half = h.rope != nullptr ? a.rotary / 2 : 0;
+  const int64_t places = half > 0 && !a.side_by_side && half % 8 == 0 ? (a.cache.dim - half) / 8 : a.cache.dim / 8;
+  const int64_t q_items = h.q == nullptr ? 0 : max_rows * places * ((h.heads + take - 1) / take);
+  const int64_t q_blocks = (q_items + 255) / 256;
+  if (kv_blocks + q_blocks * seqs >= (int64_t{1} << 31) || q_items >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   a.kv_blocks = static_cast<int>(kv_blocks);
   a.q_blocks = static_cast<int>(q_blocks);
   const unsigned grid = static_cast<unsigned>(kv_blocks + q_blocks * seqs);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool e8 = h.cache->type == PLM_CACHE_E4M3;
-  if (h.dtype == PLM_BF16) e8 ? plm::append_go<plm::DT_BF16, true>(a, grid, s) : plm::append_go<plm::DT_BF16, false>(a, grid, s);
-  else e8 ? plm::append_go<plm::DT_F16, true>(a, grid, s) : plm::append_go<plm::DT_F16, false>(a, grid, s);
+  if (h.dtype == PLM_BF16) e8 ? plm::append_go<plm::DT_BF16, true>(a, take, grid, s) : plm::append_go<plm::DT_BF16, false>(a, take, grid, s);
+  else e8 ? plm::append_go<plm::DT_F16, true>(a, take, grid, s) : plm::append_go<plm::DT_F16, false>(a, take, grid, s);
   return hipGetLastError() == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 
@@ -483,14 +602,13 @@ int plm_kv_read(const plm_read_call* call, void* stream) {
   a.width = static_cast<int>(h.table_width);
   a.seqs = static_cast<int>(h.seqs);
   a.most = static_cast<int>(h.most);
-  // Keys: an item per token and 8 dimensions; values: per quad of tokens (one more where `first` is
-  // inside a quad) and 4 dimensions, never more items than keys have but for that quad.
-  const int64_t key_items = h.most * a.cache.heads * (a.cache.dim / 8);
-  const int64_t value_items = ((h.most + 3) / 4 + 1) * a.cache.heads * (a.cache.dim / 4);
-  const int64_t blocks = ((key_items > value_items ? key_items : value_items) + 255) / 256;
-  if (blocks * h.seqs * 2 >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
-  a.blocks = static_cast<int>(blocks);
-  const unsigned grid = static_cast<unsigned>(blocks * h.seqs * 2);
+  // Keys: an item per token and 8 dimensions; values: per quad of tokens (one more where `first` is inside a quad).
+  const int64_t per = static_cast<int64_t>(a.cache.heads) * (a.cache.dim / 8);
+  const int64_t keys = ((h.most + 7) / 8 * ((per + 7) / 8) * 64 + 255) / 256, quads = (((h.most + 3) / 4 + 1) * per + 255) / 256;
+  if (keys >= (int64_t{1} << 23) || (keys + quads) * h.seqs >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
+  a.key_blocks = static_cast<int>(keys * h.seqs);
+  a.value_blocks = static_cast<int>(quads * h.seqs);
+  const unsigned grid = static_cast<unsigned>((keys + quads) * h.seqs);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool e8 = h.cache->type == PLM_CACHE_E4M3;
   if (h.dtype == PLM_BF16) {
