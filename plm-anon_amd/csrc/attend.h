@@ -35,6 +35,7 @@ struct AttendArgs {
   int target;   // workgroups that the work is split over, at most; 0: never split
   float per_target;  // a little more than 1 / target
   int least;    // steps of a range, at least
+  int whole;    // a group of so many steps is not cut
 };
 
 constexpr int kStep = 32;        // tokens of a step
@@ -57,12 +58,14 @@ __device__ __forceinline__ AttendShare attend_share(const AttendArgs& a, int b) 
   const KvSeq seq = kv_seq(a.rows, b, a.cache.page_shift);
   if (seq.rows == 0) return s;
   s.tiles = (seq.rows * a.group + COLS - 1) / COLS;
-  // With a window, the first row's place says where it begins: where a later row's place is before it,
-  // the ranges get longer, and that is all.
-  const int64_t place = a.positions != nullptr ? a.positions[seq.start] : seq.context;
   const int hi = (seq.context + seq.rows + kStep - 1) / kStep;
   int lo = 0;
-  if (a.window > 0) lo = static_cast<int>(min(max(place + 1 - a.window, int64_t{0}), static_cast<int64_t>(hi) * kStep)) / kStep;
+  if (a.window > 0) {
+    // The first row's place says where the window begins: where a later row's is before it, the ranges get longer, and
+    // that is all.
+    const int64_t place = a.positions != nullptr ? a.positions[seq.start] : seq.context;
+    lo = static_cast<int>(min(max(place + 1 - a.window, int64_t{0}), static_cast<int64_t>(hi) * kStep)) / kStep;
+  }
   s.steps = hi - lo + min((a.sinks + kStep - 1) / kStep, lo);
   return s;
 }
@@ -123,7 +126,7 @@ __device__ __forceinline__ AttendItem attend_item(const AttendArgs& a, int index
   int items = 0, slots = 0;
   for (int base = 0; base < a.rows.seqs; base += 64) {
     const AttendShare s = base == 0 ? own : attend_share<COLS>(a, base + lane);
-    const int ranges = min(max((s.steps + chunk - 1) / chunk, 1), kAttendMost);
+    const int ranges = s.steps <= a.whole ? 1 : min(max((s.steps + chunk - 1) / chunk, 1), kAttendMost);
     const int split = ranges > 1 ? s.tiles * heads : 0;  // groups of several ranges: they alone have slots
     const int mine = JOIN ? split : s.tiles * heads * ranges;
     const int to = wave_scan(mine);

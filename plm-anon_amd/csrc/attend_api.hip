@@ -11,7 +11,7 @@ namespace {
 
 struct AttendPlan {
   int columns;        // of a workgroup's tile
-  int target, least;  // AttendArgs
+  int target, least, whole;  // AttendArgs
   int64_t grid, groups, bytes;
 };
 
@@ -19,16 +19,26 @@ struct AttendPlan {
 // (attend_item), so a wide table costs nothing; `grid` bounds the workgroups that any lengths can ask for:
 // one per group and as many more as the work is cut into.
 AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t heads, int64_t total, int64_t seqs,
-                       int64_t max_rows, int64_t table_width) {
+                       int64_t max_rows, int64_t table_width, int64_t window, int64_t sinks, bool mask) {
   AttendPlan p{};
   const int64_t group = heads / kv_heads, chunks = (head_dim + 63) / 64;
   const int64_t most = max_rows * group;
-  p.columns = most <= 16 ? 16 : chunks > 2 ? 64 : most <= 32 ? 32 : most <= 256 ? 64 : 128;
+  // 128 columns need half the loads and conversions per column, once there are tiles of them for all CUs.
+  const bool many = most > 256 && kv_heads * (total * group / 128) >= 256;
+  p.columns = most <= 16 ? 16 : chunks > 2 ? 64 : most <= 32 ? 32 : many ? 128 : 64;
   p.groups = kv_heads * (seqs + total * group / p.columns);
-  const int64_t capacity = (table_width * page + kStep - 1) / kStep;
+  // Ranges are joined by a second launch and each has a walk's beginning and end: 5 to 8 us that a cut has to win back.
+  // A step of 32 tokens takes a quarter of about 0.8 us (up to 32 columns, a step per wavefront) or half of 1.2 us.
   p.least = p.columns <= 32 ? 16 : 8;
-  // A single sequence's groups are alike: where they fill the device there is nothing to even out.
-  p.target = capacity > p.least && !(seqs == 1 && p.groups >= 256) ? 512 : 0;
+  p.whole = p.columns <= 32 ? 32 : 20;
+  // What a group can be long at most: with a window the rows' own span of it.
+  const int64_t span = mask ? max_rows : std::min(max_rows, p.columns / group + 2);
+  int64_t steps = (table_width * page + kStep - 1) / kStep;
+  if (window > 0) steps = std::min(steps, (std::min(window + sinks, int64_t{1} << 30) + span) / kStep + 3);
+  // Not cut: what is short, a single sequence's groups, which are alike, where they fill the device, and groups that do
+  // and cannot be much unlike.
+  const bool full = p.groups - kv_heads >= 256;
+  p.target = steps > p.whole && !(full && (seqs == 1 || steps <= 4 * p.least)) ? 512 : 0;
   p.grid = p.groups + p.target;
   // There are 2 * target ranges of groups of several at most: a cut sequence has less than twice load / chunk of
   // them, and a chunk is load / target at least. Such a group has two at least.
@@ -50,7 +60,8 @@ bool attend_of(const plm_attend_call* call, AttendArgs& a, AttendPlan& p) {
   if (h.window < 0 || h.sinks < 0 || !(h.scale > 0.0) || !(h.scale < 3.0e38)) return false;
   if (h.mask != nullptr && (h.mask_rows < 1 || h.mask_words < 1 || h.mask_rows >= (1 << 28) || h.mask_words >= (1 << 24)))
     return false;
-  p = attend_plan(heads, a.cache.page, a.cache.dim, h.heads, h.rows.total, h.rows.seqs, h.rows.max_rows, h.rows.table_width);
+  p = attend_plan(heads, a.cache.page, a.cache.dim, h.heads, h.rows.total, h.rows.seqs, h.rows.max_rows, h.rows.table_width,
+                  h.window, h.sinks, h.mask != nullptr);
   return p.grid < (int64_t{1} << 31);
 }
 
@@ -94,6 +105,7 @@ int plm_attend(const plm_attend_call* call, void* workspace, size_t workspace_by
   a.target = p.target;
   a.per_target = p.target > 0 ? 1.001f / static_cast<float>(p.target) : 0.0f;
   a.least = p.least;
+  a.whole = p.whole;
   const unsigned grid = static_cast<unsigned>(p.grid);
   const int32_t dtype = static_cast<int32_t>(h.dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);
