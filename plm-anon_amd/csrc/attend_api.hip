@@ -9,6 +9,8 @@
 namespace plm {
 namespace {
 
+constexpr int64_t kNarrowWork = 24000;  // groups of 16 columns times steps
+
 struct AttendPlan {
   int columns;        // of a workgroup's tile
   int target, least, whole;  // AttendArgs
@@ -23,18 +25,27 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   AttendPlan p{};
   const int64_t group = heads / kv_heads, chunks = (head_dim + 63) / 64;
   const int64_t most = max_rows * group;
-  // 128 columns need half the loads and conversions per column, once there are tiles of them for all CUs.
+  // What a tile of columns sees at most: all the table holds, or with a window the rows' own span of it.
+  const int64_t far = int64_t{1} << 30;
+  const auto seen = [&](int64_t columns) {
+    const int64_t all = (table_width * page + kStep - 1) / kStep, span = mask ? max_rows : std::min(max_rows, columns / group + 2);
+    return window > 0 ? std::min(all, (std::min(window, far) + std::min(sinks, far) + span) / kStep + 3) : all;
+  };
+  // Tiles of 16 columns, whose four wavefronts take different tokens, are done soonest while all of a call's are short of
+  // work for the device; wider ones need less of it. (Rounds of 56 rows over 500 / 4007 / 16000 tokens, 16 heads over 4:
+  // 11 / 21 / 37 us against 19 / 23 / 36; 42 rows over 55237 tokens 54 against 45.) Up to 96 tokens there is nothing to
+  // take apart. 128 columns need half the loads and conversions of 64, once there are tiles of them for all CUs.
+  const int64_t narrow = kv_heads * (seqs + total * group / 16);
   const bool many = most > 256 && kv_heads * (total * group / 128) >= 256;
-  p.columns = most <= 16 ? 16 : chunks > 2 ? 64 : most <= 32 ? 32 : many ? 128 : 64;
+  if (most <= 16 || (seen(16) > 3 && narrow * seen(16) <= kNarrowWork)) p.columns = 16;
+  else if (chunks <= 2 && most <= 32) p.columns = 32;
+  else p.columns = chunks <= 2 && many ? 128 : 64;
   p.groups = kv_heads * (seqs + total * group / p.columns);
   // Ranges are joined by a second launch and each has a walk's beginning and end: 5 to 8 us that a cut has to win back.
   // A step of 32 tokens takes a quarter of about 0.8 us (up to 32 columns, a step per wavefront) or half of 1.2 us.
   p.least = p.columns <= 32 ? 16 : 8;
   p.whole = p.columns <= 32 ? 32 : 20;
-  // What a group can be long at most: with a window the rows' own span of it.
-  const int64_t span = mask ? max_rows : std::min(max_rows, p.columns / group + 2);
-  int64_t steps = (table_width * page + kStep - 1) / kStep;
-  if (window > 0) steps = std::min(steps, (std::min(window + sinks, int64_t{1} << 30) + span) / kStep + 3);
+  const int64_t steps = seen(p.columns);
   // Not cut: what is short, a single sequence's groups, which are alike, where they fill the device, and groups that do
   // and cannot be much unlike.
   const bool full = p.groups - kv_heads >= 256;
