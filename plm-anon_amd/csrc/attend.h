@@ -49,13 +49,14 @@ __host__ __device__ constexpr int64_t attend_slot_floats(int columns, int padded
 // A sequence's share of the work, the same in every workgroup.
 struct AttendShare {
   int tiles, steps;
+  KvSeq seq;
 };
 
 template <int COLS>
 __device__ __forceinline__ AttendShare attend_share(const AttendArgs& a, int b) {
-  AttendShare s{0, 0};
+  AttendShare s{0, 0, {0, 0, 0}};
   if (b >= a.rows.seqs) return s;
-  const KvSeq seq = kv_seq(a.rows, b, a.cache.page_shift);
+  const KvSeq seq = s.seq = kv_seq(a.rows, b, a.cache.page_shift);
   if (seq.rows == 0) return s;
   s.tiles = (seq.rows * a.group + COLS - 1) / COLS;
   const int hi = (seq.context + seq.rows + kStep - 1) / kStep;
@@ -100,6 +101,7 @@ __device__ __forceinline__ float wave_total(float v) {
 struct AttendItem {
   int b, tile, head, range, ranges;  // ranges == 0: nothing to do
   int slot;                          // the group's first partial slot; its ranges' are `heads` slots apart
+  KvSeq seq;
 };
 
 // Which range of which group (sequence, tile, key head) workgroup `index` takes; with JOIN, which group of several
@@ -149,6 +151,7 @@ __device__ __forceinline__ AttendItem attend_item(const AttendArgs& a, int index
         it.tile = tiles - 1 - y;  // a causal tile's work grows with its number: the longest first
       }
       it.slot = slots + of(slot_to) + (it.tile - tiles) * it.ranges * heads + it.head;
+      it.seq = {of(s.seq.start), of(s.seq.rows), of(s.seq.context)};
       return it;
     }
     items += __builtin_amdgcn_readlane(to, 63);
@@ -260,8 +263,11 @@ struct AttendColumns {
       real[n] = x < columns;
       row[n] = y / a.group;
       head[n] = it.head * a.group + y - row[n] * a.group;
-      const int64_t p = a.positions != nullptr ? a.positions[seq.start + row[n]] : seq.context + row[n];
-      window_lo[n] = a.window > 0 ? max(static_cast<int>(min(max(p, static_cast<int64_t>(-far)), static_cast<int64_t>(far))) - a.window + 1, 0) : 0;
+      window_lo[n] = 0;
+      if (a.window > 0) {
+        const int64_t p = a.positions != nullptr ? a.positions[seq.start + row[n]] : seq.context + row[n];
+        window_lo[n] = max(static_cast<int>(min(max(p, static_cast<int64_t>(-far)), static_cast<int64_t>(far))) - a.window + 1, 0);
+      }
     }
   }
 
@@ -550,10 +556,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
   const int g = lane >> 4, col = lane & 15;
   const AttendItem it = attend_item<COLS, false>(a, blockIdx.x, lane);
   if (it.ranges == 0) return;
-  KvSeq seq = kv_seq(a.rows, it.b, a.cache.page_shift);
-  seq.start = __builtin_amdgcn_readfirstlane(seq.start);
-  seq.rows = __builtin_amdgcn_readfirstlane(seq.rows);
-  seq.context = __builtin_amdgcn_readfirstlane(seq.context);
+  const KvSeq& seq = it.seq;
   const int columns = seq.rows * a.group;
 
   using Wave = AttendWave<DT, E8, C, NC>;
@@ -739,62 +742,64 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
     }
   }
 
-  // Every wavefront's result in plain units, then joined by halves through LDS.
+  // The wavefronts' results, in plain units, meet in LDS; each then joins a quarter of the dimensions, register r of its
+  // number (4 consecutive dimensions of 16).
+  static_assert(W == 4, "a wavefront per accumulator register");
+  constexpr int kWaveFloats = NC * (C * 16 + 2) * 64;
+  float* shared = reinterpret_cast<float*>(lds);
+  {
+    float* mine = shared + wave * kWaveFloats + lane * 4;
 #pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    w.l[n] = column_sum(w.l[n]);
-    if constexpr (E8) {
+    for (int n = 0; n < NC; ++n) {
+      const float scale = E8 ? w.ref : 1.0f;
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w.o[n][c][j] *= w.ref;
+        for (int r = 0; r < 4; ++r)
+          *reinterpret_cast<f32x4*>(mine + ((n * C + c) * 4 + r) * 256) =
+              f32x4{w.o[n][c][0][r], w.o[n][c][1][r], w.o[n][c][2][r], w.o[n][c][3][r]} * scale;
+      float* ends = shared + wave * kWaveFloats + NC * C * 1024 + n * 128 + lane;
+      ends[0] = w.m[n];
+      ends[64] = column_sum(w.l[n]);
     }
   }
-  constexpr int kWaveFloats = NC * (C * 16 + 2) * 64;
-  float* shared = reinterpret_cast<float*>(lds);
-  for (int half = W / 2; half > 0; half >>= 1) {
-    if (half != W / 2) __syncthreads();
-    if (wave >= half && wave < 2 * half) {
-      float* to_ = shared + (wave - half) * kWaveFloats + lane;
+  __syncthreads();
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
+  for (int n = 0; n < NC; ++n) {
+    float top = kMinusInf, m[W], sum = 0.0f;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) to_[((n * C + c) * 16 + j * 4 + r) * 64] = w.o[n][c][j][r];
-        to_[(NC * C * 16 + 2 * n) * 64] = w.m[n];
-        to_[(NC * C * 16 + 2 * n + 1) * 64] = w.l[n];
-      }
+    for (int i = 0; i < W; ++i) {
+      m[i] = shared[i * kWaveFloats + NC * C * 1024 + n * 128 + lane];
+      top = fmaxf(top, m[i]);
     }
-    __syncthreads();
-    if (wave < half) {
-      const float* other = shared + wave * kWaveFloats + lane;
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        const float m = other[(NC * C * 16 + 2 * n) * 64], l = other[(NC * C * 16 + 2 * n + 1) * 64];
-        const float top = fmaxf(w.m[n], m);
-        const float x = w.m[n] == top ? 1.0f : __builtin_amdgcn_exp2f(w.m[n] - top);
-        const float y = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-        w.m[n] = top;
-        w.l[n] = w.l[n] * x + l * y;
+    for (int i = 0; i < W; ++i) {
+      m[i] = m[i] == top ? 1.0f : __builtin_amdgcn_exp2f(m[i] - top);
+      sum += m[i] * shared[i * kWaveFloats + NC * C * 1024 + n * 128 + 64 + lane];
+    }
+    if (!cols.real[n]) continue;
+    const bool last = it.ranges == 1;
+    const float inverse = !last ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing is zero
+    constexpr int PAD = 64 * C;
+    float* slot = a.partials + static_cast<int64_t>(it.slot + it.range * a.cache.heads) * attend_slot_floats(COLS, PAD);
+    const int x = 16 * n + col;
+    uint16_t* out = a.out + (static_cast<int64_t>(seq.start + cols.row[n]) * a.heads + cols.head[n]) * a.cache.dim;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              w.o[n][c][j][r] = w.o[n][c][j][r] * x + other[((n * C + c) * 16 + j * 4 + r) * 64] * y;
-      }
+      for (int i = 0; i < W; ++i)
+        o += *reinterpret_cast<const f32x4*>(shared + i * kWaveFloats + ((n * C + c) * 4 + wave) * 256 + lane * 4) * m[i];
+      o *= inverse;
+      const int e = 64 * c + 16 * g + 4 * wave;
+      if (!last) *reinterpret_cast<f32x4*>(slot + x * PAD + e) = o;
+      else if (e < a.cache.dim) *reinterpret_cast<u32x2*>(out + e) = u32x2{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
+    }
+    if (!last && g == 0 && wave == 0) {
+      slot[COLS * PAD + x] = top;
+      slot[COLS * PAD + COLS + x] = sum;
     }
   }
-
-  if (it.ranges == 1) {
-    if (wave == 0) cols.template store<DT, C>(a, seq, g, w.o, w.l);
-    return;
-  }
-  if (wave == 0) attend_publish<NC, C>(a, it, COLS, 0, g, col, cols, w.o, w.m, w.l);
 }
 
 hipError_t attend_bf16_e4m3(const AttendArgs& a, int columns, unsigned grid, hipStream_t s);

@@ -8,21 +8,21 @@
 namespace plm {
 
 template <int DT, int COLS>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int take, int slices) {
-  __shared__ float weight[kAttendMost][kJoinColumns], sums[kAttendMost][kJoinColumns], total[kJoinColumns];
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int take, int slices, int items) {
+  __shared__ float weight[kJoinColumns][kAttendMost], total[kJoinColumns];
   __shared__ f32x4 parts[256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int pad = 64 * a.cache.chunks, dim = a.cache.dim, quads = dim >> 2;
   const int64_t apart = attend_slot_floats(COLS, pad) * a.cache.heads;  // from a range to the next
   // A thread's share: every `lanes`-th range of four dimensions of a column.
   const int work = take * quads, lanes = 256 / work, share = threadIdx.x / work;
   const int c = (threadIdx.x - share * work) / quads, e = (threadIdx.x - share * work - c * quads) << 2;
-  for (int index = blockIdx.x;; index += gridDim.x) {
-    const AttendItem it = attend_item<COLS, true>(a, index / slices, threadIdx.x & 63);
+  for (int index = blockIdx.x; index < items; index += gridDim.x) {
+    const AttendItem it = attend_item<COLS, true>(a, index / slices, lane);
     if (it.ranges < 2) return;
     const int slice = index % slices;
-    const KvSeq seq = kv_seq(a.rows, it.b, a.cache.page_shift);
     const int first = it.tile * COLS + slice * take;  // column of the sequence
-    const int live = min(take, seq.rows * a.group - first);
+    const int live = min(take, it.seq.rows * a.group - first);
     if (live <= 0) continue;
     const float* slot = a.partials + it.slot * attend_slot_floats(COLS, pad);
     // The first eight of the thread's loads go with the maxima's and sums'.
@@ -32,23 +32,18 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int take
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (mine) part[k] = *reinterpret_cast<const f32x4*>(from + min(share + k * lanes, it.ranges - 1) * apart);
-    for (int i = threadIdx.x; i < it.ranges * take; i += 256) {
-      const int range = i / take, x = i - range * take;
-      const float* at = slot + range * apart + COLS * pad + slice * take + x;
-      weight[range][x] = x < live ? at[0] : 0.0f;
-      sums[range][x] = x < live ? at[COLS] : 0.0f;
-    }
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) < take) {
-      const int x = threadIdx.x;
-      float top = -__builtin_inff(), sum = 0.0f;
-      for (int range = 0; range < it.ranges; ++range) top = fmaxf(top, weight[range][x]);
-      for (int range = 0; range < it.ranges; ++range) {
-        const float m = weight[range][x], y = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-        weight[range][x] = y;
-        sum += y * sums[range][x];
-      }
-      total[x] = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing is zero
+    // A wavefront per column, a lane per range.
+    static_assert(kAttendMost == 64, "a lane per range");
+    for (int x = wave; x < live; x += 4) {
+      const float* at = slot + min(lane, it.ranges - 1) * apart + COLS * pad + slice * take + x;
+      const float m = lane < it.ranges ? at[0] : -__builtin_inff(), l = at[COLS];
+      float top = m;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+      const float y = lane >= it.ranges ? 0.0f : m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+      weight[x][lane] = y;
+      const float sum = wave_total(lane < it.ranges ? y * l : 0.0f);
+      if (lane == 0) total[x] = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing is zero
     }
     __syncthreads();
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -61,7 +56,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int take
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (base + k * lanes < it.ranges) sum += part[k] * weight[base + k * lanes][c];
+          if (base + k * lanes < it.ranges) sum += part[k] * weight[c][base + k * lanes];
       }
     }
     parts[threadIdx.x] = sum;
@@ -70,7 +65,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int take
       for (int k = 1; k < lanes; ++k) sum += parts[threadIdx.x + k * work];
       sum *= total[c];
       const int column = first + c, row = column / a.group;
-      uint16_t* at = a.out + (static_cast<int64_t>(seq.start + row) * a.heads + it.head * a.group + column - row * a.group) * dim;
+      uint16_t* at = a.out + (static_cast<int64_t>(it.seq.start + row) * a.heads + it.head * a.group + column - row * a.group) * dim;
       *reinterpret_cast<u32x2*>(at + e) = u32x2{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
     }
     __syncthreads();
@@ -87,9 +82,10 @@ hipError_t join_go(int32_t dtype, const AttendArgs& a, int64_t groups, int colum
   int take = 1;
   while (take < kJoinColumns && 2 * take * quads <= 256 && groups * ((columns + take - 1) / take) > 512) take *= 2;
   const int slices = (columns + take - 1) / take;
-  const unsigned grid = static_cast<unsigned>(groups * slices < 2048 ? groups * slices : 2048);
-  if (dtype == PLM_BF16) attend_join_kernel<DT_BF16, COLS><<<grid, 256, 0, s>>>(a, take, slices);
-  else attend_join_kernel<DT_F16, COLS><<<grid, 256, 0, s>>>(a, take, slices);
+  const int items = static_cast<int>(groups) * slices;
+  const unsigned grid = static_cast<unsigned>(items < 2048 ? items : 2048);
+  if (dtype == PLM_BF16) attend_join_kernel<DT_BF16, COLS><<<grid, 256, 0, s>>>(a, take, slices, items);
+  else attend_join_kernel<DT_F16, COLS><<<grid, 256, 0, s>>>(a, take, slices, items);
   return hipGetLastError();
 }
 

@@ -20,7 +20,7 @@ hipError_t attend_go(Kernel kern, const AttendArgs& a, unsigned grid, unsigned t
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_stream(const AttendArgs& a, unsigned grid, hipStream_t s) {
   constexpr int W = 4;
-  constexpr size_t waves = static_cast<size_t>(W / 2) * NC * (C * 16 + 2) * 64 * 4;
+  constexpr size_t waves = static_cast<size_t>(W) * NC * (C * 16 + 2) * 64 * 4;
   return attend_go(&attend_kernel<DT, E8, C, NC, W>, a, grid, 64 * W, waves, s);
 }
 

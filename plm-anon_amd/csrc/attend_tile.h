@@ -28,10 +28,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const int g = lane >> 4, col = lane & 15;
   const AttendItem it = attend_item<COLS, false>(a, blockIdx.x, lane);
   if (it.ranges == 0) return;
-  KvSeq seq = kv_seq(a.rows, it.b, a.cache.page_shift);
-  seq.start = __builtin_amdgcn_readfirstlane(seq.start);
-  seq.rows = __builtin_amdgcn_readfirstlane(seq.rows);
-  seq.context = __builtin_amdgcn_readfirstlane(seq.context);
+  const KvSeq& seq = it.seq;
   const int columns = seq.rows * a.group;
   const int end = seq.context + seq.rows;
   const int last_page = (end + a.cache.page - 1) >> a.cache.page_shift;
