@@ -34,9 +34,10 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   // Tiles of 16 columns, whose four wavefronts take different tokens, are done soonest while all of a call's are short of
   // work for the device; wider ones need less of it. (Rounds of 56 rows over 500 / 4007 / 16000 tokens, 16 heads over 4:
   // 11 / 21 / 37 us against 19 / 23 / 36; 42 rows over 55237 tokens 54 against 45.) Up to 96 tokens there is nothing to
-  // take apart. 128 columns need half the loads and conversions of 64, once there are tiles of them for all CUs.
+  // take apart. 128 columns need half the loads and conversions of 64, once there are tiles of them for all CUs; short
+  // walks end more evenly in smaller tiles (prompts through a window of 512: 42 against 45 us).
   const int64_t narrow = kv_heads * (seqs + total * group / 16);
-  const bool many = most > 256 && kv_heads * (total * group / 128) >= 256;
+  const bool many = most > 256 && kv_heads * (total * group / 128) >= (seen(128) < 24 ? 2048 : 256);
   if (most <= 16 || (seen(16) > 3 && narrow * seen(16) <= kNarrowWork)) p.columns = 16;
   else if (chunks <= 2 && most <= 32) p.columns = 32;
   else p.columns = chunks <= 2 && many ? 128 : 64;

@@ -26,7 +26,7 @@ hipError_t attend_stream(const AttendArgs& a, unsigned grid, hipStream_t s) {
 
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_tiled(const AttendArgs& a, unsigned grid, hipStream_t s) {
-  constexpr size_t sets = static_cast<size_t>(2) * attend_set_bytes(C);
+  constexpr size_t sets = static_cast<size_t>(attend_sets(C)) * attend_set_bytes(C);
   return attend_go(&attend_tile_kernel<DT, E8, C, NC>, a, grid, 256, sets, s);
 }
 

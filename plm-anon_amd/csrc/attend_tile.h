@@ -16,12 +16,16 @@ namespace plm {
 constexpr int kTile = 64;  // tokens staged at once
 constexpr int kNoLds = 0x1e;  // __builtin_amdgcn_sched_barrier: all but LDS accesses may move across
 constexpr int attend_set_bytes(int chunks) { return 16 * chunks * 1024; }
+// Of longer heads one set: two workgroups fit a CU then, which is worth more than the barrier that it costs (prompts of
+// heads of 256: 365 us with two sets, 240 with one).
+constexpr int attend_sets(int chunks) { return chunks > 2 ? 1 : 2; }
 
 template <int DT, bool E8, int C, int NC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attend_tile_kernel(AttendArgs a) {
   constexpr int COLS = 64 * NC;
   constexpr int kUnitBytes = E8 ? 1024 : 2048, kLoads = E8 ? 1 : 2;
   constexpr int kKeys = 8 * C * 1024, kSet = attend_set_bytes(C);  // bytes of a set: keys, then values
+  constexpr int kSets = attend_sets(C);
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -323,14 +327,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     // The first turn only fetches: one copy of the code, which short walks wait for too.
 #pragma unroll 1
     for (int s = walk.from - 1; s < walk.to; ++s) {
-      const int t0 = st.t0, set = (s - walk.from) & 1;
+      const int t0 = st.t0, set = kSets == 2 ? (s - walk.from) & 1 : 0;
       const float ks[4] = {st.ks[0], st.ks[1], st.ks[2], st.ks[3]};
       const uint32_t held = st.held;
       if (s + 1 < walk.to) fetch(walk.token_of(s + 1));
       if (s >= walk.from) compute(std::false_type{}, lds + set * kSet, t0, ks, held);
       if (s + 1 < walk.to) {
         follow();
-        store(lds + (set ^ 1) * kSet);
+        if constexpr (kSets == 1) __syncthreads();
+        store(lds + (kSets == 2 ? set ^ 1 : 0) * kSet);
       }
       __syncthreads();
     }

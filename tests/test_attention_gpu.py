@@ -120,6 +120,50 @@ def test_causal(device, shape, dtype, kind):
     check(c.attend(), *c.expected())
 
 
+# A table wide enough that the sizes alone speak for much work: the 32-, 64- and 128-column kernels on small inputs,
+# and sequences cut into ranges.
+WIDE = 12000
+WIDE_SHAPES = [
+    ([70, 0, 3], [3, 1, 2], 10, 1, 64, 16),              # 32 columns, in part
+    ([901, 17], [5, 8], 8, 2, 128, 32),                  # 32 columns, two chunks
+    ([130, 5], [21, 40], 8, 2, 64, 16),                  # 64 columns, the last tile in part
+    ([1100], [56], 16, 4, 128, 64),                      # 64 columns, cut
+    ([75, 300], [33, 7], 6, 2, 80, 16),
+    ([200], [30], 4, 2, 192, 128),
+    ([40, 333], [25, 12], 4, 1, 256, 16),                # 64 columns of four chunks, one set in LDS
+    ([90], [520], 64, 1, 16, 64),                        # 128 columns
+    ([600, 10], [1040, 600], 20, 1, 72, 32),             # 128 columns, two chunks, the second in part
+]
+
+
+@pytest.mark.parametrize("dtype, kind", [(BF16, E4M3), (FP16, E4M3), (BF16, BF16), (FP16, FP16)])
+@pytest.mark.parametrize("shape", range(len(WIDE_SHAPES)))
+def test_wide_tables(device, shape, dtype, kind):
+    c = Case(device, *WIDE_SHAPES[shape], dtype=dtype, kind=kind, seed=50 + shape, wider=WIDE)
+    check(c.attend(), *c.expected())
+
+
+@pytest.mark.parametrize("window, sinks", [(16, 4), (100, 40), (777, 19)])
+@pytest.mark.parametrize("dtype, kind", [(BF16, E4M3), (FP16, FP16)])
+def test_window_of_many_columns(device, window, sinks, dtype, kind):
+    """Heads enough that a window's short walks are work for the 64-column (and, through 777, the 128-column) kernel."""
+    c = Case(device, [30], [760], 128, 128, 8, 16, dtype=dtype, kind=kind, seed=window)
+    check(c.attend(window=window, sinks=sinks), *c.expected(window, sinks))
+
+
+@pytest.mark.parametrize("k, heads, kv_heads, dim, dtype, kind", [(6, 20, 20, 80, FP16, E4M3), (7, 16, 4, 128, BF16, E4M3),
+                                                                (10, 8, 1, 64, FP16, FP16), (7, 8, 2, 256, BF16, BF16)])
+@pytest.mark.parametrize("window", [None, 50])
+def test_round_of_many_columns(device, k, heads, kv_heads, dim, dtype, kind, window):
+    rows = k + k * k
+    c = Case(device, [300, 0, 77], [rows] * 3, heads, kv_heads, dim, 32, dtype=dtype, kind=kind, seed=k, wider=WIDE)
+    bits, places = attention.round_mask(k, device=device)
+    see, want = oracle.round_rows(k)
+    at = (torch.tensor(c.contexts)[:, None] + want).flatten()
+    got = c.attend(mask=bits, positions=at.to(device), window=window, sinks=3)
+    check(got, *c.expected(window, 3, see, at))
+
+
 @pytest.mark.parametrize("window, sinks", [(1, 0), (1, 1), (16, 4), (33, 0), (100, 40), (777, 19), (10 ** 12, 5)])
 @pytest.mark.parametrize("kind", [E4M3, BF16])
 def test_window(device, window, sinks, kind):
@@ -139,8 +183,9 @@ def test_round(device, k, heads, kv_heads, dim, window):
     check(got, *c.expected(window, 3, see, at))
 
 
-def test_rows_that_see_nothing_are_zero(device):
-    c = Case(device, [0, 40], [5, 5], 4, 2, 64, 16, seed=3)
+@pytest.mark.parametrize("heads, wider", [(4, 0), (8, WIDE), (32, WIDE)])
+def test_rows_that_see_nothing_are_zero(device, heads, wider):
+    c = Case(device, [0, 40], [5, 5], heads, 2, 64, 16, seed=3, wider=wider)
     bits = torch.tensor([[0], [0b10], [0], [0b11111], [0]], dtype=torch.int32)
     see = torch.tensor([[(int(w) >> j) & 1 for j in range(5)] for w in bits[:, 0]], dtype=torch.bool)
     got = c.attend(mask=bits.to(device))
@@ -154,22 +199,26 @@ def test_rows_that_see_nothing_are_zero(device):
     check(c.attend(window=8, positions=-far), *c.expected(window=8, places=-far.cpu()))
 
 
+@pytest.mark.parametrize("heads, wider", [(4, 0), (1, WIDE), (4, WIDE)])
 @pytest.mark.parametrize("kind", [E4M3, FP16])
-def test_what_is_masked_does_not_reach_the_rows(device, kind):
+def test_what_is_masked_does_not_reach_the_rows(device, kind, heads, wider):
     """NaN and infinities in tokens past the end, outside the window, and ahead of a row in its own tile."""
-    c = Case(device, [70], [20], 4, 1, 64, 32, dtype=FP16, kind=kind, seed=5)
-    want, tol = c.expected(window=30, sinks=1)
+    c = Case(device, [70], [20], heads, 1, 64, 32, dtype=FP16, kind=kind, seed=5, wider=wider)
+    window = None if wider else 30        # 16-column tiles; the wider ones, without a window
+    want, tol = c.expected(window=window, sinks=1)
     bad = {0x7F, 0xFF} if kind == E4M3 else {0x7C00, 0xFC00, 0x7E00}
+    places = [75, 89, 90, 93, 95] if wider else [5, 41, 75, 89, 90, 93, 95]
     for name, x in (("k", c.cache.k), ("v", c.cache.v)):
         flat = oracle._bits(x)
-        for t in (5, 41, 75, 89, 90, 93, 95):    # left of every window, in row 0's alone, own rows 5 and 19, past the end
+        for t in places:    # left of every window, in row 0's alone, own rows 5 and 19, past the end
             at = oracle._flat(x, int(c.table[0, t // 32]), 1, 32, 64, name)[t % 32].flatten().to(device)
             for i, code in enumerate(sorted(bad)):
                 flat[at[i::len(bad)]] = torch.tensor(code, dtype=torch.int32, device=device).to(flat.dtype)
-    got = c.attend(window=30, sinks=1).cpu()
-    rows = torch.tensor([r for r in range(20) if not any(70 + r - 30 < t <= 70 + r for t in (5, 41, 75, 89))])
-    assert rows.tolist() == [1, 2, 3, 4]
-    dirty = [0, *range(5, 20)]
+    got = c.attend(window=window, sinks=1).cpu()
+    rows = torch.tensor([r for r in range(20) if not any((wider or 70 + r - 30 < t) and t <= 70 + r for t in places)])
+    clean = [0, 1, 2, 3, 4] if wider else [1, 2, 3, 4]
+    assert rows.tolist() == clean
+    dirty = [r for r in range(20) if r not in clean]
     check(got[rows], want[rows], tol[rows])
     assert not torch.isfinite(got[dirty].float()).all(-1).any()
 
@@ -184,17 +233,19 @@ def test_extreme_scores(device):
     check(c.attend(), *c.expected(), what="values of 2^100")
 
 
-def test_pages_of_very_unlike_scales(device):
+@pytest.mark.parametrize("heads, wider", [(4, 0), (64, WIDE)])
+def test_pages_of_very_unlike_scales(device, heads, wider):
     """8-bit pages of fp16 rows: values of 2^8 and of 2^-14 next to each other, and pages of zeros."""
-    c = Case(device, [150], [2], 4, 1, 64, 16, dtype=FP16, seed=9)
+    c = Case(device, [150], [2], heads, 1, 64, 16, dtype=FP16, seed=9, wider=wider)
     for i, s in enumerate([2.0 ** 5, 2.0 ** -20, 2.0 ** -9, 2.0 ** -64, 2.0 ** 3, 2.0 ** -6, 1.0, 2.0 ** -30, 2.0 ** -12, 2.0 ** -8]):
         c.cache.v_scale[int(c.table[0, i])] = s
         c.cache.k_scale[int(c.table[0, i])] = 2.0 ** -8 if i % 2 else 2.0 ** -9
     check(c.attend(), *c.expected())
 
 
-def test_pages_that_are_not_there(device):
-    c = Case(device, [100, 30], [4, 4], 4, 2, 64, 16, seed=10)
+@pytest.mark.parametrize("heads, wider", [(4, 0), (8, WIDE), (32, WIDE)])
+def test_pages_that_are_not_there(device, heads, wider):
+    c = Case(device, [100, 30], [4, 4], heads, 2, 64, 16, seed=10, wider=wider)
     missing = {0: [1, 3], 1: [0]}
     for b, numbers in missing.items():
         for n in numbers:
@@ -215,9 +266,10 @@ def test_pages_that_are_not_there(device):
     assert c.attend().abs().max() == 0
 
 
-def test_numbers_out_of_range_shorten_a_sequence(device):
+@pytest.mark.parametrize("heads, wider", [(4, 0), (32, WIDE)])
+def test_numbers_out_of_range_shorten_a_sequence(device, heads, wider):
     """Lengths past the table, negative ones, and starts past the rows: no access leaves a buffer, the others hold."""
-    c = Case(device, [50, 20], [4, 4], 4, 2, 64, 16, seed=11)
+    c = Case(device, [50, 20], [4, 4], heads, 2, 64, 16, seed=11, wider=wider)
     want, tol = c.expected()
     lengths = torch.tensor([10 ** 14, 20], device=device)
     got = c.attend(lengths=lengths)
