@@ -253,3 +253,24 @@ def test_oracle_pieces():
     out, _, _ = oracle.attention(torch.zeros(1, 1, 2), torch.zeros(6, 1, 2), v, torch.zeros(1, 6, dtype=torch.bool), 1.0)
     assert out.abs().max() == 0
     assert math.isclose(float(oracle.attention(torch.ones(1, 1, 2), torch.ones(6, 1, 2), v, see[:1], 0.5)[2]), 1.0)
+
+
+def test_pages_are_handed_out_and_taken_back():
+    from plm_amd.attention_layer import PageTable
+
+    cache = _stub(pages=5, page=16)
+    pages = PageTable(cache, 2, 64)
+    assert pages.table.tolist() == [[-1] * 4] * 2
+    pages.reserve(0, 17)
+    pages.reserve(1, 33)
+    held = [t for t in pages.table.flatten().tolist() if t >= 0]
+    assert len(held) == 5 and sorted(held) == [0, 1, 2, 3, 4]
+    pages.reserve(0, 32)   # already there
+    with pytest.raises(RuntimeError):
+        pages.reserve(0, 33)
+    with pytest.raises(ValueError):
+        pages.reserve(1, 65)
+    pages.free(1)
+    assert pages.table[1].tolist() == [-1] * 4
+    pages.reserve(0, 64)
+    assert sorted(pages.table[0].tolist()) == sorted({*pages.table[0].tolist()})
