@@ -1,33 +1,45 @@
 // Which kernel a launch of plm_attend takes (a translation unit per type of rows and cache includes it).
 #pragma once
 
+#include <atomic>
+
 #include "attend.h"
 #include "attend_tile.h"
 
 namespace plm {
 
-template <typename Kernel>
-hipError_t attend_go(Kernel kern, const AttendArgs& a, unsigned grid, unsigned threads, size_t bytes, hipStream_t s) {
-  if (bytes > 64 * 1024) {
-    const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                                  hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-    if (raised != hipSuccess) return raised;
-  }
-  kern<<<grid, threads, bytes, s>>>(a);
-  return hipGetLastError();
+// Lets `kern` have more than 64 KiB of LDS, once per device (`done`: a bit each).
+inline hipError_t allow_lds(const void* kern, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  const hipError_t err = hipGetDevice(&dev);
+  if (err != hipSuccess) return err;
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+  const hipError_t raised = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (raised == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return raised;
 }
 
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_stream(const AttendArgs& a, unsigned grid, hipStream_t s) {
   constexpr int W = 4;
   constexpr size_t waves = static_cast<size_t>(W) * NC * (C * 16 + 2) * 64 * 4;
-  return attend_go(&attend_kernel<DT, E8, C, NC, W>, a, grid, 64 * W, waves, s);
+  auto* kern = &attend_kernel<DT, E8, C, NC, W>;
+  if constexpr (waves > 64 * 1024) {
+    static std::atomic<uint64_t> done{0};
+    const hipError_t raised = allow_lds(reinterpret_cast<const void*>(kern), waves, done);
+    if (raised != hipSuccess) return raised;
+  }
+  kern<<<grid, 64 * W, waves, s>>>(a);
+  return hipGetLastError();
 }
 
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_tiled(const AttendArgs& a, unsigned grid, hipStream_t s) {
   constexpr size_t sets = static_cast<size_t>(attend_sets(C)) * attend_set_bytes(C);
-  return attend_go(&attend_tile_kernel<DT, E8, C, NC>, a, grid, 256, sets, s);
+  static_assert(sets <= 64 * 1024, "dynamic LDS without asking for more");
+  attend_tile_kernel<DT, E8, C, NC><<<grid, 256, sets, s>>>(a);
+  return hipGetLastError();
 }
 
 template <int DT, bool E8, int C>

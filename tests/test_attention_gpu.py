@@ -299,6 +299,17 @@ def test_strided_queries_and_wide_tables(device, kind):
     assert torch.equal(c.attend(q=odd), want)
 
 
+@pytest.mark.parametrize("heads, wider", [(4, 0), (64, WIDE)])
+def test_sequences_without_rows(device, heads, wider):
+    c = Case(device, [50, 0, 20, 7], [0, 3, 0, 2], heads, 1, 64, 16, seed=15, wider=wider)
+    check(c.attend(), *c.expected())
+    before = c.cache.k.view(torch.uint8).clone()
+    attention.append_kv(c.cache, None, c.k.to(device), c.v.to(device), **c.calls)
+    for b in (0, 2):
+        held = [p for p in c.table[b].tolist() if p >= 0]
+        assert torch.equal(before[held], c.cache.k.view(torch.uint8)[held])
+
+
 def test_many_sequences(device):
     contexts = [(37 * b) % 211 for b in range(150)]
     c = Case(device, contexts, [1 + b % 3 for b in range(150)], 4, 1, 16, 16, seed=13)
