@@ -10,7 +10,7 @@
 // comes out with 16 consecutive dimensions per lane. Keys and values go from memory straight into
 // operand registers: 16 bytes per lane, 1 KiB per load, no LDS.
 //
-// A workgroup's W wavefronts take every W-th step of 32 tokens of one range of one (sequence, tile of
+// A workgroup's four wavefronts take every fourth step of 32 tokens of one range of one (sequence, tile of
 // columns, key head), and are joined through LDS at the end. Ranges of the same (sequence, tile, head)
 // leave partial results in device memory, which a second launch joins (attend_join.hip).
 #pragma once
@@ -39,6 +39,7 @@ struct AttendArgs {
 };
 
 constexpr int kStep = 32;        // tokens of a step
+constexpr int kWaves = 4;        // wavefronts of a workgroup
 constexpr int kAttendMost = 64;  // ranges per group, at most
 constexpr int kJoinColumns = 8;  // columns that a workgroup of the joining launch takes at a time, at most
 
@@ -547,8 +548,8 @@ constexpr int attend_waves(bool e8, int chunks, int nc) {
   return e8 || chunks == 3 ? 2 : 1;
 }
 
-template <int DT, bool E8, int C, int NC, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_waves(E8, C, NC)))) void attend_kernel(AttendArgs a) {
+template <int DT, bool E8, int C, int NC>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(attend_waves(E8, C, NC)))) void attend_kernel(AttendArgs a) {
   constexpr int COLS = 16 * NC;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63;
@@ -581,7 +582,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
   auto step = [&](auto careful, int number) {
     constexpr bool CAREFUL = decltype(careful)::value;
     const int t0 = walk.token_of(number);
-    const bool more = !CAREFUL && number + W < walk.to;
+    const bool more = !CAREFUL && number + kWaves < walk.to;
     const bool edge = walk.edge(t0) || !s.held[0] || !s.held[1];
     // S^T of both units, all columns.
     f32x4 score[NC][2];
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
     }
     typename Wave::Place next = s;
     if (more) {
-      next = w.place(a, it.b, it.head, walk.token_of(number + W), last_page, lane);
+      next = w.place(a, it.b, it.head, walk.token_of(number + kWaves), last_page, lane);
       w.keys(a, next, lane);
     }
     uint32_t seen[NC];
@@ -729,11 +730,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
     s = w.place(a, it.b, it.head, walk.token_of(walk.from + wave), last_page, lane);
     w.keys(a, s, lane);
     w.values(a, s, lane);
-    for (int number = walk.from + wave; number < walk.to; number += W) step(std::false_type{}, number);
+    for (int number = walk.from + wave; number < walk.to; number += kWaves) step(std::false_type{}, number);
     if (__any(odd)) {
       w.begin();
 #pragma unroll 1
-      for (int number = walk.from + wave; number < walk.to; number += W) {
+      for (int number = walk.from + wave; number < walk.to; number += kWaves) {
         s = w.place(a, it.b, it.head, walk.token_of(number), last_page, lane);
         w.keys(a, s, lane);
         w.values(a, s, lane);
@@ -744,7 +745,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
 
   // The wavefronts' results, in plain units, meet in LDS; each then joins a quarter of the dimensions, register r of its
   // number (4 consecutive dimensions of 16).
-  static_assert(W == 4, "a wavefront per accumulator register");
+  static_assert(kWaves == 4, "a wavefront per accumulator register");
   constexpr int kWaveFloats = NC * (C * 16 + 2) * 64;
   float* shared = reinterpret_cast<float*>(lds);
   {
@@ -766,14 +767,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
-    float top = kMinusInf, m[W], sum = 0.0f;
+    float top = kMinusInf, m[kWaves], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
+    for (int i = 0; i < kWaves; ++i) {
       m[i] = shared[i * kWaveFloats + NC * C * 1024 + n * 128 + lane];
       top = fmaxf(top, m[i]);
     }
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
+    for (int i = 0; i < kWaves; ++i) {
       m[i] = m[i] == top ? 1.0f : __builtin_amdgcn_exp2f(m[i] - top);
       sum += m[i] * shared[i * kWaveFloats + NC * C * 1024 + n * 128 + 64 + lane];
     }
@@ -788,7 +789,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
     for (int c = 0; c < C; ++c) {
       f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < W; ++i)
+      for (int i = 0; i < kWaves; ++i)
         o += *reinterpret_cast<const f32x4*>(shared + i * kWaveFloats + ((n * C + c) * 4 + wave) * 256 + lane * 4) * m[i];
       o *= inverse;
       const int e = 64 * c + 16 * g + 4 * wave;

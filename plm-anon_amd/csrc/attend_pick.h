@@ -22,23 +22,27 @@ inline hipError_t allow_lds(const void* kern, size_t bytes, std::atomic<uint64_t
 
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_stream(const AttendArgs& a, unsigned grid, hipStream_t s) {
-  constexpr int W = 4;
-  constexpr size_t waves = static_cast<size_t>(W) * NC * (C * 16 + 2) * 64 * 4;
-  auto* kern = &attend_kernel<DT, E8, C, NC, W>;
+  constexpr size_t waves = static_cast<size_t>(kWaves) * NC * (C * 16 + 2) * 64 * 4;
+  auto* kern = &attend_kernel<DT, E8, C, NC>;
   if constexpr (waves > 64 * 1024) {
     static std::atomic<uint64_t> done{0};
     const hipError_t raised = allow_lds(reinterpret_cast<const void*>(kern), waves, done);
     if (raised != hipSuccess) return raised;
   }
-  kern<<<grid, 64 * W, waves, s>>>(a);
+  kern<<<grid, 64 * kWaves, waves, s>>>(a);
   return hipGetLastError();
 }
 
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_tiled(const AttendArgs& a, unsigned grid, hipStream_t s) {
   constexpr size_t sets = static_cast<size_t>(attend_sets(C)) * attend_set_bytes(C);
-  static_assert(sets <= 64 * 1024, "dynamic LDS without asking for more");
-  attend_tile_kernel<DT, E8, C, NC><<<grid, 256, sets, s>>>(a);
+  auto* kern = &attend_tile_kernel<DT, E8, C, NC>;
+  if constexpr (sets >= 64 * 1024) {  // with what the kernel has besides
+    static std::atomic<uint64_t> done{0};
+    const hipError_t raised = allow_lds(reinterpret_cast<const void*>(kern), sets, done);
+    if (raised != hipSuccess) return raised;
+  }
+  kern<<<grid, 64 * kWaves, sets, s>>>(a);
   return hipGetLastError();
 }
 
