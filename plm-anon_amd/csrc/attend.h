@@ -141,7 +141,8 @@ __device__ __forceinline__ AttendItem attend_item(const AttendArgs& a, int index
       it.b = base + at;
       it.ranges = of(ranges);
       const int tiles = of(s.tiles), rest = index - (items + of(to - mine));
-      if (rest < 0 || tiles < 1) return AttendItem{};
+      // Sequences that claim the same rows again and again can add up to more than 32 bits hold: nobody's work.
+      if (static_cast<uint32_t>(rest) >= static_cast<uint32_t>(of(mine))) return AttendItem{};
       const int x = rest / heads;
       it.head = rest - x * heads;
       if constexpr (JOIN) {
