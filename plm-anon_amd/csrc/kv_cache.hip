@@ -111,61 +111,49 @@ __device__ __forceinline__ void turned8(u32x4 lo, u32x4 hi, const float (&c)[8],
   }
 }
 
-// Queries: a thread has one place of a row, and `take` heads of it: the cosines and sines, four times a query's bytes,
-// are then read once for all of them. Where a half is whole groups of 8, a place is both partners' groups.
-template <int DT, int TAKE>
+// Queries: a thread has one place of a row and head, both partners' eight dimensions where a half is whole groups of 8.
+// (Four heads per thread, which read the cosines and sines once, measured the same over four prompts of up to 2048 rows
+// of 16 heads of 128, 22 us with the pages read back, and slower over three of 333 rows of 32 heads of 80, 20 against 19:
+// they come from L2.)
+template <int DT>
 __device__ __forceinline__ void append_queries(const AppendArgs& a, int block) {
   const int b = block / a.q_blocks;
   const KvSeq seq = kv_seq(a.rows, b, a.cache.page_shift);
   const int dim = a.cache.dim, rotary = a.rope != nullptr ? a.rotary : 0, half = rotary >> 1;
   const bool paired = rotary > 0 && !a.side_by_side && (half & 7) == 0;
-  const int places = paired ? (dim - half) >> 3 : dim >> 3, per_row = places * ((a.heads + TAKE - 1) / TAKE);
+  const int places = paired ? (dim - half) >> 3 : dim >> 3, per_row = places * a.heads;
   const int at = (block - b * a.q_blocks) * 256 + static_cast<int>(threadIdx.x), i = at / per_row;
   if (i >= seq.rows) return;
-  const int rest = at - i * per_row, part = rest / places, place = rest - part * places;
+  const int rest = at - i * per_row, head = rest / places, place = rest - head * places;
   const int64_t row = seq.start + i;
   bool none;
   const float* turn = turn_of(a, static_cast<int>(row), seq.context + i, none);
-  const uint16_t* from = a.q + row * a.q_row;
-  uint16_t* to = a.q_out + row * a.heads * dim;
-  const int head0 = part * TAKE;
-  if (paired && place < (half >> 3) && turn != nullptr) {
+  const uint16_t* from = a.q + row * a.q_row + head * a.q_head;
+  uint16_t* to = a.q_out + (row * a.heads + head) * dim;
+  const bool both = paired && place < (half >> 3);
+  if (both && turn != nullptr) {
     const int e = place << 3;
-    u32x4 lo[TAKE], hi[TAKE];
-#pragma unroll
-    for (int h = 0; h < TAKE; ++h) {
-      const uint16_t* x = from + min(head0 + h, a.heads - 1) * a.q_head + e;
-      lo[h] = *reinterpret_cast<const u32x4*>(x);
-      hi[h] = *reinterpret_cast<const u32x4*>(x + half);
-    }
-    float c[8], s[8];
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(from + e), hi = *reinterpret_cast<const u32x4*>(from + e + half);
+    float c[8], s[8], x[8], y[8];
 #pragma unroll
     for (int k = 0; k < 8; k += 4) {
       *reinterpret_cast<f32x4*>(c + k) = *reinterpret_cast<const f32x4*>(turn + e + k);
       *reinterpret_cast<f32x4*>(s + k) = *reinterpret_cast<const f32x4*>(turn + half + e + k);
     }
-#pragma unroll
-    for (int h = 0; h < TAKE; ++h) {
-      if (head0 + h >= a.heads) continue;
-      float x[8], y[8];
-      turned8<DT>(lo[h], hi[h], c, s, x, y);
-      uint16_t* out = to + (head0 + h) * dim + e;
-      *reinterpret_cast<u32x4*>(out) = pack8<DT>(x);
-      *reinterpret_cast<u32x4*>(out + half) = pack8<DT>(y);
-    }
+    turned8<DT>(lo, hi, c, s, x, y);
+    *reinterpret_cast<u32x4*>(to + e) = pack8<DT>(x);
+    *reinterpret_cast<u32x4*>(to + e + half) = pack8<DT>(y);
     return;
   }
-  // Everything else eight dimensions at a time: pairs side by side, halves of other sizes, what is not turned.
-  const bool both = paired && place < (half >> 3);  // a position that the table does not hold
+  // Everything else eight dimensions at a time: pairs side by side, halves of other sizes, what is not turned, both
+  // partners of a position that the table does not hold.
 #pragma unroll 1
-  for (int h = head0; h < min(head0 + TAKE, a.heads); ++h)
-#pragma unroll 1
-    for (int k = 0; k < (both ? 2 : 1); ++k) {
-      const int e = paired && !both ? (place << 3) + half : (place << 3) + k * half;
-      float x[8];
-      rotated8<DT>(from + h * a.q_head, e, turn, rotary, a.side_by_side != 0, x);
-      *reinterpret_cast<u32x4*>(to + h * dim + e) = pack8<DT>(x);
-    }
+  for (int k = 0; k < (both ? 2 : 1); ++k) {
+    const int e = paired && !both ? (place << 3) + half : (place << 3) + k * half;
+    float x[8];
+    rotated8<DT>(from, e, turn, rotary, a.side_by_side != 0, x);
+    *reinterpret_cast<u32x4*>(to + e) = pack8<DT>(x);
+  }
 }
 
 // A thread's 16 values of the workgroup's page. Values: 4 dimensions (i / 4, from e[0]) of 4 tokens (i % 4), one 16-byte
@@ -371,12 +359,12 @@ __device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq&
 }
 
 // A workgroup has a page of one head's keys or values (8 bits), 256 units of it (16 bits), or 256 places of queries.
-template <int DT, bool E8, int UPT, int TAKE>
+template <int DT, bool E8, int UPT>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ float red[4];
   int block = blockIdx.x;
   if (block >= a.kv_blocks) {
-    append_queries<DT, TAKE>(a, block - a.kv_blocks);
+    append_queries<DT>(a, block - a.kv_blocks);
     return;
   }
   const bool values = block & 1;
@@ -510,22 +498,17 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
 
 namespace {
 
-template <int DT, bool E8, int UPT>
-void append_take(const AppendArgs& a, int take, unsigned grid, hipStream_t s) {
-  if (take == 4) append_kernel<DT, E8, UPT, 4><<<grid, 256, 0, s>>>(a);
-  else append_kernel<DT, E8, UPT, 1><<<grid, 256, 0, s>>>(a);
-}
-
 template <int DT, bool E8>
-void append_go(const AppendArgs& a, int take, unsigned grid, hipStream_t s) {
-  const int units = a.cache.page * ((a.cache.dim + 15) / 16);
+void append_go(const AppendArgs& a, unsigned grid, hipStream_t s) {
   if constexpr (!E8) {
-    append_take<DT, false, 1>(a, take, grid, s);
+    append_kernel<DT, false, 1><<<grid, 256, 0, s>>>(a);
   } else {
-    if (units <= 256) append_take<DT, true, 1>(a, take, grid, s);
-    else if (units <= 512) append_take<DT, true, 2>(a, take, grid, s);
-    else if (units <= 1024) append_take<DT, true, 4>(a, take, grid, s);
-    else append_take<DT, true, 8>(a, take, grid, s);
+    // Units of 16 values per thread, as many as keep a page's rows in registers.
+    const int units = a.cache.page * ((a.cache.dim + 15) / 16);
+    if (units <= 256) append_kernel<DT, true, 1><<<grid, 256, 0, s>>>(a);
+    else if (units <= 512) append_kernel<DT, true, 2><<<grid, 256, 0, s>>>(a);
+    else if (units <= 1024) append_kernel<DT, true, 4><<<grid, 256, 0, s>>>(a);
+    else append_kernel<DT, true, 8><<<grid, 256, 0, s>>>(a);
   }
 }
 
@@ -564,19 +547,17 @@ int plm_kv_append(const plm_append_call* call, void* stream) {
   const bool e8 = h.cache->type == PLM_CACHE_E4M3;
   a.parts = e8 ? 1 : (a.cache.page * ((a.cache.dim + 15) / 16) + 255) / 256;
   const int64_t kv_blocks = seqs * a.page_slots * a.cache.heads * a.parts * 2;
-  // Four heads per thread once that leaves a few wavefronts for every SIMD; below, latency is all there is.
-  const int take = h.heads >= 4 && h.rows.total * h.heads * (a.cache.dim / 8) >= (1 << 19) ? 4 : 1;
   const int half = h.rope != nullptr ? a.rotary / 2 : 0;
   const int64_t places = half > 0 && !a.side_by_side && half % 8 == 0 ? (a.cache.dim - half) / 8 : a.cache.dim / 8;
-  const int64_t q_items = h.q == nullptr ? 0 : max_rows * places * ((h.heads + take - 1) / take);
+  const int64_t q_items = h.q == nullptr ? 0 : max_rows * places * h.heads;
   const int64_t q_blocks = (q_items + 255) / 256;
   if (kv_blocks + q_blocks * seqs >= (int64_t{1} << 31) || q_items >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   a.kv_blocks = static_cast<int>(kv_blocks);
   a.q_blocks = static_cast<int>(q_blocks);
   const unsigned grid = static_cast<unsigned>(kv_blocks + q_blocks * seqs);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (h.dtype == PLM_BF16) e8 ? plm::append_go<plm::DT_BF16, true>(a, take, grid, s) : plm::append_go<plm::DT_BF16, false>(a, take, grid, s);
-  else e8 ? plm::append_go<plm::DT_F16, true>(a, take, grid, s) : plm::append_go<plm::DT_F16, false>(a, take, grid, s);
+  if (h.dtype == PLM_BF16) e8 ? plm::append_go<plm::DT_BF16, true>(a, grid, s) : plm::append_go<plm::DT_BF16, false>(a, grid, s);
+  else e8 ? plm::append_go<plm::DT_F16, true>(a, grid, s) : plm::append_go<plm::DT_F16, false>(a, grid, s);
   return hipGetLastError() == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 
