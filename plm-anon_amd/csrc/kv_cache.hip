@@ -1,9 +1,10 @@
 // The paged cache's append (with the position rotation of keys and queries) and its read, declared in
 // include/plm_amd.h.
 //
-// Rotation: dimensions (a, b) of a pair become (a cos - b sin, b cos + a sin) in fp32; a pair is (i,
-// i + rotary / 2), or (2 i, 2 i + 1) side by side. A query is rounded once to the model's type, a key
-// once to what the cache holds.
+// Rotation: dimensions (a, b) of a pair become (a cos - b sin, b cos + a sin); a pair is (i, i + rotary / 2), or (2 i,
+// 2 i + 1) side by side. What becomes the model's type is computed in fp32 and rounded from there, off by half a step and
+// 2^-16 of one at most. An 8-bit code has 2^20 fp32 values to a step, so of a million keys' values about one would come out
+// on the other side of a border: what is that close is computed in fp64 and rounded once.
 //
 // 8-bit pages: codes times one power of two per (page, head). Appending rows needs their largest
 // magnitude first: a workgroup owns one (page, head) of the keys or of the values, keeps its new rows
@@ -29,11 +30,38 @@ struct AppendArgs {
   int heads, rotary, side_by_side, page_slots, parts, kv_blocks, q_blocks;
 };
 
+// a c + b s in fp32. `close` gets the bit where that is within its error, 2^-23 of the larger term at most, of a place where
+// 8-bit codes may part: at most four bits of mantissa, so 19 zeros at the end.
+__device__ __forceinline__ float turn_one(float a, float c, float b, float s, int bit, uint32_t& close) {
+  const float part = b * s, sum = fmaf(a, c, part);
+  const float border = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, sum) + 0x40000u) & 0xfff80000u);
+  close |= fabsf(sum - border) <= 0x1p-22f * fmaxf(fabsf(part), fabsf(sum)) ? 1u << bit : 0u;
+  return sum;
+}
+
+// Dimension e of a row, turned in fp64, which holds the products exactly, to the fp32 value on either side whose last bit
+// is set, if it is not one itself: rounded again to fewer bits that is as if rounded once.
+template <int DT>
+__device__ __forceinline__ float turned_exact(const uint16_t* x, int e, const float* turn, int rotary, bool side_by_side) {
+  const int half = rotary >> 1;
+  const bool low = side_by_side ? (e & 1) == 0 : e < half;
+  const int at = side_by_side ? e >> 1 : low ? e : e - half;
+  const double own = from_bits16<DT>(x[e]), other = from_bits16<DT>(x[side_by_side ? e ^ 1 : low ? e + half : e - half]);
+  const double part = other * static_cast<double>(turn[half + at]);
+  const double sum = fma(own, static_cast<double>(turn[at]), low ? -part : part);
+  const float near = static_cast<float>(sum);
+  const double off = sum - static_cast<double>(near);
+  uint32_t bits = __builtin_bit_cast(uint32_t, near);
+  if (fabs(off) > 0.0 && fabs(off) < __builtin_inf() && (bits & 1u) == 0u)
+    bits += (off < 0.0) == ((bits >> 31) != 0u) ? 1u : ~0u;
+  return __builtin_bit_cast(float, bits);
+}
+
 // Dimensions [e0, e0 + 8) of a row, as fp32, turned. `turn` is the position's row of the rotation table,
 // null where the table does not hold the position: what it would have turned is NaN.
 template <int DT>
 __device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float* turn, int rotary, bool side_by_side,
-                                         float (&out)[8]) {
+                                         uint32_t& close, float (&out)[8]) {
   const u32x4 own = *reinterpret_cast<const u32x4*>(x + e0);
 #pragma unroll
   for (int i = 0; i < 8; ++i) out[i] = from_bits16<DT>(static_cast<uint16_t>(own[i / 2] >> (16 * (i & 1))));
@@ -49,8 +77,8 @@ __device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float*
       if (e0 + i < rotary) {
         const float c = turn[(e0 + i) >> 1], s = turn[half + ((e0 + i) >> 1)];
         const float a = out[i], b = out[i + 1];
-        out[i] = fmaf(a, c, -(b * s));
-        out[i + 1] = fmaf(b, c, a * s);
+        out[i] = turn_one(a, c, -b, s, i, close);
+        out[i + 1] = turn_one(b, c, a, s, i + 1, close);
       }
     }
   } else if ((half & 7) == 0) {
@@ -67,7 +95,7 @@ __device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float*
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float o = from_bits16<DT>(static_cast<uint16_t>(other[i / 2] >> (16 * (i & 1))));
-      out[i] = fmaf(out[i], c[i], low ? -(o * s[i]) : o * s[i]);
+      out[i] = turn_one(out[i], c[i], low ? -o : o, s[i], i, close);
     }
   } else {
 #pragma unroll
@@ -77,7 +105,7 @@ __device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float*
         const bool low = e < half;
         const float o = from_bits16<DT>(x[low ? e + half : e - half]);
         const int at = low ? e : e - half;
-        out[i] = fmaf(out[i], turn[at], low ? -(o * turn[half + at]) : o * turn[half + at]);
+        out[i] = turn_one(out[i], turn[at], low ? -o : o, turn[half + at], i, close);
       }
     }
   }
@@ -101,13 +129,14 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
 
 // Eight pairs, partners in `lo` and `hi`, turned.
 template <int DT>
-__device__ __forceinline__ void turned8(u32x4 lo, u32x4 hi, const float (&c)[8], const float (&s)[8], float* x, float* y) {
+__device__ __forceinline__ void turned8(u32x4 lo, u32x4 hi, const float (&c)[8], const float (&s)[8], uint32_t& close, float* x,
+                                        float* y) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float p = from_bits16<DT>(static_cast<uint16_t>(lo[k / 2] >> (16 * (k & 1))));
     const float q = from_bits16<DT>(static_cast<uint16_t>(hi[k / 2] >> (16 * (k & 1))));
-    x[k] = fmaf(p, c[k], -(q * s[k]));
-    y[k] = fmaf(q, c[k], p * s[k]);
+    x[k] = turn_one(p, c[k], -q, s[k], k, close);
+    y[k] = turn_one(q, c[k], p, s[k], 8 + k, close);
   }
 }
 
@@ -131,6 +160,7 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, int block) {
   const uint16_t* from = a.q + row * a.q_row + head * a.q_head;
   uint16_t* to = a.q_out + (row * a.heads + head) * dim;
   const bool both = paired && place < (half >> 3);
+  uint32_t close = 0;  // of no account: queries are rounded to the model's type
   if (both && turn != nullptr) {
     const int e = place << 3;
     const u32x4 lo = *reinterpret_cast<const u32x4*>(from + e), hi = *reinterpret_cast<const u32x4*>(from + e + half);
@@ -140,7 +170,7 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, int block) {
       *reinterpret_cast<f32x4*>(c + k) = *reinterpret_cast<const f32x4*>(turn + e + k);
       *reinterpret_cast<f32x4*>(s + k) = *reinterpret_cast<const f32x4*>(turn + half + e + k);
     }
-    turned8<DT>(lo, hi, c, s, x, y);
+    turned8<DT>(lo, hi, c, s, close, x, y);
     *reinterpret_cast<u32x4*>(to + e) = pack8<DT>(x);
     *reinterpret_cast<u32x4*>(to + e + half) = pack8<DT>(y);
     return;
@@ -151,7 +181,7 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, int block) {
   for (int k = 0; k < (both ? 2 : 1); ++k) {
     const int e = paired && !both ? (place << 3) + half : (place << 3) + k * half;
     float x[8];
-    rotated8<DT>(from, e, turn, rotary, a.side_by_side != 0, x);
+    rotated8<DT>(from, e, turn, rotary, a.side_by_side != 0, close, x);
     *reinterpret_cast<u32x4*>(to + e) = pack8<DT>(x);
   }
 }
@@ -197,10 +227,10 @@ __device__ __forceinline__ PageUnit page_unit(const AppendArgs& a, int x) {
   return p;
 }
 
-// The unit's new values in fp32, zero where a token is not new.
+// The unit's new values in fp32, zero where a token is not new. Bit i of `close`: see turn_one.
 template <int DT, bool VALUES>
 __device__ __forceinline__ void new_values(const AppendArgs& a, const KvSeq& seq, const PageUnit& p, int base, int head,
-                                           float (&x)[16]) {
+                                           float (&x)[16], uint32_t& close) {
   const int end = seq.context + seq.rows;
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = 0.0f;
@@ -231,18 +261,30 @@ __device__ __forceinline__ void new_values(const AppendArgs& a, const KvSeq& seq
         *reinterpret_cast<f32x4*>(c + k) = *reinterpret_cast<const f32x4*>(turn + p.e[0] + k);
         *reinterpret_cast<f32x4*>(s + k) = *reinterpret_cast<const f32x4*>(turn + p.e[1] + k);
       }
-      turned8<DT>(lo, hi, c, s, x, x + 8);
-      return;
+      turned8<DT>(lo, hi, c, s, close, x, x + 8);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (p.e[k] < a.cache.dim) {
+          float half[8];
+          uint32_t of_half = 0;
+          rotated8<DT>(from, p.e[k], turn, rotary, a.side_by_side != 0, of_half, half);
+          close |= of_half << (8 * k);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[8 * k + i] = half[i];
+        }
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (p.e[k] < a.cache.dim) {
-        float half[8];
-        rotated8<DT>(from, p.e[k], turn, rotary, a.side_by_side != 0, half);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[8 * k + i] = half[i];
-      }
   }
+}
+
+// Element i of the unit's new keys, one that turns, exactly (turned_exact).
+template <int DT>
+__device__ __forceinline__ float exact_value(const AppendArgs& a, const KvSeq& seq, const PageUnit& p, int base, int head, int i) {
+  const int slot = base + p.token, row = seq.start + (slot - seq.context);
+  bool none;
+  const float* turn = turn_of(a, row, slot, none);
+  const uint16_t* from = a.new_k + static_cast<int64_t>(row) * a.k_row + head * a.k_head;
+  return turned_exact<DT>(from, (i < 8 ? p.e[0] : p.e[1]) + (i & 7), turn, a.rotary, a.side_by_side != 0);
 }
 
 // Rows of one page of one head into an 8-bit cache. UPT units of 16 values per thread.
@@ -257,11 +299,32 @@ __device__ __forceinline__ void append_page_fp8(const AppendArgs& a, const KvSeq
   const float before = stays ? *held : 0.0f;
   float x[UPT][16];
   PageUnit p[UPT];
+  uint64_t close[2] = {0, 0};
   float amax = 0.0f;
 #pragma unroll
   for (int u = 0; u < UPT; ++u) {
     p[u] = page_unit<VALUES, true>(a, min(static_cast<int>(threadIdx.x) + u * 256, count - 1));
-    new_values<DT, VALUES>(a, seq, p[u], base, head, x[u]);
+    uint32_t bits = 0;
+    new_values<DT, VALUES>(a, seq, p[u], base, head, x[u], bits);
+    close[u / 4] |= static_cast<uint64_t>(bits) << (16 * (u % 4));
+  }
+  // About one value in 2^16 is that close: one at a time, from memory. (All keys in fp64 from the start: prompts 25.3 us
+  // for 22.9, single tokens 9.8 for 9.5; without any of it 22.1 and 8.9.)
+  if constexpr (!VALUES) {
+    while ((close[0] | close[1]) != 0) {
+      const int word = close[0] != 0 ? 0 : 1, i = 64 * word + __builtin_ctzll(word == 0 ? close[0] : close[1]);
+      if (word == 0) close[0] &= close[0] - 1;
+      else close[1] &= close[1] - 1;
+      const PageUnit of = page_unit<false, true>(a, min(static_cast<int>(threadIdx.x) + (i >> 4) * 256, count - 1));
+      const float y = exact_value<DT>(a, seq, of, base, head, i & 15);
+#pragma unroll
+      for (int u = 0; u < UPT; ++u)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[u][k] = 16 * u + k == i ? y : x[u][k];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < UPT; ++u) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float m = fabsf(x[u][i]);
@@ -332,7 +395,8 @@ __device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq&
   const int first = base + p.token, last = first + (VALUES ? 4 : 1);
   if (last <= seq.context || first >= end) return;
   float x[16];
-  new_values<DT, VALUES>(a, seq, p, base, head, x);
+  uint32_t close = 0;  // of no account: rounded to the model's type
+  new_values<DT, VALUES>(a, seq, p, base, head, x, close);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     u32x4* to = reinterpret_cast<u32x4*>(page + p.at[h] + (VALUES ? h * 1024 : 0));

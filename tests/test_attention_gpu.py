@@ -423,6 +423,26 @@ def test_append(device, shape, dtype, kind):
         check(got[lo:hi], value[lo:hi], tol, f"{name} of page {page}")
 
 
+@pytest.mark.parametrize("dim, rotary, side", [(128, 128, False), (64, 64, True), (80, 40, False), (80, 40, True)])
+@pytest.mark.parametrize("cosine", [1.0625, 1.1875])
+def test_turned_keys_round_once(device, dim, rotary, side, cosine):
+    """Turned keys 2^-30 to either side of the middle between two codes: beyond fp32's reach, and rounded the right way."""
+    c = Case(device, [0, 3], [40, 30], 2, 2, dim, 32, seed=3)
+    c.k = torch.where(torch.randn(c.k.shape, generator=c.g) < 0, -1.0, 1.0).to(BF16)
+    c.k[::2] *= 256   # pages' scales are 1
+    half = rotary // 2
+    sine = torch.where(torch.randn(100, half, generator=c.g) < 0, -2.0 ** -30, 2.0 ** -30)
+    rope = torch.cat((torch.full((100, half), cosine), sine), 1)
+    _, pages = _expected_append(c, rope, side, None)
+    attention.append_kv(c.cache, None, c.k.to(device), c.v.to(device), c.calls["table"], c.calls["lengths"],
+                        rope=rope.to(device), interleaved=side, row_starts=c.calls["row_starts"], max_rows=c.calls["max_rows"])
+    for (name, page), (value, scale, lo, hi) in pages.items():
+        if name == "k":
+            assert torch.equal(c.cache.k_scale[page].cpu().double(), scale)
+            got = oracle.get_page(c.cache.k, c.cache.k_scale, page, c.kv_heads, c.page, c.dim, "k")
+            assert torch.equal(got[lo:hi], (oracle.e4m3(value / scale[:, None]) * scale[:, None])[lo:hi])
+
+
 def test_append_in_steps_is_what_was_appended(device):
     """A prompt, then tokens one by one and in rounds that are partly taken back, through a page's life."""
     cache = attention.PagedCache.empty(9, 2, 64, page=16, device=device)
