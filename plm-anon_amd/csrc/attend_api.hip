@@ -33,9 +33,10 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   };
   // Tiles of 16 columns, whose four wavefronts take different tokens, are done soonest while all of a call's are short of
   // work for the device; wider ones need less of it. (Rounds of 56 rows over 500 / 4007 / 16000 tokens, 16 heads over 4:
-  // 11 / 21 / 37 us against 19 / 23 / 36; 42 rows over 55237 tokens 54 against 45.) Up to 96 tokens there is nothing to
-  // take apart. 128 columns need half the loads and conversions of 64, once there are tiles of them for all CUs; short
-  // walks end more evenly in smaller tiles (prompts through a window of 512: 42 against 45 us).
+  // 10.0 / 18.4 / 35 us against 18.7 / 21.3 / 34; four sequences' over 2000, 32 heads over 8, 41.5 against 40.5.) Up to
+  // 96 tokens there is nothing to take apart. 128 columns need half the loads and conversions of 64, once there are tiles
+  // of them for all CUs (4096 rows after 4096 tokens: 266 against 340 us on the same card); short walks end more evenly in
+  // smaller tiles (prompts through a window of 512: 42 us in 128 columns, 40 in 64).
   const int64_t narrow = kv_heads * (seqs + total * group / 16);
   const bool many = most > 256 && kv_heads * (total * group / 128) >= (seen(128) < 24 ? 2048 : 256);
   if (most <= 16 || (seen(16) > 3 && narrow * seen(16) <= kNarrowWork)) p.columns = 16;
@@ -48,7 +49,8 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   p.whole = p.columns <= 32 ? 32 : 20;
   const int64_t steps = seen(p.columns);
   // Not cut: what is short, a single sequence's groups, which are alike, where they fill the device, and groups that do
-  // and cannot be much unlike.
+  // and cannot be much unlike. (Cut / not: two sequences of 131004 tokens 50 / 1029 us, 64 of 4500 on average 60 / 88, a
+  // round over 4007 18 / 33; 32 windows of 1024 53 / 49, a prompt of 4096 rows 250 / 242, through a window 48 / 41.)
   const bool full = p.groups - kv_heads >= 256;
   p.target = steps > p.whole && !(full && (seqs == 1 || steps <= 4 * p.least)) ? 512 : 0;
   p.grid = p.groups + p.target;
