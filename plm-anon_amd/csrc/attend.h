@@ -423,13 +423,16 @@ __device__ __forceinline__ void attend_publish(const AttendArgs& a, const Attend
 }
 
 // Chunk c of the unit at byte `at` (the same in every lane). Dimensions past the head's, in the last chunk, are not
-// read: a lane whose are (`inside` false) gets zeros.
-template <bool E8, int C>
+// read: a lane whose are (`inside` false) gets zeros. ONCE: no other workgroup reads them, so they are not to stay in the
+// caches (bit 1 of the load's last operand: nontemporal).
+template <bool E8, int C, bool ONCE>
 __device__ __forceinline__ void load_chunk_of(__amdgpu_buffer_rsrc_t rs, int c, int lane, bool inside, u32x4 (&x)[E8 ? 1 : 2]) {
 #pragma unroll
   for (int h = 0; h < (E8 ? 1 : 2); ++h) {
     const uint32_t off = static_cast<uint32_t>((c * (E8 ? 1 : 2) + h) * 1024 + lane * 16);
-    x[h] = buffer_load16(rs, c == C - 1 && !inside ? kOutOfRange : off);
+    const uint32_t at = c == C - 1 && !inside ? kOutOfRange : off;
+    if constexpr (ONCE) x[h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<int>(at), 0, 2));
+    else x[h] = buffer_load16(rs, at);
   }
 }
 
@@ -440,15 +443,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t unit_rsrc(const char* base, in
   return make_rsrc(reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo), bytes);
 }
 
-template <bool E8, int C>
+template <bool E8, int C, bool ONCE>
 __device__ __forceinline__ void load_unit(const char* base, int64_t at, int lane, bool inside, u32x4 (&x)[C][E8 ? 1 : 2]) {
   const __amdgpu_buffer_rsrc_t rs = unit_rsrc(base, at, C * (E8 ? 1024 : 2048));
 #pragma unroll
-  for (int c = 0; c < C; ++c) load_chunk_of<E8, C>(rs, c, lane, inside, x[c]);
+  for (int c = 0; c < C; ++c) load_chunk_of<E8, C, ONCE>(rs, c, lane, inside, x[c]);
 }
 
 // A wavefront's state and its walk over tokens.
-template <int DT, bool E8, int C, int NC>
+template <int DT, bool E8, int C, int NC, bool ONCE>
 struct AttendWave {
   static constexpr int kLoads = E8 ? 1 : 2;  // of 16 bytes per lane, unit and chunk
   static constexpr int kUnitBytes = 1024 * kLoads;
@@ -533,11 +536,11 @@ struct AttendWave {
 
   __device__ __forceinline__ void keys(const AttendArgs& a, const Place& s, int lane) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) load_unit<E8, C>(a.cache.k, s.at[u], lane, 16 * (lane >> 4) < a.cache.dim - 64 * (C - 1), k[u]);
+    for (int u = 0; u < 2; ++u) load_unit<E8, C, ONCE>(a.cache.k, s.at[u], lane, 16 * (lane >> 4) < a.cache.dim - 64 * (C - 1), k[u]);
   }
   __device__ __forceinline__ void values(const AttendArgs& a, const Place& s, int lane) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) load_unit<E8, C>(a.cache.v, s.at[u], lane, 4 * (lane & 15) < a.cache.dim - 64 * (C - 1), v[u]);
+    for (int u = 0; u < 2; ++u) load_unit<E8, C, ONCE>(a.cache.v, s.at[u], lane, 4 * (lane & 15) < a.cache.dim - 64 * (C - 1), v[u]);
   }
 };
 
@@ -555,7 +558,7 @@ constexpr int attend_waves(bool e8, int chunks, int nc) {
 // 131004 tokens 51 us for 268 MB, 5.3 TB/s; 32 windows of 1024 tokens, 16 key heads in 16 bits, 48 us for 270 MB, 5.6
 // TB/s. Where they are short, by a workgroup's beginning and end (arguments, lengths, table, scales, first loads, join:
 // 6000 to 7000 cycles): 500 tokens 7 us. Four wavefronts per workgroup: with eight the first of these took 70 us.
-template <int DT, bool E8, int C, int NC>
+template <int DT, bool E8, int C, int NC, bool ONCE>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(attend_waves(E8, C, NC)))) void attend_kernel(AttendArgs a) {
   constexpr int COLS = 16 * NC;
   extern __shared__ __align__(16) char lds[];
@@ -567,7 +570,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(att
   const KvSeq& seq = it.seq;
   const int columns = seq.rows * a.group;
 
-  using Wave = AttendWave<DT, E8, C, NC>;
+  using Wave = AttendWave<DT, E8, C, NC, ONCE>;
   Wave w;
   AttendColumns<NC> cols;
   cols.set(a, seq, it, it.tile * COLS, columns, col);

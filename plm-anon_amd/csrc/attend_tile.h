@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       if constexpr (E8) st.vs[u] = lane_float(page_vs, at);
       const uint64_t byte = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(page_hi, at))) << 32 |
                             (static_cast<uint32_t>(__builtin_amdgcn_readlane(page_lo, at)) & ~1u);
-      load_unit<E8, C>(role_base, static_cast<int64_t>(byte + static_cast<uint32_t>((t & (a.cache.page - 1)) >> 4) * (C * kUnitBytes)),
+      load_unit<E8, C, false>(role_base, static_cast<int64_t>(byte + static_cast<uint32_t>((t & (a.cache.page - 1)) >> 4) * (C * kUnitBytes)),
                        lane, inside, st.x[u]);
     }
   };
