@@ -554,9 +554,9 @@ constexpr int attend_waves(bool e8, int chunks, int nc) {
 
 // 16 NC columns. Bound, where contexts are long, by the bytes of the keys and values, each read once and used by one
 // wavefront: hence no LDS in the loop, and a key head's whole group of queries as columns of one tile. 64 sequences of
-// 4500 tokens on average, 16 heads of 128 over 4 in 8 bits: 60 us for 296 MB, 4.9 TB/s (a large copy reaches 5.1); two of
-// 131004 tokens 51 us for 268 MB, 5.3 TB/s; 32 windows of 1024 tokens, 16 key heads in 16 bits, 48 us for 270 MB, 5.6
-// TB/s. Where they are short, by a workgroup's beginning and end (arguments, lengths, table, scales, first loads, join:
+// 4500 tokens on average, 16 heads of 128 over 4 in 8 bits: 62 us for 296 MB, 4.8 TB/s with the join (a large copy reaches
+// 5.1); two of 131004 tokens 51 us for 268 MB, 5.3 TB/s; 32 windows of 1024 tokens, 16 key heads in 16 bits, 49 us for 270
+// MB, 5.5 TB/s. Where they are short, by a workgroup's beginning and end (arguments, lengths, table, scales, first loads, join:
 // 6000 to 7000 cycles): 500 tokens 7 us. Four wavefronts per workgroup: with eight the first of these took 70 us.
 template <int DT, bool E8, int C, int NC, bool ONCE>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(attend_waves(E8, C, NC)))) void attend_kernel(AttendArgs a) {

@@ -4,7 +4,7 @@
 // CU, past its caches, at about 50 GB/s (a round's 56 rows over 4007 tokens: 11 us of 25).
 // Here a workgroup takes `take` columns of a group at a time, thread by thread four dimensions of one. Bound by latency
 // (the lengths, the maxima and sums, the results: one after the other): 5.3 us behind that round's 3.7 MB of partial
-// results, 5.9 behind the 1 MB of two sequences of 131004 tokens.
+// results, 5.6 behind the 1 MB of two sequences of 131004 tokens.
 #include "attend.h"
 
 namespace plm {

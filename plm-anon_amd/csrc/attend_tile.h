@@ -8,12 +8,14 @@
 // Two sets of 64 tokens: the next one's loads are in flight in registers while the current is multiplied, and are
 // stored behind it; one barrier per 64 tokens.
 //
-// Bound by what the vector units issue beside the matrix cores (per score a scaling, an exponential, a sum, half a
-// maximum and half a rounding): 4096 rows after 4096 tokens, 16 heads of 128 over 4 in 8 bits, 240 us or 858 TFLOP/s of
-// visible pairs (a product of 8192^3 reaches 1122), the matrix cores busy for 40 % of the cycles and the vector units for
-// 56 %. At heads of 64 there are half the products to a score: 3381 rows through windows of 512, 32 heads over 8, 39 us
-// or 310 TFLOP/s, 17 % and 62 %. Measured without gain: the next step's loads two steps ahead, the sums of exponentials
-// by a product with ones, raised priority around the products.
+// Bound by three things in turn, which the two wavefronts that a SIMD holds overlap in part: the vector units (per score
+// a scaling, an exponential, a sum, half a maximum and half a rounding), the matrix cores, and LDS, from which every
+// wavefront reads every operand for its 32 columns. 4096 rows after 4096 tokens, 16 heads of 128 over 4 in 8 bits: 240 us
+// or 858 TFLOP/s of visible pairs (a product of 8192^3 reaches 1122), the vector units busy for 56 % of the cycles, the
+// matrix cores for 40 %, LDS for about 58 %. At heads of 64 there are half the products to a score: 3381 rows through
+// windows of 512, 32 heads over 8, 39 us or 310 TFLOP/s, 62 % and 17 %. Measured without gain: loads two steps ahead, the
+// sums of exponentials by a product with ones, raised priority around the products, no maxima but where a sum shows that
+// one has grown (248 us for 242).
 #pragma once
 
 #include "attend.h"
