@@ -10,8 +10,8 @@
 // comes out with 16 consecutive dimensions per lane. Keys and values go from memory straight into
 // operand registers: 16 bytes per lane, 1 KiB per load, no LDS.
 //
-// A workgroup's four wavefronts take every fourth step of 32 tokens of one range of one (sequence, tile of
-// columns, key head), and are joined through LDS at the end. Ranges of the same (sequence, tile, head)
+// A workgroup's wavefronts (four, or as many as a CU holds) take the steps of 32 tokens of one range of one (sequence,
+// tile of columns, key head) in turn, and are joined through LDS at the end. Ranges of the same (sequence, tile, head)
 // leave partial results in device memory, which a second launch joins (attend_join.hip).
 #pragma once
 
@@ -36,10 +36,11 @@ struct AttendArgs {
   float per_target;  // a little more than 1 / target
   int least;    // steps of a range, at least
   int whole;    // a group of so many steps is not cut
+  int wide;     // workgroups of attend_wide wavefronts, where that is more
 };
 
 constexpr int kStep = 32;        // tokens of a step
-constexpr int kWaves = 4;        // wavefronts of a workgroup
+constexpr int kWaves = 4;        // wavefronts of a workgroup, but for wide ones (attend_wide)
 constexpr int kAttendMost = 64;  // ranges per group, at most
 constexpr int kJoinColumns = 8;  // columns that a workgroup of the joining launch takes at a time, at most
 
@@ -552,14 +553,18 @@ constexpr int attend_waves(bool e8, int chunks, int nc) {
   return e8 || chunks == 3 ? 2 : 1;
 }
 
+// Wavefronts of a workgroup that fills a CU.
+constexpr int attend_wide(bool e8, int chunks) { return 4 * attend_waves(e8, chunks, 1); }
+
 // 16 NC columns. Bound, where contexts are long, by the bytes of the keys and values, each read once and used by one
 // wavefront: hence no LDS in the loop, and a key head's whole group of queries as columns of one tile. 64 sequences of
 // 4500 tokens on average, 16 heads of 128 over 4 in 8 bits: 62 us for 296 MB, 4.8 TB/s with the join (a large copy reaches
 // 5.1); two of 131004 tokens 51 us for 268 MB, 5.3 TB/s; 32 windows of 1024 tokens, 16 key heads in 16 bits, 49 us for 270
 // MB, 5.5 TB/s. Where they are short, by a workgroup's beginning and end (arguments, lengths, table, scales, first loads, join:
-// 6000 to 7000 cycles): 500 tokens 7 us. Four wavefronts per workgroup: with eight the first of these took 70 us.
-template <int DT, bool E8, int C, int NC, bool ONCE>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(attend_waves(E8, C, NC)))) void attend_kernel(AttendArgs a) {
+// 6000 to 7000 cycles): 500 tokens 7 us. Four wavefronts per workgroup there (with eight the first of these took 70 us); groups of
+// middling length that all find a CU are taken whole by as many as it holds (attend_plan).
+template <int DT, bool E8, int C, int NC, bool ONCE, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_waves(E8, C, NC)))) void attend_kernel(AttendArgs a) {
   constexpr int COLS = 16 * NC;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63;
@@ -592,7 +597,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(att
   auto step = [&](auto careful, int number) {
     constexpr bool CAREFUL = decltype(careful)::value;
     const int t0 = walk.token_of(number);
-    const bool more = !CAREFUL && number + kWaves < walk.to;
+    const bool more = !CAREFUL && number + W < walk.to;
     const bool edge = walk.edge(t0) || !s.held[0] || !s.held[1];
     // S^T of both units, all columns.
     f32x4 score[NC][2];
@@ -620,7 +625,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(att
     }
     typename Wave::Place next = s;
     if (more) {
-      next = w.place(a, it.b, it.head, walk.token_of(number + kWaves), last_page, lane);
+      next = w.place(a, it.b, it.head, walk.token_of(number + W), last_page, lane);
       w.keys(a, next, lane);
     }
     uint32_t seen[NC];
@@ -740,11 +745,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(att
     s = w.place(a, it.b, it.head, walk.token_of(walk.from + wave), last_page, lane);
     w.keys(a, s, lane);
     w.values(a, s, lane);
-    for (int number = walk.from + wave; number < walk.to; number += kWaves) step(std::false_type{}, number);
+    for (int number = walk.from + wave; number < walk.to; number += W) step(std::false_type{}, number);
     if (__any(odd)) {
       w.begin();
 #pragma unroll 1
-      for (int number = walk.from + wave; number < walk.to; number += kWaves) {
+      for (int number = walk.from + wave; number < walk.to; number += W) {
         s = w.place(a, it.b, it.head, walk.token_of(number), last_page, lane);
         w.keys(a, s, lane);
         w.values(a, s, lane);
@@ -753,9 +758,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(att
     }
   }
 
-  // The wavefronts' results, in plain units, meet in LDS; each then joins a quarter of the dimensions, register r of its
-  // number (4 consecutive dimensions of 16).
-  static_assert(kWaves == 4, "a wavefront per accumulator register");
+  // The wavefronts' results, in plain units, meet in LDS; each then joins some of the 4 C parts of the dimensions: part p is
+  // register p % 4 (4 consecutive dimensions of 16) of chunk p / 4.
   constexpr int kWaveFloats = NC * (C * 16 + 2) * 64;
   float* shared = reinterpret_cast<float*>(lds);
   {
@@ -777,14 +781,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(att
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
-    float top = kMinusInf, m[kWaves], sum = 0.0f;
+    float top = kMinusInf, m[W], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < W; ++i) {
       m[i] = shared[i * kWaveFloats + NC * C * 1024 + n * 128 + lane];
       top = fmaxf(top, m[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < W; ++i) {
       m[i] = m[i] == top ? 1.0f : __builtin_amdgcn_exp2f(m[i] - top);
       sum += m[i] * shared[i * kWaveFloats + NC * C * 1024 + n * 128 + 64 + lane];
     }
@@ -796,13 +800,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(att
     const int x = 16 * n + col;
     uint16_t* out = a.out + (static_cast<int64_t>(seq.start + cols.row[n]) * a.heads + cols.head[n]) * a.cache.dim;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
+    for (int first = 0; first < 4 * C; first += W) {
+      const int part = first + wave, e = 64 * (part / 4) + 16 * g + 4 * (part % 4);
+      if (4 * C % W != 0 && part >= 4 * C) break;
       f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i)
-        o += *reinterpret_cast<const f32x4*>(shared + i * kWaveFloats + ((n * C + c) * 4 + wave) * 256 + lane * 4) * m[i];
+      for (int i = 0; i < W; ++i)
+        o += *reinterpret_cast<const f32x4*>(shared + i * kWaveFloats + (n * C * 4 + part) * 256 + lane * 4) * m[i];
       o *= inverse;
-      const int e = 64 * c + 16 * g + 4 * wave;
       if (!last) *reinterpret_cast<f32x4*>(slot + x * PAD + e) = o;
       else if (e < a.cache.dim) *reinterpret_cast<u32x2*>(out + e) = u32x2{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
     }

@@ -10,10 +10,11 @@ namespace plm {
 namespace {
 
 constexpr int64_t kNarrowWork = 24000;  // groups of 16 columns times steps
+constexpr int64_t kWideGroups = 320, kWideSteps = 100, kWideBytes = 448 * 1024;
 
 struct AttendPlan {
   int columns;        // of a workgroup's tile
-  int target, least, whole;  // AttendArgs
+  int target, least, whole, wide;  // AttendArgs
   int64_t grid, groups, bytes;
 };
 
@@ -21,7 +22,7 @@ struct AttendPlan {
 // (attend_item), so a wide table costs nothing; `grid` bounds the workgroups that any lengths can ask for:
 // one per group and as many more as the work is cut into.
 AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t heads, int64_t total, int64_t seqs,
-                       int64_t max_rows, int64_t table_width, int64_t window, int64_t sinks, bool mask) {
+                       int64_t max_rows, int64_t table_width, int64_t window, int64_t sinks, bool mask, bool e8) {
   AttendPlan p{};
   const int64_t group = heads / kv_heads, chunks = (head_dim + 63) / 64;
   const int64_t most = max_rows * group;
@@ -48,11 +49,20 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   p.least = p.columns <= 32 ? 16 : 8;
   p.whole = p.columns <= 32 ? 32 : 20;
   const int64_t steps = seen(p.columns);
+  // Workgroups that fill a CU take groups of middling length whole, with a wavefront's steps and the joining launch saved,
+  // where all find a CU (`groups` counts a sequence's last tile twice). One CU reads about 60 GB/s from memory: few groups
+  // of many bytes are cut instead, but for those whose tiles share them. (Wide / not: 16 tokens after 1000, 16 heads of 128
+  // over 4 in 8 bits, 10.7 / 14.8 us, 64 after 1000 14.4 / 17, 64 after up to 3000 26 / 30; a round of 56 rows after 1000
+  // 11.7 / 14.4, after 2500 16.5 / 17.7, four of 42 through a window of 777 12.1 / 14.8. One token after 3000, 8 key heads,
+  // 20.7 / 15.6; 8 after 2000 in 16 bits 23.7 / 17.4; a round after 4007 22.5 / 18; up to 16 steps 8.7 / 8.4.)
+  const int64_t bytes = steps * kStep * chunks * (e8 ? 128 : 256);  // of a group's keys and values
+  p.wide = p.columns == 16 && attend_wide(e8, static_cast<int>(chunks)) > kWaves && p.groups <= kWideGroups &&
+           steps > 4 * kWaves && steps <= kWideSteps && (most > 16 || p.groups >= 128 || bytes <= kWideBytes);
   // Not cut: what is short, a single sequence's groups, which are alike, where they fill the device, and groups that do
   // and cannot be much unlike. (Cut / not: two sequences of 131004 tokens 50 / 1029 us, 64 of 4500 on average 60 / 88, a
   // round over 4007 18 / 33; 32 windows of 1024 53 / 49, a prompt of 4096 rows 250 / 242, through a window 48 / 41.)
   const bool full = p.groups - kv_heads >= 256;
-  p.target = steps > p.whole && !(full && (seqs == 1 || steps <= 4 * p.least)) ? 512 : 0;
+  p.target = !p.wide && steps > p.whole && !(full && (seqs == 1 || steps <= 4 * p.least)) ? 512 : 0;
   p.grid = p.groups + p.target;
   // There are 2 * target ranges of groups of several at most: a cut sequence has less than twice load / chunk of
   // them, and a chunk is load / target at least. Such a group has two at least.
@@ -75,7 +85,7 @@ bool attend_of(const plm_attend_call* call, AttendArgs& a, AttendPlan& p) {
   if (h.mask != nullptr && (h.mask_rows < 1 || h.mask_words < 1 || h.mask_rows >= (1 << 28) || h.mask_words >= (1 << 24)))
     return false;
   p = attend_plan(heads, a.cache.page, a.cache.dim, h.heads, h.rows.total, h.rows.seqs, h.rows.max_rows, h.rows.table_width,
-                  h.window, h.sinks, h.mask != nullptr);
+                  h.window, h.sinks, h.mask != nullptr, h.cache->type == PLM_CACHE_E4M3);
   return p.grid < (int64_t{1} << 31);
 }
 
@@ -120,6 +130,7 @@ int plm_attend(const plm_attend_call* call, void* workspace, size_t workspace_by
   a.per_target = p.target > 0 ? 1.001f / static_cast<float>(p.target) : 0.0f;
   a.least = p.least;
   a.whole = p.whole;
+  a.wide = p.wide;
   const unsigned grid = static_cast<unsigned>(p.grid);
   const int32_t dtype = static_cast<int32_t>(h.dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);

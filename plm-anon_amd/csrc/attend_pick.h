@@ -20,16 +20,16 @@ inline hipError_t allow_lds(const void* kern, size_t bytes, std::atomic<uint64_t
   return raised;
 }
 
-template <int DT, bool E8, int C, int NC, bool ONCE>
+template <int DT, bool E8, int C, int NC, bool ONCE, int W>
 hipError_t attend_stream_go(const AttendArgs& a, unsigned grid, hipStream_t s) {
-  constexpr size_t waves = static_cast<size_t>(kWaves) * NC * (C * 16 + 2) * 64 * 4;
-  auto* kern = &attend_kernel<DT, E8, C, NC, ONCE>;
+  constexpr size_t waves = static_cast<size_t>(W) * NC * (C * 16 + 2) * 64 * 4;
+  auto* kern = &attend_kernel<DT, E8, C, NC, ONCE, W>;
   if constexpr (waves > 64 * 1024) {
     static std::atomic<uint64_t> done{0};
     const hipError_t raised = allow_lds(reinterpret_cast<const void*>(kern), waves, done);
     if (raised != hipSuccess) return raised;
   }
-  kern<<<grid, 64 * kWaves, waves, s>>>(a);
+  kern<<<grid, 64 * W, waves, s>>>(a);
   return hipGetLastError();
 }
 
@@ -40,7 +40,12 @@ hipError_t attend_stream_go(const AttendArgs& a, unsigned grid, hipStream_t s) {
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_stream(const AttendArgs& a, unsigned grid, hipStream_t s) {
   const bool once = static_cast<int64_t>(a.rows.max_rows) * a.group <= 16 * NC;
-  return once ? attend_stream_go<DT, E8, C, NC, true>(a, grid, s) : attend_stream_go<DT, E8, C, NC, false>(a, grid, s);
+  constexpr int wide = NC == 1 ? attend_wide(E8, C) : kWaves;
+  if constexpr (wide > kWaves) {
+    if (a.wide && once) return attend_stream_go<DT, E8, C, NC, true, wide>(a, grid, s);
+    if (a.wide) return attend_stream_go<DT, E8, C, NC, false, wide>(a, grid, s);
+  }
+  return once ? attend_stream_go<DT, E8, C, NC, true, kWaves>(a, grid, s) : attend_stream_go<DT, E8, C, NC, false, kWaves>(a, grid, s);
 }
 
 template <int DT, bool E8, int C, int NC>

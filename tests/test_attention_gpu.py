@@ -143,6 +143,52 @@ def test_wide_tables(device, shape, dtype, kind):
     check(c.attend(), *c.expected())
 
 
+# Groups of 17 to 100 steps of 32 tokens that all find a CU: workgroups of as many wavefronts as it holds.
+MIDDLING_SHAPES = [
+    ([600], [1], 4, 2, 64, 64),                          # 19 steps over 16 wavefronts (in 8 bits)
+    ([1000, 3, 544, 0], [1] * 4, 8, 2, 128, 16),         # 12 wavefronts, some without a step
+    ([3100], [9], 16, 4, 128, 64),                       # three tiles, the last in part
+    ([800, 70], [6, 33], 6, 2, 80, 32),
+    ([580], [5], 8, 2, 192, 16),
+    ([900, 31], [5, 4], 12, 3, 256, 128),
+    ([1500], [40], 3, 3, 8, 32),
+]
+
+
+@pytest.mark.parametrize("dtype, kind", [(BF16, E4M3), (FP16, E4M3), (BF16, BF16), (FP16, FP16)])
+@pytest.mark.parametrize("shape", range(len(MIDDLING_SHAPES)))
+@pytest.mark.parametrize("window, sinks", [(None, 0), (577, 40)])
+def test_middling_contexts(device, shape, dtype, kind, window, sinks):
+    c = Case(device, *MIDDLING_SHAPES[shape], dtype=dtype, kind=kind, seed=70 + shape)
+    check(c.attend(window=window, sinks=sinks), *c.expected(window, sinks))
+
+
+@pytest.mark.parametrize("k, heads, kv_heads, dim, dtype, kind", [(6, 20, 20, 80, FP16, E4M3), (7, 16, 4, 128, BF16, E4M3),
+                                                                (5, 8, 2, 64, BF16, BF16)])
+@pytest.mark.parametrize("window", [None, 600])
+def test_round_after_middling_contexts(device, k, heads, kv_heads, dim, dtype, kind, window):
+    c = Case(device, [1100, 605], [k + k * k] * 2, heads, kv_heads, dim, 32, dtype=dtype, kind=kind, seed=k)
+    bits, places = attention.round_mask(k, device=device)
+    see, want = oracle.round_rows(k)
+    at = (torch.tensor(c.contexts)[:, None] + want).flatten()
+    got = c.attend(mask=bits, positions=at.to(device), window=window, sinks=3)
+    check(got, *c.expected(window, 3, see, at))
+
+
+@pytest.mark.parametrize("kind", [E4M3, BF16])
+def test_nan_after_a_middling_context_stays_with_its_row(device, kind):
+    c = Case(device, [700], [3], 4, 2, 128, 64, kind=kind, seed=5)
+    want, tol = c.expected()
+    values = oracle.get_page(c.cache.v, c.cache.v_scale, int(c.table[0, 702 // 64]), 2, 64, 128, "v")
+    scale = 1.0 if kind == BF16 else c.cache.v_scale[int(c.table[0, 702 // 64])].cpu().double()[None, :, None]
+    values = values / scale
+    values[702 % 64] = math.nan
+    oracle.put_page(c.cache.v, int(c.table[0, 702 // 64]), values.float().to(kind), "v")
+    got = c.attend()
+    check(got[:2], want[:2], tol[:2])
+    assert got[2].isnan().all()
+
+
 @pytest.mark.parametrize("window, sinks", [(16, 4), (100, 40), (777, 19)])
 @pytest.mark.parametrize("dtype, kind", [(BF16, E4M3), (FP16, FP16)])
 def test_window_of_many_columns(device, window, sinks, dtype, kind):
