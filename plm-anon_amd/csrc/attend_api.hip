@@ -10,7 +10,7 @@ namespace plm {
 namespace {
 
 constexpr int64_t kNarrowWork = 24000;  // groups of 16 columns times steps
-constexpr int64_t kWideGroups = 320, kWideSteps = 100, kWideBytes = 448 * 1024;
+constexpr int64_t kWideGroups = 320, kWideSteps = 100, kWideAlone = 56, kWideBytes = 448 * 1024;
 
 struct AttendPlan {
   int columns;        // of a workgroup's tile
@@ -51,13 +51,14 @@ AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t
   const int64_t steps = seen(p.columns);
   // Workgroups that fill a CU take groups of middling length whole, with a wavefront's steps and the joining launch saved,
   // where all find a CU (`groups` counts a sequence's last tile twice). One CU reads about 60 GB/s from memory: few groups
-  // of many bytes are cut instead, but for those whose tiles share them. (Wide / not: 16 tokens after 1000, 16 heads of 128
-  // over 4 in 8 bits, 10.7 / 14.8 us, 64 after 1000 14.4 / 17, 64 after up to 3000 26 / 30; a round of 56 rows after 1000
-  // 11.7 / 14.4, after 2500 16.5 / 17.7, four of 42 through a window of 777 12.1 / 14.8. One token after 3000, 8 key heads,
-  // 20.7 / 15.6; 8 after 2000 in 16 bits 23.7 / 17.4; a round after 4007 22.5 / 18; up to 16 steps 8.7 / 8.4.)
+  // of many steps or bytes are cut instead, but for those whose tiles share them. (Wide / not: 16 tokens after 1000, 16
+  // heads of 128 over 4 in 8 bits, 10.7 / 14.8 us, 64 after 1000 14.4 / 17, 64 after up to 3000 26 / 30; a round of 56 rows
+  // after 1000 11.7 / 14.4, after 2500 16.5 / 17.7, four of 42 through a window of 777 12.2 / 14.8. One token after 3000, 8
+  // key heads, 20.7 / 15.6; 8 after 2000 in 16 bits 23.7 / 17.4; a round after 4007 22.5 / 18; up to 16 steps 8.7 / 8.4.)
   const int64_t bytes = steps * kStep * chunks * (e8 ? 128 : 256);  // of a group's keys and values
   p.wide = p.columns == 16 && attend_wide(e8, static_cast<int>(chunks)) > kWaves && p.groups <= kWideGroups &&
-           steps > 4 * kWaves && steps <= kWideSteps && (most > 16 || p.groups >= 128 || bytes <= kWideBytes);
+           steps > 4 * kWaves && steps <= kWideSteps &&
+           (most > 16 || p.groups >= 128 || (steps <= kWideAlone && bytes <= kWideBytes));
   // Not cut: what is short, a single sequence's groups, which are alike, where they fill the device, and groups that do
   // and cannot be much unlike. (Cut / not: two sequences of 131004 tokens 50 / 1029 us, 64 of 4500 on average 60 / 88, a
   // round over 4007 18 / 33; 32 windows of 1024 53 / 49, a prompt of 4096 rows 250 / 242, through a window 48 / 41.)
