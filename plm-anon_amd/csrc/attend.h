@@ -227,6 +227,38 @@ constexpr float kSlack = 6.0f;
 template <int DT>
 constexpr float kShift = DT == DT_F16 ? 8.0f : 0.0f;
 
+// 8-bit values under fp16 rows are taken as codes times (page scale / `ref`), the accumulators being in units of `ref`, a
+// power of two. Ratios in [2^-5, 2^6] make every code a normal fp16 number, so no bit is lost; where the scales of a
+// step's pages leave that range `ref` moves, and the accumulators with it, in fp32. A page that a row does not see, or
+// barely, thus takes nothing from the others. bf16 holds codes times any scale: its accumulators are in plain units.
+template <int DT, bool E8>
+constexpr bool kUnits = E8 && DT == DT_F16;
+// Pages below this are left out: no value of theirs, 448 times it at most, reaches half of fp16's least (2^-25).
+constexpr float kSilent = 0x1p-34f;
+
+// Moves `ref` to where the pages' scales `vs` (0: no page) have ratios in range; false where no place is, 2^11 apart.
+template <int N>
+__device__ __forceinline__ bool unit_for(const float (&vs)[N], float& ref) {
+  // Powers of two are compared by their bits, which the scalar unit does.
+  constexpr int step = 1 << 23;
+  int hi = 0, lo = 0x7f000000;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const int bits = __builtin_bit_cast(int, vs[u]), x = bits >= __builtin_bit_cast(int, kSilent) ? bits : 0;
+    hi = max(hi, x);
+    lo = x > 0 ? min(lo, x) : lo;
+  }
+  const int at = __builtin_bit_cast(int, ref);
+  if (hi == 0 || (hi - at <= 6 * step && at - lo <= 5 * step)) return true;
+  if (hi - lo > 11 * step) return false;
+  ref = __builtin_bit_cast(float, hi - lo > 5 * step ? lo + 5 * step : hi);
+  return true;
+}
+
+// What accumulators in units of `from` are multiplied by to be in units of `to`. (Bounded: scales that far apart are no
+// page's whose values fp16 holds, and zeros have to stay zeros.)
+__device__ __forceinline__ float unit_ratio(float from, float to) { return fminf(from / to, 0x1p120f); }
+
 // Token x of a step's 32: its place among the eight of the lanes that hold it.
 struct TokenOf {
   int slot, holder;
@@ -468,7 +500,7 @@ struct AttendWave {
   f32x4 o[NC][C][4];
   u32x4 q[NC][C][2];
   float m[NC], l[NC];
-  float ref;  // largest scale of the values so far: the accumulators are in its units
+  float ref;  // the accumulators' unit (kUnits)
   int page_id, page_first;  // lane i: page number page_first + i of the sequence
   float page_ks, page_vs;
 
@@ -496,21 +528,20 @@ struct AttendWave {
     if constexpr (E8) {
       page_ks = good ? fmaxf(a.cache.k_scale[static_cast<int64_t>(id) * a.cache.heads + head], kLeastScale) : kLeastScale;
       page_vs = good ? a.cache.v_scale[static_cast<int64_t>(id) * a.cache.heads + head] : 0.0f;
-      float most = page_vs;
-#pragma unroll
-      for (int x = 32; x > 0; x >>= 1) most = fmaxf(most, __shfl_xor(most, x));
-      most = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, most)));
-      if (most > ref) {
-        const float less = ref / most;
-        ref = most;
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[n][c][j] *= less;
-      }
     }
+  }
+
+  // The accumulators in units of `to`.
+  __device__ __forceinline__ void follow(float to) {
+    if (to == ref) return;
+    const float by = unit_ratio(ref, to);
+    ref = to;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][c][j] *= by;
   }
 
   __device__ __forceinline__ Place place(const AttendArgs& a, int b, int head, int t0, int last_page, int lane) {
@@ -590,8 +621,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
   // One step. Keys and values have one set of registers each, refilled for the wavefront's next step as soon as the
   // product that reads them is issued, so about a step's bytes are in flight throughout.
   // CAREFUL: a value that is not finite was met in a step that some columns do not see whole, where 0 * it would reach
-  // them. The walk is then done again with one token at a time in such steps: apart from the usual one, whose registers
-  // it would take.
+  // them, or a step's two pages have scales too far apart for one unit (unit_for). The walk is then done again with one
+  // token at a time in such steps: apart from the usual one, whose registers it would take.
   typename Wave::Place s;
   bool odd = false;
   auto step = [&](auto careful, int number) {
@@ -693,12 +724,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
       for (int i = 0; i < 4; ++i) p[n][i] = pack2<DT>(e[2 * i], e[2 * i + 1]);
     }
     // O^T += V^T P^T: operand j of a chunk has dimensions 4 (l % 16) + j as rows.
-    const float less = w.ref > 0.0f ? 1.0f / w.ref : 0.0f;
     float ratio[2] = {1.0f, 1.0f};
-    if constexpr (E8) {
+    bool apart = false;
+    auto ratios = [&]() {
+      const float less = kUnits<DT, E8> ? (w.ref > 0.0f ? 1.0f / w.ref : 0.0f) : 1.0f;
       ratio[0] = s.vs[0] * less;
       ratio[1] = s.vs[1] * less;
+    };
+    if constexpr (kUnits<DT, E8>) {
+      float ref = w.ref;
+      apart = !unit_for(s.vs, ref);
+      odd = odd || apart;
+      w.follow(ref);
     }
+    if constexpr (E8) ratios();
     auto values_of = [&](int c, int j) {
       u32x4 v;
 #pragma unroll
@@ -713,7 +752,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
       }
       return v;
     };
-    if (!CAREFUL || !edge) {
+    if (!CAREFUL || !(edge || apart)) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -723,18 +762,32 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
           for (int n = 0; n < NC; ++n) w.o[n][c][j] = mfma_16x16x32<DT>(v, p[n], w.o[n][c][j]);
         }
     } else {
+      if (!edge) {
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u32x4 v = values_of(c, j);
+        for (int n = 0; n < NC; ++n) seen[n] = ~0u;
+      }
+      // Units apart one after the other, each with its own page's scale for a unit of the accumulators.
+      const float first = s.vs[0], second = s.vs[1];
 #pragma unroll 1
-          for (int x = 0; x < kStep; ++x) {
-            const TokenOf t(x, g);
-#pragma unroll
-            for (int n = 0; n < NC; ++n) take_token<DT>(v & t.only, p[n] & t.only, t.seen(seen[n], 0, col), w.o[n][c][j]);
-          }
+      for (int u = 0; u < (apart ? 2 : 1); ++u) {
+        if (apart) {
+          const float to = u == 0 ? first : second;
+          if (to >= kSilent) w.follow(to);
+          ratios();
         }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const u32x4 v = values_of(c, j);
+#pragma unroll 1
+            for (int x = 16 * u; x < (apart ? 16 * u + 16 : kStep); ++x) {
+              const TokenOf t(x, g);
+#pragma unroll
+              for (int n = 0; n < NC; ++n) take_token<DT>(v & t.only, p[n] & t.only, t.seen(seen[n], 0, col), w.o[n][c][j]);
+            }
+          }
+      }
     }
     s = next;
     if (more) w.values(a, s, lane);
@@ -766,7 +819,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
     float* mine = shared + wave * kWaveFloats + lane * 4;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      const float scale = E8 ? w.ref : 1.0f;
+      const float scale = kUnits<DT, E8> ? w.ref : 1.0f;
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll

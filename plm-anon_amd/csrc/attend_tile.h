@@ -74,12 +74,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   __syncthreads();
 
   // Pages: lane i has number page_first + i of the sequence: the byte where its head begins (bit 0: it is not there,
-  // and page 0 is read) and its scales. fp16 values are staged in units of the largest scale of their pages so far
-  // (`ref`), which keeps codes times scale inside fp16; bf16 takes any scale.
+  // and page 0 is read) and its scales. fp16 values are staged in the accumulators' unit `ref` (kUnits): one for all 64
+  // pages where their scales allow it (`calm`), looked for at every set of tokens only where not (at every set throughout:
+  // 2048 rows of 32 heads of 64 60 us for 56).
   const uint32_t page_bytes = static_cast<uint32_t>(a.cache.page >> 4) * (C * kUnitBytes);  // of a head, 128 KiB at most
   uint32_t page_lo = 1, page_hi = 0;
   int page_first = -64;
   float page_ks = kLeastScale, page_vs = 0.0f, ref = 1.0f, next_ref = 1.0f;
+  bool calm = true;
+  auto first_lane = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); };
   auto pages = [&](int number) {
     page_first = number;
     const int at = number + lane;
@@ -93,11 +96,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       const int64_t of = good ? id * a.cache.heads + it.head : 0;
       page_ks = good ? fmaxf(a.cache.k_scale[of], kLeastScale) : kLeastScale;
       page_vs = good ? a.cache.v_scale[of] : 0.0f;
-      if constexpr (DT == DT_F16) {
-        float most = page_vs;
+      if constexpr (kUnits<DT, E8>) {
+        float most = page_vs >= kSilent ? page_vs : 0.0f, least = page_vs >= kSilent ? page_vs : __builtin_inff();
 #pragma unroll
-        for (int x = 32; x > 0; x >>= 1) most = fmaxf(most, __shfl_xor(most, x));
-        next_ref = fmaxf(next_ref, __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, most))));
+        for (int x = 32; x > 0; x >>= 1) {
+          most = fmaxf(most, __shfl_xor(most, x));
+          least = fminf(least, __shfl_xor(least, x));
+        }
+        const float of_all[2] = {first_lane(most), first_lane(fminf(least, most))};
+        next_ref = ref;
+        calm = unit_for(of_all, next_ref);
       }
     }
   };
@@ -138,7 +146,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
                        lane, inside, st.x[u]);
     }
   };
-  bool odd = false;  // staged a value that is not finite for columns that may not all look (see attend_kernel)
+  bool odd = false;  // staged a value that is not finite for columns that may not all look, or `apart` (see attend_kernel)
+  bool apart = false;  // the staged tokens' pages have no unit in common: their values are the codes themselves (0 of silent ones)
   auto store = [&](char* set) {
     if (!values_role) {
 #pragma unroll
@@ -157,8 +166,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
         }
       return;
     }
-    const float less = DT == DT_F16 ? (ref > 0.0f ? 1.0f / ref : 0.0f) : 1.0f;
-    const float r0 = st.vs[0] * less, r1 = st.vs[1] * less;
+    const float less = kUnits<DT, E8> ? (ref > 0.0f ? 1.0f / ref : 0.0f) : 1.0f;
+    auto ratio = [&](float vs) { return !apart ? vs * less : vs < kSilent ? 0.0f : 1.0f; };
+    const float r0 = ratio(st.vs[0]), r1 = ratio(st.vs[1]);
     const bool edge = walk.edge(st.t0) || st.held != 15u;
     // Tokens that are no one's, past the end or of a page that is not there, have values of zero.
     u32x4 keep = {~0u, ~0u, ~0u, ~0u};
@@ -192,6 +202,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       }
   };
 
+  auto value_scale = [&](int t0, int u) { return lane_float(page_vs, ((t0 + 16 * u) >> a.cache.page_shift) - page_first); };
+  auto move = [&](float to) {
+    if (to == ref) return;
+    const float by = unit_ratio(ref, to);
+    ref = to;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][c][j] *= by;
+  };
   auto compute = [&](auto careful, const char* set, int t0, const float (&ks)[4], uint32_t held) {
     constexpr bool CAREFUL = decltype(careful)::value;
     const bool edge = walk.edge(t0) || held != 15u;
@@ -272,7 +294,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       }
       l[n] += sum;
     }
-    if (!CAREFUL || !edge) {
+    if (!CAREFUL || !(edge || apart)) {
 #pragma unroll
       for (int pc = 0; pc < 2 * C; ++pc) {
         if (pc + 1 < 2 * C) read_values(pc + 1, x[(pc + 1) & 1]);
@@ -285,36 +307,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       return;
     }
     // One token at a time, as in attend_kernel.
+    if (!edge) {
 #pragma unroll
-    for (int pair = 0; pair < 2; ++pair)
+      for (int n = 0; n < NC; ++n) seen[n] = ~0u;
+    }
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(values + ((pair * C + c) * 4 + j) * 1024);
+    for (int pair = 0; pair < 2; ++pair) {
 #pragma unroll 1
-          for (int x = 0; x < 32; ++x) {
-            const TokenOf t(x, g);
-#pragma unroll
-            for (int n = 0; n < NC; ++n)
-              take_token<DT>(v & t.only, p[n][pair] & t.only, t.seen(seen[n], pair, col), o[n][c][j]);
-          }
+      for (int u = 0; u < (apart ? 2 : 1); ++u) {
+        if (apart) {
+          const float to = value_scale(t0, 2 * pair + u);
+          if (to >= kSilent) move(to);
         }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(values + ((pair * C + c) * 4 + j) * 1024);
+#pragma unroll 1
+            for (int x = 16 * u; x < (apart ? 16 * u + 16 : 32); ++x) {
+              const TokenOf t(x, g);
+#pragma unroll
+              for (int n = 0; n < NC; ++n)
+                take_token<DT>(v & t.only, p[n][pair] & t.only, t.seen(seen[n], pair, col), o[n][c][j]);
+            }
+          }
+      }
+    }
   };
 
-  // The accumulators follow `ref` when the set that was staged with the new one is up.
+  // The accumulators take the unit of the tokens to be staged once those before are multiplied.
   auto follow = [&]() {
-    if constexpr (E8 && DT == DT_F16) {
-      if (next_ref > ref) {
-        const float less = ref / next_ref;
-        ref = next_ref;
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[n][c][j] *= less;
+    if constexpr (kUnits<DT, E8>) {
+      float to = next_ref;
+      if (!calm) {
+        const float vs[4] = {value_scale(st.t0, 0), value_scale(st.t0, 1), value_scale(st.t0, 2), value_scale(st.t0, 3)};
+        to = ref;
+        apart = !unit_for(vs, to);
+        odd = odd || apart;
+      } else {
+        apart = false;
       }
+      move(to);
     }
   };
   auto begin = [&]() {
@@ -328,7 +362,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       l[n] = 0.0f;
     }
     page_first = -64;
-    ref = next_ref = E8 && DT == DT_F16 ? 0.0f : 1.0f;
+    ref = next_ref = kUnits<DT, E8> ? 0.0f : 1.0f;
   };
 
   begin();
@@ -365,7 +399,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     l[n] = column_sum(l[n]);
-    if constexpr (E8 && DT == DT_F16) {
+    if constexpr (kUnits<DT, E8>) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
