@@ -30,8 +30,9 @@ struct AttendArgs {
   const int64_t* positions;  // [total]; null: context + row
   const uint32_t* mask;      // [mask_rows, mask_words]; null: causal
   float* partials;           // slots of attend_slot_floats(columns, padded dim)
+  int64_t window;            // 0: none
   float scale;               // times log2 e
-  int heads, group, window, sinks, mask_rows, mask_words;
+  int heads, group, sinks, mask_rows, mask_words;
   int target;   // workgroups that the work is split over, at most; 0: never split
   float per_target;  // a little more than 1 / target
   int least;    // steps of a range, at least
@@ -46,6 +47,12 @@ constexpr int kJoinColumns = 8;  // columns that a workgroup of the joining laun
 
 __host__ __device__ constexpr int64_t attend_slot_floats(int columns, int padded) {
   return static_cast<int64_t>(columns) * (padded + 2);
+}
+
+// The first token of the window of a row at `position`, held to 2^30, which no cache's tokens reach. Positions and windows
+// are what the caller says, in 64 bits: neither needs to have to do with the cache's size.
+__device__ __forceinline__ int window_first(const AttendArgs& a, int64_t position) {
+  return position < a.window ? 0 : static_cast<int>(min(position - a.window + 1, int64_t{1} << 30));
 }
 
 // A sequence's share of the work, the same in every workgroup.
@@ -66,8 +73,7 @@ __device__ __forceinline__ AttendShare attend_share(const AttendArgs& a, int b) 
   if (a.window > 0) {
     // The first row's place says where the window begins: where a later row's is before it, the ranges get longer, and
     // that is all.
-    const int64_t place = a.positions != nullptr ? a.positions[seq.start] : seq.context;
-    lo = static_cast<int>(min(max(place + 1 - a.window, int64_t{0}), static_cast<int64_t>(hi) * kStep)) / kStep;
+    lo = min(window_first(a, a.positions != nullptr ? a.positions[seq.start] : seq.context) / kStep, hi);
   }
   s.steps = hi - lo + min((a.sinks + kStep - 1) / kStep, lo);
   return s;
@@ -291,7 +297,6 @@ struct AttendColumns {
 
   __device__ __forceinline__ void set(const AttendArgs& a, const KvSeq& seq, const AttendItem& it, int first, int columns,
                                       int col) {
-    constexpr int far = 1 << 30;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int x = first + 16 * n + col, y = min(x, columns - 1);
@@ -299,10 +304,7 @@ struct AttendColumns {
       row[n] = y / a.group;
       head[n] = it.head * a.group + y - row[n] * a.group;
       window_lo[n] = 0;
-      if (a.window > 0) {
-        const int64_t p = a.positions != nullptr ? a.positions[seq.start + row[n]] : seq.context + row[n];
-        window_lo[n] = max(static_cast<int>(min(max(p, static_cast<int64_t>(-far)), static_cast<int64_t>(far))) - a.window + 1, 0);
-      }
+      if (a.window > 0) window_lo[n] = window_first(a, a.positions != nullptr ? a.positions[seq.start + row[n]] : seq.context + row[n]);
     }
   }
 

@@ -123,7 +123,7 @@ int plm_attend(const plm_attend_call* call, void* workspace, size_t workspace_by
   a.scale = static_cast<float>(h.scale * 1.44269504088896340736);
   a.heads = static_cast<int>(h.heads);
   a.group = a.heads / a.cache.heads;
-  a.window = static_cast<int>(h.window < far ? h.window : 0);  // longer than any cache: no window
+  a.window = h.window;
   a.sinks = static_cast<int>(std::min(h.sinks, far));
   a.mask_rows = static_cast<int>(h.mask_rows);
   a.mask_words = static_cast<int>(h.mask_words);

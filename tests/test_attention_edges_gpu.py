@@ -86,3 +86,21 @@ def test_nan_among_pages_of_unlike_scales(device, heads, wider, page):
     fine = [e for e in range(64) if e not in (21, 35)]
     check(got[:, :, fine], want[:, :, fine], tol[:, :, fine])
     check(got[:first, :, 35], want[:first, :, 35], tol[:first, :, 35])
+
+
+@pytest.mark.parametrize("heads, wider", [(4, 0), (32, WIDE)])
+@pytest.mark.parametrize("mask", [False, True])
+def test_windows_and_positions_past_any_cache(device, heads, wider, mask):
+    """A window is as long as it says, and a position as far, whatever a cache can hold."""
+    c = Case(device, [60, 7], [9, 9], heads, 2, 64, 16, seed=64, wider=wider)
+    see = torch.ones(9, 9, dtype=torch.bool).tril() if mask else None
+    bits = torch.tensor([[(1 << (i + 1)) - 1] for i in range(9)], dtype=torch.int32).to(device) if mask else None
+    row = torch.arange(18)
+    for window, far in ((2 ** 30 - 1, 2 ** 30 + row), (2 ** 30, 2 ** 30 + 3 * row), (2 ** 29 + 5, 2 ** 31 + row),
+                        (10 ** 12, 10 ** 12 + 20 + row % 9), (10 ** 12, 10 ** 15 + row), (2 ** 62, 2 ** 62 + 2 * row),
+                        (2 ** 62, -(2 ** 63) + row), (5, -(2 ** 63) + row), (2 ** 63 - 1, 2 ** 63 - 1 - row)):
+        # The same visibility in small numbers: the window's first token, held to what a sequence has.
+        first = [max(int(p) - window + 1, 0) for p in far]
+        places = torch.tensor([min(f, 10 ** 6) + 99 for f in first])
+        want, tol = c.expected(window=100, sinks=2, see=see, places=places)
+        check(c.attend(window=window, sinks=2, positions=far.to(device), mask=bits), want, tol, f"window {window} at {int(far[0])}")
