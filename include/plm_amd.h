@@ -567,7 +567,7 @@ int plm_kv_read(const plm_read_call* call, void* stream);
  *     mask[i, j / 32] is set;
  * and with window > 0 of these only t > position - window or t < sinks, the position being positions[r]
  * (positions NULL: lengths[b] + i); under a mask the window holds for the context alone. A row that sees
- * nothing is zero. out: contiguous [total, heads, head_dim]. scale is positive.
+ * nothing is zero. out: contiguous [total, heads, head_dim]. scale: in [2^-62, 2^126].
  * Workspace: plm_attend_workspace_bytes (0: none needed), 16-byte aligned, of any content; calls that may
  * run at the same time need workspaces of their own.
  */

@@ -82,7 +82,9 @@ bool attend_of(const plm_attend_call* call, AttendArgs& a, AttendPlan& p) {
   const int64_t heads = a.cache.heads;
   if (h.heads < heads || h.heads > 4096 || h.heads % heads != 0 || h.rows.total * (h.heads / heads) >= (int64_t{1} << 30))
     return false;
-  if (h.window < 0 || h.sinks < 0 || !(h.scale > 0.0) || !(h.scale < 3.0e38)) return false;
+  // The kernels multiply scores by the scale times log2 e times a page's scale (2^-64 at least) in fp32: what is masked
+  // would be NaN if that were zero or infinite.
+  if (h.window < 0 || h.sinks < 0 || !(h.scale >= 0x1p-62 && h.scale <= 0x1p126)) return false;
   if (h.mask != nullptr && (h.mask_rows < 1 || h.mask_words < 1 || h.mask_rows >= (1 << 28) || h.mask_words >= (1 << 24)))
     return false;
   p = attend_plan(heads, a.cache.page, a.cache.dim, h.heads, h.rows.total, h.rows.seqs, h.rows.max_rows, h.rows.table_width,

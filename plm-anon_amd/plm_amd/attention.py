@@ -30,6 +30,7 @@ PAGES = (16, 32, 64, 128)
 MAX_HEAD_DIM = 256
 _TYPES = {torch.bfloat16: _lib.PLM_CACHE_BF16, torch.float16: _lib.PLM_CACHE_F16, torch.float8_e4m3fn: _lib.PLM_CACHE_E4M3}
 LEAST_SCALE = 2.0 ** -64   # of an 8-bit page that holds nothing but zeros
+_SCALES = (2.0 ** -62, 2.0 ** 126)   # of the scores: times log2 e and a page's scale neither zero nor infinite in fp32
 
 
 def _shapes(pages: int, kv_heads: int, page: int, head_dim: int, e4m3: bool) -> tuple[tuple, tuple]:
@@ -265,8 +266,8 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: tor
         raise ValueError(f"window must be at least 1 token, got {window}")
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
-    if scale is not None and not 0 < scale < math.inf:
-        raise ValueError(f"scale must be positive, got {scale}")
+    if scale is not None and not _SCALES[0] <= scale <= _SCALES[1]:
+        raise ValueError(f"scale must be in [2^-62, 2^126], got {scale}")
     mask_at, mask_rows, mask_words = 0, 0, 0
     if mask is not None:
         most = rows[2]

@@ -104,3 +104,11 @@ def test_windows_and_positions_past_any_cache(device, heads, wider, mask):
         places = torch.tensor([min(f, 10 ** 6) + 99 for f in first])
         want, tol = c.expected(window=100, sinks=2, see=see, places=places)
         check(c.attend(window=window, sinks=2, positions=far.to(device), mask=bits), want, tol, f"window {window} at {int(far[0])}")
+
+
+@pytest.mark.parametrize("heads, wider", [(4, 0), (32, WIDE)])
+def test_least_scale(device, heads, wider):
+    """Masked tokens of pages of zeros, whose scale is the least there is, at the least scale of the scores."""
+    c = Case(device, [45], [12], heads, 1, 64, 16, seed=72, wider=wider)
+    c.cache.k_scale.fill_(attention.LEAST_SCALE)
+    check(c.attend(scale=2.0 ** -62), *c.expected(scale=2.0 ** -62))

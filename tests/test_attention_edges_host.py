@@ -1,0 +1,30 @@
+"""CPU checks of what the paged attention's calls refuse or hold to, at the ends of what they are given."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from plm_amd import _lib, attention
+from test_attention_host import _call, _stub
+
+LEAST, MOST = 2.0 ** -62, 2.0 ** 126
+
+
+@pytest.mark.parametrize("scale, fine", [(LEAST, True), (MOST, True), (1e-9, True), (1e9, True), (LEAST * (1 - 2 ** -20), False),
+                                         (MOST * (1 + 2 ** -20), False), (1e-30, False), (5e-324, False), (2.5e38, False)])
+def test_scales_that_single_precision_cannot_hold(scale, fine):
+    """A scale that fp32 turns into zero or infinity, by itself or times a page's, would make what is masked NaN."""
+    f = 1 << 20
+    handle = _lib.KvCache(f, f, f, f, 4, 2, 32, 64, _lib.PLM_CACHE_E4M3)
+    call = _lib.pack_attend(0, ctypes.addressof(handle), 6, 2, 3, f, 64, 64, f, 0, f, 256, 64, 4, f, 0, 0, 0, 0, 0, 0, scale)
+    lib = _lib.lib()
+    # A wide table needs a workspace: what is right is refused for want of it, before any launch.
+    assert lib.plm_attend(call, None, 0, None) == (-4 if fine else -1)
+    assert (lib.plm_attend_workspace_bytes(call) > 0) == fine
+    if not fine:
+        c = _call()
+        with pytest.raises(ValueError):
+            attention.attend(_stub(), c["q"], c["table"], c["lengths"], scale=scale)
