@@ -486,8 +486,9 @@ size_t plm_voronoi_assign_workspace_bytes(int64_t n_problems, int64_t n_targets,
  *
  * Rows of a call: `total` rows of `seqs` sequences, one after the other; sequence b's are
  * [row_starts[b], row_starts[b + 1]) (row_starts NULL: max_rows each, total = seqs * max_rows), at most
- * max_rows of them, and follow a context of lengths[b] tokens: row i is token lengths[b] + i. Token t
- * of sequence b is in page table[b, t / page] (int32, row stride table_stride, table_width entries).
+ * max_rows of them, and follow a context of lengths[b] tokens: row i is token lengths[b] + i. row_starts
+ * do not fall; rows that no sequence holds (before the first start, past the last one or past max_rows of
+ * a sequence) are not stored, and are zero in q_out and out. Token t of sequence b is in page table[b, t / page] (int32, row stride table_stride, table_width entries).
  * lengths, row_starts and positions are int64, all on the device. An entry outside [0, pages) is a page
  * that is not there: rows for it are not stored, its tokens are not seen, they read as zeros. Row
  * tensors have their dimensions contiguous; q_row, q_head, ... are strides in elements, multiples of 8;

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   const AttendItem it = attend_item<COLS, false>(a, blockIdx.x, lane);
-  if (it.ranges == 0) return;
+  if (it.ranges == 0) return attend_clear(a, it.idle, lane);
   const KvSeq& seq = it.seq;
   const int columns = seq.rows * a.group;
   const int end = seq.context + seq.rows;

@@ -58,6 +58,24 @@ __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int b, int page_shift) 
   return s;
 }
 
+// Rows [first, end) between sequence b's and the next one's (b = -1: before the first; `seq`: kv_seq of b), which no sequence
+// holds: gaps of row_starts, rows past max_rows, rows past the last start. Results have zeros there.
+struct KvGap {
+  int first, end;
+};
+
+__device__ __forceinline__ KvGap kv_gap(const KvRows& r, int b, const KvSeq& seq) {
+  if (r.starts == nullptr) return {0, 0};
+  const int64_t next = b + 1 < r.seqs ? min(max(r.starts[b + 1], int64_t{0}), static_cast<int64_t>(r.total)) : r.total;
+  return {b < 0 ? 0 : seq.start + seq.rows, static_cast<int>(next)};
+}
+
+// Zeros in the gap's rows of `out` ([rows, 8 row8] of 16 bits), taken by thread `at` of `threads`.
+__device__ __forceinline__ void kv_clear(uint16_t* out, const KvGap& gap, int64_t row8, int64_t at, int64_t threads) {
+  for (int64_t x = gap.first * row8 + at; x < gap.end * row8; x += threads)
+    reinterpret_cast<u32x4*>(out)[x] = u32x4{0u, 0u, 0u, 0u};
+}
+
 // Two e4m3 codes of a word as the model's type, times the power of two `scale` (exact, but for fp16
 // results below 2^-14, which keep fp16's absolute step).
 template <int DT>

@@ -160,6 +160,11 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, int block) {
   const bool paired = rotary > 0 && !a.side_by_side && (half & 7) == 0;
   const int places = paired ? (dim - half) >> 3 : dim >> 3, per_row = places * a.heads;
   const int at = (block - b * a.q_blocks) * 256 + static_cast<int>(threadIdx.x), i = at / per_row;
+  if (a.rows.starts != nullptr) {
+    const int64_t row8 = static_cast<int64_t>(a.heads) * (dim >> 3), threads = static_cast<int64_t>(a.q_blocks) * 256;
+    if (b == 0) kv_clear(a.q_out, kv_gap(a.rows, -1, seq), row8, at, threads);
+    kv_clear(a.q_out, kv_gap(a.rows, b, seq), row8, at, threads);
+  }
   if (i >= seq.rows) return;
   const int rest = at - i * per_row, head = rest / places, place = rest - head * places;
   const int64_t row = seq.start + i;

@@ -10,10 +10,11 @@ and attn-out linears.
 * ``round_mask`` — mask and places of a round's k + k*k rows.
 
 Rows are packed: ``total`` rows of ``seqs`` sequences one after the other, sequence b's in
-``[row_starts[b], row_starts[b + 1])`` (``None``: the same number each). They follow ``lengths[b]``
-cached tokens; token t of sequence b lies in page ``table[b, t // page]``. ``lengths``, ``row_starts`` and
-``positions`` are int64 tensors on the GPU and are never read on the host, so every call can be captured
-in a HIP graph and replayed as the sequences grow; only ``max_rows`` (the longest sequence's rows) and the
+``[row_starts[b], row_starts[b + 1])`` (``None``: the same number each). Rows that no sequence holds (before
+the first start, past the last one, past ``max_rows`` of a sequence) are not stored and come back as zeros, so a
+captured batch can be padded. A sequence's rows follow ``lengths[b]`` cached tokens; token t of sequence b lies
+in page ``table[b, t // page]``. ``lengths``, ``row_starts`` (which do not fall) and ``positions`` are int64
+tensors on the GPU and are never read on the host, so every call can be captured in a HIP graph and replayed as the sequences grow; only ``max_rows`` (the longest sequence's rows) and the
 tensors' shapes size a launch. Table entries outside the cache are pages that are not there.
 """
 

@@ -112,3 +112,90 @@ def test_least_scale(device, heads, wider):
     c = Case(device, [45], [12], heads, 1, 64, 16, seed=72, wider=wider)
     c.cache.k_scale.fill_(attention.LEAST_SCALE)
     check(c.attend(scale=2.0 ** -62), *c.expected(scale=2.0 ** -62))
+
+
+def _spoil(device, shape, dtype):
+    """Leaves memory of ``shape`` full of NaN to the next allocation."""
+    x = torch.full(shape, math.nan, dtype=dtype, device=device)
+    torch.cuda.synchronize()
+    del x
+
+
+# Rows of three sequences (the second without any) among rows that are no one's: before the first, past max_rows of the
+# third, after the last.
+PLACES, STARTS, MOST = [2, 3, 4, 5, 6, 7], [2, 5, 5, 9], 3
+
+
+@pytest.mark.parametrize("heads, dim, wider", [(4, 64, 0), (32, 64, WIDE), (4, 256, 0), (64, 80, WIDE)])
+@pytest.mark.parametrize("context", [40, 5000])
+@pytest.mark.parametrize("total", [12, 1500])
+def test_rows_of_no_sequence_are_zero(device, heads, dim, wider, context, total):
+    c = Case(device, [context, 5, 90], [3, 0, 3], heads, 1, dim, 64, seed=65, wider=wider)
+    q = torch.randn(total, heads, dim).to(BF16)
+    q[PLACES] = c.q
+    q = q.to(device)
+    want, tol = c.expected()
+    rest = [r for r in range(total) if r not in PLACES]
+    starts = torch.tensor(STARTS, device=device)
+    for window in (None, 10 ** 6):
+        _spoil(device, q.shape, BF16)
+        got = attention.attend(c.cache, q, c.calls["table"], c.calls["lengths"], row_starts=starts, max_rows=MOST, window=window)
+        check(got[PLACES], want, tol)
+        assert torch.equal(got[rest].cpu(), torch.zeros(len(rest), heads, dim, dtype=BF16))
+
+
+@pytest.mark.parametrize("kind", [E4M3, FP16])
+@pytest.mark.parametrize("total", [12, 1500])
+@pytest.mark.parametrize("side", [False, True])
+def test_appended_rows_of_no_sequence_are_zero(device, kind, total, side):
+    a, b = (Case(device, [40, 5, 90], [3, 0, 3], 4, 2, 80, 16, dtype=FP16, kind=kind, seed=66) for _ in range(2))
+    angle = torch.arange(200, dtype=torch.float64)[:, None] * 100.0 ** (-torch.arange(16, dtype=torch.float64) / 16)
+    rope = torch.cat((angle.cos(), angle.sin()), 1).float().to(device)
+    want = attention.append_kv(a.cache, a.q.to(device), a.k.to(device), a.v.to(device), **a.calls, rope=rope, interleaved=side)
+    rows = []
+    for x in (b.q, b.k, b.v):
+        y = torch.randn(total, *x.shape[1:]).to(FP16)
+        y[PLACES] = x
+        rows.append(y.to(device))
+    _spoil(device, rows[0].shape, FP16)
+    got = attention.append_kv(b.cache, *rows, b.calls["table"], b.calls["lengths"], rope=rope, interleaved=side,
+                              row_starts=torch.tensor(STARTS, device=device), max_rows=MOST)
+    assert torch.equal(got[PLACES], want)
+    rest = [r for r in range(total) if r not in PLACES]
+    assert torch.equal(got[rest].cpu(), torch.zeros(len(rest), 4, 80, dtype=FP16))
+    for x, y in ((a.cache.k, b.cache.k), (a.cache.v, b.cache.v)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("heads, wider", [(4, 0), (32, WIDE)])
+def test_many_sequences_among_rows_of_none(device, heads, wider):
+    """Gaps after every sequence of more than a wavefront's lanes of them."""
+    n = 150
+    c = Case(device, [(31 * b) % 190 for b in range(n)], [2] * n, heads, 1, 16, 16, seed=67, wider=wider)
+    starts = [1]
+    for b in range(n):
+        starts.append(starts[-1] + 2 + (b % 3 == 0))     # a row past max_rows
+    held = [s + i for s in starts[:-1] for i in (0, 1)]
+    total = starts[-1] + 3
+    q = torch.randn(total, heads, 16).to(BF16)
+    q[held] = c.q
+    q = q.to(device)
+    want, tol = c.expected()
+    _spoil(device, q.shape, BF16)
+    got = attention.attend(c.cache, q, c.calls["table"], c.calls["lengths"], row_starts=torch.tensor(starts, device=device), max_rows=2)
+    check(got[held], want, tol)
+    rest = [r for r in range(total) if r not in held]
+    assert rest and got[rest].abs().max() == 0
+
+
+@pytest.mark.parametrize("kind", [E4M3, BF16])
+def test_ragged_rows_without_their_most(device, kind):
+    """row_starts alone: launches go by the rows in all."""
+    a, b = (Case(device, [33, 250, 1000, 4], [3, 1, 65, 0], 8, 2, 64, 32, kind=kind, seed=68) for _ in range(2))
+    calls = {k: x for k, x in a.calls.items() if k != "max_rows"}
+    check(attention.attend(a.cache, a.q.to(device), **calls), *a.expected())
+    q1 = attention.append_kv(a.cache, a.q.to(device), a.k.to(device), a.v.to(device), **calls)
+    q2 = attention.append_kv(b.cache, b.q.to(device), b.k.to(device), b.v.to(device), **b.calls)
+    assert torch.equal(q1, q2)
+    for x, y in ((a.cache.k, b.cache.k), (a.cache.v, b.cache.v)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
