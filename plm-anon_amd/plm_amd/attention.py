@@ -40,8 +40,8 @@ def _shapes(pages: int, kv_heads: int, page: int, head_dim: int, e4m3: bool) -> 
 
 
 class PagedCache:
-    """Keys and values of ``kv_heads`` heads in pages of 16, 32, 64 or 128 tokens. The tensors are used as they
-    are, in the order the matrix instructions read (``include/plm_amd.h`` states it): 16-bit
+    """Keys and values of ``kv_heads`` heads in pages of 16, 32, 64 or 128 tokens. The tensors, which stay the
+    handle's, are used as they are, in the order the matrix instructions read (``include/plm_amd.h`` states it): 16-bit
     ``k [pages, kv_heads, page / 16, ceil(head_dim / 64), 2, 4, 16, 8]`` and ``v [.., 2, 4, 16, 2, 4]``, or e4m3
     ``k [.., 4, 16, 16]`` and ``v [.., 4, 16, 4, 4]`` with float32 ``k_scale`` and ``v_scale``
     ``[pages, kv_heads]``, powers of two. Dimensions past ``head_dim`` hold zeros. ``PagedCache.empty``
@@ -79,6 +79,16 @@ class PagedCache:
                                     0 if v_scale is None else v_scale.data_ptr(), pages, heads, page, head_dim,
                                     _TYPES[k.dtype])
         self._ref = ctypes.addressof(self._handle)
+
+    # What the kernels were told once stays: another tensor in a cache's place would leave them its freed memory, another
+    # size a shape that the checks of a call and the kernels see differently.
+    def __setattr__(self, name: str, value) -> None:
+        if name in self.__dict__:
+            raise AttributeError(f"a cache's {name} stays as it is; make another PagedCache")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name: str) -> None:
+        raise AttributeError(f"a cache keeps its {name}")
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, *, page: int = 64,

@@ -28,3 +28,17 @@ def test_scales_that_single_precision_cannot_hold(scale, fine):
         c = _call()
         with pytest.raises(ValueError):
             attention.attend(_stub(), c["q"], c["table"], c["lengths"], scale=scale)
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "dtype", "device"])
+def test_a_cache_stays_what_it_was_made_of(name):
+    """The handle holds addresses and sizes: another tensor in their place would leave it with freed memory."""
+    cache = _stub()
+    if not hasattr(cache, name):
+        setattr(cache, name, torch.zeros(1))
+    held = getattr(cache, name)
+    with pytest.raises(AttributeError):
+        setattr(cache, name, held)
+    with pytest.raises(AttributeError):
+        delattr(cache, name)
+    assert getattr(cache, name) is held
