@@ -14,8 +14,10 @@ Rows are packed: ``total`` rows of ``seqs`` sequences one after the other, seque
 the first start, past the last one, past ``max_rows`` of a sequence) are not stored and come back as zeros, so a
 captured batch can be padded. A sequence's rows follow ``lengths[b]`` cached tokens; token t of sequence b lies
 in page ``table[b, t // page]``. ``lengths``, ``row_starts`` (which do not fall) and ``positions`` are int64
-tensors on the GPU and are never read on the host, so every call can be captured in a HIP graph and replayed as the sequences grow; only ``max_rows`` (the longest sequence's rows) and the
-tensors' shapes size a launch. Table entries outside the cache are pages that are not there.
+tensors on the GPU and are never read on the host, so every call can be captured in a HIP graph and replayed as
+the sequences grow; only ``max_rows`` (the longest sequence's rows) and the tensors' shapes size a launch. Table
+entries outside the cache are pages that are not there. Nothing here has a backward: tensors that require a
+gradient are refused while gradients are recorded.
 """
 
 from __future__ import annotations
@@ -131,6 +133,8 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, cache: P
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.get_device() != cache._index:
         raise RuntimeError(f"{name} must be on the cache's GPU {cache.device}, got {t.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, and the cache's calls have none: detach it, or call under no_grad")
     at = t.data_ptr()
     if at % 16 == 0:
         if t.is_contiguous():

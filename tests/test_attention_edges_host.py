@@ -42,3 +42,19 @@ def test_a_cache_stays_what_it_was_made_of(name):
     with pytest.raises(AttributeError):
         delattr(cache, name)
     assert getattr(cache, name) is held
+
+
+def test_gradients_are_refused():
+    """There is no backward: an output without a graph would lose a gradient in silence."""
+    for name in ("q", "k", "v"):
+        c = _call()
+        c[name].requires_grad_()
+        with pytest.raises(RuntimeError, match="gradient"):
+            attention.append_kv(_stub(), c["q"], c["k"], c["v"], c["table"], c["lengths"])
+        if name == "q":
+            with pytest.raises(RuntimeError, match="gradient"):
+                attention.attend(_stub(), c["q"], c["table"], c["lengths"])
+    with torch.no_grad():      # past the refusal: 5 rows of 2 sequences
+        q = torch.zeros(5, 4, 64, dtype=torch.bfloat16, requires_grad=True)
+        with pytest.raises(ValueError, match="row_starts"):
+            attention.attend(_stub(), q, c["table"], c["lengths"])
