@@ -17,6 +17,7 @@
 
 #include <type_traits>
 
+#include "attend_plan.h"
 #include "kv_cache.h"
 
 namespace plm {
@@ -39,15 +40,6 @@ struct AttendArgs {
   int whole;    // a group of so many steps is not cut
   int wide;     // workgroups of attend_wide wavefronts, where that is more
 };
-
-constexpr int kStep = 32;        // tokens of a step
-constexpr int kWaves = 4;        // wavefronts of a workgroup, but for wide ones (attend_wide)
-constexpr int kAttendMost = 64;  // ranges per group, at most
-constexpr int kJoinColumns = 8;  // columns that a workgroup of the joining launch takes at a time, at most
-
-__host__ __device__ constexpr int64_t attend_slot_floats(int columns, int padded) {
-  return static_cast<int64_t>(columns) * (padded + 2);
-}
 
 // The first token of the window of a row at `position`, held to 2^30, which no cache's tokens reach. Positions and windows
 // are what the caller says, in 64 bits: neither needs to have to do with the cache's size.
@@ -596,17 +588,6 @@ struct AttendWave {
     for (int u = 0; u < 2; ++u) load_unit<E8, C, ONCE>(a.cache.v, s.at[u], lane, 4 * (lane & 15) < a.cache.dim - 64 * (C - 1), v[u]);
   }
 };
-
-// Wavefronts per SIMD to leave registers for: as many as hold the accumulators, the queries and a step's keys and
-// values without spilling (512 registers over them).
-constexpr int attend_waves(bool e8, int chunks, int nc) {
-  if (chunks == 1) return nc == 1 ? 4 : 3;
-  if (chunks == 2) return e8 && nc == 1 ? 3 : 2;
-  return e8 || chunks == 3 ? 2 : 1;
-}
-
-// Wavefronts of a workgroup that fills a CU.
-constexpr int attend_wide(bool e8, int chunks) { return 4 * attend_waves(e8, chunks, 1); }
 
 // 16 NC columns. Bound, where contexts are long, by the bytes of the keys and values, each read once and used by one
 // wavefront: hence no LDS in the loop, and a key head's whole group of queries as columns of one tile. 64 sequences of

@@ -1,78 +1,11 @@
 // C ABI of the attention over the paged cache (plm_attend), declared in include/plm_amd.h.
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
-
 #include "attend.h"
 #include "plm_amd.h"
 
 namespace plm {
 namespace {
-
-constexpr int64_t kNarrowWork = 24000;  // groups of 16 columns times steps
-constexpr int64_t kWideGroups = 320, kWideSteps = 100, kWideAlone = 56, kWideBytes = 448 * 1024;
-
-struct AttendPlan {
-  int columns;        // of a workgroup's tile
-  int target, least, whole, wide;  // AttendArgs
-  int64_t grid, groups, bytes;
-};
-
-// The launch of a call, from what the host knows: sizes, never the lengths. The work is cut on the device
-// (attend_item), so a wide table costs nothing; `grid` bounds the workgroups that any lengths can ask for:
-// one per group and as many more as the work is cut into.
-AttendPlan attend_plan(int64_t kv_heads, int64_t page, int64_t head_dim, int64_t heads, int64_t total, int64_t seqs,
-                       int64_t max_rows, int64_t table_width, int64_t window, int64_t sinks, bool mask, bool e8) {
-  AttendPlan p{};
-  const int64_t group = heads / kv_heads, chunks = (head_dim + 63) / 64;
-  const int64_t most = max_rows * group;
-  // What a tile of columns sees at most: all the table holds, or with a window the rows' own span of it.
-  const int64_t far = int64_t{1} << 30;
-  const auto seen = [&](int64_t columns) {
-    const int64_t all = (table_width * page + kStep - 1) / kStep, span = mask ? max_rows : std::min(max_rows, columns / group + 2);
-    return window > 0 ? std::min(all, (std::min(window, far) + std::min(sinks, far) + span) / kStep + 3) : all;
-  };
-  // Tiles of 16 columns, whose four wavefronts take different tokens, are done soonest while all of a call's are short of
-  // work for the device; wider ones need less of it. (Rounds of 56 rows over 500 / 4007 / 16000 tokens, 16 heads over 4:
-  // 10.0 / 18.4 / 35 us against 18.7 / 21.3 / 34; four sequences' over 2000, 32 heads over 8, 41.5 against 40.5.) Up to
-  // 96 tokens there is nothing to take apart. 128 columns need half the loads and conversions of 64, once there are tiles
-  // of them for all CUs (4096 rows after 4096 tokens: 266 against 340 us on the same card); short walks end more evenly in
-  // smaller tiles (prompts through a window of 512: 42 us in 128 columns, 40 in 64).
-  const int64_t narrow = kv_heads * (seqs + total * group / 16);
-  const bool many = most > 256 && kv_heads * (total * group / 128) >= (seen(128) < 24 ? 2048 : 256);
-  if (most <= 16 || (seen(16) > 3 && narrow * seen(16) <= kNarrowWork)) p.columns = 16;
-  else if (chunks <= 2 && most <= 32) p.columns = 32;
-  else p.columns = chunks <= 2 && many ? 128 : 64;
-  p.groups = kv_heads * (seqs + total * group / p.columns);
-  // Ranges are joined by a second launch and each has a walk's beginning and end: 5 to 8 us that a cut has to win back.
-  // A step of 32 tokens takes a quarter of about 0.8 us (up to 32 columns, a step per wavefront) or half of 1.2 us.
-  p.least = p.columns <= 32 ? 16 : 8;
-  p.whole = p.columns <= 32 ? 32 : 20;
-  const int64_t steps = seen(p.columns);
-  // Workgroups that fill a CU take groups of middling length whole, with a wavefront's steps and the joining launch saved,
-  // where all find a CU (`groups` counts a sequence's last tile twice). One CU reads about 60 GB/s from memory: few groups
-  // of many steps or bytes are cut instead, but for those whose tiles share them. (Wide / not: 16 tokens after 1000, 16
-  // heads of 128 over 4 in 8 bits, 10.7 / 14.8 us, 64 after 1000 14.4 / 17, 64 after up to 3000 26 / 30; a round of 56 rows
-  // after 1000 11.7 / 14.4, after 2500 16.5 / 17.7, four of 42 through a window of 777 12.2 / 14.8. One token after 3000, 8
-  // key heads, 20.7 / 15.6; 8 after 2000 in 16 bits 23.7 / 17.4; a round after 4007 22.5 / 18; up to 16 steps 8.7 / 8.4.)
-  const int64_t bytes = steps * kStep * chunks * (e8 ? 128 : 256);  // of a group's keys and values
-  p.wide = p.columns == 16 && attend_wide(e8, static_cast<int>(chunks)) > kWaves && p.groups <= kWideGroups &&
-           steps > 4 * kWaves && steps <= kWideSteps &&
-           (most > 16 || p.groups >= 128 || (steps <= kWideAlone && bytes <= kWideBytes));
-  // Not cut: what is short, a single sequence's groups, which are alike, where they fill the device, and groups that do
-  // and cannot be much unlike. (Cut / not: two sequences of 131004 tokens 50 / 1029 us, 64 of 4500 on average 60 / 88, a
-  // round over 4007 18 / 33; 32 windows of 1024 53 / 49, a prompt of 4096 rows 250 / 242, through a window 48 / 41.)
-  const bool full = p.groups - kv_heads >= 256;
-  p.target = !p.wide && steps > p.whole && !(full && (seqs == 1 || steps <= 4 * p.least)) ? 512 : 0;
-  p.grid = p.groups + p.target;
-  // There are 2 * target ranges of groups of several at most: a cut sequence has less than twice load / chunk of
-  // them, and a chunk is load / target at least. Such a group has two at least.
-  if (p.target > 0) {
-    p.groups = std::min<int64_t>(p.groups, p.target);
-    p.bytes = 2 * p.target * attend_slot_floats(p.columns, static_cast<int>(64 * chunks)) * 4;
-  }
-  return p;
-}
 
 // The plan of a call whose numbers go together; false where they do not.
 bool attend_of(const plm_attend_call* call, AttendArgs& a, AttendPlan& p) {

@@ -199,3 +199,14 @@ def test_ragged_rows_without_their_most(device, kind):
     assert torch.equal(q1, q2)
     for x, y in ((a.cache.k, b.cache.k), (a.cache.v, b.cache.v)):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("contexts, rows, heads, kv_heads, dim, kind, window", [
+    ([1800, 700, 33] * 13, [1] * 39, 8, 8, 128, BF16, 1797),     # 312 groups of up to 59 steps
+    ([900, 640], [110, 110], 20, 4, 64, E4M3, 529),              # 280
+    ([1000] * 65, [1] * 65, 4, 4, 16, E4M3, None),               # 260, without a window
+])
+def test_groups_past_the_cus(device, contexts, rows, heads, kv_heads, dim, kind, window):
+    """A few more groups of middling length than CUs."""
+    c = Case(device, contexts, rows, heads, kv_heads, dim, 128, kind=kind, seed=69)
+    check(c.attend(window=window, sinks=2 if window else 0), *c.expected(window, 2 if window else 0))
