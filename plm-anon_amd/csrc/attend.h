@@ -39,6 +39,7 @@ struct AttendArgs {
   int least;    // steps of a range, at least
   int whole;    // a group of so many steps is not cut
   int wide;     // workgroups of attend_wide wavefronts, where that is more
+  int walkers;  // workgroups of the launch that walk; those after them clear (kv_clear)
 };
 
 // The first token of the window of a row at `position`, held to 2^30, which no cache's tokens reach. Positions and windows
@@ -101,7 +102,6 @@ __device__ __forceinline__ float wave_total(float v) {
 struct AttendItem {
   int b, tile, head, range, ranges;  // ranges == 0: nothing to do
   int slot;                          // the group's first partial slot; its ranges' are `heads` slots apart
-  int64_t idle;                      // with nothing to do: which such workgroup of the launch
   KvSeq seq;
 };
 
@@ -159,25 +159,12 @@ __device__ __forceinline__ AttendItem attend_item(const AttendArgs& a, int index
     items += __builtin_amdgcn_readlane(to, 63);
     slots += __builtin_amdgcn_readlane(slot_to, 63);
   }
-  it.idle = static_cast<int64_t>(index) - items;
   return it;
 }
 
-// A workgroup without work clears its share of the rows that no sequence holds. The launch has one at least where there are
-// such rows, and as many as their tiles would have been.
-__device__ __forceinline__ void attend_clear(const AttendArgs& a, int64_t idle, int lane) {
-  if (a.rows.starts == nullptr) return;
-  const int64_t threads = (static_cast<int64_t>(gridDim.x) - blockIdx.x + idle) * blockDim.x;
-  for (int base = -1; base < a.rows.seqs; base += 64) {
-    const int b = base + lane;
-    KvGap gap = {0, 0};
-    if (b < a.rows.seqs) gap = kv_gap(a.rows, b, b < 0 ? KvSeq{0, 0, 0} : kv_seq(a.rows, b, a.cache.page_shift));
-    for (uint64_t some = __ballot(gap.end > gap.first); some != 0; some &= some - 1) {
-      const int at = __builtin_ctzll(some);
-      kv_clear(a.out, {__builtin_amdgcn_readlane(gap.first, at), __builtin_amdgcn_readlane(gap.end, at)},
-               static_cast<int64_t>(a.heads) * (a.cache.dim >> 3), idle * blockDim.x + threadIdx.x, threads);
-    }
-  }
+__device__ __forceinline__ void attend_clear(const AttendArgs& a) {
+  kv_clear(a.rows, a.cache.page_shift, a.out, static_cast<int64_t>(a.heads) * (a.cache.dim >> 3), blockIdx.x - a.walkers,
+           gridDim.x - a.walkers);
 }
 
 // The larger of two, NaN if either is: unlike fmaxf it needs no quieting of its operands, and three values are one
@@ -603,8 +590,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_w
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
+  if (static_cast<int>(blockIdx.x) >= a.walkers) return attend_clear(a);
   const AttendItem it = attend_item<COLS, false>(a, blockIdx.x, lane);
-  if (it.ranges == 0) return attend_clear(a, it.idle, lane);
+  if (it.ranges == 0) return;
   const KvSeq& seq = it.seq;
   const int columns = seq.rows * a.group;
 

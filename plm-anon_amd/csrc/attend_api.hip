@@ -22,7 +22,8 @@ bool attend_of(const plm_attend_call* call, AttendArgs& a, AttendPlan& p) {
     return false;
   p = attend_plan(heads, a.cache.page, a.cache.dim, h.heads, h.rows.total, h.rows.seqs, h.rows.max_rows, h.rows.table_width,
                   h.window, h.sinks, h.mask != nullptr, h.cache->type == PLM_CACHE_E4M3);
-  if (h.rows.row_starts != nullptr) p.grid += 1;  // a workgroup without work, for rows without a sequence (attend_clear)
+  a.walkers = static_cast<int>(std::min(p.grid, (int64_t{1} << 31) - 1));
+  p.grid += kv_clear_groups(a.rows, h.heads * (a.cache.dim / 8));
   return p.grid < (int64_t{1} << 31);
 }
 

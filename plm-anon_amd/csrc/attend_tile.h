@@ -39,8 +39,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
+  if (static_cast<int>(blockIdx.x) >= a.walkers) return attend_clear(a);
   const AttendItem it = attend_item<COLS, false>(a, blockIdx.x, lane);
-  if (it.ranges == 0) return attend_clear(a, it.idle, lane);
+  if (it.ranges == 0) return;
   const KvSeq& seq = it.seq;
   const int columns = seq.rows * a.group;
   const int end = seq.context + seq.rows;

@@ -160,11 +160,6 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, int block) {
   const bool paired = rotary > 0 && !a.side_by_side && (half & 7) == 0;
   const int places = paired ? (dim - half) >> 3 : dim >> 3, per_row = places * a.heads;
   const int at = (block - b * a.q_blocks) * 256 + static_cast<int>(threadIdx.x), i = at / per_row;
-  if (a.rows.starts != nullptr) {
-    const int64_t row8 = static_cast<int64_t>(a.heads) * (dim >> 3), threads = static_cast<int64_t>(a.q_blocks) * 256;
-    if (b == 0) kv_clear(a.q_out, kv_gap(a.rows, -1, seq), row8, at, threads);
-    kv_clear(a.q_out, kv_gap(a.rows, b, seq), row8, at, threads);
-  }
   if (i >= seq.rows) return;
   const int rest = at - i * per_row, head = rest / places, place = rest - head * places;
   const int64_t row = seq.start + i;
@@ -435,7 +430,8 @@ __device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq&
   }
 }
 
-// A workgroup has a page of one head's keys or values (8 bits), 256 units of it (16 bits), or 256 places of queries, all
+// A workgroup has a page of one head's keys or values (8 bits), 256 units of it (16 bits), 256 places of queries or a share of
+// the rows that no sequence holds, all
 // in one launch: what is bound by latency then waits once. Every row is read once, every code written once, in pieces of 8
 // or 16 bytes that lie side by side over the lanes as the units' order has them. Bound by memory where rows are many: 5327
 // rows of prompts, 16 heads of 128 over 4 in 8 bits, 15.1 us for 63 MB, 4.2 TB/s; 650 rows of 32 heads of 80 over 32 in 16
@@ -445,7 +441,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ float red[4];
   int block = blockIdx.x;
   if (block >= a.kv_blocks) {
-    append_queries<DT>(a, block - a.kv_blocks);
+    const int clears = a.kv_blocks + a.q_blocks * a.rows.seqs;
+    if (block < clears) append_queries<DT>(a, block - a.kv_blocks);
+    else kv_clear(a.rows, a.cache.page_shift, a.q_out, static_cast<int64_t>(a.heads) * (a.cache.dim >> 3), block - clears, gridDim.x - clears);
     return;
   }
   const bool values = block & 1;
@@ -634,10 +632,11 @@ int plm_kv_append(const plm_append_call* call, void* stream) {
   const int64_t places = half > 0 && !a.side_by_side && half % 8 == 0 ? (a.cache.dim - half) / 8 : a.cache.dim / 8;
   const int64_t q_items = h.q == nullptr ? 0 : max_rows * places * h.heads;
   const int64_t q_blocks = (q_items + 255) / 256;
-  if (kv_blocks + q_blocks * seqs >= (int64_t{1} << 31) || q_items >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
+  const int64_t clears = h.q == nullptr ? 0 : plm::kv_clear_groups(a.rows, h.heads * (a.cache.dim / 8));
+  if (kv_blocks + q_blocks * seqs + clears >= (int64_t{1} << 31) || q_items >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   a.kv_blocks = static_cast<int>(kv_blocks);
   a.q_blocks = static_cast<int>(q_blocks);
-  const unsigned grid = static_cast<unsigned>(kv_blocks + q_blocks * seqs);
+  const unsigned grid = static_cast<unsigned>(kv_blocks + q_blocks * seqs + clears);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (h.dtype == PLM_BF16) e8 ? plm::append_go<plm::DT_BF16, true>(a, grid, s) : plm::append_go<plm::DT_BF16, false>(a, grid, s);
   else e8 ? plm::append_go<plm::DT_F16, true>(a, grid, s) : plm::append_go<plm::DT_F16, false>(a, grid, s);
