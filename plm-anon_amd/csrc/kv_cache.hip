@@ -31,12 +31,27 @@ struct AppendArgs {
 };
 
 // a c + b s in fp32. `close` gets the bit where that is within its error, 2^-23 of the larger term at most, of a place where
-// 8-bit codes may part: at most four bits of mantissa, so 19 zeros at the end.
-__device__ __forceinline__ float turn_one(float a, float c, float b, float s, int bit, uint32_t& close) {
+// 8-bit codes may part: at most four bits of mantissa, so 19 zeros at the end. `near` is twice that error, kNear, or less than
+// nothing for a cosine of 1 and a sine of 0, which are exact and leave about one value in eight on a border. Zeros are too.
+constexpr float kNear = 0x1p-22f;
+__device__ __forceinline__ float turn_one(float a, float c, float b, float s, float near, int bit, uint32_t& close) {
   const float part = b * s, sum = fmaf(a, c, part);
   const float border = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, sum) + 0x40000u) & 0xfff80000u);
-  close |= fabsf(sum - border) <= 0x1p-22f * fmaxf(fabsf(part), fabsf(sum)) ? 1u << bit : 0u;
+  close |= fabsf(sum - border) < near * fmaxf(fabsf(part), fabsf(sum)) ? 1u << bit : 0u;
   return sum;
+}
+
+// `near` of a group of pairs: of all of them at once, which the positions that turn nothing have alike.
+template <int N>
+__device__ __forceinline__ float near_of(const float (&c)[N], const float (&s)[N]) {
+  float turned = fabsf(s[0]), least = c[0], most = c[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) {
+    turned = fmaxf(turned, fabsf(s[k]));
+    least = fminf(least, c[k]);
+    most = fmaxf(most, c[k]);
+  }
+  return turned == 0.0f && least == 1.0f && most == 1.0f ? -1.0f : kNear;
 }
 
 // Dimension e of a row, turned in fp64, which holds the products exactly, to the fp32 value on either side whose last bit
@@ -72,21 +87,24 @@ __device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float*
     for (int i = 0; i < 8; ++i)
       if (e0 + i < rotary) out[i] = __builtin_nanf("");
   } else if (side_by_side && (half & 3) == 0 && e0 + 8 <= rotary) {
-    const f32x4 c = *reinterpret_cast<const f32x4*>(turn + (e0 >> 1)), s = *reinterpret_cast<const f32x4*>(turn + half + (e0 >> 1));
+    float c[4], s[4];
+    *reinterpret_cast<f32x4*>(c) = *reinterpret_cast<const f32x4*>(turn + (e0 >> 1));
+    *reinterpret_cast<f32x4*>(s) = *reinterpret_cast<const f32x4*>(turn + half + (e0 >> 1));
+    const float near = near_of(c, s);
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       const float a = out[i], b = out[i + 1];
-      out[i] = turn_one(a, c[i / 2], -b, s[i / 2], i, close);
-      out[i + 1] = turn_one(b, c[i / 2], a, s[i / 2], i + 1, close);
+      out[i] = turn_one(a, c[i / 2], -b, s[i / 2], near, i, close);
+      out[i + 1] = turn_one(b, c[i / 2], a, s[i / 2], near, i + 1, close);
     }
   } else if (side_by_side) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       if (e0 + i < rotary) {
-        const float c = turn[(e0 + i) >> 1], s = turn[half + ((e0 + i) >> 1)];
+        const float c[1] = {turn[(e0 + i) >> 1]}, s[1] = {turn[half + ((e0 + i) >> 1)]}, near = near_of(c, s);
         const float a = out[i], b = out[i + 1];
-        out[i] = turn_one(a, c, -b, s, i, close);
-        out[i + 1] = turn_one(b, c, a, s, i + 1, close);
+        out[i] = turn_one(a, c[0], -b, s[0], near, i, close);
+        out[i + 1] = turn_one(b, c[0], a, s[0], near, i + 1, close);
       }
     }
   } else if ((half & 7) == 0) {
@@ -100,10 +118,11 @@ __device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float*
       *reinterpret_cast<f32x4*>(c + i) = *reinterpret_cast<const f32x4*>(at + i);
       *reinterpret_cast<f32x4*>(s + i) = *reinterpret_cast<const f32x4*>(at + half + i);
     }
+    const float near = near_of(c, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float o = from_bits16<DT>(static_cast<uint16_t>(other[i / 2] >> (16 * (i & 1))));
-      out[i] = turn_one(out[i], c[i], low ? -o : o, s[i], i, close);
+      out[i] = turn_one(out[i], c[i], low ? -o : o, s[i], near, i, close);
     }
   } else {
 #pragma unroll
@@ -113,7 +132,8 @@ __device__ __forceinline__ void rotated8(const uint16_t* x, int e0, const float*
         const bool low = e < half;
         const float o = from_bits16<DT>(x[low ? e + half : e - half]);
         const int at = low ? e : e - half;
-        out[i] = turn_one(out[i], turn[at], low ? -o : o, turn[half + at], i, close);
+        const float c[1] = {turn[at]}, s[1] = {turn[half + at]};
+        out[i] = turn_one(out[i], c[0], low ? -o : o, s[0], near_of(c, s), i, close);
       }
     }
   }
@@ -139,12 +159,13 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
 template <int DT>
 __device__ __forceinline__ void turned8(u32x4 lo, u32x4 hi, const float (&c)[8], const float (&s)[8], uint32_t& close, float* x,
                                         float* y) {
+  const float near = near_of(c, s);
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float p = from_bits16<DT>(static_cast<uint16_t>(lo[k / 2] >> (16 * (k & 1))));
     const float q = from_bits16<DT>(static_cast<uint16_t>(hi[k / 2] >> (16 * (k & 1))));
-    x[k] = turn_one(p, c[k], -q, s[k], k, close);
-    y[k] = turn_one(q, c[k], p, s[k], 8 + k, close);
+    x[k] = turn_one(p, c[k], -q, s[k], near, k, close);
+    y[k] = turn_one(q, c[k], p, s[k], near, 8 + k, close);
   }
 }
 
@@ -316,8 +337,9 @@ __device__ __forceinline__ void append_page_fp8(const AppendArgs& a, const KvSeq
     new_values<DT, VALUES>(a, seq, p[u], base, head, x[u], bits);
     close[u / 4] |= static_cast<uint64_t>(bits) << (16 * (u % 4));
   }
-  // About one value in 2^16 is that close: one at a time, from memory. (All keys in fp64 from the start: prompts 25.3 us
-  // for 22.9, single tokens 9.8 for 9.5; without any of it 22.1 and 8.9.)
+  // About one turned value in 2^16 is that close: one at a time, from memory. (All keys in fp64 from the start: prompts 25.3
+  // us for 22.9, single tokens 9.8 for 9.5; without any of it 22.1 and 8.9. 2048 rows of 4 heads of 256 in pages of 128 take
+  // 18 us, and 17 if they are zeros or do not turn; with those taken for close 221 and 71.)
   if constexpr (!VALUES) {
     while ((close[0] | close[1]) != 0) {
       const int word = close[0] != 0 ? 0 : 1, i = 64 * word + __builtin_ctzll(word == 0 ? close[0] : close[1]);

@@ -210,3 +210,34 @@ def test_groups_past_the_cus(device, contexts, rows, heads, kv_heads, dim, kind,
     """A few more groups of middling length than CUs."""
     c = Case(device, contexts, rows, heads, kv_heads, dim, 128, kind=kind, seed=69)
     check(c.attend(window=window, sinks=2 if window else 0), *c.expected(window, 2 if window else 0))
+
+
+def _append_us(cache, k, v, table, lengths, rope, interleaved):
+    def times(n):
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        for _ in range(n):
+            attention.append_kv(cache, None, k, v, table, lengths, rope=rope, interleaved=interleaved)
+        end.record()
+        torch.cuda.synchronize()
+        return begin.elapsed_time(end) * 1e3 / n
+
+    times(5)
+    return min(times(20) for _ in range(5))
+
+
+@pytest.mark.parametrize("side", [False, True])
+def test_keys_that_need_no_rounding_cost_no_more(device, side):
+    """Zero rows (padding), and rows at position 0, are turned exactly in fp32: they do not go one by one through fp64, which
+    takes 128 turns per thread here. The factor is far from both: about 1, and about 10."""
+    cache = attention.PagedCache.empty(16, 4, 256, page=128, device=device)
+    table = torch.arange(16, dtype=torch.int32, device=device)[None]
+    zero = torch.zeros(1, dtype=torch.int64, device=device)
+    k, v = (torch.randn(2048, 4, 256, device=device).bfloat16() for _ in range(2))
+    angle = torch.arange(2048, dtype=torch.float64)[:, None] * 100.0 ** (-torch.arange(128, dtype=torch.float64) / 128)
+    rope = torch.cat((angle.cos(), angle.sin()), 1).float().to(device)
+    still = torch.cat((torch.ones(2048, 128), torch.zeros(2048, 128)), 1).to(device)
+    usual = _append_us(cache, k, v, table, zero, rope, side)
+    zeros = _append_us(cache, torch.zeros_like(k), v, table, zero, rope, side)
+    first = _append_us(cache, k, v, table, zero, still, side)
+    assert zeros < 3 * usual and first < 3 * usual, (usual, zeros, first)
