@@ -121,7 +121,8 @@ def main() -> None:
         end.record()
         length += x.shape[0]
     torch.cuda.synchronize()
-    print(f"prompt of {a.prompt} tokens: its last chunk {1e3 * begin.elapsed_time(end):.1f} us")
+    if a.prompt:
+        print(f"prompt of {a.prompt} tokens: its last chunk {1e3 * begin.elapsed_time(end):.1f} us")
 
     mask, places = attention.round_mask(a.k, device=dev)
     x = torch.randn(rows, a.hidden, generator=g, device=dev).bfloat16()

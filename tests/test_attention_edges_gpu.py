@@ -6,6 +6,9 @@ Tolerances are those of test_attention_gpu.py, whose cases these are."""
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -241,3 +244,11 @@ def test_keys_that_need_no_rounding_cost_no_more(device, side):
     zeros = _append_us(cache, torch.zeros_like(k), v, table, zero, rope, side)
     first = _append_us(cache, k, v, table, zero, still, side)
     assert zeros < 3 * usual and first < 3 * usual, (usual, zeros, first)
+
+
+def test_the_command_without_a_prompt(device):
+    package = Path(__file__).resolve().parents[1] / "plm-anon_amd"
+    done = subprocess.run([sys.executable, "-m", "plm_amd.attention_layer", "--prompt", "0", "--rounds", "3", "--cache", "model"],
+                          cwd=package, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stderr[-2000:]
+    assert "3 rounds of 56 rows from 0 tokens on" in done.stdout and "finite True" in done.stdout
