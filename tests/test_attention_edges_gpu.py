@@ -252,3 +252,29 @@ def test_the_command_without_a_prompt(device):
                           cwd=package, capture_output=True, text=True, timeout=100)
     assert done.returncode == 0, done.stderr[-2000:]
     assert "3 rounds of 56 rows from 0 tokens on" in done.stdout and "finite True" in done.stdout
+
+
+@pytest.mark.parametrize("dtype, kind", [(BF16, E4M3), (FP16, E4M3), (BF16, BF16), (FP16, FP16)])
+@pytest.mark.parametrize("shape, wider", [
+    (([7], [1], 8, 2, 64, 64), 0),
+    (([30, 8, 0], [1] * 3, 4, 4, 128, 16), 0),
+    (([300, 40], [5, 2], 20, 4, 80, 32), 0),
+    (([130], [56], 4, 1, 256, 64), 0),
+    (([20, 0, 3], [3, 1, 2], 10, 1, 64, 16), WIDE),      # 32 columns
+    (([3000], [2], 16, 2, 128, 64), 0),                  # cut and joined
+])
+def test_probabilities_are_not_rounded_to_the_models_type(device, shape, wider, dtype, kind):
+    """Up to 32 columns the output's rounding is the only one of the type's: probabilities come in two parts, each off by half
+    a step of what is left, 2^-16 in bf16 and 2^-22 in fp16 of a probability, or half of fp16's least, 2^-25 / 2^8."""
+    c = Case(device, *shape, dtype=dtype, kind=kind, seed=73, wider=wider)
+    want, tol = c.expected()
+    half = torch.finfo(dtype).eps / 2
+    sizes, most = [], 0.0
+    for b, (n, r) in enumerate(zip(c.contexts, c.rows)):
+        k, v = c.tokens("k", b, n + r), c.tokens("v", b, n + r)
+        q = c.q[c.starts[b]:c.starts[b + 1]]
+        _, size, score = oracle.attention(q, k, v, oracle.seen(n, r, n + r, None, 0, None, None), 1 / math.sqrt(c.dim))
+        off = 2 * (2.0 ** -24 * (c.dim + 12) * score + 2.0 ** -20) + (n + r) * 2.0 ** -24 + half * half
+        sizes.append(off * size + (n + r) * 2.0 ** -33 * float(v.abs().max()))
+    off = torch.cat(sizes)
+    check(c.attend(), want, off * (1 + half) + half * want.abs() + (2.0 ** -25 if dtype == FP16 else 0.0))
