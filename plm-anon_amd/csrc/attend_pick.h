@@ -33,10 +33,12 @@ hipError_t attend_stream_go(const AttendArgs& a, unsigned grid, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Where a tile holds all of a sequence's columns its keys and values are read by no one else and need not stay in the
-// caches: from memory 64 tokens over 288352, 16 heads of 128 over 4 in 8 bits, take 62 to 64 us so and 70 to 72
+// Where a tile holds all of a sequence's columns its keys and values are read by no other tile of the sequence and need not
+// stay in the caches: from memory 64 tokens over 288352, 16 heads of 128 over 4 in 8 bits, take 62 to 64 us so and 70 to 72
 // otherwise, 32 windows of 1024 in 16 bits 51.4 and 58.5; what the Infinity Cache holds takes the same. Rounds of 42 rows,
-// three tiles of which read the same, are slower so: 16.6 against 15.6 us.
+// three tiles of which read the same, are slower so: 16.6 against 15.6 us. So are sequences that share most of their pages,
+// which sizes do not tell: 64 tokens after 4600 of which 4096 are the same 38.3 against 37.1 us (57.5 and 65.4 where nothing
+// is), 256 after 2100, 2048 the same, 58 against 54, 32 after 2300 in 16 bits and 16 key heads, 2048 the same, 46 against 39.
 template <int DT, bool E8, int C, int NC>
 hipError_t attend_stream(const AttendArgs& a, unsigned grid, hipStream_t s) {
   const bool once = static_cast<int64_t>(a.rows.max_rows) * a.group <= 16 * NC;
