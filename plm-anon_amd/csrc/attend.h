@@ -5,8 +5,8 @@
 //
 // Orientation: a wavefront computes S^T = K Q^T (16 tokens x 16 columns per MFMA chain, a column being
 // one query: row * group + head of the group) and O^T = V^T P^T. The accumulator registers of S^T (lane
-// l: tokens 4 (l / 16) + r of column l % 16) are, rounded, the B operand of the second product with no
-// move between lanes, since the values are laid out for that order of tokens (kv_cache.h); the output
+// l: tokens 4 (l / 16) + r of column l % 16) are, rounded (and, up to 32 columns, once more what that
+// loses), the B operand of the second product with no move between lanes, since the values are laid out for that order of tokens (kv_cache.h); the output
 // comes out with 16 consecutive dimensions per lane. Keys and values go from memory straight into
 // operand registers: 16 bytes per lane, 1 KiB per load, no LDS.
 //
@@ -587,7 +587,7 @@ struct AttendWave {
 // 4500 tokens on average, 16 heads of 128 over 4 in 8 bits: 62 us for 296 MB, 4.8 TB/s with the join (a large copy reaches
 // 5.1); two of 131004 tokens 51 us for 268 MB, 5.3 TB/s; 32 windows of 1024 tokens, 16 key heads in 16 bits, 49 us for 270
 // MB, 5.5 TB/s. Where they are short, by a workgroup's beginning and end (arguments, lengths, table, scales, first loads, join:
-// 6000 to 7000 cycles): 500 tokens 7 us. Four wavefronts per workgroup there (with eight the first of these took 70 us); groups of
+// 6000 to 7000 cycles): 500 tokens 6.7 us. Four wavefronts per workgroup there (with eight the first of these took 70 us); groups of
 // middling length that all find a CU are taken whole by as many as it holds (attend_plan).
 template <int DT, bool E8, int C, int NC, bool ONCE, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(attend_waves(E8, C, NC)))) void attend_kernel(AttendArgs a) {

@@ -10,10 +10,11 @@
 //
 // Bound by three things in turn, which the two wavefronts that a SIMD holds overlap in part: the vector units (per score
 // a scaling, an exponential, a sum, half a maximum and half a rounding), the matrix cores, and LDS, from which every
-// wavefront reads every operand for its 32 columns. 4096 rows after 4096 tokens, 16 heads of 128 over 4 in 8 bits: 240 us
-// or 858 TFLOP/s of visible pairs (a product of 8192^3 reaches 1122), the vector units busy for 56 % of the cycles, the
+// wavefront reads every operand for its 32 columns. 4096 rows after 4096 tokens, 16 heads of 128 over 4 in 8 bits: 242 us
+// or 853 TFLOP/s of visible pairs (a product of 8192^3 reaches 1122), the vector units busy for 56 % of the cycles, the
 // matrix cores for 40 %, LDS for about 58 %. At heads of 64 there are half the products to a score: 3381 rows through
-// windows of 512, 32 heads over 8, 39 us or 310 TFLOP/s, 62 % and 17 %. Measured without gain: loads two steps ahead, the
+// windows of 512, 32 heads over 8, 38.5 us or 316 TFLOP/s, 62 % and 17 %, 12 vector instructions to each of 60 million walked
+// scores (48 million are visible), one of them the exponential. Measured without gain: loads two steps ahead, the
 // sums of exponentials by a product with ones, raised priority around the products, no maxima but where a sum shows that
 // one has grown (248 us for 242).
 #pragma once
@@ -291,8 +292,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
           sum += e[r];
         }
         // Rounded once to the model's type. (In two parts, as attend_kernel has them: 324 us for 242 at 4096 rows after 4096
-        // tokens, 42 for 37.5 through a window, since here the matrix cores and vector units are what bounds. Of outputs that
-        // are rounded themselves the error against 64 bits is 1.3 times the output's rounding alone, 0.0023 for 0.0017 in bf16.)
+        // tokens, 42 for 37.5 through a window, since here the matrix cores and vector units are what bounds; over 8-bit pages
+        // in fp16, whose products cost the same, 3 to 8 % more for the values' units. Of outputs that are rounded themselves
+        // the error against 64 bits is 1.3 times the output's rounding alone, 0.0023 for 0.0017 in bf16.)
         p[n][u / 2][2 * (u & 1)] = pack2<DT>(e[0], e[1]);
         p[n][u / 2][2 * (u & 1) + 1] = pack2<DT>(e[2], e[3]);
       }

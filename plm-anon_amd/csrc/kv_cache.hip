@@ -455,9 +455,10 @@ __device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq&
 // A workgroup has a page of one head's keys or values (8 bits), 256 units of it (16 bits), 256 places of queries or a share of
 // the rows that no sequence holds, all
 // in one launch: what is bound by latency then waits once. Every row is read once, every code written once, in pieces of 8
-// or 16 bytes that lie side by side over the lanes as the units' order has them. Bound by memory where rows are many: 5327
-// rows of prompts, 16 heads of 128 over 4 in 8 bits, 15.1 us for 63 MB, 4.2 TB/s; 650 rows of 32 heads of 80 over 32 in 16
-// bits 9.4 us for 20 MB, 2.1 TB/s, a beginning of 4 us to it; 32 single tokens 5.6 us, all latency.
+// or 16 bytes that lie side by side over the lanes as the units' order has them. Bound by memory and the vector units (busy for
+// 69 % of the cycles) where rows are many: 5327 rows of prompts, 16 heads of 128 over 4 in 8 bits, 15.6 us for 63 MB, 4.0
+// TB/s; 650 rows of 32 heads of 80 over 32 in 16 bits 9.6 us for 20 MB, 2.1 TB/s, a beginning of 4 us to it; 32 single tokens
+// 5.6 us, all latency.
 template <int DT, bool E8, int UPT>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ float red[4];
@@ -505,8 +506,10 @@ struct ReadArgs {
 };
 
 // Pages back as rows. Thread: keys, 8 dimensions of one token; values, 8 dimensions of the 4 tokens that share their
-// words. Bound by latency and memory: 1007 tokens of 32 sequences, 4 heads of 128 in 8 bits, 4.7 us; 5459 tokens of four
-// 8.2 us for 17 MB, 2.0 TB/s; 895 tokens of 32 heads of 80 in 16 bits 7.5 us for 18 MB, 2.4 TB/s.
+// words. Bound by latency and, where tokens are many, by the vector units, which find the addresses (about 100 instructions per
+// 16 bytes written, four divisions by sizes known at run time among them; busy for 62 % of the cycles): 1007 tokens of 32
+// sequences, 4 heads of 128 in 8 bits, 4.9 us; 5459 tokens of four 8.4 us for 17 MB, 23 with the zeros behind them; 895 tokens
+// of 32 heads of 80 in 16 bits 7.5 us for 18 MB.
 template <int DT, bool E8>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const KvCache& c = a.cache;

@@ -267,7 +267,7 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: tor
     j % 32 of word j // 32 set where row i sees row j; the same for every sequence) it sees the context and those
     rows. With ``window`` it sees of these the tokens after ``position - window`` and the first ``sinks``, the
     position being ``positions[row]`` or the row's token number; under a mask the window holds for the context
-    alone. A row that sees nothing is zero. ``scale`` is 1 / sqrt(head_dim) unless given."""
+    alone. A row that sees nothing is zero. ``scale`` is 1 / sqrt(head_dim) unless given, in [2^-62, 2^126]."""
     if q.dim() != 3 or q.shape[0] < 1:
         raise ValueError(f"q must be [rows, heads, {cache.head_dim}] with at least one row, got {list(q.shape)}")
     dim, dtype = cache.head_dim, q.dtype
