@@ -453,8 +453,7 @@ __device__ __forceinline__ void append_page_16(const AppendArgs& a, const KvSeq&
 }
 
 // A workgroup has a page of one head's keys or values (8 bits), 256 units of it (16 bits), 256 places of queries or a share of
-// the rows that no sequence holds, all
-// in one launch: what is bound by latency then waits once. Every row is read once, every code written once, in pieces of 8
+// the rows that no sequence holds, all in one launch: what is bound by latency then waits once. Every row is read once, every code written once, in pieces of 8
 // or 16 bytes that lie side by side over the lanes as the units' order has them. Bound by memory and the vector units (busy for
 // 69 % of the cycles) where rows are many: 5327 rows of prompts, 16 heads of 128 over 4 in 8 bits, 15.6 us for 63 MB, 4.0
 // TB/s; 650 rows of 32 heads of 80 over 32 in 16 bits 9.6 us for 20 MB, 2.1 TB/s, a beginning of 4 us to it; 32 single tokens
