@@ -7,8 +7,8 @@
 // one query: row * group + head of the group) and O^T = V^T P^T. The accumulator registers of S^T (lane
 // l: tokens 4 (l / 16) + r of column l % 16) are, rounded (and, up to 32 columns, once more what that
 // loses), the B operand of the second product with no move between lanes, since the values are laid out
-// for that order of tokens (kv_cache.h); the output comes out with 16 consecutive dimensions per lane. Keys and values go from memory straight into
-// operand registers: 16 bytes per lane, 1 KiB per load, no LDS.
+// for that order of tokens (kv_cache.h); the output comes out with 16 consecutive dimensions per lane.
+// Keys and values go from memory straight into operand registers: 16 bytes per lane, 1 KiB per load, no LDS.
 //
 // A workgroup's wavefronts (four, or as many as a CU holds) take the steps of 32 tokens of one range of one (sequence,
 // tile of columns, key head) in turn, and are joined through LDS at the end. Ranges of the same (sequence, tile, head)
