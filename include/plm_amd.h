@@ -588,6 +588,84 @@ typedef struct plm_attend_call {
 int plm_attend(const plm_attend_call* call, void* workspace, size_t workspace_bytes, void* stream);
 size_t plm_attend_workspace_bytes(const plm_attend_call* call);
 
+/*
+ * 8-bit rows: e4m3 codes with a power of two per block of 128 along K, for activations [M, K] and weights [N, K].
+ * A block's scale is the least power of two s with (largest finite magnitude) <= 448 s, at least 2^-64, and a code the
+ * value over s, rounded to the nearest, ties to even; what is not finite becomes NaN. Rows have a scale each per block
+ * of K; a weight's are made for 128 x 128 (plm_fp8_weight) and kept per row.
+ *
+ * Order of the bytes, in fragments of 16 rows x 128 of K, ceil(rows / 16) x ceil(K / 128) of them. With f = row / 16,
+ * r = row % 16, b = k / 128:
+ *   codes   [b][f][k / 64 % 2][k / 16 % 4][r][k % 16]
+ *   scales  [b / 4][f][r][b % 4], the exponent + 127 in a byte
+ * Codes past K are zeros, rows past the last of any content. plm_fp8_codes_bytes, plm_fp8_scales_bytes: the sizes (0
+ * where there are no such rows: 1 <= rows < 2^28, 8 <= K <= 2^24, K % 8 == 0). A gate/up weight (gate rows first, N a
+ * multiple of 32) has its halves' fragments in turn: fragment 2 j has gate rows [16 j, 16 j + 16), 2 j + 1 the up
+ * rows; a half's blocks of 128 rows begin with its first.
+ */
+enum plm_fp8_out { PLM_FP8_BF16 = 0, PLM_FP8_F16 = 1, PLM_FP8_F32 = 2 };
+size_t plm_fp8_codes_bytes(int64_t rows, int64_t k);
+size_t plm_fp8_scales_bytes(int64_t rows, int64_t k);
+
+/*
+ * Rows x [rows, k] of `dtype` (row stride x_row, a multiple of 8) into 8 bits (norm 0: no residual, weight, sum or y), or
+ * with norm: t = x + residual (residual, sum NULL: x), rounded to dtype and stored in `sum`; t weight / sqrt(mean(t^2) +
+ * eps) (weight [k] of dtype, NULL: ones) into y in `dtype`, or where y is NULL into 8 bits. The norm's codes are what
+ * its exact value rounds to. sum and y are contiguous [rows, k]; every pointer is 16-byte aligned; eps in [2^-100, 2^100].
+ */
+typedef struct plm_fp8_rows_call {
+  int64_t dtype, rows, k;
+  const void* x;
+  int64_t x_row;
+  int64_t norm;
+  const void* residual;
+  int64_t residual_row;
+  void* sum;
+  const void* weight;
+  double eps;
+  void* y;
+  void* codes;
+  void* scales;
+} plm_fp8_rows_call;
+int plm_fp8_rows(const plm_fp8_rows_call* call, void* stream);
+
+/*
+ * A weight [n, k] (row stride ld) into 8 bits: `w` of `dtype`, 16-byte aligned, ld % 8 == 0, rounded with scales per 128 x
+ * 128; or, where `blocks` is not NULL, e4m3 codes (8-byte aligned, ld % 8 == 0) whose scales blocks [blocks of rows, blocks of
+ * K] (with gate_up the gate half's blocks of rows, then the up half's) are powers of two in [2^-126, 2^126].
+ */
+typedef struct plm_fp8_weight_call {
+  int64_t dtype, n, k;
+  const void* w;
+  int64_t ld;
+  const float* blocks;
+  int64_t gate_up;
+  void* codes;
+  void* scales;
+} plm_fp8_weight_call;
+int plm_fp8_weight(const plm_fp8_weight_call* call, void* stream);
+
+/* The values that 8-bit rows stand for, contiguous [rows, k] in `out_type` (plm_fp8_out), 16-byte aligned; gate_up: a
+ * gate/up weight's, gate rows first. */
+int plm_fp8_values(const void* codes, const void* scales, int64_t rows, int64_t k, int32_t gate_up, int32_t out_type, void* y,
+                   void* stream);
+
+/*
+ * y[m, n] = x[m, k] . w[n, k]^T of 8-bit rows, summed in fp32 and rounded once to `out` (plm_fp8_out); with act, over a
+ * gate/up weight, y[m, n / 2] = g / (1 + e^-g) * u of the halves' products, in fp32 up to the one rounding. ldy in
+ * elements, at least y's columns. m <= 2^21.
+ */
+typedef struct plm_fp8_linear_call {
+  int64_t m, n, k;
+  const void* x;
+  const void* x_scales;
+  const void* w;
+  const void* w_scales;
+  void* y;
+  int64_t ldy, out, act;
+} plm_fp8_linear_call;
+int plm_fp8_linear(const plm_fp8_linear_call* call, void* stream);
+
 /* Human-readable name of a status code. */
 const char* plm_status_string(int32_t status);
 

@@ -1,0 +1,91 @@
+// Rows of e4m3 codes with a power of two per block of 128 along K, as the 8-bit kernels see them: activations [M, K]
+// and weights [N, K] alike.
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 rows by 16 columns over 128 of K and takes a power of two for each
+// row and each column (32 of K at a time; all four are the block's here), so a block's scales cost no instruction of
+// their own and the sum over blocks is one chain of such products in fp32. Where in K a lane's 32 bytes lie is free as long
+// as both operands agree. With r = row % 16, f = row / 16, b = k / 128, h = k / 64 % 2, g = k / 16 % 4, j = k % 16:
+//   code   byte ((b * fragments + f) * 2 + h) * 1024 + g * 256 + r * 16 + j
+//   scale  byte ((b / 4) * fragments + f) * 64 + r * 4 + b % 4, holding the exponent + 127
+// Lane l = 16 g + r reads 16 bytes at 16 l of either half: 1 KiB side by side per load, from memory and from LDS.
+// Codes past K are zero; rows past the last hold anything, since a row's codes reach only its own outputs.
+// A gate/up weight's fragments alternate: fragment 2 j has gate rows [16 j, 16 j + 16), fragment 2 j + 1 the up rows.
+#pragma once
+
+#include "kv_cache.h"
+
+namespace plm {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kFp8Block = 128;           // of K
+constexpr int64_t kFp8Bytes = 2048;      // of a fragment: 16 rows x 128 codes
+constexpr int64_t kFp8ScaleBytes = 64;   // of a fragment's four blocks
+
+__host__ __device__ constexpr int64_t fp8_frags(int64_t rows) { return (rows + 15) / 16; }
+__host__ __device__ constexpr int64_t fp8_blocks(int64_t k) { return (k + kFp8Block - 1) / kFp8Block; }
+__host__ __device__ constexpr int64_t fp8_codes_bytes(int64_t rows, int64_t k) { return fp8_frags(rows) * fp8_blocks(k) * kFp8Bytes; }
+__host__ __device__ constexpr int64_t fp8_scales_bytes(int64_t rows, int64_t k) {
+  return fp8_frags(rows) * ((fp8_blocks(k) + 3) / 4) * kFp8ScaleBytes;
+}
+
+__device__ __forceinline__ int64_t fp8_code_at(int64_t frags, int64_t row, int64_t k) {
+  return ((k >> 7) * frags + (row >> 4)) * kFp8Bytes + ((k >> 6) & 1) * 1024 + ((k >> 4) & 3) * 256 + (row & 15) * 16 + (k & 15);
+}
+__device__ __forceinline__ int64_t fp8_scale_at(int64_t frags, int64_t row, int64_t block) {
+  return ((block >> 2) * frags + (row >> 4)) * kFp8ScaleBytes + (row & 15) * 4 + (block & 3);
+}
+
+// Where a weight's row lies: of gate/up the halves' fragments alternate (n: rows of both, a multiple of 32).
+__device__ __forceinline__ int64_t fp8_place(int64_t row, int64_t n, bool gate_up) {
+  if (!gate_up) return row;
+  const int64_t half = n >> 1, up = row >= half ? 1 : 0, i = row - up * half;
+  return ((i >> 4) * 2 + up) * 16 + (i & 15);
+}
+
+__device__ __forceinline__ uint8_t fp8_exponent(float scale) { return static_cast<uint8_t>(__builtin_bit_cast(uint32_t, scale) >> 23); }
+__device__ __forceinline__ float fp8_power(uint32_t exponent) { return __builtin_bit_cast(float, exponent << 23); }
+// 1 / scale, for scales up to 2^126.
+__device__ __forceinline__ float fp8_inverse(float scale) {
+  return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, scale));
+}
+
+// |x| for the largest magnitude of a block: what is not finite has no part in it.
+__device__ __forceinline__ float fp8_magnitude(float x) {
+  const float a = fabsf(x);
+  return a < __builtin_inff() ? a : 0.0f;
+}
+
+// c += rows of `a` times rows of `b` over one block, times the scales in the low bytes of sa and sb. The instruction adds
+// products in eights (k, k + 1, .., k + 7 of a lane), aligned to the largest of an eight and cut at 2^-14 of its power of two,
+// and the eights' sums in fp32 (measured; so does the older v_mfma_f32_16x16x32_fp8_fp8). Over random rows of 128 that is
+// off by 3e-6 of the sum of magnitudes (rms), 3e-5 of a result over 2048: a seventieth of bf16's rounding, a tenth of fp16's.
+// Results in fp32 are made by fp8_mma_exact.
+__device__ __forceinline__ f32x4 fp8_mma(i32x8 a, i32x8 b, f32x4 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
+}
+
+// The same with every product added in fp32: codes times their scales are bf16 values, exactly, four products of 32 deep.
+struct Fp8Exact {
+  u32x4 part[4];
+};
+__device__ __forceinline__ Fp8Exact fp8_exact(i32x8 v, int scale) {
+  const float s = fp8_power(static_cast<uint32_t>(scale));
+  Fp8Exact e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    e.part[i] = fp8_eight<DT_BF16>(static_cast<uint32_t>(v[2 * i]), static_cast<uint32_t>(v[2 * i + 1]), s);
+  return e;
+}
+__device__ __forceinline__ f32x4 fp8_mma_exact(const Fp8Exact& a, const Fp8Exact& b, f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = mfma_16x16x32<DT_BF16>(a.part[i], b.part[i], c);
+  return c;
+}
+
+__device__ __forceinline__ i32x8 fp8_operand(u32x4 lo, u32x4 hi) {
+  return i32x8{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
+               static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
+}
+
+}  // namespace plm

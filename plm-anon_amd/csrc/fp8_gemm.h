@@ -1,0 +1,53 @@
+// The products over e4m3 rows (plm_fp8_linear): what their kernels share.
+#pragma once
+
+#include "fp8.h"
+#include "plm_amd.h"
+
+namespace plm {
+
+struct Fp8Gemm {
+  const uint8_t* x;         // codes of [m, k]
+  const uint8_t* x_scales;
+  const uint8_t* w;         // codes of [n, k]
+  const uint8_t* w_scales;
+  void* y;
+  int64_t ldy;
+  int m, n, blocks;         // n: rows of the weight; blocks of K
+  int x_frags, w_frags, out;  // out: plm_fp8_out
+};
+
+// g / (1 + e^-g) * u in fp32; the exponential's overflow gives g / inf = -0.
+__device__ __forceinline__ float fp8_silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// Columns [n, n + 4) of row m, of `columns` in all.
+__device__ __forceinline__ void fp8_store4(const Fp8Gemm& a, int m, int n, int columns, f32x4 v) {
+  const int64_t at = m * a.ldy + n;
+  const int left = columns - n;
+  if (a.out == PLM_FP8_F32) {
+    float* y = static_cast<float*>(a.y) + at;
+    if (left >= 4 && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+      *reinterpret_cast<f32x4*>(y) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < left) y[j] = v[j];
+    }
+    return;
+  }
+  uint16_t b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = a.out == PLM_FP8_BF16 ? to_bits16<DT_BF16>(v[j]) : to_bits16<DT_F16>(v[j]);
+  uint16_t* y = static_cast<uint16_t*>(a.y) + at;
+  if (left >= 4 && (reinterpret_cast<uintptr_t>(y) & 7) == 0) {
+    *reinterpret_cast<u32x2*>(y) = u32x2{b[0] | (static_cast<uint32_t>(b[1]) << 16), b[2] | (static_cast<uint32_t>(b[3]) << 16)};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) y[j] = b[j];
+  }
+}
+
+hipError_t fp8_narrow(const Fp8Gemm& a, bool act, hipStream_t s);
+
+}  // namespace plm

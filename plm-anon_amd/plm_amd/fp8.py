@@ -1,0 +1,314 @@
+"""A decoder layer's linears in 8 bits on the HIP library: e4m3 rows and weights with a power-of-two scale per block of
+128, which the matrix instructions apply themselves.
+
+* ``Weight`` — a linear's weight ``[N, K]`` (or a fused gate/up one) in 8 bits, laid out once in the order the matrix
+  instructions read: half the bytes of the 16-bit packed weights, which a round is bound by, and twice the
+  matrix rate, which a prompt is bound by;
+* ``Rows`` — activations ``[M, K]`` in 8 bits; ``quantize`` makes them, and ``rms_norm`` with ``dtype=float8_e4m3fn``;
+* ``linear`` — rows times a weight, transposed: the 8-bit form of ``fast_gemm.hip_linear``;
+* ``gate_up_silu`` — the gate/up projection with its activation: that of ``fast_gemm.gate_up_silu``;
+* ``rms_norm`` — the root-mean-square norm between them, with the residual's addition, in 8 or 16 bits.
+
+A block's scale is the least power of two s with (largest finite magnitude) <= 448 s, at least 2^-64, as in the paged
+cache; codes are rounded to nearest even, and what is not finite becomes NaN, in its own row alone. A row's blocks are 128
+of K, a weight's 128 x 128. ``linear`` and ``gate_up_silu`` take 16-bit rows too, which they round as ``quantize`` does.
+
+Calls run on the current stream of the tensors' GPU, allocate what they return, keep nothing between calls and can be
+captured; sums are in one order, so results repeat bit for bit. Nothing here has a backward: tensors that require a
+gradient are refused while gradients are recorded.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+E4M3 = torch.float8_e4m3fn
+BLOCK = 128
+_OUT = {torch.bfloat16: _lib.PLM_FP8_BF16, torch.float16: _lib.PLM_FP8_F16, torch.float32: _lib.PLM_FP8_F32}
+_EPS = (2.0 ** -100, 2.0 ** 100)
+MAX_ROWS = 1 << 21   # of a product
+
+
+def _launch(entry, call, device: torch.device, what: str) -> None:
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = entry(call, _lib.stream_handle(device))
+    else:
+        with torch.cuda.device(index):
+            status = entry(call, _lib.stream_handle(device))
+    if status:
+        _lib.check(status, what)
+
+
+def _matrix(t: torch.Tensor, name: str, device: torch.device | None = None) -> tuple[torch.Tensor, int, int]:
+    """``t`` [rows, k] of 16 bits as a kernel can read it, its pointer and row stride."""
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be [rows, k], got {list(t.shape)}")
+    if t.dtype not in _lib.DTYPE_CODES:
+        raise TypeError(f"{name} must be bf16 or fp16, got {t.dtype}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, and the 8-bit calls have none: detach it, or call under no_grad")
+    k = t.shape[1]
+    if k < 8 or k % 8 or k > 1 << 24:
+        raise ValueError(f"{name}'s rows must have a multiple of 8 in [8, 2^24] of elements, got {k}")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise RuntimeError(f"{name} must be on {'a GPU' if device is None else device}, got {t.device}")
+    at = t.data_ptr()
+    if at % 16 == 0 and t.stride(1) == 1 and t.stride(0) % 8 == 0:
+        return t, at, t.stride(0)
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), k
+
+
+class _Eight:
+    """Codes and scales of ``rows`` rows of ``k`` (``include/plm_amd.h`` states their order); what it was made of stays."""
+
+    _gate_up = False
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int):
+        lib = _lib.lib()
+        need = int(lib.plm_fp8_codes_bytes(rows, k)), int(lib.plm_fp8_scales_bytes(rows, k))
+        if not need[0]:
+            raise ValueError(f"8-bit rows need 1 to 2^28 - 1 rows of a multiple of 8 in [8, 2^24], got [{rows}, {k}]")
+        for name, t, size, dtype in (("codes", codes, need[0], E4M3), ("scales", scales, need[1], torch.uint8)):
+            if t.dtype is not dtype or t.shape != (size,) or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} of [{rows}, {k}] must be contiguous {dtype} [{size}] on 16 bytes, got {t.dtype} "
+                                 f"{list(t.shape)}")
+        if not codes.is_cuda or scales.device != codes.device:
+            raise RuntimeError(f"codes and scales live on one GPU; got {codes.device} and {scales.device}")
+        self.__dict__.update(codes=codes, scales=scales, rows=rows, k=k, device=codes.device, codes_at=codes.data_ptr(),
+                             scales_at=scales.data_ptr())
+
+    @classmethod
+    def _new(cls, rows: int, k: int, device: torch.device):
+        """Uninitialised rows, for a kernel to fill: one allocation, no check of what is known."""
+        frags, blocks = -(-rows // 16), -(-k // BLOCK)
+        codes, scales = frags * blocks * 2048, frags * (-(-blocks // 4)) * 64
+        both = torch.empty(codes + scales, dtype=torch.uint8, device=device)
+        self = cls.__new__(cls)
+        at = both.data_ptr()
+        self.__dict__.update(_both=both, rows=rows, k=k, device=both.device, codes_at=at, scales_at=at + codes, _codes_size=codes)
+        return self
+
+    def __getattr__(self, name: str):
+        # The tensors of what a kernel filled, as views when they are asked for.
+        if name in ("codes", "scales") and "_both" in self.__dict__:
+            both, size = self.__dict__["_both"], self.__dict__["_codes_size"]
+            return both[:size].view(E4M3) if name == "codes" else both[size:]
+        raise AttributeError(name)
+
+    def __setattr__(self, name: str, value) -> None:
+        raise AttributeError(f"8-bit rows stay what they were made of: {name} cannot be set")
+
+    def __delattr__(self, name: str) -> None:
+        raise AttributeError(f"8-bit rows keep their {name}")
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.rows, self.k
+
+    def values(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """``[rows, k]``: what the codes stand for, exact in bf16 and fp32 but for codes that round up to 2^128,
+        which are infinite (fp16 has neither the range nor all steps)."""
+        if dtype not in _OUT:
+            raise TypeError(f"values come in bf16, fp16 or fp32, not {dtype}")
+        out = torch.empty(self.rows, self.k, dtype=dtype, device=self.device)
+        if not self.rows:
+            return out
+
+        def entry(call, stream: int) -> int:
+            return _lib.lib().plm_fp8_values(*call, stream)
+
+        _launch(entry, (self.codes_at, self.scales_at, self.rows, self.k, int(self._gate_up), _OUT[dtype], out.data_ptr()),
+                self.device, f"plm_fp8_values({self.rows} rows of {self.k})")
+        return out
+
+
+class Rows(_Eight):
+    """Activations ``[rows, k]`` in 8 bits, as ``quantize`` and ``rms_norm`` return them."""
+
+
+class Weight(_Eight):
+    """A weight ``[n, k]`` in 8 bits. ``Weight.quantize`` rounds one of 16 bits, ``Weight.from_blocks`` lays out codes and
+    scales that are there already; ``Weight(codes, scales, n, k, gate_up=...)`` takes ``.codes`` and ``.scales`` of
+    another (a checkpoint of this layout). ``gate_up``: a fused gate/up weight, gate rows first, for ``gate_up_silu``."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, *, gate_up: bool = False):
+        _halves(n, gate_up)
+        super().__init__(codes, scales, n, k)
+        self.__dict__["_gate_up"] = bool(gate_up)
+
+    @property
+    def n(self) -> int:
+        return self.rows
+
+    @property
+    def gate_up(self) -> bool:
+        return self._gate_up
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor, *, gate_up: bool = False) -> "Weight":
+        """``w`` (bf16 or fp16 ``[n, k]``) rounded to 8 bits."""
+        w, at, stride = _matrix(w, "w")
+        n, k = w.shape
+        if w.shape[0] > 1 and stride < k:
+            raise ValueError("w's rows overlap")
+        return cls._filled(_lib.DTYPE_CODES[w.dtype], n, k, at, max(stride, k), 0, gate_up, w.device)
+
+    @classmethod
+    def from_blocks(cls, codes: torch.Tensor, scales: torch.Tensor, *, gate_up: bool = False) -> "Weight":
+        """``codes`` float8_e4m3fn ``[n, k]`` with float32 ``scales [ceil(n / 128), ceil(k / 128)]`` (of a gate/up weight the
+        gate half's blocks of rows, then the up half's), powers of two in [2^-126, 2^126]: a weight is
+        ``codes * scales``. Reads the scales on the host; other scales are refused (round such a weight's values)."""
+        if codes.dim() != 2 or codes.dtype is not E4M3 or not codes.is_cuda:
+            raise ValueError(f"codes must be float8_e4m3fn [n, k] on a GPU, got {codes.dtype} {list(codes.shape)} on {codes.device}")
+        n, k = codes.shape
+        if n < 1 or k < 8 or k % 8:
+            raise ValueError(f"codes must have rows of a multiple of 8, got {list(codes.shape)}")
+        halves = _halves(n, gate_up)
+        shape = (halves * -(-(n // halves) // BLOCK), -(-k // BLOCK))
+        if scales.shape != shape or scales.dtype is not torch.float32 or scales.device != codes.device:
+            raise ValueError(f"scales must be float32 {list(shape)} on {codes.device}, got {scales.dtype} {list(scales.shape)} on "
+                             f"{scales.device}")
+        scales = scales.contiguous()
+        bits = scales.view(torch.int32)
+        if not bool(((bits & 0x7fffff) == 0).logical_and(bits >= 1 << 23).logical_and(bits <= 253 << 23).all()):
+            raise ValueError("scales must be powers of two in [2^-126, 2^126]")
+        if not codes.is_contiguous() or codes.data_ptr() % 8:
+            codes = codes.clone(memory_format=torch.contiguous_format)
+        return cls._filled(0, n, k, codes.data_ptr(), k, scales.data_ptr(), gate_up, codes.device)
+
+    @classmethod
+    def _filled(cls, dtype: int, n: int, k: int, at: int, stride: int, blocks: int, gate_up: bool, device: torch.device) -> "Weight":
+        _halves(n, gate_up)
+        if n < 1:
+            raise ValueError("a weight has at least one row")
+        self = cls._new(n, k, device)
+        self.__dict__["_gate_up"] = bool(gate_up)
+        _launch(_lib.lib().plm_fp8_weight,
+                _lib.pack_fp8_weight(dtype, n, k, at, stride, blocks, bool(gate_up), self.codes_at, self.scales_at), device,
+                f"plm_fp8_weight([{n}, {k}], gate_up={gate_up})")
+        return self
+
+
+def _halves(n: int, gate_up: bool) -> int:
+    if gate_up and n % 32:
+        raise ValueError(f"a fused gate/up weight needs a multiple of 32 rows, got {n}")
+    return 2 if gate_up else 1
+
+
+def quantize(x: torch.Tensor) -> Rows:
+    """``x`` (bf16 or fp16 ``[rows, k]``, k a multiple of 8) in 8 bits."""
+    x, at, stride = _matrix(x, "x")
+    rows, k = x.shape
+    out = Rows._new(rows, k, x.device)
+    if rows:
+        _launch(_lib.lib().plm_fp8_rows,
+                _lib.pack_fp8_rows(_lib.DTYPE_CODES[x.dtype], rows, k, at, stride, 0, 0, 0, 0, 0, 0.0, 0, out.codes_at,
+                                   out.scales_at), x.device, f"plm_fp8_rows({rows} rows of {k})")
+    return out
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6, *, residual: torch.Tensor | None = None,
+             dtype: torch.dtype | None = None):
+    """``t * weight / sqrt(mean(t^2) + eps)`` of ``t = x + residual``, rounded to x's type (without a residual ``t`` is
+    ``x``), ``[rows, k]``: in x's type, or with ``dtype=torch.float8_e4m3fn`` as ``Rows``. With a residual the result is
+    ``(norm, t)``, t being the residual of the next call. ``weight [k]`` is of x's type (None: ones); eps is in [2^-100,
+    2^100]. Codes are what the exact value rounds to."""
+    x, at, stride = _matrix(x, "x")
+    rows, k = x.shape
+    if dtype not in (None, x.dtype, E4M3):
+        raise TypeError(f"a norm comes in its input's type or float8_e4m3fn, not {dtype}")
+    if not _EPS[0] <= eps <= _EPS[1]:
+        raise ValueError(f"eps must be in [2^-100, 2^100], got {eps}")
+    weight_at = 0
+    if weight is not None:
+        if weight.dtype is not x.dtype or weight.shape != (k,) or weight.device != x.device:
+            raise ValueError(f"weight must be {x.dtype} [{k}] on {x.device}, got {weight.dtype} {list(weight.shape)} on {weight.device}")
+        if weight.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("weight requires a gradient, and the 8-bit calls have none: detach it, or call under no_grad")
+        if not weight.is_contiguous() or weight.data_ptr() % 16:
+            weight = weight.clone(memory_format=torch.contiguous_format)
+        weight_at = weight.data_ptr()
+    total, total_at, residual_at, residual_stride = None, 0, 0, 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype is not x.dtype:
+            raise ValueError(f"residual must be {x.dtype} {list(x.shape)} as x is, got {residual.dtype} {list(residual.shape)}")
+        residual, residual_at, residual_stride = _matrix(residual, "residual", x.device)
+        total = torch.empty(rows, k, dtype=x.dtype, device=x.device)
+        total_at = total.data_ptr()
+    if dtype is E4M3:
+        out = Rows._new(rows, k, x.device)
+        y_at, codes_at, scales_at = 0, out.codes_at, out.scales_at
+    else:
+        out = torch.empty(rows, k, dtype=x.dtype, device=x.device)
+        y_at, codes_at, scales_at = out.data_ptr(), 0, 0
+    if rows:
+        _launch(_lib.lib().plm_fp8_rows,
+                _lib.pack_fp8_rows(_lib.DTYPE_CODES[x.dtype], rows, k, at, stride, 1, residual_at, residual_stride, total_at,
+                                   weight_at, eps, y_at, codes_at, scales_at), x.device, f"plm_fp8_rows(norm of {rows} rows of {k})")
+    return out if residual is None else (out, total)
+
+
+def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dtype: torch.dtype | None, act: bool) -> torch.Tensor:
+    if not isinstance(w, Weight):
+        raise TypeError(f"w must be an fp8.Weight, got {type(w).__name__}")
+    if not isinstance(x, Rows):
+        if x.dim() != 2 or x.shape[1] != w.k:
+            raise ValueError(f"x must be [rows, {w.k}], got {list(x.shape)}")
+        if out_dtype is None:
+            out_dtype = x.dtype if out is None else out.dtype
+        x = quantize(x)
+    elif x.k != w.k:
+        raise ValueError(f"x must be [rows, {w.k}], got {list(x.shape)}")
+    elif out_dtype is None:
+        if out is None:
+            raise ValueError("rows in 8 bits have no type of their own: out_dtype or out is needed")
+        out_dtype = out.dtype
+    if x.device != w.device:
+        raise RuntimeError(f"x must be on the weight's GPU {w.device}, got {x.device}")
+    if out_dtype not in _OUT:
+        raise TypeError(f"a product comes in bf16, fp16 or fp32, not {out_dtype}")
+    if x.rows > MAX_ROWS:
+        raise ValueError(f"a product takes up to {MAX_ROWS} rows, got {x.rows}")
+    shape = (x.rows, w.rows // 2 if act else w.rows)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=w.device)
+    elif out.shape != shape or out.dtype is not out_dtype or out.device != w.device or \
+            (shape[0] and (out.stride(1) != 1 and shape[1] > 1 or out.stride(0) < shape[1] and shape[0] > 1)):
+        raise ValueError(f"out must be a row-major {list(shape)} {out_dtype} tensor on {w.device}")
+    elif out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("out requires a gradient, and the 8-bit calls have none")
+    if x.rows:
+        _launch(_lib.lib().plm_fp8_linear,
+                _lib.pack_fp8_linear(x.rows, w.rows, w.k, x.codes_at, x.scales_at, w.codes_at, w.scales_at, out.data_ptr(),
+                                     max(out.stride(0), shape[1]), _OUT[out_dtype], act), w.device,
+                f"plm_fp8_linear(M={x.rows}, N={w.rows}, K={w.k}, act={act})")
+    return out
+
+
+def linear(x: torch.Tensor | Rows, w: Weight, *, out: torch.Tensor | None = None,
+           out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``x @ w^T`` ``[rows, n]``, summed in fp32 and rounded once to ``out_dtype``: bf16, fp16 or fp32, x's type unless given
+    (``Rows`` have none). ``x`` is ``[rows, k]``, in 16 bits, which are rounded to 8 here, or ``Rows``."""
+    if isinstance(w, Weight) and w.gate_up:
+        raise ValueError("a gate/up weight goes to gate_up_silu")
+    return _product(x, w, out, out_dtype, False)
+
+
+def gate_up_silu(x: torch.Tensor | Rows, w: Weight, *, out: torch.Tensor | None = None,
+                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``silu(g) * u`` of the halves of ``x @ w^T``, ``[rows, n / 2]``: in fp32 up to the one rounding to ``out_dtype``
+    (``fast_gemm.gate_up_silu`` rounds the projections and the activation on the way). ``w`` is a gate/up weight."""
+    if isinstance(w, Weight) and not w.gate_up:
+        raise ValueError("gate_up_silu needs a weight made with gate_up=True")
+    return _product(x, w, out, out_dtype, True)
+
+
+def llama_mlp(x: torch.Tensor | Rows, gate_up: Weight, down: Weight, *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """A gated MLP over 8-bit weights, ``down(silu(g) * u)``: the 8-bit form of ``fast_gemm.llama_mlp``. The activation is
+    rounded to ``out_dtype`` (bf16 or fp16, x's type unless given) and from there to 8 bits."""
+    act = gate_up_silu(x, gate_up, out_dtype=out_dtype)
+    return linear(act, down)

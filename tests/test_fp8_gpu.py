@@ -1,0 +1,367 @@
+"""The 8-bit rows, norm and products against the definition in 64 bits.
+
+Tolerances. Codes and scales are whole numbers and equal the definition's. A norm in 16 bits is rounded once from fp32
+arithmetic of three roundings: half a step (``finfo(t).eps / 2``) and 2^-21 of the value, and half of the least subnormal.
+A product of codes is exact in fp32 and K of them are added: each addition is off by at most 2^-23 of the sum of magnitudes
+(the matrix instruction may cut instead of rounding), then the output's half step. For 16-bit results the 8-bit matrix
+instruction adds products in eights of K and cuts each at 2^-14 of the largest one's power of two: 7 of them per eight. The activation's error is its
+derivative's, |silu'| <= 1.1, times the gate's, and fp32 arithmetic with an exponential and a division, 2^-20 of its value.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import fp8_oracle as oracle
+from plm_amd import fp8
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+
+
+def _rows(m, k, dtype, seed=0, loud=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g) * (0.7 * torch.randn(m, 1, generator=g)).exp()
+    if loud:
+        x = x * (1 + 30 * (torch.rand(k, generator=g) < 0.02))
+    return x.to(dtype)
+
+
+def _same(got, want):
+    # In the type they come in: its largest values round to 2^128, which is infinite there.
+    got, want = got.cpu().double(), want.to(got.dtype).double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+SIZES = [(1, 8), (1, 128), (3, 120), (16, 136), (17, 1024), (33, 1416), (5, 2048), (56, 2560), (2, 4104), (1, 10240), (4, 16392)]
+
+
+@pytest.mark.parametrize("m,k", SIZES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_quantize(device, m, k, dtype):
+    x = _rows(m, k, dtype, seed=m * k)
+    x[m // 2, :min(k, 128)] = 0
+    got = fp8.quantize(x.to(device))
+    _same(got.values(), oracle.rounded(x))
+    codes, scales = oracle.places(m, k)
+    want = torch.stack([oracle.scale_of(x[:, a:a + 128].double().abs().amax(1)) for a in range(0, k, 128)], 1)
+    assert torch.equal(got.scales.cpu()[scales].double(), want.log2() + 127)
+    held = got.codes.cpu().view(torch.uint8)[codes].view(E4M3).float().double()
+    assert torch.equal(held * want.repeat_interleave(128, 1)[:, :k], oracle.rounded(x))
+    # Codes behind the row's end are zeros.
+    if k % 128:
+        whole, _ = oracle.places(m, -(-k // 128) * 128)
+        assert not got.codes.cpu().view(torch.uint8)[whole[:, k:]].any()
+
+
+@pytest.mark.parametrize("m", [1023, 1024, 4097])
+def test_many_rows(device, m):
+    x = _rows(m, 264, BF16, seed=m)
+    _same(fp8.quantize(x.to(device)).values(BF16), oracle.rounded(x))
+    y, t = fp8.rms_norm(x.to(device), None, 1e-6, residual=x.flip(0).contiguous().to(device), dtype=E4M3)
+    want, total = oracle.norm(x, None, 1e-6, x.flip(0))
+    assert torch.equal(t.cpu(), total)
+    _same(y.values(BF16), oracle.rounded(want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_quantize_extremes(device, dtype):
+    """Ties, the borders of scales, subnormals, the type's largest value; infinities and NaN stay in their place."""
+    x = torch.zeros(12, 256, dtype=dtype)
+    x[0, :128] = torch.linspace(-448, 448, 128)
+    x[1, :9] = torch.tensor([448.0, 1.0625, 1.1875, -1.0625, 17 * 2.0 ** -10, 2.0 ** -10, 3 * 2.0 ** -10, 2.0 ** -9, 208])
+    x[2, 0], x[2, 130] = 449 if dtype is FP16 else 450, 448
+    x[3, :2] = torch.tensor([torch.finfo(dtype).max, torch.finfo(dtype).tiny])
+    x[4, 5] = torch.finfo(dtype).smallest_normal / 8
+    x[5, :4] = torch.tensor([1.0, float("inf"), -3.0, 0.5])
+    x[6, 200] = float("nan")
+    x[6, 201] = 7
+    x[7] = float("-inf")
+    x[8] = torch.finfo(dtype).min
+    x[9, 255] = -0.0
+    x[10] = 2.0 ** -14
+    _same(fp8.quantize(x.to(device)).values(), oracle.rounded(x))
+
+
+def test_strided_rows(device):
+    base = _rows(40, 600, BF16, seed=4).to(device)
+    for x in (base[:, 8:392], base[::2, 16:400], base[:, 4:388], base.t().contiguous().t()[:, :384], base[3:4].expand(7, 600)):
+        _same(fp8.quantize(x).values(), oracle.rounded(x.cpu()))
+        y, t = fp8.rms_norm(x, None, 1e-5, residual=x, dtype=E4M3)
+        want, total = oracle.norm(x.cpu(), None, 1e-5, x.cpu())
+        assert torch.equal(t.cpu(), total)
+        _same(y.values(), oracle.rounded(want))
+
+
+@pytest.mark.parametrize("m,k", SIZES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("residual,weight", [(True, True), (False, True), (True, False), (False, False)])
+def test_norm(device, m, k, dtype, residual, weight):
+    x, r = _rows(m, k, dtype, seed=1), _rows(m, k, dtype, seed=2)
+    if m > 2:
+        x[1], r[1] = 0, 0
+    w = (1 + 0.2 * torch.randn(k, generator=torch.Generator().manual_seed(3))).to(dtype) if weight else None
+    want, total = oracle.norm(x, w, 1e-5, r if residual else None)
+    args = dict(residual=r.to(device) if residual else None)
+    on = w.to(device) if weight else None
+    for kind in (None, E4M3):
+        got = fp8.rms_norm(x.to(device), on, 1e-5, dtype=kind, **args)
+        if residual:
+            assert torch.equal(got[1].cpu(), total)
+            got = got[0]
+        if kind is E4M3:
+            _same(got.values(), oracle.rounded(want))
+        else:
+            info = torch.finfo(dtype)
+            off = (got.cpu().double() - want).abs()
+            assert (off <= want.abs() * (info.eps / 2 + 2.0 ** -21) + info.smallest_normal * info.eps / 2).all()
+
+
+def test_norm_borders(device):
+    """Rows of values that lie on the borders between codes, and of magnitudes that fp32 steps do not reach."""
+    k = 512
+    x = torch.ones(8, k, dtype=BF16)
+    x[1, :256] = 17
+    x[2] = 2.0 ** -120
+    x[3] = 2.0 ** 120
+    x[4, ::2] = -2.0 ** 60
+    x[5, 7] = float("inf")
+    x[6, 9] = float("nan")
+    x[7] = 0
+    w = torch.full((k,), 1.0, dtype=BF16)
+    w[:32] = torch.tensor([1 + i / 32 for i in range(32)])
+    w[64:96] = torch.tensor([(1 + i / 32) * 2.0 ** -8 for i in range(32)])
+    for eps in (2.0 ** -100, 1e-6, 3.0):
+        want, _ = oracle.norm(x, w, eps)
+        _same(fp8.rms_norm(x.to(device), w.to(device), eps, dtype=E4M3).values(), oracle.rounded(want))
+        got = fp8.rms_norm(x.to(device), w.to(device), eps).cpu().double()
+        want = want.to(BF16).double()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert ((got - want).nan_to_num().abs() <= want.nan_to_num().abs() * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("n,k,gate_up", [(1, 8, False), (40, 136, False), (128, 128, False), (257, 1024, False), (300, 1416, False),
+                                         (32, 8, True), (96, 128, True), (288, 264, True), (1024, 520, True)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_weight(device, n, k, gate_up, dtype):
+    w = (0.02 * torch.randn(n, k, generator=torch.Generator().manual_seed(n))).to(dtype)
+    w[n // 3, k // 2] = 3
+    want, scales = oracle.weight(w, gate_up)
+    got = fp8.Weight.quantize(w.to(device), gate_up=gate_up)
+    _same(got.values(), want)
+    half = n // 2 if gate_up else n
+    per = scales.view(2 if gate_up else 1, -1, scales.shape[1]).repeat_interleave(128, 1)[:, :half].reshape(n, -1)
+    codes = (want / per.repeat_interleave(128, 1)[:, :k]).float().to(E4M3)
+    laid = fp8.Weight.from_blocks(codes.to(device), scales.float().to(device), gate_up=gate_up)
+    at, where = oracle.places(n, k)
+    rows = oracle.order(n, gate_up)
+    for held in (got, laid, fp8.Weight(got.codes.clone(), got.scales.clone(), n, k, gate_up=gate_up)):
+        assert torch.equal(held.codes.cpu().view(torch.uint8)[at[rows]], codes.view(torch.uint8))
+        assert torch.equal(held.scales.cpu()[where[rows]].double(), per.log2() + 127)
+        _same(held.values(BF16), want)
+
+
+def _weight(n, k, seed, gate_up=False, dtype=BF16):
+    w = (0.05 * torch.randn(n, k, generator=torch.Generator().manual_seed(seed))).to(dtype)
+    return w, oracle.weight(w, gate_up)[0]
+
+
+def _largest_of_eights(x, w):
+    """The largest |product| of every eight of K, summed."""
+    x, w = (t.abs().nan_to_num().float().to("cuda") for t in (x, w))
+    total = torch.zeros(x.shape[0], w.shape[0], device="cuda")
+    for at in range(0, x.shape[1], 8):
+        largest = torch.zeros_like(total)
+        for k in range(at, at + 8):
+            torch.maximum(largest, x[:, k, None] * w[:, k], out=largest)
+        total += largest
+    return total.double().cpu()
+
+
+def _expected(x, w, out, act):
+    """(product, tolerance) of the values of rows and weight."""
+    y, size = x @ w.T, x.abs() @ w.abs().T
+    off = size * x.shape[1] * 2.0 ** -23
+    if out is not F32:
+        off += 7 * 2.0 ** -14 * _largest_of_eights(x, w)
+    if act:
+        (g, u), (dg, du) = y.chunk(2, 1), off.chunk(2, 1)
+        y = torch.sigmoid(g) * g * u
+        off = 1.1 * dg * (u.abs() + du) + (torch.sigmoid(g) * g).abs() * du + y.abs() * 2.0 ** -20
+    info = torch.finfo(out)
+    return y, off + (y.abs() + off) * info.eps / 2 + info.smallest_normal * info.eps / 2
+
+
+def _check(got, x, w, out, act=False):
+    want, off = _expected(x, w, out, act)
+    assert got.dtype is out and got.shape == want.shape
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    bad = (got - want).abs().nan_to_num() > off.nan_to_num()
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), float(((got - want).abs() / off).nan_to_num().max()))
+
+
+PRODUCTS = [(1, 1, 8), (1, 2048, 2048), (2, 40, 136), (7, 33, 128), (16, 256, 1024), (17, 257, 1416), (33, 1000, 256), (42, 2560, 2560),
+            (56, 129, 10240), (64, 512, 520), (65, 300, 1032), (110, 384, 2048), (130, 16, 264), (250, 640, 648), (517, 304, 1416),
+            (1025, 136, 392)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("dtype,out", [(BF16, None), (FP16, None), (BF16, F32)])
+def test_linear(device, m, n, k, dtype, out):
+    x = _rows(m, k, dtype, seed=m + n + k)
+    w, values = _weight(n, k, seed=n, dtype=dtype)
+    weight = fp8.Weight.quantize(w.to(device))
+    got = fp8.linear(x.to(device), weight, out_dtype=out)
+    _check(got, oracle.rounded(x), values, out or dtype)
+    # The same from 8-bit rows, bit for bit, into the caller's tensor, whose other columns stay.
+    wide = torch.full((m, n + 5), 7.0, dtype=out or dtype, device=device)
+    again = fp8.linear(fp8.quantize(x.to(device)), weight, out=wide[:, 2:n + 2])
+    assert torch.equal(again, got)
+    assert bool((wide[:, :2] == 7).all()) and bool((wide[:, n + 2:] == 7).all())
+
+
+@pytest.mark.parametrize("m,half,k", [(1, 16, 8), (1, 5632, 2048), (3, 48, 136), (16, 128, 1024), (42, 1000 // 16 * 16, 520), (56, 5632, 2048),
+                                      (65, 304, 1416), (129, 160, 264), (300, 272, 2048), (1030, 144, 392)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_gate_up(device, m, half, k, dtype):
+    x = _rows(m, k, dtype, seed=m + half, loud=False)
+    w, values = _weight(2 * half, k, seed=half, gate_up=True, dtype=dtype)
+    weight = fp8.Weight.quantize(w.to(device), gate_up=True)
+    rows = oracle.rounded(x)
+    _check(fp8.gate_up_silu(x.to(device), weight), rows, values, dtype, act=True)
+    _check(fp8.gate_up_silu(fp8.quantize(x.to(device)), weight, out_dtype=F32), rows, values, F32, act=True)
+
+
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_not_finite(device, m):
+    """What is not finite reaches its own row, and of a weight its own column."""
+    x = _rows(m, 264, BF16, seed=5)
+    x[0, 3] = float("inf")
+    x[m // 2, 200] = float("nan")
+    w, values = _weight(80, 264, seed=6)
+    w[7, 100] = float("nan")
+    values = oracle.weight(w)[0]
+    weight = fp8.Weight.quantize(w.to(device))
+    got = fp8.linear(x.to(device), weight).cpu()
+    want, off = _expected(oracle.rounded(x), values, BF16, False)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert ((got.double() - want).abs().nan_to_num() <= off.nan_to_num()).all()
+
+
+def test_large_gates(device):
+    """Gates so low that the exponential overflows give zeros, not NaN; so high, the product alone."""
+    k, half = 128, 32
+    w = torch.zeros(2 * half, k, dtype=BF16)
+    w[:half, 0] = torch.linspace(-400, 400, half)
+    w[half:, 1] = 1
+    x = torch.zeros(3, k, dtype=BF16)
+    x[:, 0], x[:, 1] = 1, 2
+    values = oracle.weight(w, True)[0]
+    got = fp8.gate_up_silu(x.to(device), fp8.Weight.quantize(w.to(device), gate_up=True))
+    _check(got, oracle.rounded(x), values, BF16, act=True)
+
+
+def test_empty_rows(device):
+    weight = fp8.Weight.quantize(_weight(32, 64, 0)[0].to(device))
+    gated = fp8.Weight.quantize(_weight(32, 64, 0)[0].to(device), gate_up=True)
+    x = torch.empty(0, 64, dtype=BF16, device=device)
+    assert fp8.linear(x, weight).shape == (0, 32) and fp8.gate_up_silu(x, gated).shape == (0, 16)
+    y, t = fp8.rms_norm(x, None, residual=x, dtype=E4M3)
+    assert y.shape == (0, 64) and t.shape == (0, 64) and y.values(BF16).shape == (0, 64)
+    assert fp8.linear(y, weight, out_dtype=F32).shape == (0, 32)
+
+
+@pytest.mark.parametrize("m", [1, 56, 300])
+def test_layer_run(device, m):
+    """A layer's MLP as it is used: norm with the residual, gate/up, activation, down, each from the one before."""
+    k, half = 512, 704
+    x, r = _rows(m, k, BF16, seed=8, loud=False), _rows(m, k, BF16, seed=9, loud=False)
+    w = (1 + 0.1 * torch.randn(k, generator=torch.Generator().manual_seed(1))).to(BF16)
+    up, up_values = _weight(2 * half, k, 10, gate_up=True)
+    down, down_values = _weight(k, half, 11)
+    gate_up, down8 = fp8.Weight.quantize(up.to(device), gate_up=True), fp8.Weight.quantize(down.to(device))
+    rows, total = fp8.rms_norm(x.to(device), w.to(device), 1e-5, residual=r.to(device), dtype=E4M3)
+    want, t = oracle.norm(x, w, 1e-5, r)
+    assert torch.equal(total.cpu(), t)
+    act = fp8.gate_up_silu(rows, gate_up, out_dtype=BF16)
+    _check(act, oracle.rounded(want), up_values, BF16, act=True)
+    y = fp8.linear(act, down8)
+    _check(y, oracle.rounded(act.cpu()), down_values, BF16)
+    assert torch.equal(fp8.llama_mlp(rows, gate_up, down8, out_dtype=BF16), y)
+
+
+def test_captured(device):
+    """A captured run follows its inputs, replay after replay, and equals eager calls on another stream bit for bit."""
+    m, k, half = 42, 768, 512
+    weight = fp8.Weight.quantize(_weight(2 * half, k, 1, gate_up=True)[0].to(device), gate_up=True)
+    down = fp8.Weight.quantize(_weight(k, half, 2)[0].to(device))
+    norm = torch.ones(k, dtype=BF16, device=device)
+    x, r = (torch.empty(m, k, dtype=BF16, device=device) for _ in range(2))
+
+    def step(x, r):
+        rows, t = fp8.rms_norm(x, norm, residual=r, dtype=E4M3)
+        return fp8.llama_mlp(rows, weight, down, out_dtype=BF16), t
+
+    x.copy_(_rows(m, k, BF16, 0)), r.copy_(_rows(m, k, BF16, 1))
+    step(x, r)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, r)
+    other = torch.cuda.Stream()
+    for seed in range(4):
+        x.copy_(_rows(m, k, BF16, 10 + seed)), r.copy_(_rows(m, k, BF16, 20 + seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            eager = step(x, r)
+        other.synchronize()
+        assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
+
+
+def test_refusals(device):
+    w = fp8.Weight.quantize(_weight(32, 64, 0)[0].to(device))
+    gated = fp8.Weight.quantize(_weight(32, 64, 0)[0].to(device), gate_up=True)
+    x = _rows(3, 64, BF16).to(device)
+    with pytest.raises(RuntimeError):
+        fp8.quantize(x.clone().requires_grad_())
+    with pytest.raises(RuntimeError):
+        fp8.rms_norm(x, torch.ones(64, dtype=BF16, device=device, requires_grad=True))
+    with torch.no_grad():
+        fp8.quantize(x.clone().requires_grad_())
+    with pytest.raises(ValueError):
+        fp8.linear(x, gated)
+    with pytest.raises(ValueError):
+        fp8.gate_up_silu(x, w)
+    with pytest.raises(ValueError):
+        fp8.linear(fp8.quantize(x), w)
+    with pytest.raises(ValueError):
+        fp8.linear(x[:, :56], w)
+    with pytest.raises(ValueError):
+        fp8.linear(fp8.quantize(x[:, :56]), w, out_dtype=BF16)
+    with pytest.raises(TypeError):
+        fp8.linear(x, w, out_dtype=torch.float64)
+    with pytest.raises(TypeError):
+        fp8.linear(x, x)
+    for out in (torch.empty(3, 31, dtype=BF16, device=device), torch.empty(32, 3, dtype=BF16, device=device).t(),
+                torch.empty(1, 32, dtype=BF16, device=device).expand(3, 32)):
+        with pytest.raises(ValueError):
+            fp8.linear(x, w, out=out)
+    with pytest.raises(ValueError):
+        fp8.linear(x, w, out=torch.empty(3, 32, dtype=BF16, device=device), out_dtype=F32)
+    with pytest.raises(AttributeError):
+        w.rows = 3
+    with pytest.raises(AttributeError):
+        del w.k
+    codes, scales = torch.zeros(32, 64, dtype=torch.uint8, device=device).view(E4M3), torch.ones(1, 1, device=device)
+    for bad in (3.0, 0.0, -1.0, float("inf"), float("nan"), 2.0 ** 127, 2.0 ** -130):
+        with pytest.raises(ValueError):
+            fp8.Weight.from_blocks(codes, scales * bad)
+    with pytest.raises(ValueError):
+        fp8.Weight.from_blocks(codes, scales, gate_up=True)
+    with pytest.raises(ValueError):
+        fp8.Weight.from_blocks(codes, scales.double())
