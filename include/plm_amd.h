@@ -598,8 +598,8 @@ size_t plm_attend_workspace_bytes(const plm_attend_call* call);
  * r = row % 16, b = k / 128:
  *   codes   [b][f][k / 64 % 2][k / 16 % 4][r][k % 16]
  *   scales  [b / 4][f][r][b % 4], the exponent + 127 in a byte
- * Codes past K are zeros, rows past the last of any content. plm_fp8_codes_bytes, plm_fp8_scales_bytes: the sizes (0
- * where there are no such rows: 1 <= rows < 2^28, 8 <= K <= 2^24, K % 8 == 0). A gate/up weight (gate rows first, N a
+ * Codes and scales past K are zeros, rows past the last of any content. plm_fp8_codes_bytes, plm_fp8_scales_bytes: the sizes (0
+ * where there are no such rows: 1 <= rows < 2^24, 8 <= K <= 2^24, K % 8 == 0). A gate/up weight (gate rows first, N a
  * multiple of 32) has its halves' fragments in turn: fragment 2 j has gate rows [16 j, 16 j + 16), 2 j + 1 the up
  * rows; a half's blocks of 128 rows begin with its first.
  */
@@ -652,19 +652,27 @@ int plm_fp8_values(const void* codes, const void* scales, int64_t rows, int64_t 
 
 /*
  * y[m, n] = x[m, k] . w[n, k]^T of 8-bit rows, summed in fp32 and rounded once to `out` (plm_fp8_out); with act, over a
- * gate/up weight, y[m, n / 2] = g / (1 + e^-g) * u of the halves' products, in fp32 up to the one rounding. ldy in
- * elements, at least y's columns. m <= 2^21.
+ * gate/up weight, y[m, n / 2] = g / (1 + e^-g) * u of the halves' products, in fp32 up to the one rounding. Results in
+ * 16 bits: the matrix instruction cuts each product of eight along K at 2^-14 of the largest one's power of two
+ * before it adds them (fp32 results are not cut). x: codes and scales, or up to 16 rows of 16 bits (x_type, row stride x_row,
+ * a multiple of 8), which are rounded as plm_fp8_rows does. ldy in elements, at least y's columns. m, n <= PLM_FP8_MOST.
+ * Workspace: plm_fp8_linear_workspace_bytes (0: none needed), 16-byte aligned, of any content; calls that may run at
+ * the same time need workspaces of their own.
  */
+#define PLM_FP8_MOST (1 << 21)
+enum plm_fp8_in { PLM_FP8_CODES = 0, PLM_FP8_ROWS_BF16 = 1, PLM_FP8_ROWS_F16 = 2 };
 typedef struct plm_fp8_linear_call {
-  int64_t m, n, k;
+  int64_t m, n, k, x_type;
   const void* x;
   const void* x_scales;
+  int64_t x_row;
   const void* w;
   const void* w_scales;
   void* y;
   int64_t ldy, out, act;
 } plm_fp8_linear_call;
-int plm_fp8_linear(const plm_fp8_linear_call* call, void* stream);
+int plm_fp8_linear(const plm_fp8_linear_call* call, void* workspace, size_t workspace_bytes, void* stream);
+size_t plm_fp8_linear_workspace_bytes(const plm_fp8_linear_call* call);
 
 /* Human-readable name of a status code. */
 const char* plm_status_string(int32_t status);

@@ -8,7 +8,7 @@
 //   code   byte ((b * fragments + f) * 2 + h) * 1024 + g * 256 + r * 16 + j
 //   scale  byte ((b / 4) * fragments + f) * 64 + r * 4 + b % 4, holding the exponent + 127
 // Lane l = 16 g + r reads 16 bytes at 16 l of either half: 1 KiB side by side per load, from memory and from LDS.
-// Codes past K are zero; rows past the last hold anything, since a row's codes reach only its own outputs.
+// Codes past K are zero, and so are scales (2^-127); rows past the last hold anything, since a row's codes reach only its own outputs.
 // A gate/up weight's fragments alternate: fragment 2 j has gate rows [16 j, 16 j + 16), fragment 2 j + 1 the up rows.
 #pragma once
 
@@ -36,6 +36,14 @@ __device__ __forceinline__ int64_t fp8_scale_at(int64_t frags, int64_t row, int6
   return ((block >> 2) * frags + (row >> 4)) * kFp8ScaleBytes + (row & 15) * 4 + (block & 3);
 }
 
+// A block's scale, and after the last block's zeros up to the next multiple of four.
+__device__ __forceinline__ void fp8_put_scale(uint8_t* scales, int64_t frags, int64_t row, int64_t block, int64_t blocks, uint8_t e) {
+  uint8_t* at = scales + fp8_scale_at(frags, row, block);
+  *at = e;
+  if (block == blocks - 1)
+    for (int i = 1; i < 4 - static_cast<int>(block & 3); ++i) at[i] = 0;
+}
+
 // Where a weight's row lies: of gate/up the halves' fragments alternate (n: rows of both, a multiple of 32).
 __device__ __forceinline__ int64_t fp8_place(int64_t row, int64_t n, bool gate_up) {
   if (!gate_up) return row;
@@ -54,6 +62,54 @@ __device__ __forceinline__ float fp8_inverse(float scale) {
 __device__ __forceinline__ float fp8_magnitude(float x) {
   const float a = fabsf(x);
   return a < __builtin_inff() ? a : 0.0f;
+}
+
+// The largest magnitude of 32 values of 16 bits, as bits: of finite ones it is their largest, else at least fp8_infinite.
+template <int DT>
+__device__ __forceinline__ constexpr uint32_t fp8_infinite() {
+  return DT == DT_BF16 ? 0x7f80u : 0x7c00u;
+}
+template <int DT, typename... W>
+__device__ __forceinline__ uint32_t fp8_most16(W... words) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 most = {0, 0};
+  auto add = [&](u32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+  };
+  (add(words), ...);
+  return max(static_cast<uint32_t>(most[0]), static_cast<uint32_t>(most[1]));
+}
+
+// Codes of four finite 16-bit values, two in a word, over a scale that bounds them.
+template <int DT>
+__device__ __forceinline__ uint32_t fp8_four(uint32_t lo, uint32_t hi, float scale) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  s16x2 w = {0, 0};
+  if constexpr (DT == DT_BF16) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, lo), scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, hi), scale, true);
+  } else {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, lo), scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, hi), scale, true);
+  }
+  return __builtin_bit_cast(uint32_t, w);
+}
+
+// Codes of 32 values of any kind and their scale; `share` gives the largest magnitude of the lanes that have a block.
+template <int DT, typename F>
+__device__ __forceinline__ float fp8_round_any(const u32x4 (&raw)[4], F share, i32x8& codes) {
+  float v[32], amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    v[i] = from_bits16<DT>(static_cast<uint16_t>(raw[i >> 3][(i & 7) >> 1] >> (16 * (i & 1))));
+    amax = fmaxf(amax, fp8_magnitude(v[i]));
+  }
+  const float scale = fp8_scale_of(share(amax)), inverse = fp8_inverse(scale);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    codes[i] = static_cast<int>(fp8_word(v[4 * i] * inverse, v[4 * i + 1] * inverse, v[4 * i + 2] * inverse, v[4 * i + 3] * inverse));
+  return scale;
 }
 
 // c += rows of `a` times rows of `b` over one block, times the scales in the low bytes of sa and sb. The instruction adds

@@ -3,35 +3,81 @@
 
 #include "fp8_gemm.h"
 
-extern "C" {
+namespace plm {
+namespace {
 
-int plm_fp8_linear(const plm_fp8_linear_call* call, void* stream) {
-  using namespace plm;
-  if (call == nullptr) return PLM_ERR_ARGUMENT;
+struct Fp8Plan {
+  bool tile;
+  Fp8TileKind kind;
+  Fp8Narrow narrow;
+  size_t bytes;   // of partial sums
+};
+
+// The plan of a call whose numbers go together; false where they do not.
+bool linear_of(const plm_fp8_linear_call* call, Fp8Gemm& a, Fp8Plan& p) {
+  if (call == nullptr) return false;
   const plm_fp8_linear_call& h = *call;
   const bool act = h.act != 0;
-  const int64_t columns = act ? h.n / 2 : h.n;
-  if (plm_fp8_codes_bytes(h.m, h.k) == 0 || plm_fp8_codes_bytes(h.n, h.k) == 0 || (act && h.n % 32 != 0)) return PLM_ERR_ARGUMENT;
-  // The second dimension of a grid has 65535 workgroups of 64 rows at least.
-  if (h.m > (int64_t{1} << 21) || h.ldy < columns || h.out < PLM_FP8_BF16 || h.out > PLM_FP8_F32) return PLM_ERR_ARGUMENT;
-  if (h.x == nullptr || h.x_scales == nullptr || h.w == nullptr || h.w_scales == nullptr || h.y == nullptr) return PLM_ERR_ARGUMENT;
-  for (const void* p : {h.x, h.x_scales, h.w, h.w_scales})
-    if (!aligned16_ptr(p)) return PLM_ERR_ALIGNMENT;
-  if (reinterpret_cast<uintptr_t>(h.y) % (h.out == PLM_FP8_F32 ? 4 : 2) != 0) return PLM_ERR_ALIGNMENT;
+  if (h.m < 1 || h.m > PLM_FP8_MOST || h.n < 1 || h.n > PLM_FP8_MOST || plm_fp8_codes_bytes(h.n, h.k) == 0 || (act && h.n % 32 != 0))
+    return false;
+  if (h.ldy < (act ? h.n / 2 : h.n) || h.out < PLM_FP8_BF16 || h.out > PLM_FP8_F32) return false;
+  if (h.x_type < PLM_FP8_CODES || h.x_type > PLM_FP8_ROWS_F16) return false;
+  if (h.x_type != PLM_FP8_CODES && (h.m > 16 || h.x_row < 0)) return false;
+  a.ldy = h.ldy;
+  a.x_row = h.x_row;
+  a.m = static_cast<int>(h.m);
+  a.n = static_cast<int>(h.n);
+  a.k = static_cast<int>(h.k);
+  a.blocks = static_cast<int>(fp8_blocks(h.k));
+  a.x_frags = static_cast<int>(fp8_frags(h.m));
+  a.w_frags = static_cast<int>(fp8_frags(h.n));
+  a.x_type = static_cast<int>(h.x_type);
+  a.out = static_cast<int>(h.out);
+  p.narrow = narrow_plan(a.x_frags, a.w_frags, a.blocks, act, h.x_type != PLM_FP8_CODES);
+  const Fp8TilePlan t = tile_plan(a.x_frags, a.w_frags, a.blocks);
+  // Results in fp32 need products that the tiles do not make.
+  p.tile = h.out != PLM_FP8_F32 && a.x_frags > 4 && t.us < p.narrow.us;
+  p.kind = t.kind;
+  p.bytes = 0;
+  if (p.tile) return true;
+  if (p.narrow.ranges > 1) p.bytes = static_cast<size_t>(p.narrow.ranges) * a.x_frags * a.w_frags * 1024;
+  return true;
+}
+
+}  // namespace
+}  // namespace plm
+
+extern "C" {
+
+size_t plm_fp8_linear_workspace_bytes(const plm_fp8_linear_call* call) {
+  plm::Fp8Gemm a{};
+  plm::Fp8Plan p{};
+  return plm::linear_of(call, a, p) ? p.bytes : 0;
+}
+
+int plm_fp8_linear(const plm_fp8_linear_call* call, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace plm;
   Fp8Gemm a{};
+  Fp8Plan p{};
+  if (!linear_of(call, a, p)) return PLM_ERR_ARGUMENT;
+  const plm_fp8_linear_call& h = *call;
+  const bool codes = h.x_type == PLM_FP8_CODES;
+  if (h.x == nullptr || (codes && h.x_scales == nullptr) || h.w == nullptr || h.w_scales == nullptr || h.y == nullptr)
+    return PLM_ERR_ARGUMENT;
+  for (const void* at : {h.x, h.x_scales, h.w, h.w_scales, static_cast<const void*>(workspace)})
+    if (!aligned16_ptr(at)) return PLM_ERR_ALIGNMENT;
+  if (!codes && h.x_row % 8 != 0) return PLM_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(h.y) % (h.out == PLM_FP8_F32 ? 4 : 2) != 0) return PLM_ERR_ALIGNMENT;
+  if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes)) return PLM_ERR_WORKSPACE;
   a.x = static_cast<const uint8_t*>(h.x);
   a.x_scales = static_cast<const uint8_t*>(h.x_scales);
   a.w = static_cast<const uint8_t*>(h.w);
   a.w_scales = static_cast<const uint8_t*>(h.w_scales);
   a.y = h.y;
-  a.ldy = h.ldy;
-  a.m = static_cast<int>(h.m);
-  a.n = static_cast<int>(h.n);
-  a.blocks = static_cast<int>(fp8_blocks(h.k));
-  a.x_frags = static_cast<int>(fp8_frags(h.m));
-  a.w_frags = static_cast<int>(fp8_frags(h.n));
-  a.out = static_cast<int>(h.out);
-  return fp8_narrow(a, act, static_cast<hipStream_t>(stream)) == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
+  a.partials = static_cast<f32x4*>(workspace);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipError_t err = p.tile ? fp8_tile(a, p.kind, h.act != 0, s) : fp8_narrow(a, p.narrow, h.act != 0, s);
+  return err == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 
 }  // extern "C"

@@ -2,19 +2,22 @@
 #pragma once
 
 #include "fp8.h"
+#include "fp8_plan.h"
 #include "plm_amd.h"
 
 namespace plm {
 
 struct Fp8Gemm {
-  const uint8_t* x;         // codes of [m, k]
+  const uint8_t* x;         // codes of [m, k], or rows of 16 bits (x_type: plm_fp8_in)
   const uint8_t* x_scales;
   const uint8_t* w;         // codes of [n, k]
   const uint8_t* w_scales;
   void* y;
-  int64_t ldy;
-  int m, n, blocks;         // n: rows of the weight; blocks of K
-  int x_frags, w_frags, out;  // out: plm_fp8_out
+  f32x4* partials;          // of products whose K is cut into ranges
+  int64_t ldy, x_row;       // x_row: stride of 16-bit rows
+  int m, n, k, blocks;      // n: rows of the weight; blocks of K
+  int range;                // blocks of a range
+  int x_frags, w_frags, x_type, out;  // out: plm_fp8_out
 };
 
 // g / (1 + e^-g) * u in fp32; the exponential's overflow gives g / inf = -0.
@@ -48,6 +51,7 @@ __device__ __forceinline__ void fp8_store4(const Fp8Gemm& a, int m, int n, int c
   }
 }
 
-hipError_t fp8_narrow(const Fp8Gemm& a, bool act, hipStream_t s);
+hipError_t fp8_narrow(Fp8Gemm a, const Fp8Narrow& p, bool act, hipStream_t s);
+hipError_t fp8_tile(const Fp8Gemm& a, Fp8TileKind kind, bool act, hipStream_t s);
 
 }  // namespace plm

@@ -159,7 +159,7 @@ __device__ __forceinline__ void emit16(const RowsArgs& a, const Norm& norm, int6
       for (int j = 0; j < 4; ++j)
         o[j] = fp8_word(y[4 * j] * inverse, y[4 * j + 1] * inverse, y[4 * j + 2] * inverse, y[4 * j + 3] * inverse);
       *reinterpret_cast<u32x4*>(a.codes + fp8_code_at(a.frags, row, at)) = o;
-      if ((threadIdx.x & 7) == 0) a.scales[fp8_scale_at(a.frags, row, block)] = fp8_exponent(scale);
+      if ((threadIdx.x & 7) == 0) fp8_put_scale(a.scales, a.frags, row, block, fp8_blocks(a.k), fp8_exponent(scale));
     }
   }
 }
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void weight_kernel(WeightArgs a) {
     }
     const int64_t place = fp8_place(half * a.half + row, a.n, a.gate_up != 0);
     *reinterpret_cast<u32x2*>(a.codes + fp8_code_at(frags, place, at)) = o;
-    if ((threadIdx.x & 15) == 0) a.scales[fp8_scale_at(frags, place, kb)] = fp8_exponent(scale);
+    if ((threadIdx.x & 15) == 0) fp8_put_scale(a.scales, frags, place, kb, a.k_blocks, fp8_exponent(scale));
   }
 }
 
@@ -354,7 +354,7 @@ hipError_t launch_rows(const RowsArgs& a, bool norm, hipStream_t s) {
 }
 
 bool sizes_fit(int64_t rows, int64_t k) {
-  return rows >= 1 && rows < (int64_t{1} << 28) && k >= 8 && k <= (1 << 24) && k % 8 == 0;
+  return rows >= 1 && rows < (int64_t{1} << 24) && k >= 8 && k <= (1 << 24) && k % 8 == 0;
 }
 
 template <typename... P>

@@ -21,6 +21,7 @@ PLM_RULE_NUCLEUS, PLM_RULE_FLOOR = 0, 1
 PLM_OUT_MODEL, PLM_OUT_F32, PLM_OUT_SILU_MUL = 0, 1, 2   # plm_chain_gemm.out_f32
 PLM_CACHE_BF16, PLM_CACHE_F16, PLM_CACHE_E4M3 = 0, 1, 2   # plm_kv_cache.type
 PLM_FP8_BF16, PLM_FP8_F16, PLM_FP8_F32 = 0, 1, 2   # plm_fp8_out
+PLM_FP8_CODES, PLM_FP8_ROWS_BF16, PLM_FP8_ROWS_F16 = 0, 1, 2   # plm_fp8_in
 DTYPE_CODES = {torch.bfloat16: PLM_BF16, torch.float16: PLM_F16}
 # PLM_WORKSPACE_COUNTER_BYTES: the zero-between-calls counter area at the start of every workspace.
 COUNTER_BYTES = 1 << 18
@@ -79,6 +80,7 @@ EXPORTS = (
     "plm_fp8_weight",
     "plm_fp8_values",
     "plm_fp8_linear",
+    "plm_fp8_linear_workspace_bytes",
     "plm_status_string",
 )
 
@@ -118,7 +120,7 @@ pack_attend = struct.Struct(f"={len(ATTEND_FIELDS) - 1}qd").pack
 FP8_ROWS_FIELDS = ("dtype", "rows", "k", "x", "x_row", "norm", "residual", "residual_row", "sum", "weight", "eps", "y", "codes",
                    "scales")
 FP8_WEIGHT_FIELDS = ("dtype", "n", "k", "w", "ld", "blocks", "gate_up", "codes", "scales")
-FP8_LINEAR_FIELDS = ("m", "n", "k", "x", "x_scales", "w", "w_scales", "y", "ldy", "out", "act")
+FP8_LINEAR_FIELDS = ("m", "n", "k", "x_type", "x", "x_scales", "x_row", "w", "w_scales", "y", "ldy", "out", "act")
 pack_fp8_rows = struct.Struct("=10qd3q").pack
 pack_fp8_weight = struct.Struct(f"={len(FP8_WEIGHT_FIELDS)}q").pack
 pack_fp8_linear = struct.Struct(f"={len(FP8_LINEAR_FIELDS)}q").pack
@@ -234,7 +236,11 @@ def _declare(lib: ctypes.CDLL) -> None:
     for name in ("plm_fp8_codes_bytes", "plm_fp8_scales_bytes"):
         getattr(lib, name).argtypes = [c_i64, c_i64]
         getattr(lib, name).restype = c_sz
-    for name in ("plm_fp8_rows", "plm_fp8_weight", "plm_fp8_linear"):
+    lib.plm_fp8_linear.argtypes = [ctypes.c_char_p, c_p, c_sz, c_p]
+    lib.plm_fp8_linear.restype = ctypes.c_int
+    lib.plm_fp8_linear_workspace_bytes.argtypes = [ctypes.c_char_p]
+    lib.plm_fp8_linear_workspace_bytes.restype = c_sz
+    for name in ("plm_fp8_rows", "plm_fp8_weight"):
         getattr(lib, name).argtypes = [ctypes.c_char_p, c_p]
         getattr(lib, name).restype = ctypes.c_int
     lib.plm_fp8_values.argtypes = [c_p, c_p, c_i64, c_i64, c_i32, c_i32, c_p, c_p]

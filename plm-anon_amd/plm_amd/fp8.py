@@ -28,7 +28,8 @@ E4M3 = torch.float8_e4m3fn
 BLOCK = 128
 _OUT = {torch.bfloat16: _lib.PLM_FP8_BF16, torch.float16: _lib.PLM_FP8_F16, torch.float32: _lib.PLM_FP8_F32}
 _EPS = (2.0 ** -100, 2.0 ** 100)
-MAX_ROWS = 1 << 21   # of a product
+_IN = {torch.bfloat16: _lib.PLM_FP8_ROWS_BF16, torch.float16: _lib.PLM_FP8_ROWS_F16}
+MOST = 1 << 21   # rows of a product's operands
 
 
 def _launch(entry, call, device: torch.device, what: str) -> None:
@@ -71,7 +72,7 @@ class _Eight:
         lib = _lib.lib()
         need = int(lib.plm_fp8_codes_bytes(rows, k)), int(lib.plm_fp8_scales_bytes(rows, k))
         if not need[0]:
-            raise ValueError(f"8-bit rows need 1 to 2^28 - 1 rows of a multiple of 8 in [8, 2^24], got [{rows}, {k}]")
+            raise ValueError(f"8-bit rows need 1 to 2^24 - 1 rows of a multiple of 8 in [8, 2^24], got [{rows}, {k}]")
         for name, t, size, dtype in (("codes", codes, need[0], E4M3), ("scales", scales, need[1], torch.uint8)):
             if t.dtype is not dtype or t.shape != (size,) or not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name} of [{rows}, {k}] must be contiguous {dtype} [{size}] on 16 bytes, got {t.dtype} "
@@ -255,37 +256,57 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6, *,
 def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dtype: torch.dtype | None, act: bool) -> torch.Tensor:
     if not isinstance(w, Weight):
         raise TypeError(f"w must be an fp8.Weight, got {type(w).__name__}")
+    kind, x_scales, stride = _lib.PLM_FP8_CODES, 0, 0
     if not isinstance(x, Rows):
-        if x.dim() != 2 or x.shape[1] != w.k:
-            raise ValueError(f"x must be [rows, {w.k}], got {list(x.shape)}")
+        x, x_at, stride = _matrix(x, "x", w.device)
+        rows, k = x.shape
         if out_dtype is None:
             out_dtype = x.dtype if out is None else out.dtype
-        x = quantize(x)
-    elif x.k != w.k:
-        raise ValueError(f"x must be [rows, {w.k}], got {list(x.shape)}")
-    elif out_dtype is None:
-        if out is None:
-            raise ValueError("rows in 8 bits have no type of their own: out_dtype or out is needed")
-        out_dtype = out.dtype
-    if x.device != w.device:
-        raise RuntimeError(f"x must be on the weight's GPU {w.device}, got {x.device}")
+        kind = _IN[x.dtype]
+    else:
+        rows, k, x_at, x_scales = x.rows, x.k, x.codes_at, x.scales_at
+        if out_dtype is None:
+            if out is None:
+                raise ValueError("rows in 8 bits have no type of their own: out_dtype or out is needed")
+            out_dtype = out.dtype
+        if x.device != w.device:
+            raise RuntimeError(f"x must be on the weight's GPU {w.device}, got {x.device}")
+    if k != w.k:
+        raise ValueError(f"x must be [rows, {w.k}], got {[rows, k]}")
     if out_dtype not in _OUT:
         raise TypeError(f"a product comes in bf16, fp16 or fp32, not {out_dtype}")
-    if x.rows > MAX_ROWS:
-        raise ValueError(f"a product takes up to {MAX_ROWS} rows, got {x.rows}")
-    shape = (x.rows, w.rows // 2 if act else w.rows)
+    if rows > MOST or w.rows > MOST:
+        raise ValueError(f"a product takes up to {MOST} rows of x and of the weight, got {rows} and {w.rows}")
+    columns = w.rows // 2 if act else w.rows
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=w.device)
-    elif out.shape != shape or out.dtype is not out_dtype or out.device != w.device or \
-            (shape[0] and (out.stride(1) != 1 and shape[1] > 1 or out.stride(0) < shape[1] and shape[0] > 1)):
-        raise ValueError(f"out must be a row-major {list(shape)} {out_dtype} tensor on {w.device}")
-    elif out.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("out requires a gradient, and the 8-bit calls have none")
-    if x.rows:
-        _launch(_lib.lib().plm_fp8_linear,
-                _lib.pack_fp8_linear(x.rows, w.rows, w.k, x.codes_at, x.scales_at, w.codes_at, w.scales_at, out.data_ptr(),
-                                     max(out.stride(0), shape[1]), _OUT[out_dtype], act), w.device,
-                f"plm_fp8_linear(M={x.rows}, N={w.rows}, K={w.k}, act={act})")
+        out = torch.empty((rows, columns), dtype=out_dtype, device=w.device)
+        out_row = columns
+    else:
+        if out.shape != (rows, columns) or out.dtype is not out_dtype or out.device != w.device or \
+                (rows and (out.stride(1) != 1 and columns > 1 or out.stride(0) < columns and rows > 1)):
+            raise ValueError(f"out must be a row-major {[rows, columns]} {out_dtype} tensor on {w.device}")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("out requires a gradient, and the 8-bit calls have none")
+        out_row = max(out.stride(0), columns)
+    if not rows:
+        return out
+    # Up to 16 rows every workgroup rounds for itself, which saves a launch (2048 x 2048 over one row 3.7 us for 6); not
+    # several for each of an LM head's many workgroups (50257 x 2048 over 16 rows 28 us for 26).
+    if kind and (rows > 16 or rows > 4 and w.rows > 16384):
+        x = quantize(x)
+        kind, x_at, x_scales = _lib.PLM_FP8_CODES, x.codes_at, x.scales_at
+    call = _lib.pack_fp8_linear(rows, w.rows, k, kind, x_at, x_scales, stride, w.codes_at, w.scales_at, out.data_ptr(), out_row,
+                                _OUT[out_dtype], act)
+    lib = _lib.lib()
+    space, size = 0, lib.plm_fp8_linear_workspace_bytes(call)
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=w.device)   # partial sums: this call's alone
+        space = work.data_ptr()
+
+    def entry(call, stream: int) -> int:
+        return lib.plm_fp8_linear(call, space, size, stream)
+
+    _launch(entry, call, w.device, f"plm_fp8_linear(M={rows}, N={w.rows}, K={k}, act={act})")
     return out
 
 

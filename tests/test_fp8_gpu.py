@@ -86,6 +86,30 @@ def test_quantize_extremes(device, dtype):
     _same(fp8.quantize(x.to(device)).values(), oracle.rounded(x))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_rows_in_the_product_round_as_their_own_launch(device, dtype):
+    """Up to 16 rows the product rounds them itself: extremes too, and short last blocks."""
+    info = torch.finfo(dtype)
+    for k in (256, 264, 392, 1032):
+        x = _rows(12, k, dtype, seed=k)
+        x[1] = 0
+        x[2, 1::2] = info.smallest_normal
+        x[3] = info.smallest_normal / 4
+        x[4, 7], x[4, 9] = info.max, -info.max
+        x[5, k - 1], x[5, 3] = float("inf"), 2.0
+        x[6, 130], x[6, 131] = float("nan"), info.max
+        x[7, :9] = torch.tensor([448.0, 1.0625, 1.1875, -1.0625, 17 * 2.0 ** -10, 2.0 ** -10, 3 * 2.0 ** -10, 2.0 ** -9, 208])
+        x[8] = x[8].sign() * 2.0 ** -10
+        x[9, 8:] = 0
+        for n in (16, 40):
+            weight = fp8.Weight.quantize(_weight(n, k, n, dtype=dtype)[0].to(device))
+            for m in (1, 5, 12):
+                rows = x[12 - m:].to(device)
+                for out in (F32, dtype):
+                    assert torch.equal(fp8.linear(rows, weight, out_dtype=out).view(torch.int32 if out is F32 else torch.int16),
+                                       fp8.linear(fp8.quantize(rows), weight, out_dtype=out).view(torch.int32 if out is F32 else torch.int16))
+
+
 def test_strided_rows(device):
     base = _rows(40, 600, BF16, seed=4).to(device)
     for x in (base[:, 8:392], base[::2, 16:400], base[:, 4:388], base.t().contiguous().t()[:, :384], base[3:4].expand(7, 600)):
@@ -204,7 +228,10 @@ def _check(got, x, w, out, act=False):
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), float(((got - want).abs() / off).nan_to_num().max()))
 
 
-PRODUCTS = [(1, 1, 8), (1, 2048, 2048), (2, 40, 136), (7, 33, 128), (16, 256, 1024), (17, 257, 1416), (33, 1000, 256), (42, 2560, 2560),
+# Each way a product is cut: whole and cut K (2048 x 8192 at 42 and 64, 512 x 10240), one and two fragments of the weight, every
+# tile (64 x 64 of 257 x 1416 at 300 to 256 x 256 at 1100 rows of 8200), short last fragments, tiles and groups of blocks.
+PRODUCTS = [(1, 1, 8), (42, 2048, 8192), (64, 2048, 8192), (20, 512, 10240), (300, 257, 1416), (700, 2056, 1032), (520, 6150, 2048),
+            (1100, 8200, 640), (1600, 8192, 2056), (513, 8208, 136), (1, 2048, 2048), (2, 40, 136), (7, 33, 128), (16, 256, 1024), (17, 257, 1416), (33, 1000, 256), (42, 2560, 2560),
             (56, 129, 10240), (64, 512, 520), (65, 300, 1032), (110, 384, 2048), (130, 16, 264), (250, 640, 648), (517, 304, 1416),
             (1025, 136, 392)]
 
@@ -224,7 +251,7 @@ def test_linear(device, m, n, k, dtype, out):
     assert bool((wide[:, :2] == 7).all()) and bool((wide[:, n + 2:] == 7).all())
 
 
-@pytest.mark.parametrize("m,half,k", [(1, 16, 8), (1, 5632, 2048), (3, 48, 136), (16, 128, 1024), (42, 1000 // 16 * 16, 520), (56, 5632, 2048),
+@pytest.mark.parametrize("m,half,k", [(1, 16, 8), (48, 512, 8192), (390, 5632, 512), (1100, 5640 // 16 * 16, 640), (1, 5632, 2048), (3, 48, 136), (16, 128, 1024), (42, 1000 // 16 * 16, 520), (56, 5632, 2048),
                                       (65, 304, 1416), (129, 160, 264), (300, 272, 2048), (1030, 144, 392)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_gate_up(device, m, half, k, dtype):

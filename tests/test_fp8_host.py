@@ -72,7 +72,7 @@ def test_every_place_is_taken_once(rows, k):
 
 
 def test_sizes_of_no_rows():
-    for rows, k in ((0, 64), (-1, 64), (1 << 28, 64), (4, 0), (4, 4), (4, 12), (4, (1 << 24) + 8), (4, -8)):
+    for rows, k in ((0, 64), (-1, 64), (1 << 24, 64), (4, 0), (4, 4), (4, 12), (4, (1 << 24) + 8), (4, -8)):
         assert fp8_bytes(rows, k) == (0, 0)
 
 
@@ -106,7 +106,7 @@ def test_c_entries_refuse_before_a_launch():
     rows = caller(lib.plm_fp8_rows, _lib.pack_fp8_rows,
                   dict(dtype=0, rows=3, k=64, x=f, x_row=64, norm=1, residual=f, residual_row=64, sum=f, weight=f, eps=1e-6, y=0,
                        codes=f, scales=f))
-    for bad in (dict(dtype=2), dict(rows=0), dict(rows=1 << 28), dict(k=60), dict(k=0), dict(x=0), dict(x_row=-8), dict(sum=0),
+    for bad in (dict(dtype=2), dict(rows=0), dict(rows=1 << 24), dict(k=60), dict(k=0), dict(x=0), dict(x_row=-8), dict(sum=0),
                 dict(residual=0), dict(codes=0), dict(scales=0), dict(norm=0), dict(norm=0, residual=0, sum=0),
                 dict(norm=0, residual=0, sum=0, weight=0, y=f), dict(eps=0.0), dict(eps=-1.0), dict(eps=math.nan), dict(eps=math.inf)):
         assert rows(**bad) == -1, bad
@@ -121,13 +121,27 @@ def test_c_entries_refuse_before_a_launch():
     for bad in (dict(w=f + 8), dict(w=f + 4, blocks=f), dict(ld=68), dict(codes=f + 2), dict(scales=f + 8)):
         assert weight(**bad) == -2, bad
 
-    linear = caller(lib.plm_fp8_linear, _lib.pack_fp8_linear,
-                    dict(m=3, n=64, k=64, x=f, x_scales=f, w=f, w_scales=f, y=f, ldy=64, out=0, act=0))
+    def product(call, stream):
+        return lib.plm_fp8_linear(call, f, 1 << 40, stream)
+
+    assert lib.plm_fp8_linear_workspace_bytes(None) == 0
+    linear = caller(product, _lib.pack_fp8_linear,
+                    dict(m=3, n=64, k=64, x_type=0, x=f, x_scales=f, x_row=0, w=f, w_scales=f, y=f, ldy=64, out=0, act=0))
     for bad in (dict(m=0), dict(m=(1 << 21) + 1), dict(n=0), dict(k=4), dict(x=0), dict(x_scales=0), dict(w=0), dict(w_scales=0),
-                dict(y=0), dict(ldy=63), dict(out=3), dict(out=-1), dict(act=1, n=48), dict(act=1, ldy=31)):
+                dict(y=0), dict(ldy=63), dict(out=3), dict(out=-1), dict(act=1, n=48), dict(act=1, ldy=31), dict(x_type=3),
+                dict(x_type=-1), dict(x_type=1, m=17), dict(x_type=2, x_row=-8), dict(n=(1 << 21) + 1, ldy=1 << 22)):
         assert linear(**bad) == -1, bad
-    for bad in (dict(x=f + 8), dict(x_scales=f + 4), dict(w=f + 2), dict(w_scales=f + 8), dict(y=f + 1), dict(y=f + 2, out=2)):
+    for bad in (dict(x=f + 8), dict(x_scales=f + 4), dict(w=f + 2), dict(w_scales=f + 8), dict(y=f + 1), dict(y=f + 2, out=2),
+                dict(x_type=1, x_row=4), dict(x_type=1, x=f + 8)):
         assert linear(**bad) == -2, bad
+
+    # Few columns over a long K: K is cut, and the partial sums need a workspace.
+    call = _lib.pack_fp8_linear(64, 2048, 8192, 0, f, f, 0, f, f, f, 2048, 0, 0)
+    need = lib.plm_fp8_linear_workspace_bytes(call)
+    assert need > 0 and need % 1024 == 0
+    assert lib.plm_fp8_linear(call, None, 0, None) == -4 and lib.plm_fp8_linear(call, f, need - 1, None) == -4
+    assert lib.plm_fp8_linear(call, f + 8, need, None) == -2
+    assert lib.plm_fp8_linear_workspace_bytes(_lib.pack_fp8_linear(64, 2048, 8196, 0, f, f, 0, f, f, f, 2048, 0, 0)) == 0
 
     for bad in ((0, f, 3, 64, 0, 0, f), (f, 0, 3, 64, 0, 0, f), (f, f, 0, 64, 0, 0, f), (f, f, 3, 60, 0, 0, f), (f, f, 48, 64, 1, 0, f),
                 (f, f, 3, 64, 0, 3, f), (f, f, 3, 64, 0, 0, 0)):
