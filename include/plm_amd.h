@@ -596,7 +596,7 @@ size_t plm_attend_workspace_bytes(const plm_attend_call* call);
  *
  * Order of the bytes, in fragments of 16 rows x 128 of K, ceil(rows / 16) x ceil(K / 128) of them. With f = row / 16,
  * r = row % 16, b = k / 128:
- *   codes   [b][f][k / 64 % 2][k / 16 % 4][r][k % 16]
+ *   codes   [b][f][k / 64 % 2][k / 8 % 4][r][k / 32 % 2][k % 8]
  *   scales  [b / 4][f][r][b % 4], the exponent + 127 in a byte
  * Codes and scales past K are zeros, rows past the last of any content. plm_fp8_codes_bytes, plm_fp8_scales_bytes: the sizes (0
  * where there are no such rows: 1 <= rows < 2^24, 8 <= K <= 2^24, K % 8 == 0). A gate/up weight (gate rows first, N a

@@ -52,7 +52,7 @@ def places(rows: int, k: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Where codes and scales of ``[rows, k]`` lie in their buffers."""
     frags = -(-rows // 16)
     r, c = torch.arange(rows)[:, None], torch.arange(k)
-    codes = (((c // 128 * frags + r // 16) * 2 + c // 64 % 2) * 4 + c // 16 % 4) * 256 + r % 16 * 16 + c % 16
+    codes = (((c // 128 * frags + r // 16) * 2 + c // 64 % 2) * 4 + c // 8 % 4) * 256 + r % 16 * 16 + c // 32 % 2 * 8 + c % 8
     b = torch.arange(-(-k // 128))
     return codes, ((b // 4 * frags + r // 16) * 16 + r % 16) * 4 + b % 4
 

@@ -4,8 +4,9 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 rows by 16 columns over 128 of K and takes a power of two for each
 // row and each column (32 of K at a time; all four are the block's here), so a block's scales cost no instruction of
 // their own and the sum over blocks is one chain of such products in fp32. Where in K a lane's 32 bytes lie is free as long
-// as both operands agree. With r = row % 16, f = row / 16, b = k / 128, h = k / 64 % 2, g = k / 16 % 4, j = k % 16:
-//   code   byte ((b * fragments + f) * 2 + h) * 1024 + g * 256 + r * 16 + j
+// as both operands agree: in pieces of 8, so that four lanes' pieces of 16-bit values are 64 bytes of a row. With r = row % 16,
+// f = row / 16, b = k / 128, h = k / 64 % 2, p = k / 32 % 2, g = k / 8 % 4, j = k % 8:
+//   code   byte ((b * fragments + f) * 2 + h) * 1024 + g * 256 + r * 16 + p * 8 + j
 //   scale  byte ((b / 4) * fragments + f) * 64 + r * 4 + b % 4, holding the exponent + 127
 // Lane l = 16 g + r reads 16 bytes at 16 l of either half: 1 KiB side by side per load, from memory and from LDS.
 // Codes past K are zero, and so are scales (2^-127); rows past the last hold anything, since a row's codes reach only its own outputs.
@@ -30,8 +31,11 @@ __host__ __device__ constexpr int64_t fp8_scales_bytes(int64_t rows, int64_t k) 
 }
 
 __device__ __forceinline__ int64_t fp8_code_at(int64_t frags, int64_t row, int64_t k) {
-  return ((k >> 7) * frags + (row >> 4)) * kFp8Bytes + ((k >> 6) & 1) * 1024 + ((k >> 4) & 3) * 256 + (row & 15) * 16 + (k & 15);
+  return ((k >> 7) * frags + (row >> 4)) * kFp8Bytes + ((k >> 6) & 1) * 1024 + ((k >> 3) & 3) * 256 + (row & 15) * 16 +
+         ((k >> 5) & 1) * 8 + (k & 7);
 }
+// Where in K the four pieces of eight of a lane lie, in its codes' order.
+__device__ __forceinline__ int fp8_piece_at(int64_t kb, int lane, int i) { return static_cast<int>(kb) * kFp8Block + i * 32 + (lane >> 4) * 8; }
 __device__ __forceinline__ int64_t fp8_scale_at(int64_t frags, int64_t row, int64_t block) {
   return ((block >> 2) * frags + (row >> 4)) * kFp8ScaleBytes + (row & 15) * 4 + (block & 3);
 }
@@ -93,6 +97,14 @@ __device__ __forceinline__ uint32_t fp8_four(uint32_t lo, uint32_t hi, float sca
     w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, lo), scale, false);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, hi), scale, true);
   }
+  return __builtin_bit_cast(uint32_t, w);
+}
+
+__device__ __forceinline__ uint32_t fp8_four(float a, float b, float c, float d, float scale) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  s16x2 w = {0, 0};
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, scale, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, scale, true);
   return __builtin_bit_cast(uint32_t, w);
 }
 

@@ -44,11 +44,11 @@ __device__ __forceinline__ void load(const Fp8Gemm& a, int kb, int f0, int t0, i
       o.xs[t] = xs[static_cast<uint32_t>(there >> 4) * static_cast<uint32_t>(kFp8ScaleBytes) + (there & 15) * 4];
     }
   } else {
-    const int r = (lane & 15) < a.m ? lane & 15 : 0, at = kb * kFp8Block + (lane >> 4) * 16;
+    const int r = (lane & 15) < a.m ? lane & 15 : 0;
     const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x) + r * a.x_row;
 #pragma unroll
     for (int i = 0; i < 4; ++i)   // past k anything: round_rows puts zeros there
-      o.raw[i] = *reinterpret_cast<const u32x4*>(x + min(at + (i >> 1) * 64 + (i & 1) * 8, a.k - 8));
+      o.raw[i] = *reinterpret_cast<const u32x4*>(x + min(fp8_piece_at(kb, lane, i), a.k - 8));
   }
 }
 
@@ -59,7 +59,7 @@ __device__ __forceinline__ void round_rows(Operands<MT, NF>& o, int kb, int k, i
   if ((kb + 1) * kFp8Block > k) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (kb * kFp8Block + (lane >> 4) * 16 + (i >> 1) * 64 + (i & 1) * 8 >= k) o.raw[i] = u32x4{0u, 0u, 0u, 0u};
+      if (fp8_piece_at(kb, lane, i) >= k) o.raw[i] = u32x4{0u, 0u, 0u, 0u};
   }
   const uint32_t most = fp8_most16<DT>(o.raw[0], o.raw[1], o.raw[2], o.raw[3]);
   const uint32_t of_row = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));

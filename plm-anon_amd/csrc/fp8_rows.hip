@@ -1,12 +1,11 @@
 // Rows into 8 bits (plm_fp8_rows), with the root-mean-square norm and the residual's addition before it or the norm in
-// 16 bits; weights into 8 bits or into the kernels' order (plm_fp8_weight, plm_fp8_pack) and back to values
-// (plm_fp8_values). Declared in include/plm_amd.h; order of the bytes: fp8.h.
+// 16 bits; weights into 8 bits or into the kernels' order (plm_fp8_weight) and back to values (plm_fp8_values). Declared in
+// include/plm_amd.h; order of the bytes: fp8.h.
 //
 // Norm: t = x + residual, rounded to the model's type (so that the norm of the returned sum is the same); y = t w / sqrt(
-// mean(t^2) + eps). The sum of squares is fp64: squares of 16-bit values are exact in fp32, four of them are added in
-// fp32 at most. y in fp32 is off by three roundings; a code has 2^20 fp32 values to a step, so of a million values one to
-// four would come out on the other side of a border between codes: what is that close is computed in fp64 and
-// rounded once, the scale's border likewise.
+// mean(t^2) + eps). The sum of squares and the root are fp64. y in fp32 is off by three roundings, 3 of its last places at
+// most; a code has 2^20 fp32 values to a step, so of a million values one to four would come out on the other side of a
+// border between codes: what is that close is computed in fp64 and rounded once, the scale's border likewise.
 #include <hip/hip_runtime.h>
 
 #include "fp8.h"
@@ -54,191 +53,316 @@ __device__ __forceinline__ float odd_float(double v) {
   return __builtin_bit_cast(float, bits);
 }
 
-// Sixteen values of a row from `at`, a multiple of 16 (k is one of 8), zeros past k.
-template <int DT>
-__device__ __forceinline__ void load16(const uint16_t* row, int at, int k, u32x4 (&v)[2]) {
-  v[0] = at < k ? *reinterpret_cast<const u32x4*>(row + at) : u32x4{0u, 0u, 0u, 0u};
-  v[1] = at + 8 < k ? *reinterpret_cast<const u32x4*>(row + at + 8) : u32x4{0u, 0u, 0u, 0u};
+// Eight values of a row from `at`, a multiple of 8 as k is one; zeros past k.
+__device__ __forceinline__ u32x4 load8(const uint16_t* row, int at, int k) {
+  return at < k ? *reinterpret_cast<const u32x4*>(row + at) : u32x4{0u, 0u, 0u, 0u};
 }
 
 // x + residual, rounded.
 template <int DT>
-__device__ __forceinline__ void add16(u32x4 (&v)[2], const u32x4 (&r)[2]) {
+__device__ __forceinline__ u32x4 add8(u32x4 v, u32x4 r) {
+  float x[8], y[8];
+  unpack8<DT>(v, x);
+  unpack8<DT>(r, y);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float x[8], y[8];
-    unpack8<DT>(v[h], x);
-    unpack8<DT>(r[h], y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] += y[i];
-    v[h] = pack8of<DT>(x);
-  }
+  for (int i = 0; i < 8; ++i) x[i] += y[i];
+  return pack8of<DT>(x);
 }
 
-__device__ __forceinline__ void store16(uint16_t* row, int at, int k, const u32x4 (&v)[2]) {
-  if (at < k) *reinterpret_cast<u32x4*>(row + at) = v[0];
-  if (at + 8 < k) *reinterpret_cast<u32x4*>(row + at + 8) = v[1];
+template <int DT>
+__device__ __forceinline__ double squares8(u32x4 v) {
+  float x[8];
+  unpack8<DT>(v, x);
+  double sum = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), sum);
+  return sum;
 }
 
 // A row's norm: 1 / sqrt(mean + eps) in both widths.
 struct Norm {
   double exact;
   float near;
-  bool wide;   // outside of what fp32 steps stay accurate in: every value in fp64
+  bool wide;   // outside of where fp32 keeps its steps: every value in fp64
 };
 
-// y of sixteen values. `close` gets the bit of each that is within its error (three roundings, 2^-22 is more than twice
-// that) of a place where codes may part: at most four bits of mantissa, so 19 zeros at the end.
-template <int DT, bool NORM, bool WEIGHT>
-__device__ __forceinline__ void normed16(const RowsArgs& a, const Norm& norm, const u32x4 (&v)[2], int at, float (&y)[16],
-                                         uint32_t& close) {
-  unpack8<DT>(v[0], y);
-  unpack8<DT>(v[1], y + 8);
-  close = 0;
-  if constexpr (NORM) {
-    float w[16];
-    if constexpr (WEIGHT) {
-      u32x4 of[2];
-      load16<DT>(a.weight, at, a.k, of);
-      unpack8<DT>(of[0], w);
-      unpack8<DT>(of[1], w + 8);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      y[i] *= norm.near;
-      if constexpr (WEIGHT) y[i] *= w[i];
-      const float border = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, y[i]) + 0x40000u) & 0xfff80000u);
-      close |= fabsf(y[i] - border) < 0x1p-22f * fabsf(y[i]) || (norm.wide && at + i < a.k) ? 1u << i : 0u;
-    }
-  }
+__device__ __forceinline__ Norm norm_of(double squares, int k, double eps) {
+  Norm n;
+  n.exact = 1.0 / sqrt(squares / k + eps);
+  n.near = static_cast<float>(n.exact);
+  n.wide = !(n.near > 0x1p-100f && n.near < 0x1p100f);
+  return n;
 }
 
-// The values of `close`, in fp64 and rounded to odd.
-template <int DT, bool WEIGHT>
-__device__ __forceinline__ void normed_exact(const RowsArgs& a, const Norm& norm, const u32x4 (&v)[2], int at, uint32_t close,
-                                             float (&y)[16]) {
-  for (; close != 0; close &= close - 1) {
-    const int j = __builtin_ctz(close);
-    uint32_t word = 0;
+// y of N / 8 pieces of eight values. Returns whether one is so close to a place where codes may part that fp32 does not tell the
+// side: those have at most four bits of mantissa, 19 zeros at the end.
+template <int DT, bool WEIGHT, int N>
+__device__ __forceinline__ bool normed(const Norm& norm, const u32x4 (&v)[N / 8], const u32x4 (&w)[N / 8], float (&y)[N]) {
+  uint32_t least = ~0u;
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
-      if (n == j >> 1) word = v[n >> 2][n & 3];
-    double exact = static_cast<double>(from_bits16<DT>(static_cast<uint16_t>(word >> (16 * (j & 1))))) * norm.exact;
-    if constexpr (WEIGHT) exact *= static_cast<double>(from_bits16<DT>(a.weight[at + j]));
+  for (int p = 0; p < N / 8; ++p) {
+    float of[8];
+    unpack8<DT>(v[p], y + 8 * p);
+    if constexpr (WEIGHT) unpack8<DT>(w[p], of);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[8 * p + i] *= norm.near;
+      if constexpr (WEIGHT) y[8 * p + i] *= of[i];
+      least = min(least, (__builtin_bit_cast(uint32_t, y[8 * p + i]) + 4u) & 0x7ffffu);
+    }
+  }
+  return least <= 8u || norm.wide;
+}
+
+// What is that close, in fp64 and rounded to odd: one value at a time, as it is rarely more than one of a wavefront's, and read
+// again, so that nothing is kept for it. `t` and `weight`: the row and the norm's weights, value i at place(i) of k.
+template <int DT, bool WEIGHT, int N, typename P>
+__device__ __forceinline__ void normed_exact(const Norm& norm, const uint16_t* t, const uint16_t* weight, int k, P place, float (&y)[N]) {
+  uint32_t close = norm.wide ? ~0u >> (32 - N) : 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) close |= ((__builtin_bit_cast(uint32_t, y[i]) + 4u) & 0x7ffffu) <= 8u ? 1u << i : 0u;
+#pragma unroll 1
+  for (; close != 0; close &= close - 1) {
+    const int i = __builtin_ctz(close), at = place(i);
+    if (at >= k) continue;
+    double exact = static_cast<double>(from_bits16<DT>(t[at])) * norm.exact;
+    if constexpr (WEIGHT) exact *= static_cast<double>(from_bits16<DT>(weight[at]));
     const float odd = odd_float(exact);
 #pragma unroll
-    for (int n = 0; n < 16; ++n)
-      if (n == j) y[n] = odd;
+    for (int n = 0; n < N; ++n) y[n] = n == i ? odd : y[n];
   }
 }
 
-// Sixteen values of a row, of `row`'s 16-bit v, into the output.
-template <int DT, bool NORM, bool WEIGHT, bool E8>
-__device__ __forceinline__ void emit16(const RowsArgs& a, const Norm& norm, int64_t row, int at, const u32x4 (&v)[2]) {
-  float y[16];
-  uint32_t close;
-  normed16<DT, NORM, WEIGHT>(a, norm, v, at, y, close);
-  if constexpr (NORM) {
-    if (E8 || norm.wide) normed_exact<DT, WEIGHT>(a, norm, v, at, close, y);
-  }
-  if constexpr (!E8) {
-    const u32x4 o[2] = {pack8of<DT>(y), pack8of<DT>(y + 8)};
-    store16(a.y + row * a.k, at, a.k, o);
-  } else {
-    // 448 is among the borders above: a value that could lie on either side of it has been computed exactly.
+// Codes of N values, and their scale; `share` gives the largest of the lanes that have a block between them. 448 is among the
+// borders above: a value that could lie on either side of it has been computed exactly.
+template <int N, typename F>
+__device__ __forceinline__ float codes_of(const float (&y)[N], F share, uint32_t (&codes)[N / 4]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) most = max(most, __builtin_bit_cast(uint32_t, y[i]) & 0x7fffffffu);
+  most = share(most);
+  if (__builtin_expect(__ballot(most >= 0x7f800000u) != 0, 0)) {   // not all finite
     float amax = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fp8_magnitude(y[j]));
+    for (int i = 0; i < N; ++i) amax = fmaxf(amax, fp8_magnitude(y[i]));
+    const float scale = fp8_scale_of(__builtin_bit_cast(float, share(__builtin_bit_cast(uint32_t, amax)))), inverse = fp8_inverse(scale);
 #pragma unroll
-    for (int d = 1; d < 8; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
-    const float scale = fp8_scale_of(amax), inverse = fp8_inverse(scale);
-    const int block = at >> 7;
-    if (block < static_cast<int>(fp8_blocks(a.k))) {
-      u32x4 o;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = fp8_word(y[4 * j] * inverse, y[4 * j + 1] * inverse, y[4 * j + 2] * inverse, y[4 * j + 3] * inverse);
-      *reinterpret_cast<u32x4*>(a.codes + fp8_code_at(a.frags, row, at)) = o;
-      if ((threadIdx.x & 7) == 0) fp8_put_scale(a.scales, a.frags, row, block, fp8_blocks(a.k), fp8_exponent(scale));
-    }
+    for (int i = 0; i < N / 4; ++i)
+      codes[i] = fp8_word(y[4 * i] * inverse, y[4 * i + 1] * inverse, y[4 * i + 2] * inverse, y[4 * i + 3] * inverse);
+    return scale;
   }
+  const float scale = fp8_scale_of(__builtin_bit_cast(float, most));
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) codes[i] = fp8_four(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3], scale);
+  return scale;
 }
 
-// Chunks of 16 values of a row; whole blocks where codes are written, whose zeros past k are part of them.
+// Chunks of 16 values of a row, 8 and 8 of every 64; whole blocks where codes are written, whose zeros past k are part of them.
 template <bool E8>
-__device__ __forceinline__ int row_chunks(int k) {
-  return E8 ? static_cast<int>(fp8_blocks(k)) * 8 : (k + 15) / 16;
+__host__ __device__ __forceinline__ int row_chunks(int k) {
+  return E8 ? static_cast<int>(fp8_blocks(k)) * 8 : (k + 63) / 64 * 4;
 }
 
-// A wavefront takes a row, a lane the sixteen values at 16 (lane + 64 i); eight lanes have a block. HELD chunks stay in
-// registers between the sum of squares and the output; the rest of a longer row is read again.
-template <int DT, bool RES, bool WEIGHT, bool E8, int HELD>
-__global__ __launch_bounds__(1024) void norm_kernel(RowsArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 6) + (threadIdx.x >> 6);
-  if (row >= a.rows) return;
-  const int turns = (row_chunks<E8>(a.k) + 63) / 64;
+// A workgroup has a row, a thread chunks thread + threads i of it, the pieces of eight at 64 (chunk / 4) + 8 (chunk % 4) and 32
+// further; eight threads have a block. The first chunk stays in
+// registers between the sum of squares and the output; the rest of a row longer than the workgroup is read again.
+template <int DT, bool RES, bool WEIGHT, bool E8>
+__global__ __launch_bounds__(1024) void row_norm_kernel(RowsArgs a) {
+  __shared__ double parts[16];
+  const int64_t row = blockIdx.x;
+  const int threads = blockDim.x, turns = (row_chunks<E8>(a.k) + threads - 1) / threads;
   const uint16_t* x = a.x + row * a.x_row;
   const uint16_t* residual = RES ? a.residual + row * a.residual_row : nullptr;
   uint16_t* sum = RES ? a.sum + row * a.k : nullptr;
-  double squares = 0.0;
-  auto add = [&](const u32x4 (&v)[2]) {
-    float f[16];
-    unpack8<DT>(v[0], f);
-    unpack8<DT>(v[1], f + 8);
+  auto read = [&](int at, u32x4 (&v)[2]) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) squares = fma(static_cast<double>(f[j]), static_cast<double>(f[j]), squares);
+    for (int h = 0; h < 2; ++h) {
+      v[h] = load8(x, at + 32 * h, a.k);
+      if constexpr (RES) {
+        v[h] = add8<DT>(v[h], load8(residual, at + 32 * h, a.k));
+        if (at + 32 * h < a.k) *reinterpret_cast<u32x4*>(sum + at + 32 * h) = v[h];
+      }
+    }
+    return squares8<DT>(v[0]) + squares8<DT>(v[1]);
   };
-  u32x4 held[HELD][2], more[RES ? HELD : 1][2];
+  auto weights = [&](int at, u32x4 (&w)[2]) {
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {   // every load before the first store, which it may not pass
-    load16<DT>(x, 16 * (lane + 64 * i), a.k, held[i]);
-    if constexpr (RES) load16<DT>(residual, 16 * (lane + 64 * i), a.k, more[i]);
-  }
+    for (int h = 0; h < 2; ++h) w[h] = WEIGHT ? load8(a.weight, at + 32 * h, a.k) : u32x4{0u, 0u, 0u, 0u};
+  };
+  auto emit = [&](const Norm& norm, int at, const u32x4 (&v)[2], const u32x4 (&w)[2]) {
+    float y[16];
+    const bool close = normed<DT, WEIGHT, 16>(norm, v, w, y);
+    if (E8 ? close : norm.wide)
+      normed_exact<DT, WEIGHT, 16>(norm, RES ? sum : x, a.weight, a.k, [&](int i) { return at + (i >> 3) * 32 + (i & 7); }, y);
+    if constexpr (E8) {
+      uint32_t c[4];
+      const float scale = codes_of<16>(y, [](uint32_t most) {
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
-    if constexpr (RES) {
-      add16<DT>(held[i], more[i]);
-      store16(sum, 16 * (lane + 64 * i), a.k, held[i]);
+        for (int d = 1; d < 8; d <<= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+        return most;
+      }, c);
+      const int block = at >> 7;
+      if (block < static_cast<int>(fp8_blocks(a.k))) {
+        *reinterpret_cast<u32x4*>(a.codes + fp8_code_at(a.frags, row, at)) = u32x4{c[0], c[1], c[2], c[3]};
+        if ((threadIdx.x & 7) == 0) fp8_put_scale(a.scales, a.frags, row, block, fp8_blocks(a.k), fp8_exponent(scale));
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (at + 32 * h < a.k) *reinterpret_cast<u32x4*>(a.y + row * a.k + at + 32 * h) = pack8of<DT>(y + 8 * h);
     }
-    add(held[i]);
-  }
-  for (int i = HELD; i < turns; ++i) {
+  };
+
+  auto chunk_at = [&](int i) {
+    const int chunk = static_cast<int>(threadIdx.x) + threads * i;
+    return (chunk >> 2) * 64 + (chunk & 3) * 8;
+  };
+  const int first = chunk_at(0);
+  u32x4 held[2], w[2];
+  weights(first, w);
+  double squares = read(first, held);
+  for (int i = 1; i < turns; ++i) {
     u32x4 v[2];
-    load16<DT>(x, 16 * (lane + 64 * i), a.k, v);
-    if constexpr (RES) {
-      u32x4 r[2];
-      load16<DT>(residual, 16 * (lane + 64 * i), a.k, r);
-      add16<DT>(v, r);
-      store16(sum, 16 * (lane + 64 * i), a.k, v);
-    }
-    add(v);
+    squares += read(chunk_at(i), v);
   }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) squares += __shfl_xor(squares, d);
-  Norm norm;
-  norm.exact = 1.0 / sqrt(squares / a.k + a.eps);
-  norm.near = static_cast<float>(norm.exact);
-  norm.wide = !(norm.near > 0x1p-100f && norm.near < 0x1p100f);
+  if (threads > 64) {
+    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = squares;
+    __syncthreads();
+    squares = parts[0];
+    for (int i = 1; i < threads >> 6; ++i) squares += parts[i];
+  }
+  const Norm norm = norm_of(squares, a.k, a.eps);
+  emit(norm, first, held, w);
+  for (int i = 1; i < turns; ++i) {
+    u32x4 v[2], of[2];
+    const int at = chunk_at(i);
 #pragma unroll
-  for (int i = 0; i < HELD; ++i)
-    if (i < turns) emit16<DT, true, WEIGHT, E8>(a, norm, row, 16 * (lane + 64 * i), held[i]);
-  for (int i = HELD; i < turns; ++i) {
-    u32x4 v[2];
-    load16<DT>(RES ? sum : x, 16 * (lane + 64 * i), a.k, v);   // of the sum this lane's own stores
-    emit16<DT, true, WEIGHT, E8>(a, norm, row, 16 * (lane + 64 * i), v);
+    for (int h = 0; h < 2; ++h) v[h] = load8(RES ? sum : x, at + 32 * h, a.k);   // of the sum this thread's own
+    weights(at, of);
+    emit(norm, at, v, of);
   }
 }
 
-// Rows as they are: every 64 chunks of a row a wavefront's of its own.
+// The lanes of a row in a wavefront that has a fragment: 16 apart.
+__device__ __forceinline__ uint32_t share_row(uint32_t most) {
+  most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
+  return max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+}
+
+// A lane's 32 codes of a fragment, 1 KiB side by side per store, and the scales of its rows.
+__device__ __forceinline__ void store_fragment(const RowsArgs& a, int64_t frag, int kb, int lane, const uint32_t (&c)[8], float scale) {
+  u32x4* to = reinterpret_cast<u32x4*>(a.codes + (kb * a.frags + frag) * kFp8Bytes) + lane;
+  to[0] = u32x4{c[0], c[1], c[2], c[3]};
+  to[64] = u32x4{c[4], c[5], c[6], c[7]};
+  if (lane < 16) fp8_put_scale(a.scales, a.frags, frag * 16 + lane, kb, fp8_blocks(a.k), fp8_exponent(scale));
+}
+
+// Sixteen rows of the norm in 8 bits: a wavefront has a fragment, row lane % 16 of it a lane, and takes the blocks of K that its
+// number gives it, the first HELD of which stay in registers. Whole lines are written, where a row to a workgroup
+// writes 16 bytes of each.
+template <int DT, bool RES, bool WEIGHT, int HELD>
+__global__ __launch_bounds__(1024) void fragment_norm_kernel(RowsArgs a) {
+  __shared__ double parts[16][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, blocks = static_cast<int>(fp8_blocks(a.k));
+  const int64_t frag = blockIdx.x, row = min(frag * 16 + (lane & 15), static_cast<int64_t>(a.rows) - 1);
+  const bool there = frag * 16 + (lane & 15) < a.rows;   // rows past the last compute the last one's, and store nothing
+  const uint16_t* x = a.x + row * a.x_row;
+  const uint16_t* residual = RES ? a.residual + row * a.residual_row : nullptr;
+  uint16_t* sum = RES ? a.sum + row * a.k : nullptr;
+  u32x4 held[HELD][4];
+  double squares = 0.0;
+  {
+    u32x4 more[HELD][4];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)   // every load before the first store, which it may not pass
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        held[i][j] = load8(x, fp8_piece_at(wave + waves * i, lane, j), a.k);
+        if constexpr (RES) more[i][j] = load8(residual, fp8_piece_at(wave + waves * i, lane, j), a.k);
+      }
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (RES) {
+          held[i][j] = add8<DT>(held[i][j], more[i][j]);
+          const int at = fp8_piece_at(wave + waves * i, lane, j);
+          if (at < a.k && there) *reinterpret_cast<u32x4*>(sum + at) = held[i][j];
+        }
+        squares += squares8<DT>(held[i][j]);
+      }
+  }
+  for (int kb = wave + waves * HELD; kb < blocks; kb += waves)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = fp8_piece_at(kb, lane, j);
+      u32x4 v = load8(x, at, a.k);
+      if constexpr (RES) {
+        v = add8<DT>(v, load8(residual, at, a.k));
+        if (at < a.k && there) *reinterpret_cast<u32x4*>(sum + at) = v;
+      }
+      squares += squares8<DT>(v);
+    }
+  squares += __shfl_xor(squares, 16);
+  squares += __shfl_xor(squares, 32);
+  if (lane < 16) parts[wave][lane] = squares;
+  __syncthreads();
+  squares = parts[0][lane & 15];
+  for (int i = 1; i < waves; ++i) squares += parts[i][lane & 15];
+  const Norm norm = norm_of(squares, a.k, a.eps);
+  auto emit = [&](int kb, const u32x4 (&v)[4]) {
+    u32x4 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = WEIGHT ? load8(a.weight, fp8_piece_at(kb, lane, j), a.k) : u32x4{0u, 0u, 0u, 0u};
+    float y[32];
+    if (normed<DT, WEIGHT, 32>(norm, v, w, y))
+      normed_exact<DT, WEIGHT, 32>(norm, RES ? sum : x, a.weight, a.k, [&](int i) { return fp8_piece_at(kb, lane, i >> 3) + (i & 7); }, y);
+    uint32_t c[8];
+    const float scale = codes_of<32>(y, share_row, c);
+    store_fragment(a, frag, kb, lane, c, scale);
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+    if (wave + waves * i < blocks) emit(wave + waves * i, held[i]);
+  for (int kb = wave + waves * HELD; kb < blocks; kb += waves) {
+    u32x4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = fp8_piece_at(kb, lane, j);
+      v[j] = load8(x, at, a.k);
+      // Read again rather than the sum, which a row past the last has not stored.
+      if constexpr (RES) v[j] = add8<DT>(v[j], load8(residual, at, a.k));
+    }
+    emit(kb, v);
+  }
+}
+
+// Rows as they are: a wavefront has a fragment.
 template <int DT>
-__global__ __launch_bounds__(1024) void round_kernel(RowsArgs a) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 6) + (threadIdx.x >> 6);
-  if (row >= a.rows) return;
-  const int at = 16 * (static_cast<int>(blockIdx.y) * 64 + static_cast<int>(threadIdx.x & 63));
-  u32x4 v[2];
-  load16<DT>(a.x + row * a.x_row, at, a.k, v);
-  emit16<DT, false, false, true>(a, Norm{0.0, 1.0f, false}, row, at, v);
+__global__ __launch_bounds__(256) void round_kernel(RowsArgs a, int64_t count) {
+  const int64_t number = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (number >= count) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t kb = number / a.frags, frag = number - kb * a.frags, row = min(frag * 16 + (lane & 15), static_cast<int64_t>(a.rows) - 1);
+  u32x4 v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = load8(a.x + row * a.x_row, fp8_piece_at(static_cast<int>(kb), lane, j), a.k);
+  uint32_t c[8];
+  const uint32_t most = share_row(fp8_most16<DT>(v[0], v[1], v[2], v[3]));
+  float scale;
+  if (__builtin_expect(__ballot(most >= fp8_infinite<DT>()) != 0, 0)) {
+    i32x8 codes;
+    scale = fp8_round_any<DT>(v, [](float amax) { return __builtin_bit_cast(float, share_row(__builtin_bit_cast(uint32_t, amax))); }, codes);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = static_cast<uint32_t>(codes[i]);
+  } else {
+    scale = fp8_scale_of(from_bits16<DT>(static_cast<uint16_t>(most)));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = fp8_four<DT>(v[i >> 1][2 * (i & 1)], v[i >> 1][2 * (i & 1) + 1], scale);
+  }
+  store_fragment(a, frag, static_cast<int>(kb), lane, c, scale);
 }
 
 struct WeightArgs {
@@ -299,50 +423,64 @@ struct ValuesArgs {
   const uint8_t* codes;
   const uint8_t* scales;
   void* y;   // contiguous [rows, k]
-  int64_t rows, k, frags, pieces;
+  int64_t rows, k, frags, count;
   int gate_up;
 };
 
-// A thread has eight values of a row; OUT: plm_fp8_out.
+// A wavefront has a fragment, a lane 32 values of a row; OUT: plm_fp8_out.
 template <int OUT>
 __global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
-  const int64_t piece = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (piece >= a.pieces) return;
-  const int64_t per = a.k >> 3, row = piece / per, at = (piece - row * per) << 3;
-  const int64_t place = fp8_place(row, a.rows, a.gate_up != 0);
-  const u32x2 word = *reinterpret_cast<const u32x2*>(a.codes + fp8_code_at(a.frags, place, at));
-  const float scale = fp8_power(a.scales[fp8_scale_at(a.frags, place, at >> 7)]);
-  float x[8];
+  const int64_t number = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (number >= a.count) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t kb = number / a.frags, frag = number - kb * a.frags;
+  const int64_t row = (a.gate_up != 0 ? (frag >> 1) * 16 + (frag & 1) * (a.rows >> 1) : frag * 16) + (lane & 15);
+  if (row >= a.rows) return;
+  const u32x4* from = reinterpret_cast<const u32x4*>(a.codes + number * kFp8Bytes) + lane;
+  const u32x4 codes[2] = {from[0], from[64]};
+  const float scale = fp8_power(a.scales[fp8_scale_at(a.frags, frag * 16 + (lane & 15), kb)]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = fp8_value(word[j >> 2], j & 3) * scale;
-  if constexpr (OUT == PLM_FP8_F32) {
-    f32x4* y = reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + row * a.k + at);
-    y[0] = f32x4{x[0], x[1], x[2], x[3]};
-    y[1] = f32x4{x[4], x[5], x[6], x[7]};
-  } else {
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) + row * a.k + at) = pack8of<OUT == PLM_FP8_BF16 ? DT_BF16 : DT_F16>(x);
+  for (int j = 0; j < 4; ++j) {
+    const int at = fp8_piece_at(static_cast<int>(kb), lane, j);
+    if (at >= a.k) continue;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fp8_value(codes[j >> 1][2 * (j & 1) + (i >> 2)], i & 3) * scale;
+    if constexpr (OUT == PLM_FP8_F32) {
+      f32x4* y = reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + row * a.k + at);
+      y[0] = f32x4{x[0], x[1], x[2], x[3]};
+      y[1] = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) + row * a.k + at) = pack8of<OUT == PLM_FP8_BF16 ? DT_BF16 : DT_F16>(x);
+    }
   }
 }
 
-// Rows of a workgroup: a fragment's sixteen write whole lines between them, few rows go to as many CUs.
-int rows_per_group(int64_t rows) { return rows >= 4096 ? 16 : rows >= 1024 ? 4 : 1; }
+// Rows from which a workgroup has sixteen: 4096 x 4096 34.7 us for 42.7, 8192 x 2048 35.7 for 39.7, 2048 x 2048 13.4 for 10.4.
+constexpr int kFragmentRows = 4096;
 
 template <int DT, bool RES, bool WEIGHT, bool E8>
 void launch_norm(const RowsArgs& a, hipStream_t s) {
-  const int per = rows_per_group(a.rows);
-  const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per)), block(64 * per);
-  if (a.k <= 1024) hipLaunchKernelGGL((norm_kernel<DT, RES, WEIGHT, E8, 1>), grid, block, 0, s, a);
-  else if (a.k <= 2048) hipLaunchKernelGGL((norm_kernel<DT, RES, WEIGHT, E8, 2>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((norm_kernel<DT, RES, WEIGHT, E8, 4>), grid, block, 0, s, a);
+  if constexpr (E8) {
+    if (a.rows >= kFragmentRows) {
+      const int blocks = static_cast<int>(fp8_blocks(a.k)), waves = blocks < 16 ? blocks : 16;
+      const dim3 grid(static_cast<unsigned>(a.frags)), block(64 * waves);
+      if (blocks <= 16) hipLaunchKernelGGL((fragment_norm_kernel<DT, RES, WEIGHT, 1>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((fragment_norm_kernel<DT, RES, WEIGHT, 2>), grid, block, 0, s, a);
+      return;
+    }
+  }
+  // Wavefronts of a row: a chunk to a thread.
+  const int waves = (row_chunks<E8>(a.k) + 63) / 64;
+  hipLaunchKernelGGL((row_norm_kernel<DT, RES, WEIGHT, E8>), dim3(static_cast<unsigned>(a.rows)), dim3(64 * (waves < 16 ? waves : 16)), 0, s, a);
 }
 
 template <int DT>
 hipError_t launch_rows(const RowsArgs& a, bool norm, hipStream_t s) {
   const bool res = a.residual != nullptr, weight = a.weight != nullptr, e8 = a.y == nullptr;
   if (!norm) {
-    const int per = rows_per_group(a.rows);
-    const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per), static_cast<unsigned>((fp8_blocks(a.k) + 7) / 8));
-    hipLaunchKernelGGL((round_kernel<DT>), grid, dim3(64 * per), 0, s, a);
+    const int64_t count = a.frags * fp8_blocks(a.k);
+    hipLaunchKernelGGL((round_kernel<DT>), dim3(static_cast<unsigned>((count + 3) / 4)), dim3(256), 0, s, a, count);
   } else if (e8) {
     if (res) weight ? launch_norm<DT, true, true, true>(a, s) : launch_norm<DT, true, false, true>(a, s);
     else weight ? launch_norm<DT, false, true, true>(a, s) : launch_norm<DT, false, false, true>(a, s);
@@ -385,6 +523,7 @@ int plm_fp8_rows(const plm_fp8_rows_call* call, void* stream) {
   if (!norm && (!e8 || h.residual != nullptr || h.weight != nullptr)) return PLM_ERR_ARGUMENT;
   if ((h.residual != nullptr) != (h.sum != nullptr)) return PLM_ERR_ARGUMENT;
   if (norm && !(h.eps >= 0x1p-100 && h.eps <= 0x1p100)) return PLM_ERR_ARGUMENT;
+  if (fp8_frags(h.rows) * fp8_blocks(h.k) >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   if (h.x_row % 8 != 0 || h.residual_row % 8 != 0 || !aligned_all(h.x, h.residual, h.sum, h.weight, h.y, h.codes, h.scales))
     return PLM_ERR_ALIGNMENT;
   RowsArgs a{};
@@ -446,9 +585,9 @@ int plm_fp8_values(const void* codes, const void* scales, int64_t rows, int64_t 
       out_type < PLM_FP8_BF16 || out_type > PLM_FP8_F32)
     return PLM_ERR_ARGUMENT;
   if (!aligned_all(codes, scales, y)) return PLM_ERR_ALIGNMENT;
-  const int64_t pieces = rows * (k / 8), grid = (pieces + 255) / 256;
+  const int64_t count = fp8_frags(rows) * fp8_blocks(k), grid = (count + 3) / 4;
   if (grid >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
-  const ValuesArgs a{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), y, rows, k, fp8_frags(rows), pieces,
+  const ValuesArgs a{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), y, rows, k, fp8_frags(rows), count,
                      gate_up != 0 ? 1 : 0};
   const dim3 blocks(static_cast<unsigned>(grid));
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -26,41 +26,49 @@ from . import _lib
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 128
+_CODES = _lib.DTYPE_CODES
 _OUT = {torch.bfloat16: _lib.PLM_FP8_BF16, torch.float16: _lib.PLM_FP8_F16, torch.float32: _lib.PLM_FP8_F32}
 _EPS = (2.0 ** -100, 2.0 ** 100)
-_IN = {torch.bfloat16: _lib.PLM_FP8_ROWS_BF16, torch.float16: _lib.PLM_FP8_ROWS_F16}
+_IN = {_lib.PLM_BF16: _lib.PLM_FP8_ROWS_BF16, _lib.PLM_F16: _lib.PLM_FP8_ROWS_F16}   # plm_fp8_in of a plm_dtype
 MOST = 1 << 21   # rows of a product's operands
 
 
-def _launch(entry, call, device: torch.device, what: str) -> None:
-    index = device.index
-    if index == torch.cuda.current_device():
-        status = entry(call, _lib.stream_handle(device))
-    else:
-        with torch.cuda.device(index):
-            status = entry(call, _lib.stream_handle(device))
-    if status:
-        _lib.check(status, what)
+# What follows is on every call's path, where the host's time counts: one look at each property, strides only of tensors that
+# are not contiguous, messages formed for refusals alone.
 
 
-def _matrix(t: torch.Tensor, name: str, device: torch.device | None = None) -> tuple[torch.Tensor, int, int]:
-    """``t`` [rows, k] of 16 bits as a kernel can read it, its pointer and row stride."""
+def _run(entry, index: int, *args) -> int:
+    """Status of a C entry on GPU ``index``, on its current stream."""
+    if index == torch._C._cuda_getDevice():
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _matrix(t: torch.Tensor, name: str, index: int | None = None) -> tuple[torch.Tensor, int, int, int, int, int, int]:
+    """``t`` [rows, k] of 16 bits as a kernel can read it, its pointer, row stride, type's code, GPU, rows and k."""
     if t.dim() != 2:
         raise ValueError(f"{name} must be [rows, k], got {list(t.shape)}")
-    if t.dtype not in _lib.DTYPE_CODES:
+    code = _CODES.get(t.dtype)
+    if code is None:
         raise TypeError(f"{name} must be bf16 or fp16, got {t.dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, and the 8-bit calls have none: detach it, or call under no_grad")
-    k = t.shape[1]
+    rows, k = t.shape
     if k < 8 or k % 8 or k > 1 << 24:
         raise ValueError(f"{name}'s rows must have a multiple of 8 in [8, 2^24] of elements, got {k}")
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise RuntimeError(f"{name} must be on {'a GPU' if device is None else device}, got {t.device}")
+    on = t.get_device()
+    if on < 0 or (index is not None and on != index):
+        raise RuntimeError(f"{name} must be on {'a GPU' if index is None else f'cuda:{index}'}, got {t.device}")
     at = t.data_ptr()
-    if at % 16 == 0 and t.stride(1) == 1 and t.stride(0) % 8 == 0:
-        return t, at, t.stride(0)
+    if at % 16 == 0:
+        if t.is_contiguous():
+            return t, at, k, code, on, rows, k
+        stride, one = t.stride()
+        if one == 1 and stride % 8 == 0:
+            return t, at, stride, code, on, rows, k
     t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.data_ptr(), k
+    return t, t.data_ptr(), k, code, on, rows, k
 
 
 class _Eight:
@@ -79,26 +87,31 @@ class _Eight:
                                  f"{list(t.shape)}")
         if not codes.is_cuda or scales.device != codes.device:
             raise RuntimeError(f"codes and scales live on one GPU; got {codes.device} and {scales.device}")
-        self.__dict__.update(codes=codes, scales=scales, rows=rows, k=k, device=codes.device, codes_at=codes.data_ptr(),
+        self.__dict__.update(codes=codes, scales=scales, rows=rows, k=k, _index=codes.get_device(), codes_at=codes.data_ptr(),
                              scales_at=scales.data_ptr())
 
     @classmethod
-    def _new(cls, rows: int, k: int, device: torch.device):
-        """Uninitialised rows, for a kernel to fill: one allocation, no check of what is known."""
-        frags, blocks = -(-rows // 16), -(-k // BLOCK)
-        codes, scales = frags * blocks * 2048, frags * (-(-blocks // 4)) * 64
-        both = torch.empty(codes + scales, dtype=torch.uint8, device=device)
+    def _new(cls, rows: int, k: int, like: torch.Tensor):
+        """Uninitialised rows on ``like``'s GPU, for a kernel to fill: one allocation, no check of what is known."""
+        frags, blocks = (rows + 15) // 16, (k + 127) // 128
+        codes = frags * blocks * 2048
+        both = like.new_empty(codes + frags * ((blocks + 3) // 4) * 64, dtype=torch.uint8)
         self = cls.__new__(cls)
         at = both.data_ptr()
-        self.__dict__.update(_both=both, rows=rows, k=k, device=both.device, codes_at=at, scales_at=at + codes, _codes_size=codes)
+        d = self.__dict__
+        d["_both"], d["rows"], d["k"], d["_index"], d["codes_at"], d["scales_at"] = both, rows, k, like.get_device(), at, at + codes
         return self
 
     def __getattr__(self, name: str):
         # The tensors of what a kernel filled, as views when they are asked for.
         if name in ("codes", "scales") and "_both" in self.__dict__:
-            both, size = self.__dict__["_both"], self.__dict__["_codes_size"]
+            both, size = self._both, self.scales_at - self.codes_at
             return both[:size].view(E4M3) if name == "codes" else both[size:]
         raise AttributeError(name)
+
+    @property
+    def device(self) -> torch.device:
+        return torch.device("cuda", self._index)
 
     def __setattr__(self, name: str, value) -> None:
         raise AttributeError(f"8-bit rows stay what they were made of: {name} cannot be set")
@@ -115,15 +128,13 @@ class _Eight:
         which are infinite (fp16 has neither the range nor all steps)."""
         if dtype not in _OUT:
             raise TypeError(f"values come in bf16, fp16 or fp32, not {dtype}")
-        out = torch.empty(self.rows, self.k, dtype=dtype, device=self.device)
-        if not self.rows:
-            return out
-
-        def entry(call, stream: int) -> int:
-            return _lib.lib().plm_fp8_values(*call, stream)
-
-        _launch(entry, (self.codes_at, self.scales_at, self.rows, self.k, int(self._gate_up), _OUT[dtype], out.data_ptr()),
-                self.device, f"plm_fp8_values({self.rows} rows of {self.k})")
+        like = self.__dict__.get("_both")
+        out = (self.codes if like is None else like).new_empty((self.rows, self.k), dtype=dtype)
+        if self.rows:
+            status = _run(_lib.lib().plm_fp8_values, self._index, self.codes_at, self.scales_at, self.rows, self.k, self._gate_up,
+                          _OUT[dtype], out.data_ptr())
+            if status:
+                _lib.check(status, f"plm_fp8_values({self.rows} rows of {self.k})")
         return out
 
 
@@ -152,11 +163,10 @@ class Weight(_Eight):
     @classmethod
     def quantize(cls, w: torch.Tensor, *, gate_up: bool = False) -> "Weight":
         """``w`` (bf16 or fp16 ``[n, k]``) rounded to 8 bits."""
-        w, at, stride = _matrix(w, "w")
-        n, k = w.shape
-        if w.shape[0] > 1 and stride < k:
+        w, at, stride, code, _, n, k = _matrix(w, "w")
+        if n > 1 and stride < k:
             raise ValueError("w's rows overlap")
-        return cls._filled(_lib.DTYPE_CODES[w.dtype], n, k, at, max(stride, k), 0, gate_up, w.device)
+        return cls._filled(code, n, k, at, max(stride, k), 0, gate_up, w)
 
     @classmethod
     def from_blocks(cls, codes: torch.Tensor, scales: torch.Tensor, *, gate_up: bool = False) -> "Weight":
@@ -179,18 +189,19 @@ class Weight(_Eight):
             raise ValueError("scales must be powers of two in [2^-126, 2^126]")
         if not codes.is_contiguous() or codes.data_ptr() % 8:
             codes = codes.clone(memory_format=torch.contiguous_format)
-        return cls._filled(0, n, k, codes.data_ptr(), k, scales.data_ptr(), gate_up, codes.device)
+        return cls._filled(0, n, k, codes.data_ptr(), k, scales.data_ptr(), gate_up, codes)
 
     @classmethod
-    def _filled(cls, dtype: int, n: int, k: int, at: int, stride: int, blocks: int, gate_up: bool, device: torch.device) -> "Weight":
+    def _filled(cls, dtype: int, n: int, k: int, at: int, stride: int, blocks: int, gate_up: bool, like: torch.Tensor) -> "Weight":
         _halves(n, gate_up)
-        if n < 1:
-            raise ValueError("a weight has at least one row")
-        self = cls._new(n, k, device)
+        if not _lib.lib().plm_fp8_codes_bytes(n, k):
+            raise ValueError(f"a weight has 1 to 2^24 - 1 rows, got [{n}, {k}]")
+        self = cls._new(n, k, like)
         self.__dict__["_gate_up"] = bool(gate_up)
-        _launch(_lib.lib().plm_fp8_weight,
-                _lib.pack_fp8_weight(dtype, n, k, at, stride, blocks, bool(gate_up), self.codes_at, self.scales_at), device,
-                f"plm_fp8_weight([{n}, {k}], gate_up={gate_up})")
+        status = _run(_lib.lib().plm_fp8_weight, self._index,
+                      _lib.pack_fp8_weight(dtype, n, k, at, stride, blocks, bool(gate_up), self.codes_at, self.scales_at))
+        if status:
+            _lib.check(status, f"plm_fp8_weight([{n}, {k}], gate_up={gate_up})")
         return self
 
 
@@ -202,13 +213,17 @@ def _halves(n: int, gate_up: bool) -> int:
 
 def quantize(x: torch.Tensor) -> Rows:
     """``x`` (bf16 or fp16 ``[rows, k]``, k a multiple of 8) in 8 bits."""
-    x, at, stride = _matrix(x, "x")
-    rows, k = x.shape
-    out = Rows._new(rows, k, x.device)
+    x, at, stride, code, index, rows, k = _matrix(x, "x")
+    return _quantized(x, at, stride, code, index, rows, k)
+
+
+def _quantized(x: torch.Tensor, at: int, stride: int, code: int, index: int, rows: int, k: int) -> Rows:
+    out = Rows._new(rows, k, x)
     if rows:
-        _launch(_lib.lib().plm_fp8_rows,
-                _lib.pack_fp8_rows(_lib.DTYPE_CODES[x.dtype], rows, k, at, stride, 0, 0, 0, 0, 0, 0.0, 0, out.codes_at,
-                                   out.scales_at), x.device, f"plm_fp8_rows({rows} rows of {k})")
+        status = _run(_lib.lib().plm_fp8_rows, index,
+                      _lib.pack_fp8_rows(code, rows, k, at, stride, 0, 0, 0, 0, 0, 0.0, 0, out.codes_at, out.scales_at))
+        if status:
+            _lib.check(status, f"plm_fp8_rows({rows} rows of {k})")
     return out
 
 
@@ -218,73 +233,78 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6, *,
     ``x``), ``[rows, k]``: in x's type, or with ``dtype=torch.float8_e4m3fn`` as ``Rows``. With a residual the result is
     ``(norm, t)``, t being the residual of the next call. ``weight [k]`` is of x's type (None: ones); eps is in [2^-100,
     2^100]. Codes are what the exact value rounds to."""
-    x, at, stride = _matrix(x, "x")
-    rows, k = x.shape
-    if dtype not in (None, x.dtype, E4M3):
+    x, at, stride, code, index, rows, k = _matrix(x, "x")
+    eight = dtype is E4M3
+    if not eight and dtype is not None and dtype is not x.dtype:
         raise TypeError(f"a norm comes in its input's type or float8_e4m3fn, not {dtype}")
     if not _EPS[0] <= eps <= _EPS[1]:
         raise ValueError(f"eps must be in [2^-100, 2^100], got {eps}")
     weight_at = 0
     if weight is not None:
-        if weight.dtype is not x.dtype or weight.shape != (k,) or weight.device != x.device:
-            raise ValueError(f"weight must be {x.dtype} [{k}] on {x.device}, got {weight.dtype} {list(weight.shape)} on {weight.device}")
+        if weight.dtype is not x.dtype or weight.shape != (k,) or weight.get_device() != index:
+            raise ValueError(f"weight must be {x.dtype} [{k}] on cuda:{index}, got {weight.dtype} {list(weight.shape)} on {weight.device}")
         if weight.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("weight requires a gradient, and the 8-bit calls have none: detach it, or call under no_grad")
-        if not weight.is_contiguous() or weight.data_ptr() % 16:
-            weight = weight.clone(memory_format=torch.contiguous_format)
         weight_at = weight.data_ptr()
+        if weight_at % 16 or not weight.is_contiguous():
+            weight = weight.clone(memory_format=torch.contiguous_format)
+            weight_at = weight.data_ptr()
     total, total_at, residual_at, residual_stride = None, 0, 0, 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype is not x.dtype:
-            raise ValueError(f"residual must be {x.dtype} {list(x.shape)} as x is, got {residual.dtype} {list(residual.shape)}")
-        residual, residual_at, residual_stride = _matrix(residual, "residual", x.device)
-        total = torch.empty(rows, k, dtype=x.dtype, device=x.device)
+        if residual.shape != (rows, k) or residual.dtype is not x.dtype:
+            raise ValueError(f"residual must be {x.dtype} {[rows, k]} as x is, got {residual.dtype} {list(residual.shape)}")
+        residual, residual_at, residual_stride, *_ = _matrix(residual, "residual", index)
+        total = x.new_empty((rows, k))
         total_at = total.data_ptr()
-    if dtype is E4M3:
-        out = Rows._new(rows, k, x.device)
+    if eight:
+        out = Rows._new(rows, k, x)
         y_at, codes_at, scales_at = 0, out.codes_at, out.scales_at
     else:
-        out = torch.empty(rows, k, dtype=x.dtype, device=x.device)
+        out = x.new_empty((rows, k))
         y_at, codes_at, scales_at = out.data_ptr(), 0, 0
     if rows:
-        _launch(_lib.lib().plm_fp8_rows,
-                _lib.pack_fp8_rows(_lib.DTYPE_CODES[x.dtype], rows, k, at, stride, 1, residual_at, residual_stride, total_at,
-                                   weight_at, eps, y_at, codes_at, scales_at), x.device, f"plm_fp8_rows(norm of {rows} rows of {k})")
+        status = _run(_lib.lib().plm_fp8_rows, index,
+                      _lib.pack_fp8_rows(code, rows, k, at, stride, 1, residual_at, residual_stride, total_at, weight_at, eps, y_at,
+                                         codes_at, scales_at))
+        if status:
+            _lib.check(status, f"plm_fp8_rows(norm of {rows} rows of {k})")
     return out if residual is None else (out, total)
 
 
 def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dtype: torch.dtype | None, act: bool) -> torch.Tensor:
-    if not isinstance(w, Weight):
-        raise TypeError(f"w must be an fp8.Weight, got {type(w).__name__}")
-    kind, x_scales, stride = _lib.PLM_FP8_CODES, 0, 0
-    if not isinstance(x, Rows):
-        x, x_at, stride = _matrix(x, "x", w.device)
-        rows, k = x.shape
-        if out_dtype is None:
-            out_dtype = x.dtype if out is None else out.dtype
-        kind = _IN[x.dtype]
+    index, n, k = w._index, w.rows, w.k
+    if type(x) is Rows:
+        kind, rows, x_at, x_scales, stride, like = _lib.PLM_FP8_CODES, x.rows, x.codes_at, x.scales_at, 0, w.__dict__.get("_both")
+        if out_dtype is None and out is None:
+            raise ValueError("rows in 8 bits have no type of their own: out_dtype or out is needed")
+        if x.k != k:
+            raise ValueError(f"x must be [rows, {k}], got {[rows, x.k]}")
+        if x._index != index:
+            raise RuntimeError(f"x must be on the weight's GPU cuda:{index}, got cuda:{x._index}")
+        if like is None:
+            like = w.codes
     else:
-        rows, k, x_at, x_scales = x.rows, x.k, x.codes_at, x.scales_at
-        if out_dtype is None:
-            if out is None:
-                raise ValueError("rows in 8 bits have no type of their own: out_dtype or out is needed")
-            out_dtype = out.dtype
-        if x.device != w.device:
-            raise RuntimeError(f"x must be on the weight's GPU {w.device}, got {x.device}")
-    if k != w.k:
-        raise ValueError(f"x must be [rows, {w.k}], got {[rows, k]}")
-    if out_dtype not in _OUT:
+        x, x_at, stride, code, _, rows, own = _matrix(x, "x", index)
+        if own != k:
+            raise ValueError(f"x must be [rows, {k}], got {[rows, own]}")
+        like, x_scales, kind = x, 0, _IN[code]
+        if out_dtype is None and out is None:
+            out_dtype = x.dtype
+    if out_dtype is None:
+        out_dtype = out.dtype
+    kind_out = _OUT.get(out_dtype)
+    if kind_out is None:
         raise TypeError(f"a product comes in bf16, fp16 or fp32, not {out_dtype}")
-    if rows > MOST or w.rows > MOST:
-        raise ValueError(f"a product takes up to {MOST} rows of x and of the weight, got {rows} and {w.rows}")
-    columns = w.rows // 2 if act else w.rows
+    if rows > MOST or n > MOST:
+        raise ValueError(f"a product takes up to {MOST} rows of x and of the weight, got {rows} and {n}")
+    columns = n // 2 if act else n
     if out is None:
-        out = torch.empty((rows, columns), dtype=out_dtype, device=w.device)
+        out = like.new_empty((rows, columns), dtype=out_dtype)
         out_row = columns
     else:
-        if out.shape != (rows, columns) or out.dtype is not out_dtype or out.device != w.device or \
+        if out.shape != (rows, columns) or out.dtype is not out_dtype or out.get_device() != index or \
                 (rows and (out.stride(1) != 1 and columns > 1 or out.stride(0) < columns and rows > 1)):
-            raise ValueError(f"out must be a row-major {[rows, columns]} {out_dtype} tensor on {w.device}")
+            raise ValueError(f"out must be a row-major {[rows, columns]} {out_dtype} tensor on cuda:{index}")
         if out.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("out requires a gradient, and the 8-bit calls have none")
         out_row = max(out.stride(0), columns)
@@ -292,21 +312,18 @@ def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dt
         return out
     # Up to 16 rows every workgroup rounds for itself, which saves a launch (2048 x 2048 over one row 3.7 us for 6); not
     # several for each of an LM head's many workgroups (50257 x 2048 over 16 rows 28 us for 26).
-    if kind and (rows > 16 or rows > 4 and w.rows > 16384):
-        x = quantize(x)
-        kind, x_at, x_scales = _lib.PLM_FP8_CODES, x.codes_at, x.scales_at
-    call = _lib.pack_fp8_linear(rows, w.rows, k, kind, x_at, x_scales, stride, w.codes_at, w.scales_at, out.data_ptr(), out_row,
-                                _OUT[out_dtype], act)
+    if kind and (rows > 16 or rows > 4 and n > 16384):
+        x = _quantized(x, x_at, stride, code, index, rows, k)
+        kind, x_at, x_scales, stride = _lib.PLM_FP8_CODES, x.codes_at, x.scales_at, 0
+    call = _lib.pack_fp8_linear(rows, n, k, kind, x_at, x_scales, stride, w.codes_at, w.scales_at, out.data_ptr(), out_row, kind_out, act)
     lib = _lib.lib()
     space, size = 0, lib.plm_fp8_linear_workspace_bytes(call)
     if size:
-        work = torch.empty(size, dtype=torch.uint8, device=w.device)   # partial sums: this call's alone
+        work = like.new_empty(size, dtype=torch.uint8)   # partial sums: this call's alone
         space = work.data_ptr()
-
-    def entry(call, stream: int) -> int:
-        return lib.plm_fp8_linear(call, space, size, stream)
-
-    _launch(entry, call, w.device, f"plm_fp8_linear(M={rows}, N={w.rows}, K={k}, act={act})")
+    status = _run(lib.plm_fp8_linear, index, call, space, size)
+    if status:
+        _lib.check(status, f"plm_fp8_linear(M={rows}, N={n}, K={k}, act={act})")
     return out
 
 
@@ -314,7 +331,9 @@ def linear(x: torch.Tensor | Rows, w: Weight, *, out: torch.Tensor | None = None
            out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x @ w^T`` ``[rows, n]``, summed in fp32 and rounded once to ``out_dtype``: bf16, fp16 or fp32, x's type unless given
     (``Rows`` have none). ``x`` is ``[rows, k]``, in 16 bits, which are rounded to 8 here, or ``Rows``."""
-    if isinstance(w, Weight) and w.gate_up:
+    if not isinstance(w, Weight):
+        raise TypeError(f"w must be an fp8.Weight, got {type(w).__name__}")
+    if w._gate_up:
         raise ValueError("a gate/up weight goes to gate_up_silu")
     return _product(x, w, out, out_dtype, False)
 
@@ -323,7 +342,9 @@ def gate_up_silu(x: torch.Tensor | Rows, w: Weight, *, out: torch.Tensor | None 
                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``silu(g) * u`` of the halves of ``x @ w^T``, ``[rows, n / 2]``: in fp32 up to the one rounding to ``out_dtype``
     (``fast_gemm.gate_up_silu`` rounds the projections and the activation on the way). ``w`` is a gate/up weight."""
-    if isinstance(w, Weight) and not w.gate_up:
+    if not isinstance(w, Weight):
+        raise TypeError(f"w must be an fp8.Weight, got {type(w).__name__}")
+    if not w._gate_up:
         raise ValueError("gate_up_silu needs a weight made with gate_up=True")
     return _product(x, w, out, out_dtype, True)
 
