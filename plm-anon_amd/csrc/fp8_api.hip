@@ -7,10 +7,10 @@ namespace plm {
 namespace {
 
 struct Fp8Plan {
-  bool tile;
+  bool tile, round;   // round: rows of 16 bits first, by a launch of their own
   Fp8TileKind kind;
   Fp8Narrow narrow;
-  size_t bytes;   // of partial sums
+  size_t codes, scales, bytes;   // of a workspace's rounded rows and, behind them, all of it with the partial sums
 };
 
 // The plan of a call whose numbers go together; false where they do not.
@@ -22,7 +22,11 @@ bool linear_of(const plm_fp8_linear_call* call, Fp8Gemm& a, Fp8Plan& p) {
     return false;
   if (h.ldy < (act ? h.n / 2 : h.n) || h.out < PLM_FP8_BF16 || h.out > PLM_FP8_F32) return false;
   if (h.x_type < PLM_FP8_CODES || h.x_type > PLM_FP8_ROWS_F16) return false;
-  if (h.x_type != PLM_FP8_CODES && (h.m > 16 || h.x_row < 0)) return false;
+  const bool in16 = h.x_type != PLM_FP8_CODES;
+  if (in16 && (h.x_row < 0 || plm_fp8_codes_bytes(h.m, h.k) == 0)) return false;
+  // Up to 16 rows every workgroup rounds for itself, which saves a launch (2048 x 2048 over one row 3.7 us for 6); not several
+  // for each of an LM head's many workgroups (50257 x 2048 over 16 rows 28 us for 26).
+  p.round = in16 && (h.m > 16 || (h.m > 4 && h.n > 16384));
   a.ldy = h.ldy;
   a.x_row = h.x_row;
   a.m = static_cast<int>(h.m);
@@ -31,16 +35,17 @@ bool linear_of(const plm_fp8_linear_call* call, Fp8Gemm& a, Fp8Plan& p) {
   a.blocks = static_cast<int>(fp8_blocks(h.k));
   a.x_frags = static_cast<int>(fp8_frags(h.m));
   a.w_frags = static_cast<int>(fp8_frags(h.n));
-  a.x_type = static_cast<int>(h.x_type);
+  a.x_type = p.round ? static_cast<int>(PLM_FP8_CODES) : static_cast<int>(h.x_type);
   a.out = static_cast<int>(h.out);
-  p.narrow = narrow_plan(a.x_frags, a.w_frags, a.blocks, act, h.x_type != PLM_FP8_CODES);
+  p.narrow = narrow_plan(a.x_frags, a.w_frags, a.blocks, act, a.x_type != PLM_FP8_CODES);
   const Fp8TilePlan t = tile_plan(a.x_frags, a.w_frags, a.blocks);
   // Results in fp32 need products that the tiles do not make.
   p.tile = h.out != PLM_FP8_F32 && a.x_frags > 4 && t.us < p.narrow.us;
   p.kind = t.kind;
-  p.bytes = 0;
-  if (p.tile) return true;
-  if (p.narrow.ranges > 1) p.bytes = static_cast<size_t>(p.narrow.ranges) * a.x_frags * a.w_frags * 1024;
+  p.codes = p.round ? plm_fp8_codes_bytes(h.m, h.k) : 0;
+  p.scales = p.round ? plm_fp8_scales_bytes(h.m, h.k) : 0;
+  p.bytes = p.codes + p.scales;
+  if (!p.tile && p.narrow.ranges > 1) p.bytes += static_cast<size_t>(p.narrow.ranges) * a.x_frags * a.w_frags * 1024;
   return true;
 }
 
@@ -74,9 +79,17 @@ int plm_fp8_linear(const plm_fp8_linear_call* call, void* workspace, size_t work
   a.w = static_cast<const uint8_t*>(h.w);
   a.w_scales = static_cast<const uint8_t*>(h.w_scales);
   a.y = h.y;
-  a.partials = static_cast<f32x4*>(workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const hipError_t err = p.tile ? fp8_tile(a, p.kind, h.act != 0, s) : fp8_narrow(a, p.narrow, h.act != 0, s);
+  hipError_t err = hipSuccess;
+  uint8_t* space = static_cast<uint8_t*>(workspace);
+  if (p.round) {
+    err = fp8_round(h.x_type == PLM_FP8_ROWS_BF16 ? PLM_BF16 : PLM_F16, h.x, h.x_row, h.m, h.k, space, space + p.codes, s);
+    a.x = space;
+    a.x_scales = space + p.codes;
+  }
+  if (err != hipSuccess) return PLM_ERR_LAUNCH;
+  a.partials = reinterpret_cast<f32x4*>(space + p.codes + p.scales);
+  err = p.tile ? fp8_tile(a, p.kind, h.act != 0, s) : fp8_narrow(a, p.narrow, h.act != 0, s);
   return err == hipSuccess ? PLM_OK : PLM_ERR_LAUNCH;
 }
 

@@ -51,6 +51,8 @@ __device__ __forceinline__ void fp8_store4(const Fp8Gemm& a, int m, int n, int c
   }
 }
 
+// Rows of 16 bits (plm_dtype) into codes and scales.
+hipError_t fp8_round(int dtype, const void* x, int64_t x_row, int64_t rows, int64_t k, uint8_t* codes, uint8_t* scales, hipStream_t s);
 hipError_t fp8_narrow(Fp8Gemm a, const Fp8Narrow& p, bool act, hipStream_t s);
 hipError_t fp8_tile(const Fp8Gemm& a, Fp8TileKind kind, bool act, hipStream_t s);
 

@@ -8,8 +8,7 @@
 // border between codes: what is that close is computed in fp64 and rounded once, the scale's border likewise.
 #include <hip/hip_runtime.h>
 
-#include "fp8.h"
-#include "plm_amd.h"
+#include "fp8_gemm.h"
 
 namespace plm {
 namespace {
@@ -491,8 +490,10 @@ hipError_t launch_rows(const RowsArgs& a, bool norm, hipStream_t s) {
   return hipGetLastError();
 }
 
+// What fits a grid of a wavefront to a fragment, among others.
 bool sizes_fit(int64_t rows, int64_t k) {
-  return rows >= 1 && rows < (int64_t{1} << 24) && k >= 8 && k <= (1 << 24) && k % 8 == 0;
+  return rows >= 1 && rows < (int64_t{1} << 24) && k >= 8 && k <= (1 << 24) && k % 8 == 0 &&
+         fp8_frags(rows) * fp8_blocks(k) < (int64_t{1} << 31);
 }
 
 template <typename... P>
@@ -501,6 +502,19 @@ bool aligned_all(const P*... p) {
 }
 
 }  // namespace
+
+hipError_t fp8_round(int dtype, const void* x, int64_t x_row, int64_t rows, int64_t k, uint8_t* codes, uint8_t* scales, hipStream_t s) {
+  RowsArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.codes = codes;
+  a.scales = scales;
+  a.x_row = x_row;
+  a.frags = fp8_frags(rows);
+  a.rows = static_cast<int>(rows);
+  a.k = static_cast<int>(k);
+  return dtype == PLM_BF16 ? launch_rows<DT_BF16>(a, false, s) : launch_rows<DT_F16>(a, false, s);
+}
+
 }  // namespace plm
 
 extern "C" {
@@ -523,7 +537,6 @@ int plm_fp8_rows(const plm_fp8_rows_call* call, void* stream) {
   if (!norm && (!e8 || h.residual != nullptr || h.weight != nullptr)) return PLM_ERR_ARGUMENT;
   if ((h.residual != nullptr) != (h.sum != nullptr)) return PLM_ERR_ARGUMENT;
   if (norm && !(h.eps >= 0x1p-100 && h.eps <= 0x1p100)) return PLM_ERR_ARGUMENT;
-  if (fp8_frags(h.rows) * fp8_blocks(h.k) >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   if (h.x_row % 8 != 0 || h.residual_row % 8 != 0 || !aligned_all(h.x, h.residual, h.sum, h.weight, h.y, h.codes, h.scales))
     return PLM_ERR_ALIGNMENT;
   RowsArgs a{};
@@ -586,7 +599,6 @@ int plm_fp8_values(const void* codes, const void* scales, int64_t rows, int64_t 
     return PLM_ERR_ARGUMENT;
   if (!aligned_all(codes, scales, y)) return PLM_ERR_ALIGNMENT;
   const int64_t count = fp8_frags(rows) * fp8_blocks(k), grid = (count + 3) / 4;
-  if (grid >= (int64_t{1} << 31)) return PLM_ERR_ARGUMENT;
   const ValuesArgs a{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), y, rows, k, fp8_frags(rows), count,
                      gate_up != 0 ? 1 : 0};
   const dim3 blocks(static_cast<unsigned>(grid));

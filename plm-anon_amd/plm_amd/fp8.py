@@ -214,10 +214,6 @@ def _halves(n: int, gate_up: bool) -> int:
 def quantize(x: torch.Tensor) -> Rows:
     """``x`` (bf16 or fp16 ``[rows, k]``, k a multiple of 8) in 8 bits."""
     x, at, stride, code, index, rows, k = _matrix(x, "x")
-    return _quantized(x, at, stride, code, index, rows, k)
-
-
-def _quantized(x: torch.Tensor, at: int, stride: int, code: int, index: int, rows: int, k: int) -> Rows:
     out = Rows._new(rows, k, x)
     if rows:
         status = _run(_lib.lib().plm_fp8_rows, index,
@@ -284,7 +280,7 @@ def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dt
         if like is None:
             like = w.codes
     else:
-        x, x_at, stride, code, _, rows, own = _matrix(x, "x", index)
+        x, x_at, stride, code, _, rows, own = _matrix(x, "x", index)   # rounded in the call, as quantize does
         if own != k:
             raise ValueError(f"x must be [rows, {k}], got {[rows, own]}")
         like, x_scales, kind = x, 0, _IN[code]
@@ -310,16 +306,11 @@ def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dt
         out_row = max(out.stride(0), columns)
     if not rows:
         return out
-    # Up to 16 rows every workgroup rounds for itself, which saves a launch (2048 x 2048 over one row 3.7 us for 6); not
-    # several for each of an LM head's many workgroups (50257 x 2048 over 16 rows 28 us for 26).
-    if kind and (rows > 16 or rows > 4 and n > 16384):
-        x = _quantized(x, x_at, stride, code, index, rows, k)
-        kind, x_at, x_scales, stride = _lib.PLM_FP8_CODES, x.codes_at, x.scales_at, 0
     call = _lib.pack_fp8_linear(rows, n, k, kind, x_at, x_scales, stride, w.codes_at, w.scales_at, out.data_ptr(), out_row, kind_out, act)
     lib = _lib.lib()
     space, size = 0, lib.plm_fp8_linear_workspace_bytes(call)
     if size:
-        work = like.new_empty(size, dtype=torch.uint8)   # partial sums: this call's alone
+        work = like.new_empty(size, dtype=torch.uint8)   # rounded rows, partial sums: this call's alone
         space = work.data_ptr()
     status = _run(lib.plm_fp8_linear, index, call, space, size)
     if status:

@@ -129,7 +129,7 @@ def test_c_entries_refuse_before_a_launch():
                     dict(m=3, n=64, k=64, x_type=0, x=f, x_scales=f, x_row=0, w=f, w_scales=f, y=f, ldy=64, out=0, act=0))
     for bad in (dict(m=0), dict(m=(1 << 21) + 1), dict(n=0), dict(k=4), dict(x=0), dict(x_scales=0), dict(w=0), dict(w_scales=0),
                 dict(y=0), dict(ldy=63), dict(out=3), dict(out=-1), dict(act=1, n=48), dict(act=1, ldy=31), dict(x_type=3),
-                dict(x_type=-1), dict(x_type=1, m=17), dict(x_type=2, x_row=-8), dict(n=(1 << 21) + 1, ldy=1 << 22)):
+                dict(x_type=-1), dict(x_type=2, x_row=-8), dict(n=(1 << 21) + 1, ldy=1 << 22)):
         assert linear(**bad) == -1, bad
     for bad in (dict(x=f + 8), dict(x_scales=f + 4), dict(w=f + 2), dict(w_scales=f + 8), dict(y=f + 1), dict(y=f + 2, out=2),
                 dict(x_type=1, x_row=4), dict(x_type=1, x=f + 8)):
@@ -141,6 +141,9 @@ def test_c_entries_refuse_before_a_launch():
     assert need > 0 and need % 1024 == 0
     assert lib.plm_fp8_linear(call, None, 0, None) == -4 and lib.plm_fp8_linear(call, f, need - 1, None) == -4
     assert lib.plm_fp8_linear(call, f + 8, need, None) == -2
+    rows = _lib.pack_fp8_linear(64, 2048, 8192, 1, f, 0, 8192, f, f, f, 2048, 0, 0)   # rounded first, into the workspace
+    assert lib.plm_fp8_linear_workspace_bytes(rows) == need + sum(fp8_bytes(64, 8192))
+    assert lib.plm_fp8_linear(rows, f, need, None) == -4
     assert lib.plm_fp8_linear_workspace_bytes(_lib.pack_fp8_linear(64, 2048, 8196, 0, f, f, 0, f, f, f, 2048, 0, 0)) == 0
 
     for bad in ((0, f, 3, 64, 0, 0, f), (f, 0, 3, 64, 0, 0, f), (f, f, 0, 64, 0, 0, f), (f, f, 3, 60, 0, 0, f), (f, f, 48, 64, 1, 0, f),
