@@ -455,16 +455,17 @@ __global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
   }
 }
 
-// Rows from which a workgroup has sixteen: 4096 x 4096 34.7 us for 42.7, 8192 x 2048 35.7 for 39.7, 2048 x 2048 13.4 for 10.4.
+// Rows from which a workgroup has sixteen: 4096 x 4096 34.7 us for 42.7, 8192 x 2048 33.5 for 39.5, 2048 x 2048 13.4 for 10.4.
 constexpr int kFragmentRows = 4096;
 
 template <int DT, bool RES, bool WEIGHT, bool E8>
 void launch_norm(const RowsArgs& a, hipStream_t s) {
   if constexpr (E8) {
     if (a.rows >= kFragmentRows) {
-      const int blocks = static_cast<int>(fp8_blocks(a.k)), waves = blocks < 16 ? blocks : 16;
+      // Two blocks to a wavefront, so that two workgroups fit a CU at 2048 columns (33.5 us for 35.7 with one of 16).
+      const int blocks = static_cast<int>(fp8_blocks(a.k)), waves = blocks <= 8 ? blocks : blocks <= 16 ? 8 : 16;
       const dim3 grid(static_cast<unsigned>(a.frags)), block(64 * waves);
-      if (blocks <= 16) hipLaunchKernelGGL((fragment_norm_kernel<DT, RES, WEIGHT, 1>), grid, block, 0, s, a);
+      if (blocks <= 8) hipLaunchKernelGGL((fragment_norm_kernel<DT, RES, WEIGHT, 1>), grid, block, 0, s, a);
       else hipLaunchKernelGGL((fragment_norm_kernel<DT, RES, WEIGHT, 2>), grid, block, 0, s, a);
       return;
     }
