@@ -20,6 +20,10 @@ struct Fp8Gemm {
   int x_frags, w_frags, x_type, out;  // out: plm_fp8_out
 };
 
+// 16 and 8 bytes at any even address, which one store writes: rows of an odd length begin anywhere.
+typedef u32x4 fp8_any16 __attribute__((aligned(2)));
+typedef u32x2 fp8_any8 __attribute__((aligned(2)));
+
 // g / (1 + e^-g) * u in fp32; the exponential's overflow gives g / inf = -0.
 __device__ __forceinline__ float fp8_silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
@@ -29,8 +33,8 @@ __device__ __forceinline__ void fp8_store4(const Fp8Gemm& a, int m, int n, int c
   const int left = columns - n;
   if (a.out == PLM_FP8_F32) {
     float* y = static_cast<float*>(a.y) + at;
-    if (left >= 4 && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
-      *reinterpret_cast<f32x4*>(y) = v;
+    if (left >= 4) {
+      *reinterpret_cast<fp8_any16*>(y) = __builtin_bit_cast(u32x4, v);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -42,8 +46,8 @@ __device__ __forceinline__ void fp8_store4(const Fp8Gemm& a, int m, int n, int c
 #pragma unroll
   for (int j = 0; j < 4; ++j) b[j] = a.out == PLM_FP8_BF16 ? to_bits16<DT_BF16>(v[j]) : to_bits16<DT_F16>(v[j]);
   uint16_t* y = static_cast<uint16_t*>(a.y) + at;
-  if (left >= 4 && (reinterpret_cast<uintptr_t>(y) & 7) == 0) {
-    *reinterpret_cast<u32x2*>(y) = u32x2{b[0] | (static_cast<uint32_t>(b[1]) << 16), b[2] | (static_cast<uint32_t>(b[3]) << 16)};
+  if (left >= 4) {
+    *reinterpret_cast<fp8_any8*>(y) = u32x2{b[0] | (static_cast<uint32_t>(b[1]) << 16), b[2] | (static_cast<uint32_t>(b[3]) << 16)};
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)

@@ -143,7 +143,6 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Fp8Gemm a, Tiles til
   stage(now, t0, 2, set2, 0, kX);
   tile_sync<2 * kX>();   // the first set's have arrived
   xo[0] = fp8_operand(set0[x_at], set0[x_at + 64]);
-  const bool aligned = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.ldy % 8 == 0;
   const int columns = ACT ? a.n / 2 : a.n;
 
   // The wait before the barrier: of the loads since the next set's, the set after it (kX) and the weight's next operands (2 FN)
@@ -207,12 +206,12 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Fp8Gemm a, Tiles til
           for (int j = 0; j < 4; ++j) v[f][j] = fp8_silu_mul(v[f][j], acc[2 * f + 1][t][j]);
         }
       }
-      if (kOut % 2 == 0 && aligned && n0 + kOut * 16 <= columns) {
+      if (kOut % 2 == 0 && n0 + kOut * 16 <= columns) {
 #pragma unroll
         for (int f = 0; f + 1 < kOut; f += 2) {
           const u32x4 o = eight_columns(four16<DT>(v[f]), four16<DT>(v[f + 1]));
           const int n = n0 + (f + ((column >> 4) & 1)) * 16 + (column >> 5) * 8;
-          if (m < a.m) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) + m * a.ldy + n) = o;
+          if (m < a.m) *reinterpret_cast<fp8_any16*>(static_cast<uint16_t*>(a.y) + m * a.ldy + n) = o;
         }
       } else if (m < a.m) {
 #pragma unroll
