@@ -1,13 +1,17 @@
 // Products over e4m3 rows for many rows of X: bound by the matrix cores.
 //
-// A workgroup has a tile of 16 WN FN rows of the weight x 16 WM FM rows of X, a wavefront FN x FM fragments of it. X comes
-// into LDS (four sets, two blocks of K ahead), the weight's operands straight from memory into registers, a block ahead: read
-// from LDS too, both operands of 256 x 256 took LDS as many cycles as the products take the matrix cores. The fragments'
-// order is what a wavefront's 16-byte reads want: no bank met twice, no address to compute.
+// A workgroup has a tile of rows of the weight x rows of X, a wavefront FD x FS fragments of it. One operand comes into LDS (four
+// sets, two blocks of K ahead), the other's fragments straight from memory into registers, a block ahead or three: read
+// from LDS too, both operands of 256 x 256 took LDS as many cycles as the products take the matrix cores (8192 x 8192 x 2048
+// 137 us). The fragments' order is what a wavefront's 16-byte reads want: no bank met twice, no address to compute.
 //
 // One barrier a block, in its middle, where the next block's set must have arrived; the operand that the next block
 // begins with is read before this one's end, so the matrix cores do not run dry at either. Workgroups stay, and the loads run
 // ahead into the next tile while the last one is stored.
+//
+// Measured, rows in 8 bits, weights from memory: 8192 x 8192 x 2048 112 us (2450 TFLOP/s; 26 us of it is what the stores take a
+// copy), 8192^3 370 (2970), 2048 x 8192 x 8192 94. Of the last 70 remain with no loads at all: the products and the
+// barriers, at the clock that they leave.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -70,51 +74,58 @@ __device__ __forceinline__ void place_of(const Tiles& g, int tile, int& tn, int&
   tm = group * kGroup + rest - tn * deep;
 }
 
-template <int WN, int WM, int FN, int FM, int AHEAD, int DT, bool ACT>
-__global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Fp8Gemm a, Tiles tiles) {
-  constexpr int kWaves = WN * WM, TN = WN * FN, TM = WM * FM, kX = 2 * TM / kWaves;
+// D is the operand whose fragments a wavefront reads into registers, FD of them, S the one that goes through LDS, FS; WL: S is the
+// weight, else X. Weights are read from memory and X mostly from L2, so that the largest tiles, whose registers hold one block
+// ahead only, have the weight in LDS: 8192 x 8192 x 2048 112.3 us for 117.4.
+template <int WD, int WS, int FD, int FS, int AHEAD, bool WL, int DT, bool ACT>
+__global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles tiles) {
+  constexpr int kWaves = WD * WS, TD = WD * FD, TS = WS * FS, kStaged = 2 * TS / kWaves;
+  constexpr int TN = WL ? TS : TD, TM = WL ? TD : TS, FN = WL ? FS : FD, FM = WL ? FD : FS;
   static_assert(AHEAD == 1 || AHEAD == 3, "operands of two or four blocks");
-  static_assert(2 * TM % kWaves == 0 && FM % 2 == 0, "every wavefront stages as many pieces of 1 KiB");
-  __shared__ __attribute__((aligned(16))) u32x4 set0[TM * 128], set1[TM * 128], set2[TM * 128], set3[TM * 128];
+  static_assert(2 * TS % kWaves == 0 && FS % 2 == 0, "every wavefront stages as many pieces of 1 KiB");
+  __shared__ __attribute__((aligned(16))) u32x4 set0[TS * 128], set1[TS * 128], set2[TS * 128], set3[TS * 128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int base = (blockIdx.x & 7) * tiles.per_xcd, count = min(tiles.per_xcd, tiles.n * tiles.m - base);
   const int stride = gridDim.x >> 3;
   int local = blockIdx.x >> 3;
   if (local >= count) return;
-  const int wn = wave / WM, wm = wave - wn * WM, at_lane = lane * 16;
-  const uint32_t w_block = static_cast<uint32_t>(a.w_frags) * kFp8Bytes, x_block = static_cast<uint32_t>(a.x_frags) * kFp8Bytes;
-  const uint32_t w_scale_block = static_cast<uint32_t>(a.w_frags) * kFp8ScaleBytes;
-  const uint32_t x_scale_block = static_cast<uint32_t>(a.x_frags) * kFp8ScaleBytes;
+  const int wd = wave / WS, ws = wave - wd * WS, at_lane = lane * 16;
+  const uint8_t *d_codes = WL ? a.x : a.w, *s_codes = WL ? a.w : a.x;
+  const uint8_t *d_scales = WL ? a.x_scales : a.w_scales, *s_scales = WL ? a.w_scales : a.x_scales;
+  const uint32_t d_frags = WL ? a.x_frags : a.w_frags, s_frags = WL ? a.w_frags : a.x_frags;
+  const uint32_t d_block = d_frags * static_cast<uint32_t>(kFp8Bytes), s_block = s_frags * static_cast<uint32_t>(kFp8Bytes);
+  const uint32_t d_scale_block = d_frags * static_cast<uint32_t>(kFp8ScaleBytes);
+  const uint32_t s_scale_block = s_frags * static_cast<uint32_t>(kFp8ScaleBytes);
 
   // Four blocks of K from kb on: an operand's bytes there, and where in it a block's fragment lies. Fragments past the operand's
   // last are the next block's first, or zeros without traffic past its end; they reach no output that is stored. So are
-  // the weight's blocks past K; X has its last one again there, since a set's older codes may be another row's NaN.
+  // D's blocks past K; S has its last one again there, since a set's older codes may be another row's NaN.
   struct Group {
-    __amdgpu_buffer_rsrc_t w, x;
+    __amdgpu_buffer_rsrc_t d, s;
     int kb;
   };
   auto group_at = [&](int kb, bool in) {
     const uint32_t left = in ? static_cast<uint32_t>(min(a.blocks - kb, 4)) : 0u;
-    return Group{make_rsrc(a.w + static_cast<int64_t>(kb) * w_block, left * w_block),
-                 make_rsrc(a.x + static_cast<int64_t>(kb) * x_block, left * x_block), kb};
+    return Group{make_rsrc(d_codes + static_cast<int64_t>(kb) * d_block, left * d_block),
+                 make_rsrc(s_codes + static_cast<int64_t>(kb) * s_block, left * s_block), kb};
   };
-  // Pieces [i0, i1) of a block of X into a set, and of the weight's operands into registers: 1 KiB a load.
-  auto stage = [&](const Group& g, int t0, int j, u32x4* set, int i0, int i1) {
-    const uint32_t at = static_cast<uint32_t>(min(j, a.blocks - 1 - g.kb)) * x_block + static_cast<uint32_t>(t0) * kFp8Bytes;
+  // Pieces [i0, i1) of a block of S into a set, and of D's operands into registers: 1 KiB a load.
+  auto stage = [&](const Group& g, int s0, int j, u32x4* set, int i0, int i1) {
+    const uint32_t at = static_cast<uint32_t>(min(j, a.blocks - 1 - g.kb)) * s_block + static_cast<uint32_t>(s0) * kFp8Bytes;
 #pragma unroll
-    for (int i = 0; i < kX; ++i)
-      if (i >= i0 && i < i1) load_lds16(g.x, set + (i * kWaves + wave) * 64, at_lane + wave * 1024, at + i * (kWaves * 1024));
+    for (int i = 0; i < kStaged; ++i)
+      if (i >= i0 && i < i1) load_lds16(g.s, set + (i * kWaves + wave) * 64, at_lane + wave * 1024, at + i * (kWaves * 1024));
   };
-  auto weights = [&](const Group& g, int f0, int j, i32x8 (&w)[FN], int i0, int i1) {
-    const uint32_t at = static_cast<uint32_t>(j) * w_block + static_cast<uint32_t>(f0) * kFp8Bytes;
+  auto direct = [&](const Group& g, int d0, int j, i32x8 (&o)[FD], int i0, int i1) {
+    const uint32_t at = static_cast<uint32_t>(j) * d_block + static_cast<uint32_t>(d0) * kFp8Bytes;
     const int here = anew(at_lane);
 #pragma unroll
-    for (int f = 0; f < FN; ++f) {
-      if (f < i0 || f >= i1) continue;
+    for (int i = 0; i < FD; ++i) {
+      if (i < i0 || i >= i1) continue;
       // Two fragments are within the 4 KiB of an instruction's own offset.
-      const int from = static_cast<int>(at + (f & ~1) * kFp8Bytes), in_lane = here + (f & 1) * static_cast<int>(kFp8Bytes);
-      w[f] = fp8_operand(__builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(g.w, in_lane, from, 0)),
-                         __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(g.w, in_lane + 1024, from, 0)));
+      const int from = static_cast<int>(at + (i & ~1) * kFp8Bytes), in_lane = here + (i & 1) * static_cast<int>(kFp8Bytes);
+      o[i] = fp8_operand(__builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(g.d, in_lane, from, 0)),
+                         __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(g.d, in_lane + 1024, from, 0)));
     }
   };
   // Four blocks' scales of fragments [f, f1) of an operand, a byte each. Past K they are zeros, which stand for 2^-127.
@@ -125,85 +136,88 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Fp8Gemm a, Tiles til
     for (int i = i0; i < i1; ++i) s[i] = __builtin_amdgcn_raw_buffer_load_b32(r, here + i * 64, first * static_cast<int>(kFp8ScaleBytes), 0);
   };
 
-  f32x4 acc[FN][FM];
-  int ws[FN], xs[FM], next_ws[FN];
-  i32x8 w[AHEAD + 1][FN], xo[2];
-  const int x_at = wm * FM * 128 + lane;
-  int f0, t0;
-  place_of(tiles, base + local, f0, t0);
-  f0 = f0 * TN + wn * FN;
-  t0 *= TM;
-  scales(a.w_scales, w_scale_block, 0, true, f0, 0, FN, next_ws);
-  scales(a.x_scales, x_scale_block, 0, true, t0 + wm * FM, 0, FM, xs);
+  f32x4 acc[FD][FS];
+  int ds[FD], ss[FS], next_ds[FD];
+  i32x8 d[AHEAD + 1][FD], so[2];
+  const int s_at = ws * FS * 128 + lane;
+  // The tile's first fragments: of this wavefront's D, and of S.
+  auto first_of = [&](int tile, int& d0, int& s0) {
+    int tn, tm;
+    place_of(tiles, tile, tn, tm);
+    d0 = (WL ? tm : tn) * TD + wd * FD;
+    s0 = (WL ? tn : tm) * TS;
+  };
+  int d0, s0;
+  first_of(base + local, d0, s0);
+  scales(d_scales, d_scale_block, 0, true, d0, 0, FD, next_ds);
+  scales(s_scales, s_scale_block, 0, true, s0 + ws * FS, 0, FS, ss);
   Group now = group_at(0, true);
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j) weights(now, f0, j, w[j], 0, FN);
-  stage(now, t0, 0, set0, 0, kX);
-  stage(now, t0, 1, set1, 0, kX);
-  stage(now, t0, 2, set2, 0, kX);
-  tile_sync<2 * kX>();   // the first set's have arrived
-  xo[0] = fp8_operand(set0[x_at], set0[x_at + 64]);
+  for (int j = 0; j < AHEAD; ++j) direct(now, d0, j, d[j], 0, FD);
+  stage(now, s0, 0, set0, 0, kStaged);
+  stage(now, s0, 1, set1, 0, kStaged);
+  stage(now, s0, 2, set2, 0, kStaged);
+  tile_sync<2 * kStaged>();   // the first set's have arrived
+  so[0] = fp8_operand(set0[s_at], set0[s_at + 64]);
   const int columns = ACT ? a.n / 2 : a.n;
 
-  // The wait before the barrier: of the loads since the next set's, the set after it (kX) and the weight's next operands (2 FN)
+  // The wait before the barrier: of the loads since the next set's, the set after it (kStaged) and D's next operands (2 FD)
   // may be outstanding. A barrier alone does not wait for loads into LDS.
 #define PLM_HALF(J, SET, NEXT, FROM, LOAD)                                                                                \
-  _Pragma("unroll") for (int t = FROM; t < FROM + FM / 2; ++t) {                                                          \
-    const u32x4* p = t + 1 < FM ? SET + x_at + (t + 1) * 128 : NEXT + x_at;                                               \
-    xo[(t + 1) & 1] = fp8_operand(p[0], p[64]);                                                                           \
-    _Pragma("unroll") for (int f = 0; f < FN; ++f)                                                                        \
-        acc[f][t] = mma_at<J>(w[J % (AHEAD + 1)][f], xo[t & 1], acc[f][t], ws[f], xs[t]);                                 \
+  _Pragma("unroll") for (int t = FROM; t < FROM + FS / 2; ++t) {                                                          \
+    const u32x4* p = t + 1 < FS ? SET + s_at + (t + 1) * 128 : NEXT + s_at;                                               \
+    so[(t + 1) & 1] = fp8_operand(p[0], p[64]);                                                                           \
+    _Pragma("unroll") for (int i = 0; i < FD; ++i)                                                                        \
+        acc[i][t] = WL ? mma_at<J>(so[t & 1], d[J % (AHEAD + 1)][i], acc[i][t], ss[t], ds[i])                             \
+                       : mma_at<J>(d[J % (AHEAD + 1)][i], so[t & 1], acc[i][t], ds[i], ss[t]);                            \
     LOAD;                                                                                                                 \
     __builtin_amdgcn_sched_barrier(0);                                                                                    \
   }
 #define PLM_STEP(J, SET, NEXT, LAST, MORE, COUNT)                                                                         \
   PLM_HALF(J, SET, NEXT, 0,                                                                                               \
-           MORE; weights(J + AHEAD < 4 ? now : next, J + AHEAD < 4 ? f0 : fn, (J + AHEAD) & 3, w[(J + AHEAD) % (AHEAD + 1)], \
-                         t * 2 * FN / FM, (t + 1) * 2 * FN / FM))                                                         \
-  tile_sync<kX + 2 * FN * (AHEAD == 1 ? 1 : 2) + COUNT>();                                                                \
-  PLM_HALF(J, SET, NEXT, FM / 2,                                                                                          \
-           MORE; stage(J == 0 ? now : next, J == 0 ? t0 : tn, (J + 3) & 3, LAST, (t - FM / 2) * 2 * kX / FM,              \
-                       (t + 1 - FM / 2) * 2 * kX / FM))
+           MORE; direct(J + AHEAD < 4 ? now : next, J + AHEAD < 4 ? d0 : dn, (J + AHEAD) & 3, d[(J + AHEAD) % (AHEAD + 1)], \
+                        t * 2 * FD / FS, (t + 1) * 2 * FD / FS))                                                          \
+  tile_sync<kStaged + 2 * FD * (AHEAD == 1 ? 1 : 2) + COUNT>();                                                           \
+  PLM_HALF(J, SET, NEXT, FS / 2,                                                                                          \
+           MORE; stage(J == 0 ? now : next, J == 0 ? s0 : sn, (J + 3) & 3, LAST, (t - FS / 2) * 2 * kStaged / FS,         \
+                       (t + 1 - FS / 2) * 2 * kStaged / FS))
 
   for (;;) {
     const bool more = local + stride < count;
-    int f1 = 0, t1 = 0;
-    if (more) {
-      place_of(tiles, base + local + stride, f1, t1);
-      f1 = f1 * TN + wn * FN;
-      t1 *= TM;
-    }
+    int d1 = 0, s1 = 0;
+    if (more) first_of(base + local + stride, d1, s1);
 #pragma unroll
-    for (int f = 0; f < FN; ++f)
+    for (int i = 0; i < FD; ++i)
 #pragma unroll
-      for (int t = 0; t < FM; ++t) acc[f][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int t = 0; t < FS; ++t) acc[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
     for (int kb = 0; kb < a.blocks; kb += 4) {
       const bool last = kb + 4 >= a.blocks, in = !last || more;
-      const int fn = last ? f1 : f0, tn = last ? t1 : t0;
+      const int dn = last ? d1 : d0, sn = last ? s1 : s0;
       const Group next = group_at(last ? 0 : kb + 4, in);
 #pragma unroll
-      for (int f = 0; f < FN; ++f) ws[f] = next_ws[f];
+      for (int i = 0; i < FD; ++i) ds[i] = next_ds[i];
       PLM_STEP(0, set0, set1, set3, , 0)
       PLM_STEP(1, set1, set2, set0, , 0)
       PLM_STEP(2, set2, set3, set1, , 0)
-      scales(a.w_scales, w_scale_block, next.kb, in, fn, 0, FN, next_ws);
-      PLM_STEP(3, set3, set0, set2, scales(a.x_scales, x_scale_block, next.kb, in, tn + wm * FM, t, t + 1, xs), FN + FM / 2)
+      scales(d_scales, d_scale_block, next.kb, in, dn, 0, FD, next_ds);
+      PLM_STEP(3, set3, set0, set2, scales(s_scales, s_scale_block, next.kb, in, sn + ws * FS, t, t + 1, ss), FD + FS / 2)
       now = next;
     }
 
     constexpr int kOut = ACT ? FN / 2 : FN;
-    const int n0 = f0 / (ACT ? 2 : 1) * 16, column = anew(lane);
+    const int n0 = (WL ? s0 + ws * FS : d0) / (ACT ? 2 : 1) * 16, m0 = (WL ? d0 : s0 + ws * FS) * 16, column = anew(lane);
 #pragma unroll
     for (int t = 0; t < FM; ++t) {
-      const int m = (t0 + wm * FM + t) * 16 + (column & 15);
+      const int m = m0 + t * 16 + (column & 15);
       f32x4 v[kOut];
 #pragma unroll
       for (int f = 0; f < kOut; ++f) {
-        v[f] = acc[ACT ? 2 * f : f][t];
+        const int g = ACT ? 2 * f : f;
+        v[f] = WL ? acc[t][g] : acc[g][t];
         if constexpr (ACT) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[f][j] = fp8_silu_mul(v[f][j], acc[2 * f + 1][t][j]);
+          for (int j = 0; j < 4; ++j) v[f][j] = fp8_silu_mul(v[f][j], (WL ? acc[t][g + 1] : acc[g + 1][t])[j]);
         }
       }
       if (kOut % 2 == 0 && n0 + kOut * 16 <= columns) {
@@ -226,33 +240,34 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Fp8Gemm a, Tiles til
     }
     if (!more) break;
     local += stride;
-    f0 = f1;
-    t0 = t1;
+    d0 = d1;
+    s0 = s1;
   }
 #undef PLM_STEP
 #undef PLM_HALF
   __builtin_amdgcn_s_waitcnt(0x0f70);   // no load may arrive in this workgroup's LDS after its end
 }
 
-template <int WN, int WM, int FN, int FM, int AHEAD, int DT, bool ACT>
+template <int WD, int WS, int FD, int FS, int AHEAD, bool WL, int DT, bool ACT>
 hipError_t launch(const Fp8Gemm& a, hipStream_t s) {
-  const int tiles_n = (a.w_frags + WN * FN - 1) / (WN * FN), tiles_m = (a.x_frags + WM * FM - 1) / (WM * FM);
+  constexpr int TN = WL ? WS * FS : WD * FD, TM = WL ? WD * FD : WS * FS;
+  const int tiles_n = (a.w_frags + TN - 1) / TN, tiles_m = (a.x_frags + TM - 1) / TM;
   const int64_t tiles = static_cast<int64_t>(tiles_n) * tiles_m, per_xcd = (tiles + 7) / 8;
   if (tiles >= (int64_t{1} << 28)) return hipErrorInvalidValue;
   // As many workgroups as the CUs of an XCD hold at once, by their LDS.
-  constexpr int64_t resident = kFp8Cus / 8 * (4 * WM * FM * 2048 > 80 * 1024 ? 1 : 2);
-  hipLaunchKernelGGL((tile_kernel<WN, WM, FN, FM, AHEAD, DT, ACT>), dim3(static_cast<unsigned>(8 * std::min(per_xcd, resident))),
-                     dim3(64 * WN * WM), 0, s, a, Tiles{tiles_n, tiles_m, static_cast<int>(per_xcd)});
+  constexpr int64_t resident = kFp8Cus / 8 * (4 * WS * FS * 2048 > 80 * 1024 ? 1 : 2);
+  hipLaunchKernelGGL((tile_kernel<WD, WS, FD, FS, AHEAD, WL, DT, ACT>), dim3(static_cast<unsigned>(8 * std::min(per_xcd, resident))),
+                     dim3(64 * WD * WS), 0, s, a, Tiles{tiles_n, tiles_m, static_cast<int>(per_xcd)});
   return hipGetLastError();
 }
 
 template <int DT, bool ACT>
 hipError_t pick(const Fp8Gemm& a, Fp8TileKind kind, hipStream_t s) {
-  switch (kind) {   // fragments of a tile: kFp8Tiles
-    case kTile64x64: return launch<2, 1, 2, 4, 3, DT, ACT>(a, s);
-    case kTile128x64: return launch<4, 1, 2, 4, 3, DT, ACT>(a, s);
-    case kTile128x128: return launch<4, 1, 2, 8, 3, DT, ACT>(a, s);
-    default: return launch<4, 2, 4, 8, 1, DT, ACT>(a, s);
+  switch (kind) {
+    case kTile64x64: return launch<2, 1, 2, 4, 3, false, DT, ACT>(a, s);
+    case kTile128x64: return launch<4, 1, 2, 4, 3, false, DT, ACT>(a, s);
+    case kTile128x128: return launch<4, 1, 2, 8, 3, false, DT, ACT>(a, s);
+    default: return launch<4, 2, 4, 8, 1, true, DT, ACT>(a, s);
   }
 }
 
