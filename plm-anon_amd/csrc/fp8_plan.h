@@ -57,19 +57,22 @@ struct Fp8TilePlan {
   double us;
 };
 
-inline Fp8TilePlan tile_plan(int64_t x_frags, int64_t w_frags, int64_t blocks) {
+// `exact`: results in fp32, from products in bf16; tiles of 128 x 64 and 128 x 128.
+inline Fp8TilePlan tile_plan(int64_t x_frags, int64_t w_frags, int64_t blocks, bool exact) {
   struct Size {
     int n, m;             // fragments
     double step, end;     // us a block of K, and a tile's beginning and end
+    double exact;         // a block's step in fp32, 0 for none
   };
-  constexpr Size sizes[] = {{4, 4, 0.27, 1.0}, {8, 4, 0.40, 1.5}, {8, 8, 0.53, 2.0}, {16, 16, 1.07, 5.6}};
+  constexpr Size sizes[] = {{4, 4, 0.27, 1.0, 0.0}, {8, 4, 0.40, 1.5, 0.6}, {8, 8, 0.53, 2.0, 1.02}, {16, 16, 1.07, 5.6, 0.0}};
   const double steps = static_cast<double>((blocks + 3) / 4 * 4);
   Fp8TilePlan best{kTile64x64, 1e30};
   for (int k = kTile64x64; k <= kTile256x256; ++k) {
     const Size& z = sizes[k];
+    if (exact && z.exact == 0.0) continue;
     const int64_t tiles = ((w_frags + z.n - 1) / z.n) * ((x_frags + z.m - 1) / z.m);
     // The largest are bound by the matrix cores, whose clock falls as more of them work.
-    const double step = k == kTile256x256 ? z.step + 0.3 * std::min(1.0, static_cast<double>(tiles) / kFp8Cus) : z.step;
+    const double step = exact ? z.exact : k == kTile256x256 ? z.step + 0.3 * std::min(1.0, static_cast<double>(tiles) / kFp8Cus) : z.step;
     const double us = k == kTile256x256 ? 2.2 + fp8_turns(tiles) * (steps * step + z.end) : 2.2 + z.end + fp8_turns(tiles) * steps * step;
     if (us < best.us) best = {static_cast<Fp8TileKind>(k), us};
   }

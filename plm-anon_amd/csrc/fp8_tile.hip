@@ -12,6 +12,10 @@
 // Measured, rows in 8 bits, weights from memory: 8192 x 8192 x 2048 112 us (2450 TFLOP/s; 26 us of it is what the stores take a
 // copy), 8192^3 370 (2970), 2048 x 8192 x 8192 94. Of the last 70 remain with no loads at all: the products and the
 // barriers, at the clock that they leave.
+//
+// Results in fp32 are sums of bf16 products, exact ones: a fragment's codes times their scales, 16 conversions for each of an
+// operand's, 128 x 64 and 128 x 128 only. 2048 x 8192 x 2048 69 us (1000 TFLOP/s, of the 1650 that bf16's products reach; each
+// wavefront converts all of X), 65 with tiles of 256 x 128, 127 the way of few rows.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -60,6 +64,8 @@ __device__ __forceinline__ u32x2 four16(f32x4 v) {
                to_bits16<DT>(v[2]) | (static_cast<uint32_t>(to_bits16<DT>(v[3])) << 16)};
 }
 
+constexpr int kExact = -1;
+
 struct Tiles {
   int n, m, per_xcd;
 };
@@ -77,10 +83,13 @@ __device__ __forceinline__ void place_of(const Tiles& g, int tile, int& tn, int&
 // D is the operand whose fragments a wavefront reads into registers, FD of them, S the one that goes through LDS, FS; WL: S is the
 // weight, else X. Weights are read from memory and X mostly from L2, so that the largest tiles, whose registers hold one block
 // ahead only, have the weight in LDS: 8192 x 8192 x 2048 112.3 us for 117.4.
+// DT: the result's, 16 bits, or kExact: fp32, of products added in fp32.
 template <int WD, int WS, int FD, int FS, int AHEAD, bool WL, int DT, bool ACT>
 __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles tiles) {
   constexpr int kWaves = WD * WS, TD = WD * FD, TS = WS * FS, kStaged = 2 * TS / kWaves;
   constexpr int TN = WL ? TS : TD, TM = WL ? TD : TS, FN = WL ? FS : FD, FM = WL ? FD : FS;
+  constexpr bool kWide = DT == kExact;
+  static_assert(!kWide || !WL, "the exact products have X in LDS");
   static_assert(AHEAD == 1 || AHEAD == 3, "operands of two or four blocks");
   static_assert(2 * TS % kWaves == 0 && FS % 2 == 0, "every wavefront stages as many pieces of 1 KiB");
   __shared__ __attribute__((aligned(16))) u32x4 set0[TS * 128], set1[TS * 128], set2[TS * 128], set3[TS * 128];
@@ -139,6 +148,7 @@ __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles til
   f32x4 acc[FD][FS];
   int ds[FD], ss[FS], next_ds[FD];
   i32x8 d[AHEAD + 1][FD], so[2];
+  [[maybe_unused]] Fp8Exact exact[FD];
   const int s_at = ws * FS * 128 + lane;
   // The tile's first fragments: of this wavefront's D, and of S.
   auto first_of = [&](int tile, int& d0, int& s0) {
@@ -167,13 +177,19 @@ __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles til
   _Pragma("unroll") for (int t = FROM; t < FROM + FS / 2; ++t) {                                                          \
     const u32x4* p = t + 1 < FS ? SET + s_at + (t + 1) * 128 : NEXT + s_at;                                               \
     so[(t + 1) & 1] = fp8_operand(p[0], p[64]);                                                                           \
+    [[maybe_unused]] Fp8Exact other;                                                                                      \
+    if constexpr (kWide) other = fp8_exact(so[t & 1], ss[t] >> (8 * J) & 255);                                            \
     _Pragma("unroll") for (int i = 0; i < FD; ++i)                                                                        \
-        acc[i][t] = WL ? mma_at<J>(so[t & 1], d[J % (AHEAD + 1)][i], acc[i][t], ss[t], ds[i])                             \
-                       : mma_at<J>(d[J % (AHEAD + 1)][i], so[t & 1], acc[i][t], ds[i], ss[t]);                            \
+        acc[i][t] = kWide ? fp8_mma_exact(exact[i], other, acc[i][t])                                                     \
+                    : WL  ? mma_at<J>(so[t & 1], d[J % (AHEAD + 1)][i], acc[i][t], ss[t], ds[i])                          \
+                          : mma_at<J>(d[J % (AHEAD + 1)][i], so[t & 1], acc[i][t], ds[i], ss[t]);                         \
     LOAD;                                                                                                                 \
     __builtin_amdgcn_sched_barrier(0);                                                                                    \
   }
 #define PLM_STEP(J, SET, NEXT, LAST, MORE, COUNT)                                                                         \
+  if constexpr (kWide) {                                                                                                  \
+    _Pragma("unroll") for (int i = 0; i < FD; ++i) exact[i] = fp8_exact(d[J % (AHEAD + 1)][i], ds[i] >> (8 * J) & 255);   \
+  }                                                                                                                       \
   PLM_HALF(J, SET, NEXT, 0,                                                                                               \
            MORE; direct(J + AHEAD < 4 ? now : next, J + AHEAD < 4 ? d0 : dn, (J + AHEAD) & 3, d[(J + AHEAD) % (AHEAD + 1)], \
                         t * 2 * FD / FS, (t + 1) * 2 * FD / FS))                                                          \
@@ -220,7 +236,13 @@ __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles til
           for (int j = 0; j < 4; ++j) v[f][j] = fp8_silu_mul(v[f][j], (WL ? acc[t][g + 1] : acc[g + 1][t])[j]);
         }
       }
-      if (kOut % 2 == 0 && n0 + kOut * 16 <= columns) {
+      if constexpr (kWide) {
+#pragma unroll
+        for (int f = 0; f < kOut; ++f) {
+          const int n = n0 + f * 16 + (column >> 4) * 4;
+          if (m < a.m && n < columns) fp8_store4(a, m, n, columns, v[f]);
+        }
+      } else if (kOut % 2 == 0 && n0 + kOut * 16 <= columns) {
 #pragma unroll
         for (int f = 0; f + 1 < kOut; f += 2) {
           const u32x4 o = eight_columns(four16<DT>(v[f]), four16<DT>(v[f + 1]));
@@ -271,9 +293,15 @@ hipError_t pick(const Fp8Gemm& a, Fp8TileKind kind, hipStream_t s) {
   }
 }
 
+template <bool ACT>
+hipError_t pick_exact(const Fp8Gemm& a, Fp8TileKind kind, hipStream_t s) {
+  return kind == kTile128x64 ? launch<4, 1, 2, 4, 3, false, kExact, ACT>(a, s) : launch<4, 1, 2, 8, 1, false, kExact, ACT>(a, s);
+}
+
 }  // namespace
 
 hipError_t fp8_tile(const Fp8Gemm& a, Fp8TileKind kind, bool act, hipStream_t s) {
+  if (a.out == PLM_FP8_F32) return act ? pick_exact<true>(a, kind, s) : pick_exact<false>(a, kind, s);
   if (a.out == PLM_FP8_BF16) return act ? pick<DT_BF16, true>(a, kind, s) : pick<DT_BF16, false>(a, kind, s);
   return act ? pick<DT_F16, true>(a, kind, s) : pick<DT_F16, false>(a, kind, s);
 }

@@ -279,6 +279,20 @@ def test_not_finite(device, m):
     assert ((got.double() - want).abs().nan_to_num() <= off.nan_to_num()).all()
 
 
+@pytest.mark.parametrize("out", [BF16, FP16, F32])
+@pytest.mark.parametrize("m,n,k", [(700, 5000, 264), (1030, 8200, 648)])
+def test_not_finite_in_tiles(device, m, n, k, out):
+    """The same where tiles are used, K ends inside a group of four blocks, and an infinity stands in the last of them."""
+    x = _rows(m, k, BF16, seed=7)
+    x[m - 1, k - 1] = float("-inf")
+    x[m // 3, 5] = float("nan")
+    w, _ = _weight(n, k, seed=8)
+    w[n - 1, k - 2] = float("inf")
+    w[n // 2, 130] = float("nan")
+    got = fp8.linear(x.to(device), fp8.Weight.quantize(w.to(device)), out_dtype=out)
+    _check(got, oracle.rounded(x), oracle.weight(w)[0], out)
+
+
 def test_large_gates(device):
     """Gates so low that the exponential overflows give zeros, not NaN; so high, the product alone."""
     k, half = 128, 32
