@@ -599,7 +599,7 @@ size_t plm_attend_workspace_bytes(const plm_attend_call* call);
  *   codes   [b][f][k / 64 % 2][k / 8 % 4][r][k / 32 % 2][k % 8]
  *   scales  [b / 4][f][r][b % 4], the exponent + 127 in a byte
  * Codes and scales past K are zeros, rows past the last of any content. plm_fp8_codes_bytes, plm_fp8_scales_bytes: the sizes (0
- * where there are no such rows: 1 <= rows < 2^24, 8 <= K <= 2^24, K % 8 == 0). A gate/up weight (gate rows first, N a
+ * where there are no such rows: 1 <= rows < 2^24, 8 <= K <= 2^24, K % 8 == 0, at most 2^25 fragments). A gate/up weight (gate rows first, N a
  * multiple of 32) has its halves' fragments in turn: fragment 2 j has gate rows [16 j, 16 j + 16), 2 j + 1 the up
  * rows; a half's blocks of 128 rows begin with its first.
  */
@@ -632,7 +632,7 @@ int plm_fp8_rows(const plm_fp8_rows_call* call, void* stream);
 /*
  * A weight [n, k] (row stride ld) into 8 bits: `w` of `dtype`, 16-byte aligned, ld % 8 == 0, rounded with scales per 128 x
  * 128; or, where `blocks` is not NULL, e4m3 codes (8-byte aligned, ld % 8 == 0) whose scales blocks [blocks of rows, blocks of
- * K] (with gate_up the gate half's blocks of rows, then the up half's) are powers of two in [2^-126, 2^126].
+ * K] (with gate_up the gate half's blocks of rows, then the up half's) are powers of two in [2^-64, 2^119].
  */
 typedef struct plm_fp8_weight_call {
   int64_t dtype, n, k;
@@ -656,6 +656,7 @@ int plm_fp8_values(const void* codes, const void* scales, int64_t rows, int64_t 
  * 16 bits: the matrix instruction cuts each product of eight along K at 2^-14 of the largest one's power of two
  * before it adds them (fp32 results are not cut). x: codes and scales, or rows of 16 bits (x_type, row stride x_row, a
  * multiple of 8), which are rounded as plm_fp8_rows does. ldy in elements, at least y's columns. m, n <= PLM_FP8_MOST.
+ * y overlaps no operand.
  * Workspace: plm_fp8_linear_workspace_bytes (0: none needed), 16-byte aligned, of any content; calls that may run at
  * the same time need workspaces of their own.
  */

@@ -8,6 +8,8 @@
 // border between codes: what is that close is computed in fp64 and rounded once, the scale's border likewise.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "fp8_gemm.h"
 
 namespace plm {
@@ -470,9 +472,10 @@ void launch_norm(const RowsArgs& a, hipStream_t s) {
       return;
     }
   }
-  // Wavefronts of a row: a chunk to a thread.
-  const int waves = (row_chunks<E8>(a.k) + 63) / 64;
-  hipLaunchKernelGGL((row_norm_kernel<DT, RES, WEIGHT, E8>), dim3(static_cast<unsigned>(a.rows)), dim3(64 * (waves < 16 ? waves : 16)), 0, s, a);
+  // Wavefronts of a row: a chunk to a thread, in a launch of less than 2^32 threads (four for 2^24 rows).
+  const int64_t fit = 0xffffffffll / (64 * static_cast<int64_t>(a.rows));
+  const int waves = static_cast<int>(std::min({(row_chunks<E8>(a.k) + int64_t{63}) / 64, int64_t{16}, fit}));
+  hipLaunchKernelGGL((row_norm_kernel<DT, RES, WEIGHT, E8>), dim3(static_cast<unsigned>(a.rows)), dim3(64 * waves), 0, s, a);
 }
 
 template <int DT>
@@ -491,10 +494,10 @@ hipError_t launch_rows(const RowsArgs& a, bool norm, hipStream_t s) {
   return hipGetLastError();
 }
 
-// What fits a grid of a wavefront to a fragment, among others.
+// What fits a launch of a wavefront to a fragment, whose threads are less than 2^32, among others.
 bool sizes_fit(int64_t rows, int64_t k) {
   return rows >= 1 && rows < (int64_t{1} << 24) && k >= 8 && k <= (1 << 24) && k % 8 == 0 &&
-         fp8_frags(rows) * fp8_blocks(k) < (int64_t{1} << 31);
+         fp8_frags(rows) * fp8_blocks(k) <= (int64_t{1} << 25);
 }
 
 template <typename... P>

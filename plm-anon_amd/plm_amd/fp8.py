@@ -47,6 +47,8 @@ def _run(entry, index: int, *args) -> int:
 
 def _matrix(t: torch.Tensor, name: str, index: int | None = None) -> tuple[torch.Tensor, int, int, int, int, int, int]:
     """``t`` [rows, k] of 16 bits as a kernel can read it, its pointer, row stride, type's code, GPU, rows and k."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dim() != 2:
         raise ValueError(f"{name} must be [rows, k], got {list(t.shape)}")
     code = _CODES.get(t.dtype)
@@ -80,7 +82,8 @@ class _Eight:
         lib = _lib.lib()
         need = int(lib.plm_fp8_codes_bytes(rows, k)), int(lib.plm_fp8_scales_bytes(rows, k))
         if not need[0]:
-            raise ValueError(f"8-bit rows need 1 to 2^24 - 1 rows of a multiple of 8 in [8, 2^24], got [{rows}, {k}]")
+            raise ValueError(f"8-bit rows need 1 to 2^24 - 1 rows of a multiple of 8 in [8, 2^24], at most 2^25 fragments, got "
+                             f"[{rows}, {k}]")
         for name, t, size, dtype in (("codes", codes, need[0], E4M3), ("scales", scales, need[1], torch.uint8)):
             if t.dtype is not dtype or t.shape != (size,) or not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name} of [{rows}, {k}] must be contiguous {dtype} [{size}] on 16 bytes, got {t.dtype} "
@@ -108,6 +111,10 @@ class _Eight:
             both, size = self._both, self.scales_at - self.codes_at
             return both[:size].view(E4M3) if name == "codes" else both[size:]
         raise AttributeError(name)
+
+    def __reduce__(self):
+        # A copy's addresses are its own tensors'; bytes, as pickle knows no float8.
+        return _again, (type(self), self.codes.view(torch.uint8), self.scales, self.rows, self.k, self._gate_up)
 
     @property
     def device(self) -> torch.device:
@@ -171,8 +178,8 @@ class Weight(_Eight):
     @classmethod
     def from_blocks(cls, codes: torch.Tensor, scales: torch.Tensor, *, gate_up: bool = False) -> "Weight":
         """``codes`` float8_e4m3fn ``[n, k]`` with float32 ``scales [ceil(n / 128), ceil(k / 128)]`` (of a gate/up weight the
-        gate half's blocks of rows, then the up half's), powers of two in [2^-126, 2^126]: a weight is
-        ``codes * scales``. Reads the scales on the host; other scales are refused (round such a weight's values)."""
+        gate half's blocks of rows, then the up half's), powers of two in [2^-64, 2^119]: a weight is
+        ``codes * scales``, finite. Reads the scales on the host; other scales are refused (round such a weight's values)."""
         if codes.dim() != 2 or codes.dtype is not E4M3 or not codes.is_cuda:
             raise ValueError(f"codes must be float8_e4m3fn [n, k] on a GPU, got {codes.dtype} {list(codes.shape)} on {codes.device}")
         n, k = codes.shape
@@ -185,8 +192,8 @@ class Weight(_Eight):
                              f"{scales.device}")
         scales = scales.contiguous()
         bits = scales.view(torch.int32)
-        if not bool(((bits & 0x7fffff) == 0).logical_and(bits >= 1 << 23).logical_and(bits <= 253 << 23).all()):
-            raise ValueError("scales must be powers of two in [2^-126, 2^126]")
+        if not bool(((bits & 0x7fffff) == 0).logical_and(bits >= 63 << 23).logical_and(bits <= 246 << 23).all()):
+            raise ValueError("scales must be powers of two in [2^-64, 2^119]")
         if not codes.is_contiguous() or codes.data_ptr() % 8:
             codes = codes.clone(memory_format=torch.contiguous_format)
         return cls._filled(0, n, k, codes.data_ptr(), k, scales.data_ptr(), gate_up, codes)
@@ -195,7 +202,7 @@ class Weight(_Eight):
     def _filled(cls, dtype: int, n: int, k: int, at: int, stride: int, blocks: int, gate_up: bool, like: torch.Tensor) -> "Weight":
         _halves(n, gate_up)
         if not _lib.lib().plm_fp8_codes_bytes(n, k):
-            raise ValueError(f"a weight has 1 to 2^24 - 1 rows, got [{n}, {k}]")
+            raise ValueError(f"a weight has 1 to 2^24 - 1 rows and at most 2^25 fragments, got [{n}, {k}]")
         self = cls._new(n, k, like)
         self.__dict__["_gate_up"] = bool(gate_up)
         status = _run(_lib.lib().plm_fp8_weight, self._index,
@@ -203,6 +210,13 @@ class Weight(_Eight):
         if status:
             _lib.check(status, f"plm_fp8_weight([{n}, {k}], gate_up={gate_up})")
         return self
+
+
+def _again(cls, codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int, gate_up: bool):
+    if not rows:
+        return cls._new(rows, k, codes)
+    codes = codes.view(E4M3)
+    return cls(codes, scales, rows, k, gate_up=True) if gate_up else cls(codes, scales, rows, k)
 
 
 def _halves(n: int, gate_up: bool) -> int:
@@ -267,9 +281,18 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6, *,
     return out if residual is None else (out, total)
 
 
+def _overlap(a: int, a_row: int, a_width: int, b: int, b_row: int, b_width: int, rows: int) -> bool:
+    """Whether two matrices of as many rows share memory, by their addresses, row strides and widths in bytes; columns of one wide
+    matrix do not."""
+    if a + (rows - 1) * a_row + a_width <= b or b + (rows - 1) * b_row + b_width <= a:
+        return False
+    apart = (b - a) % a_row if a_row else 0
+    return a_row != b_row or apart < a_width or apart + b_width > a_row
+
+
 def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dtype: torch.dtype | None, act: bool) -> torch.Tensor:
     index, n, k = w._index, w.rows, w.k
-    if type(x) is Rows:
+    if isinstance(x, Rows):
         kind, rows, x_at, x_scales, stride, like = _lib.PLM_FP8_CODES, x.rows, x.codes_at, x.scales_at, 0, w.__dict__.get("_both")
         if out_dtype is None and out is None:
             raise ValueError("rows in 8 bits have no type of their own: out_dtype or out is needed")
@@ -304,6 +327,9 @@ def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dt
         if out.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("out requires a gradient, and the 8-bit calls have none")
         out_row = max(out.stride(0), columns)
+        if not x_scales and rows and _overlap(x_at, 2 * stride, 2 * k, out.data_ptr(), out.element_size() * out_row,
+                                              out.element_size() * columns, rows):
+            raise ValueError("out overlaps x, which workgroups read while others write")
     if not rows:
         return out
     call = _lib.pack_fp8_linear(rows, n, k, kind, x_at, x_scales, stride, w.codes_at, w.scales_at, out.data_ptr(), out_row, kind_out, act)

@@ -10,6 +10,9 @@ derivative's, |silu'| <= 1.1, times the gate's, and fp32 arithmetic with an expo
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -406,3 +409,63 @@ def test_refusals(device):
         fp8.Weight.from_blocks(codes, scales, gate_up=True)
     with pytest.raises(ValueError):
         fp8.Weight.from_blocks(codes, scales.double())
+    for bad in (2.0 ** 120, 2.0 ** -65):   # of which a value, or a value of the format's own, has no bf16
+        with pytest.raises(ValueError):
+            fp8.Weight.from_blocks(codes, scales * bad)
+    for call in (fp8.quantize, lambda t: fp8.linear(t, w), lambda t: fp8.rms_norm(t, None)):
+        for wrong in (w, None, 3.0):
+            with pytest.raises(TypeError):
+                call(wrong)
+
+
+def test_out_beside_x(device):
+    """x and out may be columns of one matrix, and not the same ones."""
+    wide = _rows(40, 264, BF16, seed=3, loud=False).to(device)
+    w = fp8.Weight.quantize((0.1 * torch.randn(72, 64, generator=torch.Generator().manual_seed(2))).to(BF16).to(device))
+    for m in (1, 5, 40):
+        want = fp8.linear(wide[:m, 64:128].clone(), w)
+        assert torch.equal(fp8.linear(wide[:m, 64:128], w, out=wide[:m, 128:200]), want)
+        assert torch.equal(fp8.linear(wide[:m, 64:128], w, out=wide[:m, 192:264]), want)
+        for out in (wide[:m, 64:136], wide[:m, 120:192], wide[:m, 0:72]):
+            with pytest.raises(ValueError):
+                fp8.linear(wide[:m, 64:128], w, out=out)
+    square = fp8.Weight.quantize(torch.eye(64, dtype=BF16, device=device))
+    x = wide[:7, :64].clone()
+    with pytest.raises(ValueError):
+        fp8.linear(x, square, out=x)
+
+
+@pytest.mark.parametrize("gate_up", [False, True])
+def test_copies(device, gate_up):
+    """Copies, also through a file, read their own memory."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(3, 136, generator=g).to(BF16).to(device)
+    w = fp8.Weight.quantize(torch.randn(64, 136, generator=g).to(BF16).to(device), gate_up=gate_up)
+    rows = fp8.quantize(x)
+    call = fp8.gate_up_silu if gate_up else fp8.linear
+    want = call(x, w)
+    for remade in (copy.deepcopy, copy.copy, lambda t: pickle.loads(pickle.dumps(t))):
+        again, them = remade(w), remade(rows)
+        assert again.gate_up == gate_up and again.shape == w.shape
+        for t in (again, them):
+            assert t.codes_at == t.codes.data_ptr() and t.scales_at == t.scales.data_ptr()
+        if remade is not copy.copy:
+            assert again.codes_at != w.codes_at and them.scales_at != rows.scales_at
+        assert torch.equal(call(them, again, out_dtype=BF16), want)
+    none = copy.deepcopy(fp8.quantize(x[:0]))
+    assert none.shape == (0, 136) and call(none, w, out_dtype=BF16).shape[0] == 0
+
+
+def test_many_rows(device):
+    """Rows of which a wavefront each, and 16 to a row, would be more threads than a launch has; offsets past 32 bits."""
+    rows, k = 1 << 22, 8192
+    if torch.cuda.mem_get_info(device)[0] < 3 * rows * k:
+        pytest.skip("the norm takes 64 GiB")
+    x = _rows(1, k, BF16, seed=9).to(device)
+    got = fp8.rms_norm(x.expand(rows, k), None)
+    want = fp8.rms_norm(x, None)
+    for at in (0, 1, (1 << 18) - 1, 1 << 18, (1 << 20) + 77, rows - 1):
+        assert torch.equal(got[at:at + 1], want)
+    assert bool((got[::4099] == want).all())
+    del got
+    torch.cuda.empty_cache()
