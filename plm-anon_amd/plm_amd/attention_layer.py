@@ -114,6 +114,8 @@ class DecoderLayer:
                  down: torch.Tensor | fp8.Weight, eps: float = 1e-6):
         if attention.norm is None:
             raise ValueError("a decoder layer's attention needs its norm")
+        if isinstance(gate_up, fp8.Weight) is not isinstance(down, fp8.Weight):
+            raise TypeError("gate_up and down are both tensors or both an fp8.Weight")
         self.attention, self.norm, self.gate_up, self.down, self.eps = attention, norm, gate_up, down, eps
 
     def __call__(self, x: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, residual: torch.Tensor | None = None,

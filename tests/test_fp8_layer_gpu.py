@@ -103,6 +103,13 @@ def test_refusals(device):
         AttentionLayer(layer.attention.out_weight, layer.attention.out_weight, layer.attention.cache, HEADS)
 
 
+def test_weights_of_two_kinds_are_refused(device):
+    layer, _ = _layer(device, True)
+    plain = torch.zeros(layer.down.shape, dtype=torch.bfloat16, device=device)
+    with pytest.raises(TypeError):
+        DecoderLayer(layer.attention, layer.norm, layer.gate_up, plain)
+
+
 @pytest.mark.parametrize("weights,mlp", [("e4m3", "0"), ("e4m3", "384"), ("model", "384")])
 def test_the_command_runs(device, weights, mlp):
     root = Path(__file__).resolve().parents[1]
