@@ -6,6 +6,11 @@
 // mean(t^2) + eps). The sum of squares and the root are fp64. y in fp32 is off by three roundings, 3 of its last places at
 // most; a code has 2^20 fp32 values to a step, so of a million values one to four would come out on the other side of a
 // border between codes: what is that close is computed in fp64 and rounded once, the scale's border likewise.
+//
+// Measured (medians, a large copy 5.1 TB/s): norm with residual into 8 bits 8192 x 2048 33.5 us, 117 MB, 3.5 TB/s (a row's values
+// are held in registers between the sum and the codes; two workgroups of a CU read while the other computes), 56 x 2048 4.5
+// and 1 x 1024 in 16 bits 2.3 us, of which 2.2 are a launch; rounding alone 8192 x 2048 14 to 17 us, 50 MB, 3.2 TB/s; values of
+// 8192 x 2048 in bf16 10.5 us, 4.8 TB/s; a weight of 11264 x 2048 15.6 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
