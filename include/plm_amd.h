@@ -611,7 +611,8 @@ size_t plm_fp8_scales_bytes(int64_t rows, int64_t k);
  * Rows x [rows, k] of `dtype` (row stride x_row, a multiple of 8) into 8 bits (norm 0: no residual, weight, sum or y), or
  * with norm: t = x + residual (residual, sum NULL: x), rounded to dtype and stored in `sum`; t weight / sqrt(mean(t^2) +
  * eps) (weight [k] of dtype, NULL: ones) into y in `dtype`, or where y is NULL into 8 bits. The norm's codes are what
- * its exact value rounds to. sum and y are contiguous [rows, k]; every pointer is 16-byte aligned; eps in [2^-100, 2^100].
+ * its exact value rounds to. sum and y are contiguous [rows, k] and overlap no input; every pointer is 16-byte aligned; eps in
+ * [2^-100, 2^100].
  */
 typedef struct plm_fp8_rows_call {
   int64_t dtype, rows, k;

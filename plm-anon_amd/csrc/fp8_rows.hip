@@ -9,7 +9,7 @@
 //
 // Measured (medians, a large copy 5.1 TB/s): norm with residual into 8 bits 8192 x 2048 33.5 us, 117 MB, 3.5 TB/s (a row's values
 // are held in registers between the sum and the codes; two workgroups of a CU read while the other computes), 56 x 2048 4.5
-// and 1 x 1024 in 16 bits 2.3 us, of which 2.2 are a launch; rounding alone 8192 x 2048 14 to 17 us, 50 MB, 3.2 TB/s; values of
+// and 1 x 1024 in 16 bits 2.3 us, of which 2.2 are a launch; rounding alone 8192 x 2048 12.7 us, 50 MB, 4.0 TB/s; values of
 // 8192 x 2048 in bf16 10.5 us, 4.8 TB/s; a weight of 11264 x 2048 15.6 us.
 #include <hip/hip_runtime.h>
 
@@ -171,11 +171,13 @@ __host__ __device__ __forceinline__ int row_chunks(int k) {
 
 // A workgroup has a row, a thread chunks thread + threads i of it, the pieces of eight at 64 (chunk / 4) + 8 (chunk % 4) and 32
 // further; eight threads have a block. The first chunk stays in
-// registers between the sum of squares and the output; the rest of a row longer than the workgroup is read again.
-template <int DT, bool RES, bool WEIGHT, bool E8>
+// registers between the sum of squares and the output; the rest of a row longer than the workgroup is read again. GROUPED: of 128
+// workgroups the sixteen of an XCD (number % 8) have the sixteen rows of a fragment; the grid is a multiple of 128.
+template <int DT, bool RES, bool WEIGHT, bool E8, bool GROUPED>
 __global__ __launch_bounds__(1024) void row_norm_kernel(RowsArgs a) {
   __shared__ double parts[16];
-  const int64_t row = blockIdx.x;
+  const int64_t row = GROUPED ? (blockIdx.x & ~127u) | ((blockIdx.x & 7u) << 4) | ((blockIdx.x >> 3) & 15u) : blockIdx.x;
+  if (GROUPED && row >= a.rows) return;
   const int threads = blockDim.x, turns = (row_chunks<E8>(a.k) + threads - 1) / threads;
   const uint16_t* x = a.x + row * a.x_row;
   const uint16_t* residual = RES ? a.residual + row * a.residual_row : nullptr;
@@ -265,8 +267,8 @@ __device__ __forceinline__ void store_fragment(const RowsArgs& a, int64_t frag, 
   if (lane < 16) fp8_put_scale(a.scales, a.frags, frag * 16 + lane, kb, fp8_blocks(a.k), fp8_exponent(scale));
 }
 
-// Sixteen rows of the norm in 8 bits: a wavefront has a fragment, row lane % 16 of it a lane, and takes the blocks of K that its
-// number gives it, the first HELD of which stay in registers. Whole lines are written, where a row to a workgroup
+// Sixteen rows of the norm in 8 bits: a wavefront has a fragment, row lane % 16 of it a lane, and has HELD blocks of K,
+// which stay in registers. Whole lines are written, where a row to a workgroup
 // writes 16 bytes of each.
 template <int DT, bool RES, bool WEIGHT, int HELD>
 __global__ __launch_bounds__(1024) void fragment_norm_kernel(RowsArgs a) {
@@ -300,17 +302,6 @@ __global__ __launch_bounds__(1024) void fragment_norm_kernel(RowsArgs a) {
         squares += squares8<DT>(held[i][j]);
       }
   }
-  for (int kb = wave + waves * HELD; kb < blocks; kb += waves)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = fp8_piece_at(kb, lane, j);
-      u32x4 v = load8(x, at, a.k);
-      if constexpr (RES) {
-        v = add8<DT>(v, load8(residual, at, a.k));
-        if (at < a.k && there) *reinterpret_cast<u32x4*>(sum + at) = v;
-      }
-      squares += squares8<DT>(v);
-    }
   squares += __shfl_xor(squares, 16);
   squares += __shfl_xor(squares, 32);
   if (lane < 16) parts[wave][lane] = squares;
@@ -332,26 +323,16 @@ __global__ __launch_bounds__(1024) void fragment_norm_kernel(RowsArgs a) {
 #pragma unroll
   for (int i = 0; i < HELD; ++i)
     if (wave + waves * i < blocks) emit(wave + waves * i, held[i]);
-  for (int kb = wave + waves * HELD; kb < blocks; kb += waves) {
-    u32x4 v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = fp8_piece_at(kb, lane, j);
-      v[j] = load8(x, at, a.k);
-      // Read again rather than the sum, which a row past the last has not stored.
-      if constexpr (RES) v[j] = add8<DT>(v[j], load8(residual, at, a.k));
-    }
-    emit(kb, v);
-  }
 }
 
-// Rows as they are: a wavefront has a fragment.
+// Rows as they are: a wavefront has a fragment, its neighbours the blocks of K beside it, so that rows are read on: 8192 x 2048
+// 12.7 us for 14.9 where they had the rows below, 8192 x 8192 40.0 for 49.8 (5.0 TB/s).
 template <int DT>
 __global__ __launch_bounds__(256) void round_kernel(RowsArgs a, int64_t count) {
-  const int64_t number = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t number = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 6) + (threadIdx.x >> 6);
   if (number >= count) return;
   const int lane = threadIdx.x & 63;
-  const int64_t kb = number / a.frags, frag = number - kb * a.frags, row = min(frag * 16 + (lane & 15), static_cast<int64_t>(a.rows) - 1);
+  const int64_t blocks = fp8_blocks(a.k), frag = number / blocks, kb = number - frag * blocks, row = min(frag * 16 + (lane & 15), static_cast<int64_t>(a.rows) - 1);
   u32x4 v[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = load8(a.x + row * a.x_row, fp8_piece_at(static_cast<int>(kb), lane, j), a.k);
@@ -462,25 +443,32 @@ __global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
   }
 }
 
-// Rows from which a workgroup has sixteen: 4096 x 4096 34.7 us for 42.7, 8192 x 2048 33.5 for 39.5, 2048 x 2048 13.4 for 10.4.
-constexpr int kFragmentRows = 4096;
+// Rows from which a workgroup has sixteen, and the blocks of K that it holds: 4096 x 4096 34.5 us for 38.0, 8192 x 2048 33.5 for
+// 36.3, 2048 x 2048 13.9 for 9.5; 8192 x 8192, half of it read again, 142 for 128.
+constexpr int kFragmentRows = 4096, kFragmentBlocks = 32;
 
 template <int DT, bool RES, bool WEIGHT, bool E8>
 void launch_norm(const RowsArgs& a, hipStream_t s) {
+  // Wavefronts of a row: a chunk to a thread, in a launch of less than 2^32 threads (four for 2^24 rows).
+  const int64_t fit = 0xffffffffll / (64 * ((static_cast<int64_t>(a.rows) + 127) / 128 * 128));
+  const int waves = static_cast<int>(std::min({(row_chunks<E8>(a.k) + int64_t{63}) / 64, int64_t{16}, fit}));
+  const unsigned rows = static_cast<unsigned>(a.rows);
   if constexpr (E8) {
-    if (a.rows >= kFragmentRows) {
+    const int blocks = static_cast<int>(fp8_blocks(a.k));
+    if (a.rows >= kFragmentRows && blocks <= kFragmentBlocks) {
       // Two blocks to a wavefront, so that two workgroups fit a CU at 2048 columns (33.5 us for 35.7 with one of 16).
-      const int blocks = static_cast<int>(fp8_blocks(a.k)), waves = blocks <= 8 ? blocks : blocks <= 16 ? 8 : 16;
-      const dim3 grid(static_cast<unsigned>(a.frags)), block(64 * waves);
+      const dim3 grid(static_cast<unsigned>(a.frags)), block(64 * (blocks <= 8 ? blocks : blocks <= 16 ? 8 : 16));
       if (blocks <= 8) hipLaunchKernelGGL((fragment_norm_kernel<DT, RES, WEIGHT, 1>), grid, block, 0, s, a);
       else hipLaunchKernelGGL((fragment_norm_kernel<DT, RES, WEIGHT, 2>), grid, block, 0, s, a);
       return;
     }
+    // A fragment's rows on one XCD, in whose L2 their pieces of its lines meet: 2048 x 4096 19.5 us for 21.9.
+    if (a.rows >= 128) {
+      hipLaunchKernelGGL((row_norm_kernel<DT, RES, WEIGHT, true, true>), dim3((rows + 127) / 128 * 128), dim3(64 * waves), 0, s, a);
+      return;
+    }
   }
-  // Wavefronts of a row: a chunk to a thread, in a launch of less than 2^32 threads (four for 2^24 rows).
-  const int64_t fit = 0xffffffffll / (64 * static_cast<int64_t>(a.rows));
-  const int waves = static_cast<int>(std::min({(row_chunks<E8>(a.k) + int64_t{63}) / 64, int64_t{16}, fit}));
-  hipLaunchKernelGGL((row_norm_kernel<DT, RES, WEIGHT, E8>), dim3(static_cast<unsigned>(a.rows)), dim3(64 * waves), 0, s, a);
+  hipLaunchKernelGGL((row_norm_kernel<DT, RES, WEIGHT, E8, false>), dim3(rows), dim3(64 * waves), 0, s, a);
 }
 
 template <int DT>
@@ -488,7 +476,8 @@ hipError_t launch_rows(const RowsArgs& a, bool norm, hipStream_t s) {
   const bool res = a.residual != nullptr, weight = a.weight != nullptr, e8 = a.y == nullptr;
   if (!norm) {
     const int64_t count = a.frags * fp8_blocks(a.k);
-    hipLaunchKernelGGL((round_kernel<DT>), dim3(static_cast<unsigned>((count + 3) / 4)), dim3(256), 0, s, a, count);
+    const int waves = count < 4096 ? 2 : 4;   // 42 x 10240 2.5 us for 2.9 of four, 4096 x 2048 8.0 for 7.7
+    hipLaunchKernelGGL((round_kernel<DT>), dim3(static_cast<unsigned>((count + waves - 1) / waves)), dim3(64 * waves), 0, s, a, count);
   } else if (e8) {
     if (res) weight ? launch_norm<DT, true, true, true>(a, s) : launch_norm<DT, true, false, true>(a, s);
     else weight ? launch_norm<DT, false, true, true>(a, s) : launch_norm<DT, false, false, true>(a, s);

@@ -70,6 +70,17 @@ def test_many_rows(device, m):
     _same(y.values(BF16), oracle.rounded(want))
 
 
+# A workgroup to a row, in groups of 128 rows from there on, and to 16 rows of up to 32 blocks from 4096 on.
+@pytest.mark.parametrize("m,k", [(127, 512), (128, 520), (300, 2056), (4095, 392), (4099, 1160), (4096, 4096), (4100, 4104)])
+def test_norm_ways(device, m, k):
+    x = _rows(m, k, BF16, seed=m + k)
+    r, w = x.flip(0).contiguous(), (1 + 0.1 * torch.randn(k, generator=torch.Generator().manual_seed(k))).to(BF16)
+    y, t = fp8.rms_norm(x.to(device), w.to(device), 1e-5, residual=r.to(device), dtype=E4M3)
+    want, total = oracle.norm(x, w, 1e-5, r)
+    assert torch.equal(t.cpu(), total)
+    _same(y.values(), oracle.rounded(want))
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_quantize_extremes(device, dtype):
     """Ties, the borders of scales, subnormals, the type's largest value; infinities and NaN stay in their place."""
@@ -456,7 +467,7 @@ def test_copies(device, gate_up):
     assert none.shape == (0, 136) and call(none, w, out_dtype=BF16).shape[0] == 0
 
 
-def test_many_rows(device):
+def test_norm_of_most_rows(device):
     """Rows of which a wavefront each, and 16 to a row, would be more threads than a launch has; offsets past 32 bits."""
     rows, k = 1 << 22, 8192
     if torch.cuda.mem_get_info(device)[0] < 3 * rows * k:

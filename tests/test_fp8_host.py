@@ -167,3 +167,29 @@ def test_oracle_pieces():
     w[16:] = 512
     values, scales = oracle.weight(w, gate_up=True)
     assert torch.equal(values, w.double()) and scales.flatten().tolist() == [2.0 ** -8, 2.0]
+
+
+def test_sizes_have_a_largest():
+    """2^25 fragments: more threads than a launch has would be needed for more."""
+    most = 1 << 25
+    assert fp8_bytes(16 * 2, 128 * (1 << 17)) == (2048 << 18, 64 << 16)
+    assert fp8_bytes((1 << 24) - 1, 128 * 32)[0] == most * 2048
+    assert fp8_bytes((1 << 24) - 1, 128 * 32 + 8) == (0, 0)
+    assert fp8_bytes(16 * (most >> 17) + 1, 128 << 17) == (0, 0)
+
+
+def test_overlap():
+    """Against a map of the bytes."""
+    for rows in (1, 2, 3):
+        for a_row in (0, 8, 12):
+            for b_row in (8, 12):
+                for a_width in (2, 4, 8):
+                    for b_width in (2, 6):
+                        for b in range(0, 60):
+                            def held(at, row, width):
+                                return {at + r * row + i for r in range(rows) for i in range(width)}
+                            meet = bool(held(20, a_row, a_width) & held(b, b_row, b_width))
+                            got = fp8._overlap(20, a_row, a_width, b, b_row, b_width, rows)
+                            assert got or not meet
+                            if a_row == b_row and a_row >= max(a_width, b_width) and abs(b - 20) < a_row:
+                                assert got == meet   # columns of one matrix
