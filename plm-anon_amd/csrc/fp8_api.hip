@@ -41,7 +41,7 @@ bool linear_of(const plm_fp8_linear_call* call, Fp8Gemm& a, Fp8Plan& p) {
   const bool exact = h.out == PLM_FP8_F32;
   const Fp8TilePlan t = tile_plan(a.x_frags, a.w_frags, a.blocks, exact);
   // Results in fp32 are a fifth to a half slower the narrow way (128 x 8192 x 2048 11.5 us for 9.2, 256 19 for 14.6).
-  p.tile = a.x_frags > 4 && t.us < (exact ? 1.25 : 1.0) * p.narrow.us;
+  p.tile = a.x_frags >= kFp8TileFrags && t.us < (exact ? 1.25 : 1.0) * p.narrow.us;
   p.kind = t.kind;
   p.codes = p.round ? plm_fp8_codes_bytes(h.m, h.k) : 0;
   p.scales = p.round ? plm_fp8_scales_bytes(h.m, h.k) : 0;

@@ -5,8 +5,8 @@
 // order. A CU pulls about 24 GB/s from memory and 94 from its L2, so all of them have to read: where a weight has few rows, K
 // is cut into ranges of workgroups, whose partial sums a second launch adds (narrow_plan).
 //
-// Measured, weights from memory: 50257 x 2048 over 16 rows 21.7 us (4.7 TB/s), 11264 x 2048 gate/up over 56 rows 10.4 (2.2 TB/s: of
-// a CU's reads two thirds are X), 6144 x 2048 over 56 rows 6.1, 2048 x 2048 over one row 3.4. Four fragments of the weight to a
+// Measured, weights from memory: 50257 x 2048 over 16 rows 21.7 us (4.7 TB/s), over 56 32.5 (of a CU's reads two thirds are X, so
+// tiles take it, 27.2), 6144 x 2048 over 56 rows 6.1, 2048 x 2048 over one row 3.4. Four fragments of the weight to a
 // workgroup, so that X is read half as often: gate/up 10.2 for 10.7, but the LM head at 56 rows 35 for 33.4, 6144 x 2048 8.7 for
 // 6.7. Nontemporal loads of the weight: 2 to 12 % less from memory (down of 2560 x 10240 at 42 rows 11.6 for 12.6), 3 to 30 %
 // more for weights that the 256 MB cache still holds (10.2 for 9.1); not done.

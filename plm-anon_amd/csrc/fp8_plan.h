@@ -1,8 +1,8 @@
-// How a product over e4m3 rows is cut into workgroups: by what each way takes, estimated from what a CU pulls.
+// How a product over e4m3 rows is cut into workgroups: by what each way takes, estimated from what a CU pulls and what comes from
+// memory.
 //
-// Measured at 2048 x 2048 to 50257 x 2048 and 2560 x 10240 over 1 to 2048 rows, weights from memory: the way with the least
-// estimate is the fastest measured one, or within a tenth of it. What bounds nearly all of them is a CU's reads, 55 to 65 GB/s
-// of both operands where several wavefronts share them, 24 of weights and 94 of X where each reads its own.
+// Measured at 2048 x 2048 to 50257 x 2048, 8192 x 8192 and 2560 x 10240 over 1 to 2048 rows, weights from memory: the way with the
+// least estimate is the fastest measured one, or within a tenth of it.
 #pragma once
 
 #include <stdint.h>
@@ -19,6 +19,12 @@ inline double fp8_turns(int64_t groups) {
   return whole == 1 ? 1.0 : 0.5 * (static_cast<double>(groups) / kFp8Cus + static_cast<double>(whole));
 }
 
+// us that a weight takes from memory, at a copy's rate; and with `work` us on the CUs, which hides the shorter of the two in part.
+inline double fp8_memory(int64_t w_frags, int64_t blocks) { return static_cast<double>(w_frags * blocks) * 2048 / 5.1e6; }
+inline double fp8_beside(double work, double memory, double shown) {
+  return 2.2 + std::max(work, memory) + shown * std::min(work, memory);
+}
+
 // Few rows: a workgroup has `rows` fragments of X and `width` of the weight and `waves` wavefronts, and K is cut into `ranges`,
 // whose sums a second launch joins.
 struct Fp8Narrow {
@@ -29,6 +35,7 @@ struct Fp8Narrow {
 // `in16`: rows of 16 bits, which every workgroup rounds.
 inline Fp8Narrow narrow_plan(int64_t x_frags, int64_t w_frags, int64_t blocks, bool act, bool in16) {
   const int64_t down = (x_frags + 3) / 4;
+  const double memory = fp8_memory(w_frags, blocks);
   Fp8Narrow best{static_cast<int>((x_frags + down - 1) / down), 2, 8, 1, 1e30};
   // Above 256 fragments of the weight two at a time: 6144 x 2048 at 56 rows 6.3 us for 7.6; at 128 fragments one: 4.2 for 4.7.
   for (int width = act || w_frags > 256 ? 2 : 1; width <= 2; ++width) {
@@ -37,9 +44,10 @@ inline Fp8Narrow narrow_plan(int64_t x_frags, int64_t w_frags, int64_t blocks, b
     // ranges, at 16 rows 8.3 and 8.7; 2560 x 10240 at 42 rows 15.2 whole, 12.5 in three.
     const int64_t most = std::min(std::max<int64_t>(kFp8Cus / across, 1), (blocks + 7) / 8);
     for (int64_t ranges = 1; ranges <= most; ranges = ranges < most ? most : most + 1) {
-      const double kib = 2.048 * static_cast<double>((blocks + ranges - 1) / ranges);   // of a fragment, in thousands of bytes
+      // Of a fragment, in thousands of bytes; a CU reads 24 to 28 GB/s of weights and 94 to 110 of X.
+      const double kib = 2.048 * static_cast<double>((blocks + ranges - 1) / ranges);
       const double each = width == 1 ? kib / 24 + kib * best.rows / 94 : kib * 2 / 28 + kib * best.rows / 110;
-      const double us = 2.2 + each * fp8_turns(across * ranges) + (ranges > 1 ? 4.5 : 0.0);
+      const double us = fp8_beside(each * fp8_turns(across * ranges), memory, 0.35) + (ranges > 1 ? 4.5 : 0.0);
       if (us < best.us) best = {best.rows, width, 8, static_cast<int>(ranges), us};
     }
   }
@@ -49,7 +57,10 @@ inline Fp8Narrow narrow_plan(int64_t x_frags, int64_t w_frags, int64_t blocks, b
   return best;
 }
 
-// More than 64 rows: tiles of the weight's rows x rows of X. (Fewer fill no tile: gate/up of 11264 x 2048 at 42 rows 13.5 us for 9.9.)
+// Many rows, or a weight of so many that X is read too often otherwise: tiles of the weight's rows x rows of X. 50257 x 2048 over
+// 56 rows 27.2 us for 32.5 the way of few rows, over 30 rows 26.5 for 26.9; 28672 x 2048 gate/up over 64 15.3 for 20.2,
+// 11264 x 2048 10.6 for 10.8.
+constexpr int kFp8TileFrags = 3;
 enum Fp8TileKind { kTile64x64, kTile128x64, kTile128x128, kTile256x256 };
 
 struct Fp8TilePlan {
@@ -61,19 +72,19 @@ struct Fp8TilePlan {
 inline Fp8TilePlan tile_plan(int64_t x_frags, int64_t w_frags, int64_t blocks, bool exact) {
   struct Size {
     int n, m;             // fragments
-    double step, end;     // us a block of K, and a tile's beginning and end
-    double exact;         // a block's step in fp32, 0 for none
+    double step, exact;   // us a block of K; in fp32, 0 for none
   };
-  constexpr Size sizes[] = {{4, 4, 0.27, 1.0, 0.0}, {8, 4, 0.40, 1.5, 0.6}, {8, 8, 0.53, 2.0, 1.02}, {16, 16, 1.07, 5.6, 0.0}};
-  const double steps = static_cast<double>((blocks + 3) / 4 * 4);
+  constexpr Size sizes[] = {{4, 4, 0.27, 0.0}, {8, 4, 0.40, 0.6}, {8, 8, 0.53, 1.02}, {16, 16, 1.07, 0.0}};
+  const double steps = static_cast<double>((blocks + 3) / 4 * 4), memory = fp8_memory(w_frags, blocks);
   Fp8TilePlan best{kTile64x64, 1e30};
   for (int k = kTile64x64; k <= kTile256x256; ++k) {
     const Size& z = sizes[k];
     if (exact && z.exact == 0.0) continue;
     const int64_t tiles = ((w_frags + z.n - 1) / z.n) * ((x_frags + z.m - 1) / z.m);
-    // The largest are bound by the matrix cores, whose clock falls as more of them work.
-    const double step = exact ? z.exact : k == kTile256x256 ? z.step + 0.3 * std::min(1.0, static_cast<double>(tiles) / kFp8Cus) : z.step;
-    const double us = k == kTile256x256 ? 2.2 + fp8_turns(tiles) * (steps * step + z.end) : 2.2 + z.end + fp8_turns(tiles) * steps * step;
+    // The largest are bound by the matrix cores, whose clock falls as more of them work, and by a tile's stores, 5.6 us.
+    const double us = k == kTile256x256
+                          ? 2.2 + fp8_turns(tiles) * (steps * (z.step + 0.3 * std::min(1.0, static_cast<double>(tiles) / kFp8Cus)) + 5.6)
+                          : fp8_beside(fp8_turns(tiles) * steps * (exact ? z.exact : z.step), memory, 0.5);
     if (us < best.us) best = {static_cast<Fp8TileKind>(k), us};
   }
   return best;

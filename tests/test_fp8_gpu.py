@@ -265,6 +265,15 @@ def test_linear(device, m, n, k, dtype, out):
     assert bool((wide[:, :2] == 7).all()) and bool((wide[:, n + 2:] == 7).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(33, 50257, 264), (50, 30000, 520), (64, 28672, 1032)])
+@pytest.mark.parametrize("out", [FP16, F32])
+def test_tiles_of_few_rows(device, m, n, k, out):
+    """A weight of many rows goes to the tiles from 33 rows of x on."""
+    x = _rows(m, k, FP16, seed=m)
+    w, values = _weight(n, k, seed=k, dtype=FP16)
+    _check(fp8.linear(x.to(device), fp8.Weight.quantize(w.to(device)), out_dtype=out), oracle.rounded(x), values, out)
+
+
 @pytest.mark.parametrize("m,half,k", [(1, 16, 8), (48, 512, 8192), (390, 5632, 512), (1100, 5640 // 16 * 16, 640), (1, 5632, 2048), (3, 48, 136), (16, 128, 1024), (42, 1000 // 16 * 16, 520), (56, 5632, 2048),
                                       (65, 304, 1416), (129, 160, 264), (300, 272, 2048), (1030, 144, 392)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
