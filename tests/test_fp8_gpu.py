@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import copy
 import pickle
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -385,6 +386,51 @@ def test_captured(device):
             eager = step(x, r)
         other.synchronize()
         assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
+
+
+def test_calls_at_once(device):
+    """Products with rounded rows and partial sums on two streams at the same time, from two threads."""
+    jobs = []
+    for seed, (m, n, k) in enumerate([(42, 512, 8192), (64, 256, 10240)]):
+        w = fp8.Weight.quantize(_weight(n, k, seed)[0].to(device))
+        x = _rows(m, k, BF16, seed).to(device)
+        jobs.append((x, w, fp8.linear(x, w)))
+    torch.cuda.synchronize()
+
+    def work(x, w, want):
+        with torch.cuda.stream(torch.cuda.Stream(device)):
+            got = [fp8.linear(x, w) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(y, want) for y in got)
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(lambda job: work(*job), jobs * 4))
+
+
+@pytest.mark.parametrize("which", ["weight", "x"])
+def test_offsets_past_32_bits(device, which):
+    """2^21 rows of 2176: codes of more than 4 GiB. Small whole numbers, whose sums are exact."""
+    many, k = 1 << 21, 2176
+    if torch.cuda.mem_get_info(device)[0] < 24 * many * k // 4:
+        pytest.skip("27 GB are needed")
+    g = torch.Generator(device=device).manual_seed(1)
+    large = torch.randint(-4, 5, (many, k), generator=g, device=device, dtype=torch.int8).to(BF16)
+    some = torch.cat([torch.arange(0, 130), torch.arange(many // 2 - 3, many // 2 + 200), torch.arange(many - 140, many)]).to(device)
+    picked = large[some].float()
+    if which == "weight":
+        w = fp8.Weight.quantize(large)
+        del large
+        for m, out in ((1, F32), (1, BF16), (40, BF16), (40, F32), (200, BF16)):
+            x = torch.randint(-2, 3, (m, k), generator=g, device=device, dtype=torch.int8).to(BF16)
+            assert torch.equal(fp8.linear(x, w, out_dtype=out)[:, some], (x.float() @ picked.T).to(out))
+    else:
+        for n, out in ((16, BF16), (136, BF16), (24, F32)):
+            w = torch.randint(-2, 3, (n, k), generator=g, device=device, dtype=torch.int8).to(BF16)
+            assert torch.equal(fp8.linear(large, fp8.Weight.quantize(w), out_dtype=out)[some], (picked @ w.float().T).to(out))
+        rows = fp8.rms_norm(large, None, dtype=E4M3)
+        want = fp8.rms_norm(large[some], None, dtype=E4M3).values(BF16)
+        assert torch.equal(rows.values(BF16)[some], want)
+    torch.cuda.empty_cache()
 
 
 def test_refusals(device):
