@@ -330,6 +330,26 @@ def test_large_gates(device):
     _check(got, oracle.rounded(x), values, BF16, act=True)
 
 
+@pytest.mark.parametrize("m", [1, 70, 600])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_activation(device, m, out):
+    """Gates over the whole range in which the activation is neither g nor 0, each of one product and so exact: the activation's own
+    error, 2^-20, its rounding, and what fp32 cannot hold of the smallest."""
+    half, k = 4096, 128
+    gates = torch.cat([torch.linspace(-104, 90, half // 2), torch.logspace(-30, 6, half // 2, base=2.0)])
+    w = torch.zeros(2 * half, k, dtype=BF16)
+    w[:half, 0], w[half:, 2] = gates.to(BF16), 1
+    x = torch.zeros(m, k, dtype=BF16)
+    x[:, 0] = 2.0 ** (torch.arange(m) % 3 - 1)
+    x[:, 2] = 1
+    got = fp8.gate_up_silu(x.to(device), fp8.Weight.quantize(w.to(device), gate_up=True), out_dtype=out).cpu().double()
+    gate = x[:, :1].double() * oracle.weight(w, True)[0][:half, 0].double()
+    want = gate * torch.sigmoid(gate)
+    off = want.abs() * 2.0 ** -20 + 2.0 ** -149
+    info = torch.finfo(out)
+    assert ((got - want).abs() <= off + (want.abs() + off) * info.eps / 2 + info.smallest_normal * info.eps / 2).all()
+
+
 def test_empty_rows(device):
     weight = fp8.Weight.quantize(_weight(32, 64, 0)[0].to(device))
     gated = fp8.Weight.quantize(_weight(32, 64, 0)[0].to(device), gate_up=True)
