@@ -17,6 +17,19 @@
 
 namespace plm {
 
+// Two values in 16 bits each, as to_bits16 rounds them, by one instruction.
+template <int DT>
+__device__ __forceinline__ uint32_t two_bits16(float a, float b) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  if constexpr (DT == DT_BF16) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, pair));
+  } else {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, pair));
+  }
+}
+
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kFp8Block = 128;           // of K

@@ -53,16 +53,15 @@ __device__ __forceinline__ void fp8_store4(const Fp8Gemm& a, int m, int n, int c
     }
     return;
   }
-  uint16_t b[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = a.out == PLM_FP8_BF16 ? to_bits16<DT_BF16>(v[j]) : to_bits16<DT_F16>(v[j]);
+  const uint32_t lo = a.out == PLM_FP8_BF16 ? two_bits16<DT_BF16>(v[0], v[1]) : two_bits16<DT_F16>(v[0], v[1]);
+  const uint32_t hi = a.out == PLM_FP8_BF16 ? two_bits16<DT_BF16>(v[2], v[3]) : two_bits16<DT_F16>(v[2], v[3]);
   uint16_t* y = static_cast<uint16_t*>(a.y) + at;
   if (left >= 4) {
-    *reinterpret_cast<fp8_any8*>(y) = u32x2{b[0] | (static_cast<uint32_t>(b[1]) << 16), b[2] | (static_cast<uint32_t>(b[3]) << 16)};
+    *reinterpret_cast<fp8_any8*>(y) = u32x2{lo, hi};
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (j < left) y[j] = b[j];
+      if (j < left) y[j] = static_cast<uint16_t>((j < 2 ? lo : hi) >> (16 * (j & 1)));
   }
 }
 

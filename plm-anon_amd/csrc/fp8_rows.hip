@@ -43,8 +43,7 @@ template <int DT>
 __device__ __forceinline__ u32x4 pack8of(const float* x) {
   u32x4 o;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    o[i] = to_bits16<DT>(x[2 * i]) | (static_cast<uint32_t>(to_bits16<DT>(x[2 * i + 1])) << 16);
+  for (int i = 0; i < 4; ++i) o[i] = two_bits16<DT>(x[2 * i], x[2 * i + 1]);
   return o;
 }
 

@@ -60,8 +60,7 @@ __device__ __forceinline__ u32x4 eight_columns(u32x2 a, u32x2 b) {
 
 template <int DT>
 __device__ __forceinline__ u32x2 four16(f32x4 v) {
-  return u32x2{to_bits16<DT>(v[0]) | (static_cast<uint32_t>(to_bits16<DT>(v[1])) << 16),
-               to_bits16<DT>(v[2]) | (static_cast<uint32_t>(to_bits16<DT>(v[3])) << 16)};
+  return u32x2{two_bits16<DT>(v[0], v[1]), two_bits16<DT>(v[2], v[3])};
 }
 
 constexpr int kExact = -1;
