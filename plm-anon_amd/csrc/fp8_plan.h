@@ -61,7 +61,7 @@ inline Fp8Narrow narrow_plan(int64_t x_frags, int64_t w_frags, int64_t blocks, b
 // 56 rows 27.2 us for 32.5 the way of few rows, over 30 rows 26.5 for 26.9; 28672 x 2048 gate/up over 64 15.3 for 20.2,
 // 11264 x 2048 10.6 for 10.8.
 constexpr int kFp8TileFrags = 3;
-enum Fp8TileKind { kTile64x64, kTile128x64, kTile128x128, kTile256x256 };
+enum Fp8TileKind { kTile64x64, kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
 
 struct Fp8TilePlan {
   Fp8TileKind kind;
@@ -72,19 +72,20 @@ struct Fp8TilePlan {
 inline Fp8TilePlan tile_plan(int64_t x_frags, int64_t w_frags, int64_t blocks, bool exact) {
   struct Size {
     int n, m;             // fragments
-    double step, exact;   // us a block of K; in fp32, 0 for none
+    double step, end;     // us a block of K, and a tile's stores
+    double exact;         // a block of K in fp32, 0 for none
   };
-  constexpr Size sizes[] = {{4, 4, 0.27, 0.0}, {8, 4, 0.40, 0.6}, {8, 8, 0.53, 1.02}, {16, 16, 1.07, 0.0}};
+  constexpr Size sizes[] = {{4, 4, 0.27, 0.0, 0.0}, {8, 4, 0.40, 0.0, 0.6}, {8, 8, 0.53, 0.0, 1.02}, {8, 16, 0.80, 3.0, 0.0}, {16, 16, 1.07, 5.6, 0.0}};
   const double steps = static_cast<double>((blocks + 3) / 4 * 4), memory = fp8_memory(w_frags, blocks);
   Fp8TilePlan best{kTile64x64, 1e30};
   for (int k = kTile64x64; k <= kTile256x256; ++k) {
     const Size& z = sizes[k];
     if (exact && z.exact == 0.0) continue;
     const int64_t tiles = ((w_frags + z.n - 1) / z.n) * ((x_frags + z.m - 1) / z.m);
-    // The largest are bound by the matrix cores, whose clock falls as more of them work, and by a tile's stores, 5.6 us.
-    const double us = k == kTile256x256
-                          ? 2.2 + fp8_turns(tiles) * (steps * (z.step + 0.3 * std::min(1.0, static_cast<double>(tiles) / kFp8Cus)) + 5.6)
-                          : fp8_beside(fp8_turns(tiles) * steps * (exact ? z.exact : z.step), memory, 0.5);
+    // The largest are bound by the matrix cores, whose clock falls as more of them work.
+    const double step = exact ? z.exact : k == kTile256x256 ? z.step + 0.3 * std::min(1.0, static_cast<double>(tiles) / kFp8Cus) : z.step;
+    const double work = fp8_turns(tiles) * (steps * step + z.end);
+    const double us = k == kTile256x256 ? 2.2 + work : fp8_beside(work, memory, 0.5);
     if (us < best.us) best = {static_cast<Fp8TileKind>(k), us};
   }
   return best;

@@ -9,6 +9,9 @@
 // begins with is read before this one's end, so the matrix cores do not run dry at either. Workgroups stay, and the loads run
 // ahead into the next tile while the last one is stored.
 //
+// Tiles of 128 x 256 are for products of about as many of them as CUs: 4096 x 2048 x 5632 45 us for 51 with 128 x 128 and 56 with
+// 256 x 256, 1024 x 8192 x 8192 64, 70 and 82.
+//
 // Measured, rows in 8 bits, weights from memory: 8192 x 8192 x 2048 112 us (2450 TFLOP/s; 26 us of it is what the stores take a
 // copy), 8192^3 370 (2970), 2048 x 8192 x 8192 94. Of the last 70 remain with no loads at all: the products and the
 // barriers, at the clock that they leave.
@@ -288,6 +291,7 @@ hipError_t pick(const Fp8Gemm& a, Fp8TileKind kind, hipStream_t s) {
     case kTile64x64: return launch<2, 1, 2, 4, 3, false, DT, ACT>(a, s);
     case kTile128x64: return launch<4, 1, 2, 4, 3, false, DT, ACT>(a, s);
     case kTile128x128: return launch<4, 1, 2, 8, 3, false, DT, ACT>(a, s);
+    case kTile128x256: return launch<4, 2, 2, 8, 3, false, DT, ACT>(a, s);
     default: return launch<4, 2, 4, 8, 1, true, DT, ACT>(a, s);
   }
 }

@@ -275,6 +275,16 @@ def test_tiles_of_few_rows(device, m, n, k, out):
     _check(fp8.linear(x.to(device), fp8.Weight.quantize(w.to(device)), out_dtype=out), oracle.rounded(x), values, out)
 
 
+@pytest.mark.parametrize("m,n,k,act", [(2040, 4090, 2056, False), (1000, 8192, 2056, False), (2040, 4096, 2056, True)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_wide_tiles(device, m, n, k, act, dtype):
+    """Tiles of 128 x 256: as many as there are CUs."""
+    x = _rows(m, k, dtype, seed=m, loud=False)
+    w, values = _weight(n, k, seed=n, gate_up=act, dtype=dtype)
+    weight = fp8.Weight.quantize(w.to(device), gate_up=act)
+    _check((fp8.gate_up_silu if act else fp8.linear)(x.to(device), weight), oracle.rounded(x), values, dtype, act)
+
+
 @pytest.mark.parametrize("m,half,k", [(1, 16, 8), (48, 512, 8192), (390, 5632, 512), (1100, 5640 // 16 * 16, 640), (1, 5632, 2048), (3, 48, 136), (16, 128, 1024), (42, 1000 // 16 * 16, 520), (56, 5632, 2048),
                                       (65, 304, 1416), (129, 160, 264), (300, 272, 2048), (1030, 144, 392)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
