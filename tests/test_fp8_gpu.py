@@ -463,6 +463,33 @@ def test_offsets_past_32_bits(device, which):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("m,n", [(2, 16), (20, 40), (200, 300)])
+def test_longest_rows(device, m, n):
+    """K of 2^24, of which eight places are not zero in x: sums that are exact."""
+    k = 1 << 24 if m * n < 1000 else 1 << 21
+    g = torch.Generator(device=device).manual_seed(m)
+    places = torch.tensor([0, 127, 128, k // 2 - 1, k // 2 + 640, k - 129, k - 128, k - 1], device=device)
+    x = torch.zeros(m, k, dtype=BF16, device=device)
+    x[:, places] = torch.randint(-3, 4, (m, 8), generator=g, device=device, dtype=torch.int8).to(BF16)
+    w = torch.randint(-4, 5, (n, k), generator=g, device=device, dtype=torch.int8).to(BF16)
+    want = x[:, places].float() @ w[:, places].float().T
+    weight = fp8.Weight.quantize(w)
+    for out in (BF16, F32):
+        assert torch.equal(fp8.linear(x, weight, out_dtype=out), want.to(out))
+    # Of 8 values v the norm is v / sqrt(sum v^2 / k), where there are any.
+    rows = x[:2]
+    got = fp8.rms_norm(rows, None, 2.0 ** -100)[:, places].double()
+    v = rows[:, places].double()
+    want = v / (v.pow(2).sum(1, keepdim=True) / k + 2.0 ** -100).sqrt()
+    assert ((got - want).abs() <= want.abs() * 2.0 ** -8).all()
+    eight = fp8.rms_norm(rows, None, 2.0 ** -100, dtype=E4M3).values()
+    blocks = (places // 128).unique()
+    exact = torch.zeros(2, len(blocks), 128, dtype=torch.float64)
+    exact[:, torch.searchsorted(blocks, places // 128).cpu(), (places % 128).cpu()] = want.cpu()
+    _same(eight.view(2, -1, 128)[:, blocks].flatten(1), oracle.rounded(exact.flatten(1)))
+    assert int((eight != 0).sum()) == int((v != 0).sum())
+
+
 def test_refusals(device):
     w = fp8.Weight.quantize(_weight(32, 64, 0)[0].to(device))
     gated = fp8.Weight.quantize(_weight(32, 64, 0)[0].to(device), gate_up=True)
