@@ -34,7 +34,7 @@ MOST = 1 << 21   # rows of a product's operands
 
 
 # What follows is on every call's path, where the host's time counts: one look at each property, strides only of tensors that
-# are not contiguous, messages formed for refusals alone.
+# are not contiguous, messages formed for refusals alone, sizes given one by one (a tuple of them costs an allocation 0.2 us more).
 
 
 def _run(entry, index: int, *args) -> int:
@@ -136,7 +136,7 @@ class _Eight:
         if dtype not in _OUT:
             raise TypeError(f"values come in bf16, fp16 or fp32, not {dtype}")
         like = self.__dict__.get("_both")
-        out = (self.codes if like is None else like).new_empty((self.rows, self.k), dtype=dtype)
+        out = (self.codes if like is None else like).new_empty(self.rows, self.k, dtype=dtype)
         if self.rows:
             status = _run(_lib.lib().plm_fp8_values, self._index, self.codes_at, self.scales_at, self.rows, self.k, self._gate_up,
                           _OUT[dtype], out.data_ptr())
@@ -264,13 +264,13 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6, *,
         if residual.shape != (rows, k) or residual.dtype is not x.dtype:
             raise ValueError(f"residual must be {x.dtype} {[rows, k]} as x is, got {residual.dtype} {list(residual.shape)}")
         residual, residual_at, residual_stride, *_ = _matrix(residual, "residual", index)
-        total = x.new_empty((rows, k))
+        total = x.new_empty(rows, k)
         total_at = total.data_ptr()
     if eight:
         out = Rows._new(rows, k, x)
         y_at, codes_at, scales_at = 0, out.codes_at, out.scales_at
     else:
-        out = x.new_empty((rows, k))
+        out = x.new_empty(rows, k)
         y_at, codes_at, scales_at = out.data_ptr(), 0, 0
     if rows:
         status = _run(_lib.lib().plm_fp8_rows, index,
@@ -318,7 +318,7 @@ def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dt
         raise ValueError(f"a product takes up to {MOST} rows of x and of the weight, got {rows} and {n}")
     columns = n // 2 if act else n
     if out is None:
-        out = like.new_empty((rows, columns), dtype=out_dtype)
+        out = like.new_empty(rows, columns, dtype=out_dtype)
         out_row = columns
     else:
         if out.shape != (rows, columns) or out.dtype is not out_dtype or out.get_device() != index or \
