@@ -10,7 +10,7 @@
 // Measured (medians, a large copy 5.1 TB/s): norm with residual into 8 bits 8192 x 2048 33.5 us, 117 MB, 3.5 TB/s (a row's values
 // are held in registers between the sum and the codes; two workgroups of a CU read while the other computes), 56 x 2048 4.5
 // and 1 x 1024 in 16 bits 2.3 us, of which 2.2 are a launch; rounding alone 8192 x 2048 12.7 us, 50 MB, 4.0 TB/s; values of
-// 8192 x 2048 in bf16 10.5 us, 4.8 TB/s; a weight of 11264 x 2048 15.6 us.
+// 8192 x 2048 in bf16 15 us, 3.4 TB/s (10.5 where part of it is cached); a weight of 11264 x 2048 15.6 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -413,16 +413,17 @@ struct ValuesArgs {
   int gate_up;
 };
 
-// A wavefront has a fragment, a lane 32 values of a row; OUT: plm_fp8_out.
+// A wavefront has a fragment, its neighbours the blocks of K beside it (8192 x 8192 50 us for 62 where they had the rows below),
+// a lane 32 values of a row; OUT: plm_fp8_out.
 template <int OUT>
 __global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
   const int64_t number = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (number >= a.count) return;
   const int lane = threadIdx.x & 63;
-  const int64_t kb = number / a.frags, frag = number - kb * a.frags;
+  const int64_t blocks = fp8_blocks(a.k), frag = number / blocks, kb = number - frag * blocks;
   const int64_t row = (a.gate_up != 0 ? (frag >> 1) * 16 + (frag & 1) * (a.rows >> 1) : frag * 16) + (lane & 15);
   if (row >= a.rows) return;
-  const u32x4* from = reinterpret_cast<const u32x4*>(a.codes + number * kFp8Bytes) + lane;
+  const u32x4* from = reinterpret_cast<const u32x4*>(a.codes + (kb * a.frags + frag) * kFp8Bytes) + lane;
   const u32x4 codes[2] = {from[0], from[64]};
   const float scale = fp8_power(a.scales[fp8_scale_at(a.frags, frag * 16 + (lane & 15), kb)]);
 #pragma unroll
