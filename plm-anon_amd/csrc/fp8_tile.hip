@@ -24,6 +24,7 @@
 #include <algorithm>
 
 #include "fp8_gemm.h"
+#include "fp8_waits.h"
 
 namespace plm {
 namespace {
@@ -94,6 +95,7 @@ __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles til
   static_assert(!kWide || !WL, "the exact products have X in LDS");
   static_assert(AHEAD == 1 || AHEAD == 3, "operands of two or four blocks");
   static_assert(2 * TS % kWaves == 0 && FS % 2 == 0, "every wavefront stages as many pieces of 1 KiB");
+  constexpr Fp8TileLoads kLoads{FD, FS, kStaged, AHEAD};
   __shared__ __attribute__((aligned(16))) u32x4 set0[TS * 128], set1[TS * 128], set2[TS * 128], set3[TS * 128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int base = (blockIdx.x & 7) * tiles.per_xcd, count = min(tiles.per_xcd, tiles.n * tiles.m - base);
@@ -169,12 +171,12 @@ __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles til
   stage(now, s0, 0, set0, 0, kStaged);
   stage(now, s0, 1, set1, 0, kStaged);
   stage(now, s0, 2, set2, 0, kStaged);
-  tile_sync<2 * kStaged>();   // the first set's have arrived
+  tile_sync<fp8_first_wait(kLoads)>();   // the first set's have arrived, and the second's where step 0 does not wait for them
   so[0] = fp8_operand(set0[s_at], set0[s_at + 64]);
   const int columns = ACT ? a.n / 2 : a.n;
 
-  // The wait before the barrier: of the loads since the next set's, the set after it (kStaged) and D's next operands (2 FD)
-  // may be outstanding. A barrier alone does not wait for loads into LDS.
+  // The wait before the barrier (fp8_waits.h): the loads issued since the next set's may be in flight. A barrier alone does not wait
+  // for loads into LDS.
 #define PLM_HALF(J, SET, NEXT, FROM, LOAD)                                                                                \
   _Pragma("unroll") for (int t = FROM; t < FROM + FS / 2; ++t) {                                                          \
     const u32x4* p = t + 1 < FS ? SET + s_at + (t + 1) * 128 : NEXT + s_at;                                               \
@@ -188,14 +190,14 @@ __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles til
     LOAD;                                                                                                                 \
     __builtin_amdgcn_sched_barrier(0);                                                                                    \
   }
-#define PLM_STEP(J, SET, NEXT, LAST, MORE, COUNT)                                                                         \
+#define PLM_STEP(J, SET, NEXT, LAST, MORE)                                                                                \
   if constexpr (kWide) {                                                                                                  \
     _Pragma("unroll") for (int i = 0; i < FD; ++i) exact[i] = fp8_exact(d[J % (AHEAD + 1)][i], ds[i] >> (8 * J) & 255);   \
   }                                                                                                                       \
   PLM_HALF(J, SET, NEXT, 0,                                                                                               \
            MORE; direct(J + AHEAD < 4 ? now : next, J + AHEAD < 4 ? d0 : dn, (J + AHEAD) & 3, d[(J + AHEAD) % (AHEAD + 1)], \
                         t * 2 * FD / FS, (t + 1) * 2 * FD / FS))                                                          \
-  tile_sync<kStaged + 2 * FD * (AHEAD == 1 ? 1 : 2) + COUNT>();                                                           \
+  tile_sync<fp8_step_wait(kLoads, J)>();                                                                                  \
   PLM_HALF(J, SET, NEXT, FS / 2,                                                                                          \
            MORE; stage(J == 0 ? now : next, J == 0 ? s0 : sn, (J + 3) & 3, LAST, (t - FS / 2) * 2 * kStaged / FS,         \
                        (t + 1 - FS / 2) * 2 * kStaged / FS))
@@ -215,11 +217,11 @@ __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles til
       const Group next = group_at(last ? 0 : kb + 4, in);
 #pragma unroll
       for (int i = 0; i < FD; ++i) ds[i] = next_ds[i];
-      PLM_STEP(0, set0, set1, set3, , 0)
-      PLM_STEP(1, set1, set2, set0, , 0)
-      PLM_STEP(2, set2, set3, set1, , 0)
+      PLM_STEP(0, set0, set1, set3, )
+      PLM_STEP(1, set1, set2, set0, )
+      PLM_STEP(2, set2, set3, set1, )
       scales(d_scales, d_scale_block, next.kb, in, dn, 0, FD, next_ds);
-      PLM_STEP(3, set3, set0, set2, scales(s_scales, s_scale_block, next.kb, in, sn + ws * FS, t, t + 1, ss), FD + FS / 2)
+      PLM_STEP(3, set3, set0, set2, scales(s_scales, s_scale_block, next.kb, in, sn + ws * FS, t, t + 1, ss))
       now = next;
     }
 
