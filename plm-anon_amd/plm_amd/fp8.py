@@ -14,13 +14,15 @@ cache; codes are rounded to nearest even, and what is not finite becomes NaN, in
 of K, a weight's 128 x 128. ``linear`` and ``gate_up_silu`` take 16-bit rows too, which they round as ``quantize`` does.
 
 Calls run on the current stream of the tensors' GPU, allocate what they return, keep nothing between calls and can be
-captured; sums are in one order, so results repeat bit for bit. Nothing here has a backward: tensors that require a
-gradient are refused while gradients are recorded.
+captured; sums are in one order, so results repeat bit for bit. Nothing here has a derivative: tensors that require a
+gradient are refused while gradients are recorded, and so are those that carry a forward-mode tangent, and calls while a
+tracer records.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -39,10 +41,21 @@ MOST = 1 << 21   # rows of a product's operands
 
 def _run(entry, index: int, *args) -> int:
     """Status of a C entry on GPU ``index``, on its current stream."""
+    if torch._C._is_tracing():
+        raise RuntimeError("a tracer would record the 8-bit calls' allocations and not what fills them: call them outside of it")
     if index == torch._C._cuda_getDevice():
         return entry(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
         return entry(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _derivative(t: torch.Tensor, name: str) -> None:
+    """Refuses a tensor whose derivative a call would drop."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, and the 8-bit calls have none: detach it, or call under no_grad")
+    # Tangents live inside a dual level only; asking for one takes ten times as long as asking for the level.
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name} carries a forward-mode tangent, and the 8-bit calls have none: detach it")
 
 
 def _matrix(t: torch.Tensor, name: str, index: int | None = None) -> tuple[torch.Tensor, int, int, int, int, int, int]:
@@ -54,8 +67,8 @@ def _matrix(t: torch.Tensor, name: str, index: int | None = None) -> tuple[torch
     code = _CODES.get(t.dtype)
     if code is None:
         raise TypeError(f"{name} must be bf16 or fp16, got {t.dtype}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} requires a gradient, and the 8-bit calls have none: detach it, or call under no_grad")
+    if t.requires_grad or forward_ad._current_level >= 0:
+        _derivative(t, name)
     rows, k = t.shape
     if k < 8 or k % 8 or k > 1 << 24:
         raise ValueError(f"{name}'s rows must have a multiple of 8 in [8, 2^24] of elements, got {k}")
@@ -88,6 +101,7 @@ class _Eight:
             if t.dtype is not dtype or t.shape != (size,) or not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name} of [{rows}, {k}] must be contiguous {dtype} [{size}] on 16 bytes, got {t.dtype} "
                                  f"{list(t.shape)}")
+        _derivative(codes, "codes")
         if not codes.is_cuda or scales.device != codes.device:
             raise RuntimeError(f"codes and scales live on one GPU; got {codes.device} and {scales.device}")
         self.__dict__.update(codes=codes, scales=scales, rows=rows, k=k, _index=codes.get_device(), codes_at=codes.data_ptr(),
@@ -190,6 +204,8 @@ class Weight(_Eight):
         if scales.shape != shape or scales.dtype is not torch.float32 or scales.device != codes.device:
             raise ValueError(f"scales must be float32 {list(shape)} on {codes.device}, got {scales.dtype} {list(scales.shape)} on "
                              f"{scales.device}")
+        _derivative(codes, "codes")
+        _derivative(scales, "scales")
         scales = scales.contiguous()
         bits = scales.view(torch.int32)
         if not bool(((bits & 0x7fffff) == 0).logical_and(bits >= 63 << 23).logical_and(bits <= 246 << 23).all()):
@@ -253,8 +269,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6, *,
     if weight is not None:
         if weight.dtype is not x.dtype or weight.shape != (k,) or weight.get_device() != index:
             raise ValueError(f"weight must be {x.dtype} [{k}] on cuda:{index}, got {weight.dtype} {list(weight.shape)} on {weight.device}")
-        if weight.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("weight requires a gradient, and the 8-bit calls have none: detach it, or call under no_grad")
+        if weight.requires_grad or forward_ad._current_level >= 0:
+            _derivative(weight, "weight")
         weight_at = weight.data_ptr()
         if weight_at % 16 or not weight.is_contiguous():
             weight = weight.clone(memory_format=torch.contiguous_format)
@@ -324,8 +340,8 @@ def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dt
         if out.shape != (rows, columns) or out.dtype is not out_dtype or out.get_device() != index or \
                 (rows and (out.stride(1) != 1 and columns > 1 or out.stride(0) < columns and rows > 1)):
             raise ValueError(f"out must be a row-major {[rows, columns]} {out_dtype} tensor on cuda:{index}")
-        if out.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("out requires a gradient, and the 8-bit calls have none")
+        if out.requires_grad or forward_ad._current_level >= 0:
+            _derivative(out, "out")
         out_row = max(out.stride(0), columns)
         if not x_scales and rows and _overlap(x_at, 2 * stride, 2 * k, out.data_ptr(), out.element_size() * out_row,
                                               out.element_size() * columns, rows):
