@@ -58,6 +58,11 @@ def _derivative(t: torch.Tensor, name: str) -> None:
         raise RuntimeError(f"{name} carries a forward-mode tangent, and the 8-bit calls have none: detach it")
 
 
+def _no_memory(name: str) -> None:
+    # A stand-in for a tensor (a tracer's, a wrapper's): its null would be taken for an argument that is not given.
+    raise RuntimeError(f"{name} has no memory that a kernel could read")
+
+
 def _matrix(t: torch.Tensor, name: str, index: int | None = None) -> tuple[torch.Tensor, int, int, int, int, int, int]:
     """``t`` [rows, k] of 16 bits as a kernel can read it, its pointer, row stride, type's code, GPU, rows and k."""
     if not isinstance(t, torch.Tensor):
@@ -76,6 +81,8 @@ def _matrix(t: torch.Tensor, name: str, index: int | None = None) -> tuple[torch
     if on < 0 or (index is not None and on != index):
         raise RuntimeError(f"{name} must be on {'a GPU' if index is None else f'cuda:{index}'}, got {t.device}")
     at = t.data_ptr()
+    if not at and rows:
+        _no_memory(name)
     if at % 16 == 0:
         if t.is_contiguous():
             return t, at, k, code, on, rows, k
@@ -206,6 +213,10 @@ class Weight(_Eight):
                              f"{scales.device}")
         _derivative(codes, "codes")
         _derivative(scales, "scales")
+        if not codes.data_ptr():
+            _no_memory("codes")
+        if not scales.data_ptr():
+            _no_memory("scales")
         scales = scales.contiguous()
         bits = scales.view(torch.int32)
         if not bool(((bits & 0x7fffff) == 0).logical_and(bits >= 63 << 23).logical_and(bits <= 246 << 23).all()):
@@ -272,6 +283,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6, *,
         if weight.requires_grad or forward_ad._current_level >= 0:
             _derivative(weight, "weight")
         weight_at = weight.data_ptr()
+        if not weight_at:
+            _no_memory("weight")
         if weight_at % 16 or not weight.is_contiguous():
             weight = weight.clone(memory_format=torch.contiguous_format)
             weight_at = weight.data_ptr()

@@ -37,3 +37,15 @@ def test_derivatives_of_every_argument_are_refused(device):
             call()
         with torch.no_grad():
             call()
+
+
+def test_a_weight_without_memory_is_refused(device):
+    """It is not a norm without weights, whose pointer is null."""
+    from torch._subclasses import FakeTensorMode
+
+    x = torch.ones(3, 64, dtype=BF16, device=device)
+    with FakeTensorMode():
+        weight = torch.empty(64, dtype=BF16, device="cuda")
+    for dtype in (BF16, E4M3):
+        with pytest.raises(RuntimeError, match="no memory"):
+            fp8.rms_norm(x, weight, dtype=dtype)

@@ -63,3 +63,15 @@ def test_tracers_are_refused():
     with pytest.raises(RuntimeError, match="tracer"):
         torch.jit.trace(traced, torch.zeros(3))
     assert not called
+
+
+def test_tensors_without_memory_are_refused():
+    from torch._subclasses import FakeTensorMode
+
+    mode = FakeTensorMode()
+    with mode:
+        x, codes, scales = (torch.empty(3, 64, device="cuda", dtype=dtype) for dtype in (BF16, E4M3, torch.float32))
+    for call in (fp8.quantize, fp8.Weight.quantize, lambda t: fp8.rms_norm(t, None), lambda t: fp8.linear(t, _weight()),
+                 lambda t: fp8.Weight.from_blocks(codes, scales[:1, :1])):
+        with pytest.raises(RuntimeError, match="no memory"):
+            call(x)
