@@ -5,7 +5,9 @@
 // Norm: t = x + residual, rounded to the model's type (so that the norm of the returned sum is the same); y = t w / sqrt(
 // mean(t^2) + eps). The sum of squares and the root are fp64. y in fp32 is off by three roundings, 3 of its last places at
 // most; a code has 2^20 fp32 values to a step, so of a million values one to four would come out on the other side of a
-// border between codes: what is that close is computed in fp64 and rounded once, the scale's border likewise.
+// border between codes: what is that close is computed in fp64 and rounded once, the scale's border likewise. So is all of
+// a row whose root fp32 does not hold well, and in bf16 a lane's values of which one's quotient by the root is subnormal in
+// fp32, where a weight of 2^7 or more would bring it back without the bits that it lost.
 //
 // Measured (medians, a large copy 5.1 TB/s): norm with residual into 8 bits 8192 x 2048 33.5 us, 117 MB, 3.5 TB/s (a row's values
 // are held in registers between the sum and the codes; its 512 workgroups are all there at once and read, compute and write
@@ -89,7 +91,7 @@ __device__ __forceinline__ double squares8(u32x4 v) {
 struct Norm {
   double exact;
   float near;
-  bool wide;   // outside of where fp32 keeps its steps: every value in fp64
+  bool wide;   // outside of where fp32 keeps its steps
 };
 
 __device__ __forceinline__ Norm norm_of(double squares, int k, double eps) {
@@ -100,11 +102,36 @@ __device__ __forceinline__ Norm norm_of(double squares, int k, double eps) {
   return n;
 }
 
-// y of N / 8 pieces of eight values. Returns whether one is so close to a place where codes may part that fp32 does not tell the
-// side: those have at most four bits of mantissa, 19 zeros at the end.
+// What of a lane's values fp32 does not settle.
+struct Unsettled {
+  bool close;   // one is so close to a place where codes may part that fp32 does not tell the side
+  bool wide;    // they may have left fp32's range on the way: all of them
+};
+
+// y of N / 8 pieces of eight values. Places where codes may part have at most four bits of mantissa, 19 zeros at the end.
+// A subnormal quotient is off by 2^-150. Times a weight below 2^7 that is 2^-8 of half of bf16's least step, and the value far
+// under the least code.
 template <int DT, bool WEIGHT, int N>
-__device__ __forceinline__ bool normed(const Norm& norm, const u32x4 (&v)[N / 8], const u32x4 (&w)[N / 8], float (&y)[N]) {
+__device__ __forceinline__ Unsettled normed(const Norm& norm, const u32x4 (&v)[N / 8], const u32x4 (&w)[N / 8], float (&y)[N]) {
   uint32_t least = ~0u;
+  bool wide = norm.wide;
+  if constexpr (WEIGHT && DT == DT_BF16) {
+    uint32_t any = 0u;
+#pragma unroll
+    for (int p = 0; p < N / 8; ++p) any |= w[p][0] | w[p][1] | w[p][2] | w[p][3];
+    if ((any & 0x40004000u) != 0u) {   // a weight of 2 or more
+      uint32_t most = 0u;
+#pragma unroll
+      for (int p = 0; p < N / 8; ++p) most = max(most, fp8_most16<DT>(w[p]));
+      if (most >= 0x4300u) {           // of 2^7
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float t = from_bits16<DT>(static_cast<uint16_t>(v[i >> 3][(i & 7) >> 1] >> (16 * (i & 1))));
+          wide = wide || (t != 0.0f && fabsf(t * norm.near) < 0x1p-126f);
+        }
+      }
+    }
+  }
 #pragma unroll
   for (int p = 0; p < N / 8; ++p) {
     float of[8];
@@ -117,14 +144,14 @@ __device__ __forceinline__ bool normed(const Norm& norm, const u32x4 (&v)[N / 8]
       least = min(least, (__builtin_bit_cast(uint32_t, y[8 * p + i]) + 4u) & 0x7ffffu);
     }
   }
-  return least <= 8u || norm.wide;
+  return {least <= 8u, wide};
 }
 
 // What is that close, in fp64 and rounded to odd: one value at a time, as it is rarely more than one of a wavefront's, and read
 // again, so that nothing is kept for it. `t` and `weight`: the row and the norm's weights, value i at place(i) of k.
 template <int DT, bool WEIGHT, int N, typename P>
-__device__ __forceinline__ void normed_exact(const Norm& norm, const uint16_t* t, const uint16_t* weight, int k, P place, float (&y)[N]) {
-  uint32_t close = norm.wide ? ~0u >> (32 - N) : 0u;
+__device__ __forceinline__ void normed_exact(const Norm& norm, bool wide, const uint16_t* t, const uint16_t* weight, int k, P place, float (&y)[N]) {
+  uint32_t close = wide ? ~0u >> (32 - N) : 0u;
 #pragma unroll
   for (int i = 0; i < N; ++i) close |= ((__builtin_bit_cast(uint32_t, y[i]) + 4u) & 0x7ffffu) <= 8u ? 1u << i : 0u;
 #pragma unroll 1
@@ -199,9 +226,9 @@ __global__ __launch_bounds__(1024) void row_norm_kernel(RowsArgs a) {
   };
   auto emit = [&](const Norm& norm, int at, const u32x4 (&v)[2], const u32x4 (&w)[2]) {
     float y[16];
-    const bool close = normed<DT, WEIGHT, 16>(norm, v, w, y);
-    if (E8 ? close : norm.wide)
-      normed_exact<DT, WEIGHT, 16>(norm, RES ? sum : x, a.weight, a.k, [&](int i) { return at + (i >> 3) * 32 + (i & 7); }, y);
+    const Unsettled some = normed<DT, WEIGHT, 16>(norm, v, w, y);
+    if ((E8 && some.close) || some.wide)
+      normed_exact<DT, WEIGHT, 16>(norm, some.wide, RES ? sum : x, a.weight, a.k, [&](int i) { return at + (i >> 3) * 32 + (i & 7); }, y);
     if constexpr (E8) {
       uint32_t c[4];
       const float scale = codes_of<16>(y, [](uint32_t most) {
@@ -314,8 +341,9 @@ __global__ __launch_bounds__(1024) void fragment_norm_kernel(RowsArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = WEIGHT ? load8(a.weight, fp8_piece_at(kb, lane, j), a.k) : u32x4{0u, 0u, 0u, 0u};
     float y[32];
-    if (normed<DT, WEIGHT, 32>(norm, v, w, y))
-      normed_exact<DT, WEIGHT, 32>(norm, RES ? sum : x, a.weight, a.k, [&](int i) { return fp8_piece_at(kb, lane, i >> 3) + (i & 7); }, y);
+    const Unsettled some = normed<DT, WEIGHT, 32>(norm, v, w, y);
+    if (some.close || some.wide)
+      normed_exact<DT, WEIGHT, 32>(norm, some.wide, RES ? sum : x, a.weight, a.k, [&](int i) { return fp8_piece_at(kb, lane, i >> 3) + (i & 7); }, y);
     uint32_t c[8];
     const float scale = codes_of<32>(y, share_row, c);
     store_fragment(a, frag, kb, lane, c, scale);

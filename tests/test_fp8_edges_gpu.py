@@ -7,6 +7,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
+from oracle import fp8_oracle as oracle
 from plm_amd import fp8
 
 pytestmark = pytest.mark.gpu
@@ -49,3 +50,37 @@ def test_a_weight_without_memory_is_refused(device):
     for dtype in (BF16, E4M3):
         with pytest.raises(RuntimeError, match="no memory"):
             fp8.rms_norm(x, weight, dtype=dtype)
+
+
+def _same(got, want):
+    got, want = got.cpu().double(), want.to(got.dtype).double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+# A row to a workgroup, sixteen to a fragment's workgroup.
+@pytest.mark.parametrize("m,k", [(5, 1416), (130, 512), (4096, 264)])
+@pytest.mark.parametrize("size", [2.0 ** 3, 2.0 ** 10, 2.0 ** 60, 2.0 ** 120])
+def test_norm_of_rows_wider_than_fp32(device, m, k, size):
+    """A value so far below its row's size that their quotient is subnormal in fp32, or zero, until the weight multiplies it.
+    The tolerance in 16 bits is that of any norm: half a step and 2^-21 of the value, half of the least subnormal."""
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(m, k, generator=g)
+    x[:, 1::2] *= 2.0 ** -86
+    x[:, 2::7] *= 2.0 ** -120
+    x[:, 5::11] = 0
+    x[:, :128] = 0
+    x[:, 0] = 2.0 ** 60
+    x[m // 2] *= 2.0 ** -20
+    x = x.to(BF16)
+    w = (size * (1 + 0.3 * torch.randn(k, generator=g))).to(BF16)
+    for r in (None, x.flip(0)):
+        want, total = oracle.norm(x, w, 1e-5, r)
+        on = None if r is None else r.to(device)
+        eight, sixteen = (fp8.rms_norm(x.to(device), w.to(device), 1e-5, residual=on, dtype=kind) for kind in (E4M3, None))
+        if r is not None:
+            assert torch.equal(eight[1].cpu(), total) and torch.equal(sixteen[1].cpu(), total)
+            eight, sixteen = eight[0], sixteen[0]
+        _same(eight.values(), oracle.rounded(want))
+        off = (sixteen.cpu().double() - want).abs()
+        assert (off <= want.abs() * (2.0 ** -8 + 2.0 ** -21) + 2.0 ** -134).all()
