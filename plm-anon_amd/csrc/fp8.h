@@ -146,12 +146,15 @@ __device__ __forceinline__ f32x4 fp8_mma(i32x8 a, i32x8 b, f32x4 c, int sa, int 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
 
-// The same with every product added in fp32: codes times their scales are bf16 values, exactly, four products of 32 deep.
+// The same with every product added in fp32: codes times half their scales are bf16 values, exactly, four products of 32 deep.
+// Half, since the largest of a row may have rounded up to 2^128, which bf16 does not hold; sums are a quarter of what they
+// stand for (kFp8Exact), without a loss at the other end: products are whole numbers of 2^-148.
+constexpr float kFp8Exact = 4.0f;
 struct Fp8Exact {
   u32x4 part[4];
 };
 __device__ __forceinline__ Fp8Exact fp8_exact(i32x8 v, int scale) {
-  const float s = fp8_power(static_cast<uint32_t>(scale));
+  const float s = 0.5f * fp8_power(static_cast<uint32_t>(scale));
   Fp8Exact e;
 #pragma unroll
   for (int i = 0; i < 4; ++i)

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(64 * KW) void narrow_kernel(Fp8Gemm a) {
 #pragma unroll
   for (int f = 0; f < NF; ++f)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) red[((wave * NF + f) * MT + t) * 64 + lane] = acc[f][t];
+    for (int t = 0; t < MT; ++t) red[((wave * NF + f) * MT + t) * 64 + lane] = EXACT ? acc[f][t] * kFp8Exact : acc[f][t];
   __syncthreads();
   auto sum = [&](int at) {
     f32x4 v = red[at * 64 + lane];

@@ -231,13 +231,17 @@ __global__ __launch_bounds__(64 * WD * WS) void tile_kernel(Fp8Gemm a, Tiles til
     for (int t = 0; t < FM; ++t) {
       const int m = m0 + t * 16 + (column & 15);
       f32x4 v[kOut];
+      auto sum = [&](int g) {
+        const f32x4 s = WL ? acc[t][g] : acc[g][t];
+        return kWide ? s * kFp8Exact : s;
+      };
 #pragma unroll
       for (int f = 0; f < kOut; ++f) {
-        const int g = ACT ? 2 * f : f;
-        v[f] = WL ? acc[t][g] : acc[g][t];
+        v[f] = sum(ACT ? 2 * f : f);
         if constexpr (ACT) {
+          const f32x4 u = sum(2 * f + 1);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[f][j] = fp8_silu_mul(v[f][j], (WL ? acc[t][g + 1] : acc[g + 1][t])[j]);
+          for (int j = 0; j < 4; ++j) v[f][j] = fp8_silu_mul(v[f][j], u[j]);
         }
       }
       if constexpr (kWide) {

@@ -84,3 +84,48 @@ def test_norm_of_rows_wider_than_fp32(device, m, k, size):
         _same(eight.values(), oracle.rounded(want))
         off = (sixteen.cpu().double() - want).abs()
         assert (off <= want.abs() * (2.0 ** -8 + 2.0 ** -21) + 2.0 ** -134).all()
+
+
+# In place, after a launch that rounds, K in ranges, tiles.
+RANGES = [(3, 40, 264), (20, 40, 264), (42, 512, 10240), (700, 2056, 1032)]
+
+
+@pytest.mark.parametrize("m,n,k", RANGES)
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_codes_of_two_to_the_128th(device, m, n, k, out):
+    """bf16's largest values round up to 2^128, which fp32 does not hold but a product with a small weight does. Each row of the
+    result is the sum of one such product and one of ordinary size that it swallows, so that the result is the product."""
+    x = torch.zeros(m, k, dtype=BF16)
+    x[:, k - 3] = torch.finfo(BF16).max
+    x[1::2, k - 3] = torch.finfo(BF16).min
+    x[:, 2] = 1
+    w = torch.zeros(n, k, dtype=BF16)
+    w[:, k - 3] = 2.0 ** -(10 + torch.arange(n) % 5)
+    w[3::4, k - 3] = 0
+    w[:, 2] = 1
+    want = x[:, k - 3].sign().double()[:, None] * 2.0 ** 128 * w[:, k - 3].double()
+    want = torch.where(want == 0, 1.0, want)
+    got = fp8.linear(x.to(device), fp8.Weight.quantize(w.to(device)), out_dtype=out)
+    assert torch.equal(got.cpu().double(), want)
+    # The same of a weight's, and of both, which is past the range of any type.
+    got = fp8.linear(w.to(device), fp8.Weight.quantize(x.to(device)), out_dtype=out)
+    assert torch.equal(got.cpu().double(), want.T)
+    got = fp8.linear(x.to(device), fp8.Weight.quantize(x[:2].to(device)), out_dtype=out)
+    assert torch.equal(got.cpu().double(), x[:, k - 3:k - 2].sign().double() * x[:2, k - 3].sign().double() * float("inf"))
+
+
+@pytest.mark.parametrize("m", [3, 20, 600])
+def test_gates_past_fp32(device, m):
+    """The activation in fp32 with such a code in the up row, and one in the gate row."""
+    half, k = 2048, 264
+    w = torch.zeros(2 * half, k, dtype=BF16)
+    w[:half, 0], w[half:, 1] = 1, torch.finfo(BF16).max
+    w[half // 2:half, 0], w[half + half // 2:, 1] = torch.finfo(BF16).max, 1
+    x = torch.zeros(m, k, dtype=BF16)
+    x[:, 0], x[:, 1] = 2.0 ** -30, 2.0 ** -40
+    x[:, 130] = 1
+    got = fp8.gate_up_silu(x.to(device), fp8.Weight.quantize(w.to(device), gate_up=True), out_dtype=F32).cpu().double()
+    g = torch.tensor([2.0 ** -30, 2.0 ** 98], dtype=torch.float64).repeat_interleave(half // 2)
+    u = torch.tensor([2.0 ** 88, 2.0 ** -40], dtype=torch.float64).repeat_interleave(half // 2)
+    want = (g * torch.sigmoid(g) * u).expand(m, half)
+    assert ((got - want).abs() <= want * (2.0 ** -20 + 2.0 ** -24)).all()
