@@ -129,3 +129,26 @@ def test_gates_past_fp32(device, m):
     u = torch.tensor([2.0 ** 88, 2.0 ** -40], dtype=torch.float64).repeat_interleave(half // 2)
     want = (g * torch.sigmoid(g) * u).expand(m, half)
     assert ((got - want).abs() <= want * (2.0 ** -20 + 2.0 ** -24)).all()
+
+
+@pytest.mark.parametrize("m", [1, 70, 600])
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("up", [2.0 ** 20, -2.0 ** 60, 2.0 ** 100])
+def test_low_gates_beside_large_values(device, m, out, up):
+    """Gates whose activation is below fp32's normal range while its product with the up value is not. The exponential e^(-|g| / 2)
+    is normal down to -174."""
+    half, k = 2048, 128
+    gates = torch.cat([torch.linspace(-174, -80, half // 2), torch.linspace(-104, -87, half // 2)])
+    w = torch.zeros(2 * half, k, dtype=BF16)
+    w[:half, 0], w[half:, 2] = gates.to(BF16), up
+    x = torch.zeros(m, k, dtype=BF16)
+    x[:, 0] = x[:, 2] = 1
+    weight = fp8.Weight.quantize(w.to(device), gate_up=True)
+    gate = oracle.weight(w, True)[0][:half, 0].double().clamp(min=-174)
+    got = fp8.gate_up_silu(x.to(device), weight, out_dtype=out).cpu().double()
+    within = oracle.weight(w, True)[0][:half, 0] >= -174
+    want = gate * torch.sigmoid(gate) * up
+    off = want.abs() * 2.0 ** -20 + 2.0 ** -149
+    info = torch.finfo(out)
+    bad = (got - want).abs() > off + (want.abs() + off) * info.eps / 2 + info.smallest_normal * info.eps / 2
+    assert not (bad & within).any()
