@@ -152,3 +152,37 @@ def test_low_gates_beside_large_values(device, m, out, up):
     info = torch.finfo(out)
     bad = (got - want).abs() > off + (want.abs() + off) * info.eps / 2 + info.smallest_normal * info.eps / 2
     assert not (bad & within).any()
+
+
+# Narrow in place, its ranges of K, an LM head, tiles of either size, all with a long K.
+LONG = [(1, 2048, 2048), (16, 50257, 2048), (42, 512, 10240), (64, 2048, 8192), (110, 2048, 2048), (700, 2056, 2056), (513, 640, 8192)]
+
+
+@pytest.mark.parametrize("m,n,k", LONG)
+def test_fp32_results_keep_small_terms(device, m, n, k):
+    """In every eight of K two large products cancel and the others are so small that an instruction which cuts an eight's
+    products at 2^-14 of the largest loses them. The sums are whole numbers of 2^-2 below 2^22, whatever their order, so
+    fp32 holds them exactly."""
+    g = torch.Generator().manual_seed(m)
+    x = torch.randint(-2, 3, (m, k), generator=g).float() / 2
+    w = torch.randint(-2, 3, (n, k), generator=g).float() / 2
+    x[:, 0::8], x[:, 5::8] = 256, 256
+    w[:, 0::8], w[:, 5::8] = 256, -256
+    weight = fp8.Weight.quantize(w.to(BF16).to(device))
+    want = (x.to(device).double() @ w.to(device).double().T.contiguous()).float()
+    for rows in (x.to(BF16).to(device), fp8.quantize(x.to(BF16).to(device))):
+        assert torch.equal(fp8.linear(rows, weight, out_dtype=F32), want)
+    # The 8-bit instruction would not: its 16-bit results have lost what they were made for.
+    if m <= 64:
+        assert not torch.equal(fp8.linear(x.to(BF16).to(device), weight), want.to(BF16))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (42, 512, 10240), (56, 6144, 2048), (517, 2048, 1416), (1100, 8200, 640)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_the_cut_has_no_sign(device, m, n, k, dtype):
+    """Products are cut toward zero, whatever their sign: negative rows have the negative results, bit for bit."""
+    g = torch.Generator(device=device).manual_seed(k)
+    x = torch.randn(m, k, generator=g, device=device) * (1 + 15 * (torch.rand(k, generator=g, device=device) < 0.01))
+    weight = fp8.Weight.quantize((0.05 * torch.randn(n, k, generator=g, device=device)).to(dtype))
+    x = x.to(dtype)
+    assert torch.equal(fp8.linear(-x, weight), -fp8.linear(x, weight))
