@@ -319,6 +319,13 @@ def _overlap(a: int, a_row: int, a_width: int, b: int, b_row: int, b_width: int,
     return a_row != b_row or apart < a_width or apart + b_width > a_row
 
 
+def _meets(begin: int, end: int, eight: _Eight) -> bool:
+    """Whether [begin, end) shares memory with 8-bit rows."""
+    frags, blocks = (eight.rows + 15) // 16, (eight.k + 127) // 128
+    return (begin < eight.codes_at + frags * blocks * 2048 and eight.codes_at < end
+            or begin < eight.scales_at + frags * ((blocks + 3) // 4) * 64 and eight.scales_at < end)
+
+
 def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dtype: torch.dtype | None, act: bool) -> torch.Tensor:
     index, n, k = w._index, w.rows, w.k
     if isinstance(x, Rows):
@@ -356,6 +363,11 @@ def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dt
         if out.requires_grad or forward_ad._current_level >= 0:
             _derivative(out, "out")
         out_row = max(out.stride(0), columns)
+        if rows:
+            begin = out.data_ptr()
+            end = begin + out.element_size() * ((rows - 1) * out_row + columns)
+            if _meets(begin, end, w) or x_scales and _meets(begin, end, x):
+                raise ValueError("out overlaps an operand, which workgroups read while others write")
         if not x_scales and rows and _overlap(x_at, 2 * stride, 2 * k, out.data_ptr(), out.element_size() * out_row,
                                               out.element_size() * columns, rows):
             raise ValueError("out overlaps x, which workgroups read while others write")

@@ -186,3 +186,26 @@ def test_the_cut_has_no_sign(device, m, n, k, dtype):
     weight = fp8.Weight.quantize((0.05 * torch.randn(n, k, generator=g, device=device)).to(dtype))
     x = x.to(dtype)
     assert torch.equal(fp8.linear(-x, weight), -fp8.linear(x, weight))
+
+
+def test_out_on_an_operand_is_refused(device):
+    """A result may not lie on 8-bit rows or weights either, on their codes or their scales; beside them it may."""
+    ones = torch.ones(64, 256, dtype=BF16, device=device)
+    w = fp8.Weight.quantize(ones)
+    x = fp8.quantize(ones)
+    size, after = x.codes.numel(), x.codes.numel() + 64 * 64 * 2
+    store = torch.zeros(1 << 16, dtype=torch.uint8, device=device)
+    store[:size], store[after:after + x.scales.numel()] = x.codes.view(torch.uint8), x.scales
+    codes, scales = store[:size].view(E4M3), store[after:after + x.scales.numel()]
+
+    def out(begin):
+        return store[begin:begin + 64 * 64 * 2].view(BF16).view(64, 64)
+
+    for rows, weight in ((fp8.Rows(codes, scales, 64, 256), w), (x, fp8.Weight(codes, scales, 64, 256))):
+        for begin in (0, size - 16, size + 16, after, after + x.scales.numel() - 16):
+            with pytest.raises(ValueError, match="overlaps an operand"):
+                fp8.linear(rows, weight, out=out(begin))
+        for begin in (size, after + x.scales.numel()):
+            assert bool((fp8.linear(rows, weight, out=out(begin)) == 256).all())
+    with pytest.raises(ValueError, match="overlaps an operand"):
+        fp8.linear(ones, fp8.Weight(codes, scales, 64, 256), out=out(0))
