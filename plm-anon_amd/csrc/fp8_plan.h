@@ -1,8 +1,9 @@
 // How a product over e4m3 rows is cut into workgroups: by what each way takes, estimated from what a CU pulls and what comes from
 // memory.
 //
-// Measured at 2048 x 2048 to 50257 x 2048, 8192 x 8192 and 2560 x 10240 over 1 to 2048 rows, weights from memory: the way with the
-// least estimate is the fastest measured one, or within a tenth of it.
+// Measured at 2048 x 2048 to 50257 x 2048, 8192 x 8192, 2560 x 10240 and two gate/up weights, 16-bit and fp32 results, over 1 to
+// 2048 rows, each way by itself: of 210 choices all but two are the fastest way or within a tenth of it, gate/up of 28672 x 2048
+// over 30 rows (16.0 us for 13.8) and of 11264 x 2048 over 512 in fp32 (33.1 for 29.6).
 #pragma once
 
 #include <stdint.h>
@@ -58,8 +59,8 @@ inline Fp8Narrow narrow_plan(int64_t x_frags, int64_t w_frags, int64_t blocks, b
 }
 
 // Many rows, or a weight of so many that X is read too often otherwise: tiles of the weight's rows x rows of X. 50257 x 2048 over
-// 56 rows 27.2 us for 32.5 the way of few rows, over 30 rows 26.5 for 26.9; 28672 x 2048 gate/up over 64 15.3 for 20.2,
-// 11264 x 2048 10.6 for 10.8.
+// 56 rows 26.7 us for 32.8 the way of few rows, 28672 x 2048 gate/up over 64 15.2 for 19.7, 11264 x 2048 over 56 10.1 for 10.6.
+// Below 33 rows they are not tried; of what was measured there only these weights would gain (24.6 for 26.2, 13.8 for 16.0 over 30).
 constexpr int kFp8TileFrags = 3;
 enum Fp8TileKind { kTile64x64, kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
 

@@ -9,11 +9,11 @@
 // a row whose root fp32 does not hold well, and in bf16 a lane's values of which one's quotient by the root is subnormal in
 // fp32, where a weight of 2^7 or more would bring it back without the bits that it lost.
 //
-// Measured (medians, a large copy 5.1 TB/s): norm with residual into 8 bits 8192 x 2048 33.5 us, 117 MB, 3.5 TB/s (a row's values
-// are held in registers between the sum and the codes; its 512 workgroups are all there at once and read, compute and write
-// nearly in step), 56 x 2048 4.5
-// and 1 x 1024 in 16 bits 2.3 us, of which 2.2 are a launch; rounding alone 8192 x 2048 12.7 us, 50 MB, 4.0 TB/s; values of
-// 8192 x 2048 in bf16 15 us, 3.4 TB/s (10.5 where part of it is cached); a weight of 11264 x 2048 15.6 us.
+// Measured (replayed over inputs from memory; a large copy 5.1 TB/s). Norm with residual into 8 bits: 8192 x 2048 34.4 us,
+// 117 MB, 3.4 TB/s (a row's values are held in registers between the sum and the codes; its 512 workgroups are all there at
+// once and read, compute and write nearly in step), 16384 x 2048 61.5, 56 x 2048 4.0. Norm in 16 bits: 8192 x 2048 with
+// residual 34.3, 134 MB, 3.9 TB/s; 1 x 1024 2.3, of which 2.2 are a launch. Rounding alone: 8192 x 2048 12.7, 50 MB, 4.0 TB/s.
+// Values of 8192 x 2048 in bf16: 15, 3.4 TB/s (10.5 where part of it is cached). A weight of 11264 x 2048: 15.6.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -472,13 +472,13 @@ __global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
   }
 }
 
-// Rows from which a workgroup has sixteen, and the blocks of K that it holds: 4096 x 4096 34.5 us for 38.0, 8192 x 2048 33.5 for
-// 36.3, 2048 x 2048 13.9 for 9.5; 8192 x 8192, half of it read again, 142 for 128.
+// Rows from which a workgroup has sixteen, and the blocks of K that its registers hold: 4096 x 2048 20.2 us for
+// 21.6 with one, 4096 x 4096 34.6 for 39.1, 8192 x 2048 34.4 for 36.9, but 2048 x 2048 16.5 for 12.2 and 512 x 2048 13.5 for 5.7.
 constexpr int kFragmentRows = 4096, kFragmentBlocks = 32;
 
 template <int DT, bool RES, bool WEIGHT, bool E8>
 void launch_norm(const RowsArgs& a, hipStream_t s) {
-  // Wavefronts of a row: a chunk to a thread, in a launch of less than 2^32 threads (four for 2^24 rows).
+  // Wavefronts of a row: a chunk to a thread, in a launch of less than 2^32 threads (three for the most rows).
   const int64_t fit = 0xffffffffll / (64 * ((static_cast<int64_t>(a.rows) + 127) / 128 * 128));
   const int waves = static_cast<int>(std::min({(row_chunks<E8>(a.k) + int64_t{63}) / 64, int64_t{16}, fit}));
   const unsigned rows = static_cast<unsigned>(a.rows);
@@ -491,7 +491,8 @@ void launch_norm(const RowsArgs& a, hipStream_t s) {
       else hipLaunchKernelGGL((fragment_norm_kernel<DT, RES, WEIGHT, 2>), grid, block, 0, s, a);
       return;
     }
-    // A fragment's rows on one XCD, in whose L2 their pieces of its lines meet: 2048 x 4096 19.5 us for 21.9.
+    // A fragment's rows on one XCD, in whose L2 their pieces of its lines meet: 2048 x 4096 21.8 us for 24.4, 8192 x 8192 115 for
+    // 144, 128 x 2048 4.1 for 4.1.
     if (a.rows >= 128) {
       hipLaunchKernelGGL((row_norm_kernel<DT, RES, WEIGHT, true, true>), dim3((rows + 127) / 128 * 128), dim3(64 * waves), 0, s, a);
       return;

@@ -388,7 +388,9 @@ def _product(x: torch.Tensor | Rows, w: Weight, out: torch.Tensor | None, out_dt
 def linear(x: torch.Tensor | Rows, w: Weight, *, out: torch.Tensor | None = None,
            out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x @ w^T`` ``[rows, n]``, summed in fp32 and rounded once to ``out_dtype``: bf16, fp16 or fp32, x's type unless given
-    (``Rows`` have none). ``x`` is ``[rows, k]``, in 16 bits, which are rounded to 8 here, or ``Rows``."""
+    (``Rows`` have none). ``x`` is ``[rows, k]``, in 16 bits, which are rounded to 8 here, or ``Rows``. For 16-bit results the
+    matrix instruction cuts, toward zero, each product of an eight along k at 2^-14 of the power of two of the largest, 1.5e-5
+    to 4e-5 of a result's size (rms); for float32 every product is added whole, at up to twice the time."""
     if not isinstance(w, Weight):
         raise TypeError(f"w must be an fp8.Weight, got {type(w).__name__}")
     if w._gate_up:
@@ -399,7 +401,8 @@ def linear(x: torch.Tensor | Rows, w: Weight, *, out: torch.Tensor | None = None
 def gate_up_silu(x: torch.Tensor | Rows, w: Weight, *, out: torch.Tensor | None = None,
                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``silu(g) * u`` of the halves of ``x @ w^T``, ``[rows, n / 2]``: in fp32 up to the one rounding to ``out_dtype``
-    (``fast_gemm.gate_up_silu`` rounds the projections and the activation on the way). ``w`` is a gate/up weight."""
+    (``fast_gemm.gate_up_silu`` rounds the projections and the activation on the way), the sums as ``linear``'s, the
+    activation good to 2^-20 of its value for gates down to -174. ``w`` is a gate/up weight."""
     if not isinstance(w, Weight):
         raise TypeError(f"w must be an fp8.Weight, got {type(w).__name__}")
     if not w._gate_up:
