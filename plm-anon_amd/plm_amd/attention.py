@@ -16,8 +16,8 @@ captured batch can be padded. A sequence's rows follow ``lengths[b]`` cached tok
 in page ``table[b, t // page]``. ``lengths``, ``row_starts`` (which do not fall) and ``positions`` are int64
 tensors on the GPU and are never read on the host, so every call can be captured in a HIP graph and replayed as
 the sequences grow; only ``max_rows`` (the longest sequence's rows) and the tensors' shapes size a launch. Table
-entries outside the cache are pages that are not there. Nothing here has a backward: tensors that require a
-gradient are refused while gradients are recorded.
+entries outside the cache are pages that are not there. Nothing here has a derivative: rows that require a
+gradient are refused while gradients are recorded, and so are those that carry a forward-mode tangent.
 """
 
 from __future__ import annotations
@@ -26,6 +26,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -135,6 +136,8 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, cache: P
         raise RuntimeError(f"{name} must be on the cache's GPU {cache.device}, got {t.device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, and the cache's calls have none: detach it, or call under no_grad")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name} carries a forward-mode tangent, and the cache's calls have none: detach it")
     at = t.data_ptr()
     if at % 16 == 0:
         if t.is_contiguous():

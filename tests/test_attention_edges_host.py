@@ -58,3 +58,18 @@ def test_gradients_are_refused():
         q = torch.zeros(5, 4, 64, dtype=torch.bfloat16, requires_grad=True)
         with pytest.raises(ValueError, match="row_starts"):
             attention.attend(_stub(), q, c["table"], c["lengths"])
+
+
+def test_tangents_are_refused():
+    """Nor a forward-mode derivative: an output without a tangent would lose it in silence."""
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        for name in ("q", "k", "v"):
+            c = _call()
+            c[name] = forward_ad.make_dual(c[name], torch.ones_like(c[name]))
+            with pytest.raises(RuntimeError, match="tangent"):
+                attention.append_kv(_stub(), c["q"], c["k"], c["v"], c["table"], c["lengths"])
+            if name == "q":
+                with pytest.raises(RuntimeError, match="tangent"):
+                    attention.attend(_stub(), c["q"], c["table"], c["lengths"])
