@@ -389,8 +389,8 @@ def linear(x: torch.Tensor | Rows, w: Weight, *, out: torch.Tensor | None = None
            out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x @ w^T`` ``[rows, n]``, summed in fp32 and rounded once to ``out_dtype``: bf16, fp16 or fp32, x's type unless given
     (``Rows`` have none). ``x`` is ``[rows, k]``, in 16 bits, which are rounded to 8 here, or ``Rows``. For 16-bit results the
-    matrix instruction cuts, toward zero, each product of an eight along k at 2^-14 of the power of two of the largest, 1.5e-5
-    to 4e-5 of a result's size (rms); for float32 every product is added whole, at up to twice the time."""
+    matrix instruction cuts, toward zero, each product of an eight along k at 2^-13 of two to the largest sum of two factors'
+    exponents, which is 1.5e-5 to 4e-5 of a result's size (rms); for float32 every product is added whole, at up to twice the time."""
     if not isinstance(w, Weight):
         raise TypeError(f"w must be an fp8.Weight, got {type(w).__name__}")
     if w._gate_up:

@@ -209,3 +209,27 @@ def test_out_on_an_operand_is_refused(device):
             assert bool((fp8.linear(rows, weight, out=out(begin)) == 256).all())
     with pytest.raises(ValueError, match="overlaps an operand"):
         fp8.linear(ones, fp8.Weight(codes, scales, 64, 256), out=out(0))
+
+
+@pytest.mark.parametrize("a,b,unit", [(256, 256, 3), (448, 448, 3), (240, 256, 2), (240, 240, 1), (1, 1, -13), (2.0 ** -6, 256, -11),
+                                      (2.0 ** -9, 256, -11), (7 * 2.0 ** -9, 448, -11)])
+def test_where_an_eight_is_cut(device, a, b, unit):
+    """At 2^-13 of two to the largest sum of two factors' exponents, a subnormal code's being -6: what is below goes, toward
+    zero, in its own eight alone, and fp32 results keep it."""
+    def one(small, out, at=2):
+        x, w = torch.zeros(2, 256, dtype=BF16), torch.zeros(16, 256, dtype=BF16)
+        x[:, 126::128], w[:, 125::128] = 448, 448          # scales of 1, and products of zero in an eight of their own
+        x[0, 0], x[0, 1], w[:, 0], w[:, 1] = a, a, b, -b
+        half = max(-9, min(8, unit))          # factors that are codes: the other one normal
+        x[0, at], w[:, at] = 2.0 ** half, small * 2.0 ** -half
+        x[1] = -x[0]
+        w8 = fp8.Weight.quantize(w.to(device))
+        assert torch.equal(w8.values().cpu(), w.float())
+        got = fp8.linear(x.to(device), w8, out_dtype=out).cpu()
+        assert torch.equal(got[0], -got[1])
+        return float(got[0, 0])
+
+    for small, kept in ((2.0 ** unit, 2.0 ** unit), (1.875 * 2.0 ** unit, 2.0 ** unit), (2.0 ** (unit - 1), 0.0), (1.5 * 2.0 ** (unit - 1), 0.0)):
+        assert one(small, BF16) == kept
+        assert one(small, BF16, at=8) == small
+        assert one(small, F32) == small
